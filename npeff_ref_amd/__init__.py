@@ -48,4 +48,11 @@ from .binding import (  # noqa: F401
     op_dot,
     op_spsp_dense,
     op_init_uniform,
+    op_linear,
+    op_linear_backward,
+    op_example_grads,
+    op_vocab_loss,
+    op_vocab_loss_backward,
+    linear_workspace,
+    vocab_loss_workspace,
 )

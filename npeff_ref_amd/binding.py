@@ -5,6 +5,7 @@ from __future__ import annotations
 import ctypes as C
 import math
 import os
+import sys
 import time
 from dataclasses import dataclass
 from typing import Callable, Optional
@@ -136,6 +137,30 @@ SIGNATURES = {
     "dnpeff_op_spsp_dense": (C.c_int, [_p, _p, _p]),
     "dnpeff_op_copy": (C.c_int, [_i64, _p, _p]),
     "dnpeff_op_init_uniform": (C.c_int, [C.c_int, _i64, _i64, _u64, _p]),
+    "dnpeff_linear_workspace": (C.c_int, [C.c_int, _i64, _i64, _i64, C.c_int, C.POINTER(_i64), C.POINTER(_i64)]),
+    "dnpeff_linear": (
+        C.c_int,
+        [_p, C.c_int, _i64, _i64, _i64, _p, _i64, _p, _i64, _i64, _p, C.c_int, _p, _i64, _p, _i64, _p, _i64, C.c_int, _p,
+         _p, _i64],
+    ),
+    "dnpeff_linear_backward": (
+        C.c_int,
+        [_p, C.c_int, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _p, _i64, C.c_int, _p, _i64, _p, _i64, _i64,
+         _p, C.c_int, _p, _p, _i64],
+    ),
+    "dnpeff_example_grads": (
+        C.c_int,
+        [_p, C.c_int, _i64, _i64, _i64, _p, _i64, _p, _i64, C.c_int, _p, _p, C.c_int],
+    ),
+    "dnpeff_vocab_loss_workspace": (C.c_int, [C.c_int, _i64, _i64, _i64, C.POINTER(_i64), C.POINTER(_i64)]),
+    "dnpeff_vocab_loss": (
+        C.c_int,
+        [_p, C.c_int, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _p, _p, _p, _i64],
+    ),
+    "dnpeff_vocab_loss_backward": (
+        C.c_int,
+        [_p, C.c_int, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _p, _p, _p, _i64, _p, _i64, _p, _i64],
+    ),
 }
 
 for _name, (_res, _args) in SIGNATURES.items():
@@ -401,6 +426,230 @@ def op_threshold_compact(x: "DeviceArray", divisor: float, threshold: float):
         raise
     _check(lib.dnpeff_threshold_take(found, idx.ctypes.data, val.ctypes.data))
     return idx, val
+
+
+# ---- operators of a language model whose Fishers are wanted ----------------------------------------------------
+# Operands are DeviceArrays (float32, float16, or uint16 holding the bits of bfloat16) or tensors of a library with
+# torch's interface on the GPU, all of one kind in a call.  Calls are queued on `stream` (a stream's handle): by default the
+# library's for DeviceArrays, the tensors' library's current one for tensors.
+
+F32, F16, BF16 = 0, 1, 2
+ACTS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+_KINDS = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16, "torch.int32": "i4", "torch.int64": "i8",
+          "float32": F32, "float16": F16, "uint16": BF16, "int32": "i4", "int64": "i8"}
+_KIND_OF = {}  # dtype objects seen so far
+
+
+class _Call:
+    """The operands of one call: checks of their kind, shape and layout; pointers, and where to queue it."""
+
+    def __init__(self, what, first):
+        self.what = what
+        self.own = isinstance(first, DeviceArray)
+        self.first = first
+        self.type = self.kind(first)
+        if self.type not in (F32, F16, BF16):
+            self.refuse(f"operands of {first.dtype}: float32, float16 or bfloat16 is wanted")
+
+    def refuse(self, why):
+        raise DnpeffError(f"{self.what}: {why}")
+
+    def kind(self, a):
+        k = _KIND_OF.get(a.dtype)
+        if k is None:
+            k = _KIND_OF[a.dtype] = _KINDS.get(str(a.dtype), str(a.dtype))
+        return k
+
+    def array(self, name, a, shape, kind=None):
+        """(address, elements from one row to the next, ... from one matrix to the next); None: a NULL."""
+        if a is None:
+            return None, 0, 0
+        if isinstance(a, DeviceArray) != self.own:
+            self.refuse(f"{name}: DeviceArrays and tensors do not mix in a call")
+        if self.kind(a) != (self.type if kind is None else kind):
+            self.refuse(f"{name} is of {a.dtype}")
+        if tuple(a.shape) != shape:
+            self.refuse(f"{name} is {tuple(a.shape)}, not {shape}")
+        width = shape[-1]
+        if self.own:
+            return a.ptr.value, width, (shape[-2] * width if len(shape) > 2 else 0)
+        if not a.is_cuda or a.device != self.first.device:
+            self.refuse(f"{name} is on {a.device}")
+        st = a.stride()
+        if st[-1] != 1 and width > 1:
+            self.refuse(f"{name}: elements of a row have to be next to each other")
+        ld = st[-2] if len(shape) > 1 and shape[-2] > 1 else width
+        if len(shape) > 1 and ld < width:
+            self.refuse(f"{name}: rows overlap")
+        group = 0
+        if len(shape) > 2:
+            group = st[-3] if shape[-3] > 1 else shape[-2] * ld
+            if group < (shape[-2] - 1) * ld + width:
+                self.refuse(f"{name}: matrices overlap")
+        return a.data_ptr(), ld, group
+
+    def dense(self, name, a, shape, kind=None):
+        p, ld, group = self.array(name, a, shape, kind)
+        if len(shape) > 1 and p is not None and (ld != shape[-1] or (len(shape) > 2 and group != shape[-2] * shape[-1])):
+            self.refuse(f"{name} has to be dense")
+        return p
+
+    def stream(self, stream):
+        if stream is not None:
+            return stream
+        if self.own:
+            return lib.dnpeff_stream()
+        return sys.modules[type(self.first).__module__.split(".")[0]].cuda.current_stream(self.first.device).cuda_stream
+
+    def run(self, fn, args, bytes_needed, workspace, stream):
+        """fn(stream, *args, workspace, bytes), with a workspace of the call's own where none is given."""
+        st = self.stream(stream)
+        if workspace is not None:
+            p, _, _ = (workspace.ptr.value, 0, 0) if isinstance(workspace, DeviceArray) else (workspace.data_ptr(), 0, 0)
+            n = workspace.nbytes if isinstance(workspace, DeviceArray) else workspace.numel() * workspace.element_size()
+            return _check(fn(st, *args, p, n))
+        if bytes_needed == 0:
+            return _check(fn(st, *args, None, 0))
+        if not self.own:
+            if stream is not None:
+                self.refuse("a workspace has to be given with a stream")
+            torch = sys.modules[type(self.first).__module__.split(".")[0]]
+            w = torch.empty(bytes_needed, dtype=torch.uint8, device=self.first.device)
+            return _check(fn(st, *args, w.data_ptr(), bytes_needed))
+        if stream is not None and stream != lib.dnpeff_stream():
+            self.refuse("a workspace has to be given with a stream")
+        w = C.c_void_p()
+        _check(lib.dnpeff_scratch_malloc(bytes_needed, C.byref(w)))
+        try:
+            _check(fn(st, *args, w, bytes_needed))
+        finally:
+            lib.dnpeff_scratch_free(w)
+
+
+_BYTES = {}  # sizes of workspaces asked for so far
+
+
+def _bytes(fn, *sizes):
+    """(forward, backward) bytes of a workspace."""
+    got = _BYTES.get((fn, sizes))
+    if got is None:
+        f, b = _i64(0), _i64(0)
+        _check(getattr(lib, fn)(*sizes, C.byref(f), C.byref(b)))
+        if len(_BYTES) > 4096:
+            _BYTES.clear()
+        got = _BYTES[fn, sizes] = f.value, b.value
+    return got
+
+
+def linear_workspace(rows, n_in, n_out, dtype="float32", n_groups=0):
+    """(forward, backward) bytes of workspace that op_linear and op_linear_backward take."""
+    return _bytes("dnpeff_linear_workspace", _KINDS[str(dtype)], rows, n_in, n_out, n_groups)
+
+
+def vocab_loss_workspace(rows, n_in, n_words, dtype="float32"):
+    """The same of op_vocab_loss and op_vocab_loss_backward."""
+    return _bytes("dnpeff_vocab_loss_workspace", _KINDS[str(dtype)], rows, n_in, n_words)
+
+
+def _layer(c, X_rows, W, groups):
+    """rows, n_in, n_out, leading shape of weights, number of groups, their ends' address."""
+    if groups is None:
+        if len(W.shape) != 2:
+            c.refuse(f"W is {tuple(W.shape)}: one weight is a matrix")
+        return W.shape[1], W.shape[0], (), 0, None
+    if len(W.shape) != 3:
+        c.refuse(f"W is {tuple(W.shape)}: the weights of groups have three dimensions")
+    n = W.shape[0]
+    return W.shape[2], W.shape[1], (n,), n, c.dense("groups", groups, (n + 1,), "i8")
+
+
+def op_linear(X, W, Y, bias=None, act="none", residual=None, pre=None, groups=None, workspace=None, stream=None):
+    """Y = act(X W^T + bias) + residual; pre receives X W^T + bias.  groups: the ends of the rows of each of
+    W's matrices (include/dnpeff.h, dnpeff_linear)."""
+    c = _Call("op_linear", X)
+    if act not in ACTS:
+        c.refuse(f"unknown activation {act!r}")
+    if len(X.shape) != 2:
+        c.refuse(f"X is {tuple(X.shape)}")
+    rows = X.shape[0]
+    n_in, n_out, lead, n, ends = _layer(c, rows, W, groups)
+    x, ldx, _ = c.array("X", X, (rows, n_in))
+    w, ldw, w_group = c.array("W", W, lead + (n_out, n_in))
+    y, ldy, _ = c.array("Y", Y, (rows, n_out))
+    b = c.dense("bias", bias, lead + (n_out,))
+    r, ldr, _ = c.array("residual", residual, (rows, n_out))
+    p, ldp, _ = c.array("pre", pre, (rows, n_out))
+    need = 0 if workspace is not None else _bytes("dnpeff_linear_workspace", c.type, rows, n_in, n_out, n)[0]
+    c.run(lib.dnpeff_linear, (c.type, rows, n_in, n_out, x, ldx, w, ldw, w_group, b, ACTS[act], r, ldr, y, ldy, p, ldp, n,
+                              ends), need, workspace, stream)
+
+
+def op_linear_backward(dY, X, W, pre=None, act="none", dX=None, dW=None, dbias=None, groups=None, workspace=None,
+                       stream=None):
+    """The gradients of op_linear for dY, into those of dX, dW and dbias that are given (dnpeff_linear_backward)."""
+    c = _Call("op_linear_backward", dY)
+    if act not in ACTS:
+        c.refuse(f"unknown activation {act!r}")
+    if len(dY.shape) != 2:
+        c.refuse(f"dY is {tuple(dY.shape)}")
+    rows = dY.shape[0]
+    n_in, n_out, lead, n, ends = _layer(c, rows, W, groups)
+    g, lddy, _ = c.array("dY", dY, (rows, n_out))
+    x, ldx, _ = c.array("X", X, (rows, n_in))
+    w, ldw, w_group = c.array("W", W, lead + (n_out, n_in))
+    p, ldp, _ = c.array("pre", pre, (rows, n_out))
+    gx, lddx, _ = c.array("dX", dX, (rows, n_in))
+    gw, lddw, dw_group = c.array("dW", dW, lead + (n_out, n_in))
+    b = c.dense("dbias", dbias, lead + (n_out,))
+    need = 0 if workspace is not None else _bytes("dnpeff_linear_workspace", c.type, rows, n_in, n_out, n)[1]
+    c.run(lib.dnpeff_linear_backward, (c.type, rows, n_in, n_out, g, lddy, x, ldx, w, ldw, w_group, p, ldp, ACTS[act], gx,
+                                       lddx, gw, lddw, dw_group, b, n, ends), need, workspace, stream)
+
+
+def op_example_grads(dY, X, examples, out, square=False, stream=None):
+    """out[e] = dY_e^T X_e (float32 [examples, n_out, n_in]), squared where asked for: with dY the gradient of the log
+    likelihood, rows of the diagonal Fisher.  examples: the ends of their rows (dnpeff_example_grads)."""
+    c = _Call("op_example_grads", dY)
+    if len(dY.shape) != 2 or len(X.shape) != 2:
+        c.refuse(f"dY is {tuple(dY.shape)}, X {tuple(X.shape)}")
+    rows, n_out = dY.shape
+    n_in, n = X.shape[1], examples.shape[0] - 1
+    g, lddy, _ = c.array("dY", dY, (rows, n_out))
+    x, ldx, _ = c.array("X", X, (rows, n_in))
+    ends = c.dense("examples", examples, (n + 1,), "i8")
+    o = c.dense("out", out, (n, n_out, n_in), F32)
+    _check(lib.dnpeff_example_grads(c.stream(stream), c.type, rows, n_in, n_out, g, lddy, x, ldx, n, ends, o, 1 if square else 0))
+
+
+def op_vocab_loss(X, E, labels, loss=None, lse=None, workspace=None, stream=None):
+    """Token losses lse - x . e_label and lse = log sum exp over the vocabulary E (dnpeff_vocab_loss)."""
+    c = _Call("op_vocab_loss", X)
+    if len(X.shape) != 2 or len(E.shape) != 2:
+        c.refuse(f"X is {tuple(X.shape)}, E {tuple(E.shape)}")
+    (rows, n_in), words = X.shape, E.shape[0]
+    x, ldx, _ = c.array("X", X, (rows, n_in))
+    e, lde, _ = c.array("E", E, (words, n_in))
+    need = 0 if workspace is not None else _bytes("dnpeff_vocab_loss_workspace", c.type, rows, n_in, words)[0]
+    c.run(lib.dnpeff_vocab_loss, (c.type, rows, n_in, words, x, ldx, e, lde, c.dense("labels", labels, (rows,), "i4"),
+                                  c.dense("loss", loss, (rows,), F32), c.dense("lse", lse, (rows,), F32)),
+          need, workspace, stream)
+
+
+def op_vocab_loss_backward(X, E, labels, lse, dloss, dX=None, dE=None, workspace=None, stream=None):
+    """The gradients of op_vocab_loss for dloss, into those of dX and dE that are given (dnpeff_vocab_loss_backward)."""
+    c = _Call("op_vocab_loss_backward", X)
+    if len(X.shape) != 2 or len(E.shape) != 2:
+        c.refuse(f"X is {tuple(X.shape)}, E {tuple(E.shape)}")
+    (rows, n_in), words = X.shape, E.shape[0]
+    x, ldx, _ = c.array("X", X, (rows, n_in))
+    e, lde, _ = c.array("E", E, (words, n_in))
+    gx, lddx, _ = c.array("dX", dX, (rows, n_in))
+    ge, ldde, _ = c.array("dE", dE, (words, n_in))
+    need = 0 if workspace is not None else _bytes("dnpeff_vocab_loss_workspace", c.type, rows, n_in, words)[1]
+    c.run(lib.dnpeff_vocab_loss_backward,
+          (c.type, rows, n_in, words, x, ldx, e, lde, c.dense("labels", labels, (rows,), "i4"),
+           c.dense("lse", lse, (rows,), F32), c.dense("dloss", dloss, (rows,), F32), gx, lddx, ge, ldde),
+          need, workspace, stream)
 
 
 class Csr:

@@ -1,0 +1,269 @@
+// Products of a layer with their epilogues, one weight for all rows or one per group of rows, their backward pass, and
+// weight gradients per example: the dense Fisher rows that dnpeff_topk_rows takes.
+//
+//   Z = X W^T + b,  Y = act(Z) + R
+//   dZ = dY act'(Z),  dX = dZ W,  dW = dZ^T X,  db = column sums of dZ          (per group: rows and W of the group)
+//   out[e] = dY_e^T X_e, squared where asked for                                 (e: the rows of an example)
+#include "tiles.hpp"
+
+using namespace dn;
+using namespace dn::tl;
+
+namespace dn {
+namespace tl {
+DN_STORE_PRODUCTS(, float)
+DN_STORE_PRODUCTS(, _Float16)
+DN_STORE_PRODUCTS(, __bf16)
+}  // namespace tl
+}  // namespace dn
+
+namespace {
+
+constexpr int DZ_ROWS = 128;  // rows of a group that one workgroup of k_slopes takes
+constexpr int DZ_COLS = 256;  // (a lane: four columns; a wave: every fourth row)
+
+// dZ = dY act'(Z), and the column sums of each tile of rows.
+template <class T>
+__global__ __launch_bounds__(256) void k_slopes(group_rows G, int64_t N, const T* dY, int64_t ldy, const T* Z, int64_t ldz, int act, T* dZ,
+                                                int64_t ldd, float* sums, int wide) {
+  constexpr bool EXACT = sizeof(T) == 4;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int group, within;
+  group_of_tile(G, DZ_ROWS, lane, blockIdx.x, &group, &within);
+  if (group < 0) return;
+  const int64_t m0 = G.first(group) + (int64_t)within * DZ_ROWS, m_end = G.last(group);
+  const bool held = group < G.groups;
+  const int64_t n = (int64_t)blockIdx.y * DZ_COLS + lane * 4;
+  const int there = n < N ? (int)(N - n < 4 ? N - n : 4) : 0;
+  const bool whole = wide && there == 4;
+  v4f sum = {0.f, 0.f, 0.f, 0.f};
+  if (there > 0 || (dZ && n < ldd)) {  // (columns of dZ past the last of dY: zero)
+#pragma unroll 4
+    for (int r = wave; r < DZ_ROWS; r += 4) {
+      const int64_t m = m0 + r;
+      if (m >= m_end) break;
+      v4f g = {0.f, 0.f, 0.f, 0.f};
+      if (held) {
+        g = load4(dY + m * ldy + n, whole, there);
+        if (act != DNPEFF_ACT_NONE) {
+          const v4f z = load4(Z + m * ldz + n, whole, there);
+#pragma unroll
+          for (int t = 0; t < 4; t++) g[t] *= slope_of<EXACT>(z[t], act);
+        }
+      }
+      if (dZ) store4(dZ + m * ldd + n, g, true, 4);
+      sum += g;
+    }
+  }
+  if (!sums) return;
+  __shared__ v4f side[4][64];
+  side[wave][lane] = sum;
+  __syncthreads();
+  if (wave == 0 && there > 0) {
+    const v4f s = (side[0][lane] + side[1][lane]) + (side[2][lane] + side[3][lane]);
+    store4(sums + blockIdx.x * N + n, s, N % 4 == 0, there);
+  }
+}
+
+// db[g] = the sums of the group's tiles, in their order.
+template <class T>
+__global__ __launch_bounds__(256) void k_bias_sums(group_rows G, int64_t N, const float* sums, int tiles_most, T* db) {
+  const int lane = threadIdx.x & 63, g = blockIdx.y;
+  int before = 0;
+  for (int b = 0; b < g; b += 64) {
+    const int t = b + lane < g ? (int)((G.count(b + lane) + DZ_ROWS - 1) / DZ_ROWS) : 0;
+    before += __shfl(wave_scan(t, lane), 63, 64);
+  }
+  int tiles = (int)((G.count(g) + DZ_ROWS - 1) / DZ_ROWS);
+  if (tiles > tiles_most - before) tiles = tiles_most - before;  // (groups that overlap: no more than there were)
+  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (n >= N) return;
+  float s = 0.f;
+  for (int t = 0; t < tiles; t++) s += sums[(int64_t)(before + t) * N + n];
+  db[g * N + n] = (T)s;
+}
+
+int64_t slope_tiles(int64_t rows, int groups) { return rows / DZ_ROWS + (groups + 1 < rows ? groups + 1 : rows); }
+
+struct layer {
+  int64_t rows, n_in, n_out;
+  int groups;
+  const int64_t* ends;
+  bool grouped() const { return ends != nullptr; }
+};
+
+int check_layer(const char* what, int type, const layer& l) {
+  DN_CHECK(type == DNPEFF_F32 || type == DNPEFF_F16 || type == DNPEFF_BF16, "%s: unknown type %d", what, type);
+  DN_CHECK(l.rows >= 0 && l.n_in >= 1 && l.n_out >= 1, "%s: rows = %lld, n_in = %lld, n_out = %lld", what, (long long)l.rows,
+           (long long)l.n_in, (long long)l.n_out);
+  DN_CHECK(l.rows < ((int64_t)1 << 31) && l.n_in < ((int64_t)1 << 31) && l.n_out < ((int64_t)1 << 31), "%s: sizes of 2^31 and more",
+           what);
+  DN_CHECK((l.ends == nullptr) == (l.groups == 0) && l.groups >= 0 && l.groups <= 65535, "%s: %d groups, their ends %s (65535 at most)",
+           what, l.groups, l.ends ? "given" : "not given");
+  return 0;
+}
+int check_act(const char* what, int act) {
+  DN_CHECK(act >= DNPEFF_ACT_NONE && act <= DNPEFF_ACT_SILU, "%s: unknown activation %d", what, act);
+  return 0;
+}
+group_rows rows_of(const layer& l) { return group_rows{l.ends, l.grouped() ? l.groups : 1, l.rows}; }
+
+template <class T>
+int64_t forward_ws(const layer& l) {
+  return l.grouped() ? 0 : round256(4 * split_floats<T>(l.rows, l.n_out, l.n_in));
+}
+template <class T>
+struct backward_ws {
+  int64_t dz, sums, parts, all;
+  backward_ws(const layer& l) {
+    dz = round256(l.rows * ((l.n_out + 7) / 8 * 8) * (int64_t)sizeof(T));
+    sums = round256(slope_tiles(l.rows, l.grouped() ? l.groups : 1) * l.n_out * 4);
+    const int64_t x = l.grouped() ? 0 : split_floats<T>(l.rows, l.n_in, l.n_out), w = l.grouped() ? 0 : split_floats<T>(l.n_out, l.n_in, l.rows);
+    parts = round256(4 * (x > w ? x : w));
+    all = dz + sums + parts;
+  }
+};
+
+template <class T>
+int forward(hipStream_t st, const layer& l, const void* X, int64_t ldx, const void* W, int64_t ldw, int64_t w_group, const void* bias, int act,
+            const void* residual, int64_t ldr, void* Y, int64_t ldy, void* pre, int64_t ldp, void* ws) {
+  args p{};
+  p.A = X, p.lda = ldx, p.B = W, p.ldb = ldw, p.b_group = w_group;
+  p.M = l.rows, p.N = l.n_out, p.K = l.n_in;
+  p.mode = l.grouped() ? BY_ROWS : ONE;
+  p.G = rows_of(l);
+  p.out = Y, p.ldc = ldy, p.pre = pre, p.ldp = ldp, p.residual = residual, p.ldr = ldr, p.bias = bias, p.act = act;
+  p.wide = fours<T>(Y, ldy) && fours<T>(pre, ldp) && fours<T>(residual, ldr) && fours<T>(bias, l.n_out);
+  return launch_product<T, true, true, E_LINEAR>(p, false, false, (float*)ws, st);
+}
+
+template <class T>
+int backward(hipStream_t st, const layer& l, const void* dY, int64_t lddy, const void* X, int64_t ldx, const void* W, int64_t ldw,
+             int64_t w_group, const void* pre, int64_t ldp, int act, void* dX, int64_t lddx, void* dW, int64_t lddw, int64_t dw_group,
+             void* dbias, char* ws) {
+  const backward_ws<T> room(l);
+  const group_rows G = rows_of(l);
+  const void* dz = dY;
+  int64_t ldz = lddy;
+  float* sums = dbias ? (float*)(ws + room.dz) : nullptr;
+  float* parts = room.parts > 0 ? (float*)(ws + room.dz + room.sums) : nullptr;
+  const bool slopes = act != DNPEFF_ACT_NONE && (dX || dW);
+  if (slopes) {  // (rows of whole 16 bytes, whatever those of dY are)
+    dz = ws;
+    ldz = (l.n_out + 7) / 8 * 8;
+  }
+  if ((slopes || dbias) && l.rows > 0) {
+    const bool wide = fours<T>(dY, lddy) && (act == DNPEFF_ACT_NONE || fours<T>(pre, ldp));
+    const dim3 grid((unsigned)slope_tiles(l.rows, G.groups), (unsigned)ceil_div(l.n_out, DZ_COLS));
+    DN_CHECK(grid.y <= 65535, "dnpeff_linear_backward: n_out = %lld is too wide for one launch", (long long)l.n_out);
+    k_slopes<T><<<grid, 256, 0, st>>>(G, l.n_out, (const T*)dY, lddy, (const T*)pre, ldp, act, slopes ? (T*)ws : nullptr, ldz, sums, wide);
+    DN_LAUNCH_CHECK();
+  }
+  if (dbias) {
+    k_bias_sums<T><<<dim3((unsigned)ceil_div(l.n_out, 256), (unsigned)G.groups), 256, 0, st>>>(G, l.n_out, sums, (int)slope_tiles(l.rows, G.groups), (T*)dbias);
+    DN_LAUNCH_CHECK();
+  }
+  if (dX) {
+    args p{};
+    p.A = dz, p.lda = ldz, p.B = W, p.ldb = ldw, p.b_group = w_group;
+    p.M = l.rows, p.N = l.n_in, p.K = l.n_out;
+    p.mode = l.grouped() ? BY_ROWS : ONE;
+    p.G = G;
+    p.out = dX, p.ldo = lddx, p.wide = fours<T>(dX, lddx);
+    DN_TRY((launch_product<T, true, false, E_STORE>(p, slopes, false, parts, st)));
+  }
+  if (dW) {
+    args p{};
+    p.A = dz, p.lda = ldz, p.B = X, p.ldb = ldx;
+    p.M = l.n_out, p.N = l.n_in, p.K = l.rows;
+    p.mode = l.grouped() ? BY_REDUCTION : ONE;
+    p.G = G;
+    p.out = dW, p.ldo = lddw, p.c_group = dw_group, p.wide = fours<T>(dW, lddw) && dw_group % 4 == 0;
+    DN_TRY((launch_product<T, false, false, E_STORE>(p, slopes, false, parts, st)));
+  }
+  return 0;
+}
+
+template <class T>
+int example_grads(hipStream_t st, const layer& l, const void* dY, int64_t lddy, const void* X, int64_t ldx, float* out, int square) {
+  args p{};
+  p.A = dY, p.lda = lddy, p.B = X, p.ldb = ldx;
+  p.M = l.n_out, p.N = l.n_in, p.K = l.rows;
+  p.mode = BY_REDUCTION;
+  p.G = rows_of(l);
+  p.out = out, p.out_f32 = 1, p.square = square, p.ldo = l.n_in, p.c_group = l.n_out * l.n_in;
+  p.wide = fours<float>(out, l.n_in);
+  return launch_product<T, false, false, E_STORE>(p, false, false, nullptr, st);
+}
+
+}  // namespace
+
+DN_API int dnpeff_linear_workspace(int type, int64_t rows, int64_t n_in, int64_t n_out, int n_groups, int64_t* forward_bytes,
+                                   int64_t* backward_bytes) {
+  clear_error();
+  static const int64_t some = 0;
+  const layer l{rows, n_in, n_out, n_groups, n_groups > 0 ? &some : nullptr};
+  DN_TRY(check_layer("dnpeff_linear_workspace", type, l));
+  if (forward_bytes) *forward_bytes = DN_BY_TYPE(type, forward_ws<T>(l));
+  if (backward_bytes) *backward_bytes = DN_BY_TYPE(type, backward_ws<T>(l).all);
+  return 0;
+}
+
+DN_API int dnpeff_linear(void* stream, int type, int64_t rows, int64_t n_in, int64_t n_out, const void* X, int64_t ldx, const void* W,
+                         int64_t ldw, int64_t w_group, const void* bias, int act, const void* residual, int64_t ldr, void* Y, int64_t ldy,
+                         void* pre, int64_t ldp, int n_groups, const int64_t* ends, void* workspace, int64_t workspace_bytes) {
+  clear_error();
+  const char* me = "dnpeff_linear";
+  const layer l{rows, n_in, n_out, n_groups, ends};
+  DN_TRY(check_layer(me, type, l));
+  DN_TRY(check_act(me, act));
+  if (rows == 0) return 0;
+  DN_TRY(check_array(me, "X", X, ldx, n_in, type, false));
+  DN_TRY(check_array(me, "W", W, ldw, n_in, type, false));
+  DN_TRY(check_array(me, "Y", Y, ldy, n_out, type, false));
+  DN_TRY(check_array(me, "bias", bias, n_out, n_out, type, true));
+  DN_TRY(check_array(me, "residual", residual, ldr, n_out, type, true));
+  DN_TRY(check_array(me, "pre", pre, ldp, n_out, type, true));
+  const int64_t need = DN_BY_TYPE(type, forward_ws<T>(l));
+  DN_CHECK(need == 0 || (workspace != nullptr && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0),
+           "%s: a workspace of %lld bytes, aligned to 16, is needed", me, (long long)need);
+  return DN_BY_TYPE(type, forward<T>((hipStream_t)stream, l, X, ldx, W, ldw, w_group, bias, act, residual, ldr, Y, ldy, pre, ldp,
+                                     need ? workspace : nullptr));
+}
+
+DN_API int dnpeff_linear_backward(void* stream, int type, int64_t rows, int64_t n_in, int64_t n_out, const void* dY, int64_t lddy,
+                                  const void* X, int64_t ldx, const void* W, int64_t ldw, int64_t w_group, const void* pre, int64_t ldp,
+                                  int act, void* dX, int64_t lddx, void* dW, int64_t lddw, int64_t dw_group, void* dbias, int n_groups,
+                                  const int64_t* ends, void* workspace, int64_t workspace_bytes) {
+  clear_error();
+  const char* me = "dnpeff_linear_backward";
+  const layer l{rows, n_in, n_out, n_groups, ends};
+  DN_TRY(check_layer(me, type, l));
+  DN_TRY(check_act(me, act));
+  DN_TRY(check_array(me, "dY", dY, lddy, n_out, type, rows == 0));
+  DN_TRY(check_array(me, "X", X, ldx, n_in, type, rows == 0 || !dW));
+  DN_TRY(check_array(me, "W", W, ldw, n_in, type, !dX));
+  DN_TRY(check_array(me, "pre", pre, ldp, n_out, type, rows == 0 || act == DNPEFF_ACT_NONE));
+  DN_TRY(check_array(me, "dX", dX, lddx, n_in, type, true));
+  DN_TRY(check_array(me, "dW", dW, lddw, n_in, type, true));
+  DN_TRY(check_array(me, "dbias", dbias, n_out, n_out, type, true));
+  const int64_t need = DN_BY_TYPE(type, backward_ws<T>(l).all);
+  DN_CHECK(need == 0 || (workspace != nullptr && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0),
+           "%s: a workspace of %lld bytes, aligned to 16, is needed", me, (long long)need);
+  return DN_BY_TYPE(type, backward<T>((hipStream_t)stream, l, dY, lddy, X, ldx, W, ldw, w_group, pre, ldp, act, dX, lddx, dW, lddw,
+                                      dw_group, dbias, (char*)workspace));
+}
+
+DN_API int dnpeff_example_grads(void* stream, int type, int64_t rows, int64_t n_in, int64_t n_out, const void* dY, int64_t lddy,
+                                const void* X, int64_t ldx, int n_examples, const int64_t* ends, float* out, int square) {
+  clear_error();
+  const char* me = "dnpeff_example_grads";
+  const layer l{rows, n_in, n_out, n_examples, ends};
+  DN_CHECK(n_examples >= 0, "%s: %d examples", me, n_examples);
+  if (n_examples == 0) return 0;
+  DN_TRY(check_layer(me, type, l));
+  DN_TRY(check_array(me, "dY", dY, lddy, n_out, type, rows == 0));
+  DN_TRY(check_array(me, "X", X, ldx, n_in, type, rows == 0));
+  DN_TRY(check_array(me, "out", out, n_in, n_in, DNPEFF_F32, false));
+  return DN_BY_TYPE(type, example_grads<T>((hipStream_t)stream, l, dY, lddy, X, ldx, out, square));
+}

@@ -1,0 +1,224 @@
+// Softmax cross entropy of hidden states over a vocabulary, without keeping the logits, and its gradients.
+//
+//   z[t, v] = x_t . e_v,  lse_t = log sum_v exp z[t, v],  loss_t = lse_t - z[t, label_t]
+//   g[t, v] = (exp(z[t, v] - lse_t) - [v = label_t]) dloss_t,  dX = g E,  dE = g^T X
+//
+// Forward: every tile of logits leaves the maximum and the sum of exponentials of its words, eight bytes per token and
+// tile; a second kernel joins them.  Backward: the vocabulary goes by in pieces; the logits of a piece are formed again,
+// turned into g where they are summed, and multiplied on both sides.  g is rounded to the operands' type, once: its
+// products run on the matrix cores of that type, and the rounding (2^-9 of a value in bf16) is that of the results.
+#include "tiles.hpp"
+
+#include <type_traits>
+
+using namespace dn;
+using namespace dn::tl;
+
+namespace dn {
+namespace tl {
+DN_STORE_PRODUCTS(extern, float)
+DN_STORE_PRODUCTS(extern, _Float16)
+DN_STORE_PRODUCTS(extern, __bf16)
+}  // namespace tl
+}  // namespace dn
+
+namespace {
+
+// One wave per token.
+__global__ __launch_bounds__(256) void k_join_loss(int64_t rows, int parts_n, const float2* parts, const float* hit, const int32_t* labels,
+                                                   int64_t words, float* loss, float* lse) {
+  const int64_t m = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
+  const int lane = threadIdx.x & 63;
+  if (m >= rows) return;
+  float top = -INFINITY;
+  for (int i = lane; i < parts_n; i += 64) top = fmaxf(top, parts[m * parts_n + i].x);
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
+  const float from = top == -INFINITY ? 0.f : top;
+  float sum = 0.f;
+  for (int i = lane; i < parts_n; i += 64) {
+    const float2 s = parts[m * parts_n + i];
+    if (s.x != -INFINITY || s.y != 0.f) sum += s.y * expf(s.x - from);
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d, 64);
+  if (lane == 0) {
+    const float l = logf(sum) + from;
+    const int32_t label = labels[m];
+    if (lse) lse[m] = l;
+    if (loss) loss[m] = label < 0 ? 0.f : label >= words ? __builtin_nanf("") : l - hit[m];
+  }
+}
+
+// 16-bit types: both[0] brings the largest |dloss| of a labelled token to 1 (fp16: to 2^14, so that g stays below the
+// type's largest value and probabilities down to 4e-9 above its subnormal ones), both[1] takes the results back.  With
+// equal weights, as of a mean, a label's g is then -1 but for p, and its rounding not the same for every token: left as
+// they come, weights of 1 / 2000 put gradients off by up to 2^-11 (fp16) or 2^-8 as a whole.
+template <class T>
+__global__ __launch_bounds__(1024) void k_shrink(int64_t rows, const int32_t* labels, const float* dloss, float* both) {
+  __shared__ float side[16];
+  float most = 0.f;
+  for (int64_t i = threadIdx.x; i < rows; i += 1024) {
+    const float a = fabsf(dloss[i]);
+    if (labels[i] >= 0 && a < INFINITY) most = fmaxf(most, a);
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) most = fmaxf(most, __shfl_xor(most, d, 64));
+  if (threadIdx.x % 64 == 0) side[threadIdx.x / 64] = most;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 16; i++) most = fmaxf(most, side[i]);
+    const float top = std::is_same<T, _Float16>::value ? 16384.f : 1.f;
+    most = most > 0.f ? fmaxf(most, 1e-36f) : 1.f;
+    both[0] = top / most;
+    both[1] = most / top;
+  }
+}
+
+constexpr int64_t PIECE_BYTES = (int64_t)512 << 20;  // of g at a time
+// Words per piece: even pieces, whole tiles.
+int64_t piece_words(int64_t rows, int64_t words, int size) {
+  int64_t most = PIECE_BYTES / (size * (rows > 0 ? rows : 1)) / 256 * 256;
+  if (most < 1024) most = 1024;
+  if (most >= words) return words;
+  return ceil_div(ceil_div(words, ceil_div(words, most)), 256) * 256;
+}
+int64_t padded(int64_t words) { return ceil_div(words, 64) * 64; }
+
+template <class T>
+struct room {
+  int64_t piece, g, sums, parts, all;
+  room(int64_t rows, int64_t n_in, int64_t words) {
+    piece = piece_words(rows, words, sizeof(T));
+    g = round256(rows * padded(piece) * (int64_t)sizeof(T));
+    sums = piece < words ? round256(rows * (ceil_div(n_in, 4) * 4) * 4) : 0;
+    const int64_t x = split_floats<T>(rows, n_in, piece), e = split_floats<T>(piece, n_in, rows);
+    const int64_t last = words - (ceil_div(words, piece) - 1) * piece;
+    const int64_t x1 = split_floats<T>(rows, n_in, last), e1 = split_floats<T>(last, n_in, rows);
+    int64_t most = x > e ? x : e;
+    if (x1 > most) most = x1;
+    if (e1 > most) most = e1;
+    parts = round256(4 * most);
+    all = 256 + g + sums + parts;
+  }
+};
+int64_t forward_bytes_of(int64_t rows, int64_t words) { return round256(rows * ceil_div(words, 128) * 8) + round256(rows * 4); }
+
+template <class T>
+int loss_forward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, const void* X, int64_t ldx, const void* E, int64_t lde,
+                 const int32_t* labels, float* loss, float* lse, char* ws) {
+  args p{};
+  p.A = X, p.lda = ldx, p.B = E, p.ldb = lde;
+  p.M = rows, p.N = words, p.K = n_in;
+  p.mode = ONE;
+  p.labels = labels, p.words = words, p.word0 = 0;
+  p.parts = (float2*)ws;
+  p.hit = (float*)(ws + round256(rows * ceil_div(words, 128) * 8));
+  int tile = 0;
+  DN_TRY((launch_product<T, true, true, E_LOSS>(p, false, false, nullptr, st, &tile)));
+  k_join_loss<<<(unsigned)ceil_div(rows, 4), 256, 0, st>>>(rows, (int)ceil_div(words, tile), p.parts, p.hit, labels, words, loss, lse);
+  DN_LAUNCH_CHECK();
+  return 0;
+}
+
+template <class T>
+int loss_backward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, const void* X, int64_t ldx, const void* E, int64_t lde,
+                  const int32_t* labels, const float* lse, const float* dloss, void* dX, int64_t lddx, void* dE, int64_t ldde, char* ws) {
+  const room<T> r(rows, n_in, words);
+  float* both = (float*)ws;
+  char* g = ws + 256;
+  float* sums = (float*)(g + r.g);
+  float* parts = r.parts ? (float*)(g + r.g + r.sums) : nullptr;
+  const float *shrink = nullptr, *grow = nullptr;
+  if constexpr (sizeof(T) == 2) {
+    k_shrink<T><<<1, 1024, 0, st>>>(rows, labels, dloss, both);
+    DN_LAUNCH_CHECK();
+    shrink = both, grow = both + 1;
+  }
+  for (int64_t w0 = 0; w0 < words; w0 += r.piece) {
+    const int64_t n = words - w0 < r.piece ? words - w0 : r.piece;
+    const T* Ep = (const T*)E + w0 * lde;
+    const bool first = w0 == 0, last = w0 + n == words;
+    args p{};
+    p.A = X, p.lda = ldx, p.B = Ep, p.ldb = lde;
+    p.M = rows, p.N = n, p.K = n_in;
+    p.mode = ONE;
+    p.labels = labels, p.lse = lse, p.dloss = dloss, p.shrink = shrink, p.word0 = w0, p.words = words;
+    p.out = g, p.ldc = padded(n);
+    DN_TRY((launch_product<T, true, true, E_LOSS_GRAD>(p, false, false, nullptr, st)));
+    if (dX) {
+      args q{};
+      q.A = g, q.lda = padded(n), q.B = Ep, q.ldb = lde;
+      q.M = rows, q.N = n_in, q.K = n;
+      q.mode = ONE;
+      q.sums = first && last ? nullptr : sums, q.add_sums = !first;
+      q.ldc = ceil_div(n_in, 4) * 4;
+      if (last) q.out = dX, q.ldo = lddx, q.wide = fours<T>(dX, lddx), q.scale = grow;
+      DN_TRY((launch_product<T, true, false, E_STORE>(q, true, false, parts, st)));
+    }
+    if (dE) {
+      args q{};
+      q.A = g, q.lda = padded(n), q.B = X, q.ldb = ldx;
+      q.M = n, q.N = n_in, q.K = rows;
+      q.mode = ONE;
+      T* to = (T*)dE + w0 * ldde;
+      q.out = to, q.ldo = ldde, q.wide = fours<T>(to, ldde), q.scale = grow;
+      DN_TRY((launch_product<T, false, false, E_STORE>(q, true, false, parts, st)));
+    }
+  }
+  return 0;
+}
+
+int check_head(const char* me, int type, int64_t rows, int64_t n_in, int64_t words) {
+  DN_CHECK(type == DNPEFF_F32 || type == DNPEFF_F16 || type == DNPEFF_BF16, "%s: unknown type %d", me, type);
+  DN_CHECK(rows >= 0 && n_in >= 1 && words >= 1 && rows < ((int64_t)1 << 31) && n_in < ((int64_t)1 << 31) && words < ((int64_t)1 << 31),
+           "%s: rows = %lld, n_in = %lld, n_words = %lld", me, (long long)rows, (long long)n_in, (long long)words);
+  return 0;
+}
+
+}  // namespace
+
+DN_API int dnpeff_vocab_loss_workspace(int type, int64_t rows, int64_t n_in, int64_t n_words, int64_t* forward_bytes, int64_t* backward_bytes) {
+  clear_error();
+  DN_TRY(check_head("dnpeff_vocab_loss_workspace", type, rows, n_in, n_words));
+  if (forward_bytes) *forward_bytes = forward_bytes_of(rows, n_words);
+  if (backward_bytes) *backward_bytes = DN_BY_TYPE(type, (room<T>(rows, n_in, n_words).all));
+  return 0;
+}
+
+DN_API int dnpeff_vocab_loss(void* stream, int type, int64_t rows, int64_t n_in, int64_t n_words, const void* X, int64_t ldx, const void* E,
+                             int64_t lde, const int32_t* labels, float* loss, float* lse, void* workspace, int64_t workspace_bytes) {
+  clear_error();
+  const char* me = "dnpeff_vocab_loss";
+  DN_TRY(check_head(me, type, rows, n_in, n_words));
+  if (rows == 0) return 0;
+  DN_TRY(check_array(me, "X", X, ldx, n_in, type, false));
+  DN_TRY(check_array(me, "E", E, lde, n_in, type, false));
+  DN_TRY(check_array(me, "labels", labels, 1, 1, DNPEFF_F32, false));
+  DN_TRY(check_array(me, "loss", loss, 1, 1, DNPEFF_F32, true));
+  DN_TRY(check_array(me, "lse", lse, 1, 1, DNPEFF_F32, true));
+  const int64_t need = forward_bytes_of(rows, n_words);
+  DN_CHECK(workspace != nullptr && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0,
+           "%s: a workspace of %lld bytes, aligned to 16, is needed", me, (long long)need);
+  return DN_BY_TYPE(type, loss_forward<T>((hipStream_t)stream, rows, n_in, n_words, X, ldx, E, lde, labels, loss, lse, (char*)workspace));
+}
+
+DN_API int dnpeff_vocab_loss_backward(void* stream, int type, int64_t rows, int64_t n_in, int64_t n_words, const void* X, int64_t ldx,
+                                      const void* E, int64_t lde, const int32_t* labels, const float* lse, const float* dloss, void* dX,
+                                      int64_t lddx, void* dE, int64_t ldde, void* workspace, int64_t workspace_bytes) {
+  clear_error();
+  const char* me = "dnpeff_vocab_loss_backward";
+  DN_TRY(check_head(me, type, rows, n_in, n_words));
+  DN_TRY(check_array(me, "X", X, ldx, n_in, type, rows == 0));
+  DN_TRY(check_array(me, "E", E, lde, n_in, type, rows == 0));
+  DN_TRY(check_array(me, "labels", labels, 1, 1, DNPEFF_F32, rows == 0));
+  DN_TRY(check_array(me, "lse", lse, 1, 1, DNPEFF_F32, rows == 0));
+  DN_TRY(check_array(me, "dloss", dloss, 1, 1, DNPEFF_F32, rows == 0));
+  DN_TRY(check_array(me, "dX", dX, lddx, n_in, type, true));
+  DN_TRY(check_array(me, "dE", dE, ldde, n_in, type, true));
+  const int64_t need = DN_BY_TYPE(type, (room<T>(rows, n_in, n_words).all));
+  DN_CHECK(workspace != nullptr && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0,
+           "%s: a workspace of %lld bytes, aligned to 16, is needed", me, (long long)need);
+  return DN_BY_TYPE(type, loss_backward<T>((hipStream_t)stream, rows, n_in, n_words, X, ldx, E, lde, labels, lse, dloss, dX, lddx, dE,
+                                           ldde, (char*)workspace));
+}

@@ -1,0 +1,361 @@
+"""Products of a layer with their epilogues, by group and alone, their backward pass and the per-example gradients, against
+the formulas in 64 bits.
+
+A result is a sum of k products of exact operands in fp32, in some order, then a few fp32 operations and one rounding:
+off by at most (k + 40) 2^-24 times the sum of the products' sizes, carried through the epilogue (slopes of the activations
+are at most 1.13; the 40 covers the epilogue's own operations), and half a unit in the last place of the result.  dZ is rounded to
+the type before its products: another half unit of each term."""
+
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+import npeff_ref_amd as d
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+HALF = {k: torch.finfo(t).eps / 2 for k, t in DTYPES.items()}  # relative half unit in the last place
+TINY = {"f32": 0.0, "f16": 2.0**-25, "bf16": 0.0}  # absolute, where results are subnormal
+EPS32 = 2.0**-24
+ACTS = {
+    "none": lambda z: z,
+    "relu": torch.relu,
+    "silu": torch.nn.functional.silu,
+    "gelu": torch.nn.functional.gelu,
+    "gelu_tanh": lambda z: torch.nn.functional.gelu(z, approximate="tanh"),
+}
+
+
+def rand(shape, dt, seed, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale).to(DTYPES[dt]).cuda()
+
+
+def wide(t, extra, shift):
+    """The same values in rows that are `extra` elements further apart and begin `shift` elements late."""
+    shape = t.shape[:-1] + (t.shape[-1] + extra,)
+    big = torch.full((int(np.prod(shape)) + shift,), 7.0, dtype=t.dtype, device="cuda")
+    v = big[shift:].view(shape)[..., : t.shape[-1]]
+    v.copy_(t)
+    return v
+
+
+def ends_of(sizes):
+    return torch.tensor([0] + list(np.cumsum(sizes)), dtype=torch.int64).cuda()
+
+
+def close(got, want, sums, k, dt, more=0.0):
+    """sums: of the sizes of the products behind each result; more: a further error of each."""
+    got, want = got.double().cpu(), want.double().cpu()
+    bound = HALF[dt] * 1.01 * want.abs() + (k + 40) * EPS32 * 1.2 * sums.double().cpu() + more + TINY[dt]
+    off = (got - want).abs() - bound
+    assert torch.isfinite(got).all()
+    assert (off <= 0).all(), f"worst {off.max().item():g} past its bound, at {np.unravel_index(int(off.argmax()), off.shape)}"
+
+
+def segments(rows, sizes):
+    ends = [0] + list(np.cumsum(sizes))
+    return [(g, a, b) for g, (a, b) in enumerate(zip(ends, ends[1:]))]
+
+
+def reference(X, W, b, act, R, sizes):
+    """(Y, Z, sums of sizes) in 64 bits on the host; sizes: rows of each group, or None."""
+    X, W = X.double().cpu(), W.double().cpu()
+    rows, n_out = X.shape[0], W.shape[-2]
+    Z, S = torch.zeros(rows, n_out, dtype=torch.float64), torch.zeros(rows, n_out, dtype=torch.float64)
+    Y = torch.zeros_like(Z)
+    for g, i, j in [(None, 0, rows)] if sizes is None else segments(rows, sizes):
+        w, bias = (W, b) if g is None else (W[g], None if b is None else b[g])
+        Z[i:j], S[i:j] = X[i:j] @ w.T, X[i:j].abs() @ w.T.abs()
+        if bias is not None:
+            Z[i:j] += bias.double().cpu()
+            S[i:j] += bias.double().cpu().abs()
+        Y[i:j] = ACTS[act](Z[i:j])
+    if R is not None:
+        Y, S = Y + R.double().cpu(), S + R.double().cpu().abs()
+    return Y, Z, S
+
+
+def check_forward(rows, n_in, n_out, dt, act="none", bias=False, residual=False, sizes=None, lay=(0, 0), seed=0):
+    lead = () if sizes is None else (len(sizes),)
+    X = rand((rows, n_in), dt, seed)
+    W = rand(lead + (n_out, n_in), dt, seed + 1, n_in**-0.5)
+    b = rand(lead + (n_out,), dt, seed + 2) if bias else None
+    R = rand((rows, n_out), dt, seed + 3) if residual else None
+    Y, Z, S = reference(X, W, b, act, R, sizes)
+    put = lambda t: None if t is None else wide(t, *lay)  # noqa: E731
+    y, pre = put(torch.zeros(rows, n_out, dtype=DTYPES[dt], device="cuda")), put(torch.zeros(rows, n_out, dtype=DTYPES[dt], device="cuda"))
+    d.op_linear(put(X), put(W), y, bias=b, act=act, residual=put(R), pre=pre, groups=None if sizes is None else ends_of(sizes))
+    close(y, Y, S, n_in, dt)
+    close(pre, Z, S, n_in, dt)
+
+
+def check_backward(rows, n_in, n_out, dt, act="none", sizes=None, lay=(0, 0), seed=0, bias=True):
+    lead = () if sizes is None else (len(sizes),)
+    X, W = rand((rows, n_in), dt, seed), rand(lead + (n_out, n_in), dt, seed + 1, n_in**-0.5)
+    dY, pre = rand((rows, n_out), dt, seed + 2), rand((rows, n_out), dt, seed + 3)
+    # the formula: act' from autograd in 64 bits at the given pre
+    z = pre.double().cpu().requires_grad_(True)
+    ACTS[act](z).sum().backward()
+    dZ = dY.double().cpu() * z.grad
+    x, w = X.double().cpu(), W.double().cpu()
+    dX, sX = torch.zeros(rows, n_in, dtype=torch.float64), torch.zeros(rows, n_in, dtype=torch.float64)
+    dW, sW = torch.zeros(W.shape, dtype=torch.float64), torch.zeros(W.shape, dtype=torch.float64)
+    db, sb = torch.zeros(lead + (n_out,), dtype=torch.float64), torch.zeros(lead + (n_out,), dtype=torch.float64)
+    for g, i, j in [((), 0, rows)] if sizes is None else segments(rows, sizes):
+        dX[i:j], sX[i:j] = dZ[i:j] @ w[g], dZ[i:j].abs() @ w[g].abs()
+        dW[g], sW[g] = dZ[i:j].T @ x[i:j], dZ[i:j].abs().T @ x[i:j].abs()
+        db[g], sb[g] = dZ[i:j].sum(0), dZ[i:j].abs().sum(0)
+    zX, zW = sX.clone(), sW.clone()
+    put = lambda t: None if t is None else wide(t, *lay)  # noqa: E731
+    gx, gw = put(torch.zeros_like(X)), put(torch.zeros_like(W))
+    gb = torch.zeros(lead + (n_out,), dtype=DTYPES[dt], device="cuda") if bias else None
+    d.op_linear_backward(put(dY), put(X), put(W), pre=put(pre), act=act, dX=gx, dW=gw, dbias=gb,
+                         groups=None if sizes is None else ends_of(sizes))
+    rounded = 0.0 if act == "none" else HALF[dt] * 1.01
+    # a slope's own error: four units of fp32 of terms that are at most 3 in size (it crosses zero, they do not)
+    slope = 0.0 if act in ("none", "relu") else 12 * EPS32
+    sub = TINY[dt] * 4
+    a, one = dY.double().cpu().abs(), torch.ones(rows, 1, dtype=torch.float64)
+    for g, i, j in [((), 0, rows)] if sizes is None else segments(rows, sizes):
+        sX[i:j] = sX[i:j] * rounded + slope * a[i:j] @ w[g].abs()
+        sW[g] = sW[g] * rounded + slope * a[i:j].T @ x[i:j].abs()
+        sb[g] = (rows + 40) * EPS32 * sb[g] + slope * (a[i:j].T @ one[i:j])[:, 0]
+    close(gx, dX, zX, n_out, dt, sX + sub * n_out)
+    close(gw, dW, zW, rows, dt, sW + sub * rows)
+    if bias:
+        close(gb, db, sb * 0, 0, dt, sb)
+
+
+SHAPES = [(1, 1, 1), (1, 64, 16), (2, 200, 65), (16, 512, 256), (17, 63, 129), (127, 65, 127), (128, 128, 128), (129, 136, 200), (300, 1003, 77)]
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("shape", SHAPES)
+def test_forward_sizes(shape, dt):
+    check_forward(*shape, dt, act="gelu", bias=True, residual=True, seed=sum(shape))
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("shape", SHAPES)
+def test_backward_sizes(shape, dt):
+    check_backward(*shape, dt, act="silu", seed=sum(shape))
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("act", list(ACTS))
+def test_activations(act, dt):
+    check_forward(130, 96, 72, dt, act=act, bias=True)
+    check_backward(130, 96, 72, dt, act=act)
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("lay", [(8, 0), (8, 8), (1, 0), (3, 1), (4, 4)])
+def test_strides_and_alignments(lay, dt):
+    check_forward(140, 144, 136, dt, act="relu", bias=True, residual=True, lay=lay)
+    check_backward(140, 144, 136, dt, act="gelu_tanh", lay=lay)
+
+
+# enough tiles of 256 x 256 for the large kernel, rests in every direction; reductions that are split
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+def test_large_tiles(dt):
+    check_forward(3601, 200, 3848, dt, act="silu", bias=True)
+    check_backward(3601, 3848, 200, dt, act="none", bias=False)
+    check_backward(200, 3600, 3848, dt, act="gelu")
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+def test_split_reductions(dt):
+    check_forward(100, 5000, 96, dt, act="gelu", bias=True, residual=True)
+    check_backward(2500, 90, 100, dt, act="relu")
+    check_backward(64, 72, 4111, dt, act="none")
+
+
+GROUPS = [[5, 0, 130, 1, 0, 0, 64], [0, 0, 3], [300], [0, 0], [1] * 70 + [0] * 9 + [200], [128, 256, 127, 129]]
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("sizes", GROUPS, ids=lambda s: f"{len(s)}_{sum(s)}")
+@pytest.mark.parametrize("padding", [0, 7])
+def test_groups(sizes, padding, dt):
+    rows = sum(sizes) + padding
+    check_forward(rows, 72, 136, dt, act="silu", bias=True, residual=True, sizes=sizes)
+    check_backward(rows, 72, 136, dt, act="gelu", sizes=sizes)
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+def test_groups_on_large_tiles(dt):
+    sizes = [700, 0, 256, 1300, 3, 1741]
+    check_forward(sum(sizes) + 9, 136, 3000, dt, act="gelu_tanh", sizes=sizes)
+    check_backward(sum(sizes) + 9, 3000, 136, dt, sizes=sizes, bias=False)
+    check_backward(sum(sizes) + 9, 1000, 2000, dt, sizes=sizes, act="silu")
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("n_in,n_out", [(64, 128), (77, 33), (1, 1), (136, 264)])
+@pytest.mark.parametrize("square", [False, True])
+def test_example_grads(n_in, n_out, square, dt):
+    sizes = [1, 0, 200, 33, 64, 65]
+    rows = sum(sizes) + 2
+    dY, X = rand((rows, n_out), dt, 1), rand((rows, n_in), dt, 2)
+    out = torch.full((len(sizes), n_out, n_in), 9.0, device="cuda")
+    d.op_example_grads(dY, X, ends_of(sizes), out, square=square)
+    for e, i, j in segments(rows, sizes):
+        a, b = dY[i:j].double().cpu(), X[i:j].double().cpu()
+        want, sums = a.T @ b, a.T.abs() @ b.abs()
+        if square:
+            want, sums = want**2, 2 * want.abs() * sums + (j - i + 40) * EPS32 * 1.2 * sums**2
+        close(out[e], want, sums, j - i, "f32")
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+def test_gradient_against_differences(dt):
+    """Of the formulas above in 64 bits: the slope that the gradients are held to is that of the forward pass."""
+    rows, n_in, n_out = 6, 9, 7
+    X, W, b, R = rand((rows, n_in), dt, 1), rand((n_out, n_in), dt, 2, 0.3), rand((n_out,), dt, 3), rand((rows, n_out), dt, 4)
+    dY = rand((rows, n_out), dt, 5)
+    for act in ("silu", "gelu", "gelu_tanh"):
+        _, Z, _ = reference(X, W, b, act, R, None)
+        pre = Z.to(DTYPES[dt]).cuda()
+        gx = torch.zeros_like(X)
+        d.op_linear_backward(dY, X, W, pre=pre, act=act, dX=gx)
+        h, gX = 1e-5, torch.zeros(rows, n_in, dtype=torch.float64)
+        for i in range(rows):
+            for j in range(n_in):
+                lo, hi = X.double().cpu().clone(), X.double().cpu().clone()
+                lo[i, j] -= h
+                hi[i, j] += h
+                f = [(reference(t, W, b, act, R, None)[0] * dY.double().cpu()).sum() for t in (lo, hi)]
+                gX[i, j] = (f[1] - f[0]) / (2 * h)
+        size = dY.double().cpu().abs() @ W.double().cpu().abs()
+        # pre is rounded (slopes change by at most 1.2 times that), dZ is, the result is; differences: h^2 and 1e-16 / h
+        bound = size * (HALF[dt] * (1.2 * Z.abs().max() + 1.13) + 1e-5) + HALF[dt] * gX.abs() + 1e-8 + 32 * TINY[dt]
+        assert ((gx.double().cpu() - gX).abs() <= bound).all()
+
+
+def test_no_rows():
+    X, W, Y = (torch.zeros(s, device="cuda") for s in ((0, 8), (4, 8), (0, 4)))
+    d.op_linear(X, W, Y)
+    dW, db = torch.ones(4, 8, device="cuda"), torch.ones(4, device="cuda")
+    d.op_linear_backward(Y, X, W, dX=torch.zeros_like(X), dW=dW, dbias=db)
+    assert not dW.any() and not db.any()
+    out = torch.ones(2, 4, 8, device="cuda")
+    d.op_example_grads(Y, X, ends_of([0, 0]), out)
+    assert not out.any()
+
+
+def test_infinities_and_nan_stay_in_their_rows():
+    X, W = rand((300, 64), "bf16", 1), rand((200, 64), "bf16", 2)
+    Y, clean = torch.zeros(300, 200, dtype=torch.bfloat16, device="cuda"), torch.zeros(300, 200, dtype=torch.bfloat16, device="cuda")
+    d.op_linear(X, W, clean, act="relu")
+    X[5, 3], X[200, 0] = float("nan"), float("inf")
+    d.op_linear(X, W, Y, act="relu")
+    assert Y[5].isnan().all()
+    rest = torch.ones(300, dtype=torch.bool)
+    rest[[5, 200]] = False
+    assert torch.equal(Y[rest], clean[rest])
+
+
+def test_falling_and_wild_ends_stay_inside():
+    """No promise of values, but every access is inside the arrays: guards around the outputs keep theirs."""
+    X, W = rand((64, 64), "bf16", 1), rand((4, 128, 64), "bf16", 2)
+    for ends in ([0, 50, 20, 64, 10], [0, 1 << 40, -5, 3, 64], [7, 7, 7, 7, 7]):
+        e = torch.tensor(ends, dtype=torch.int64, device="cuda")
+        guard = torch.full((66, 128), 3.0, dtype=torch.bfloat16, device="cuda")
+        dW = torch.full((6, 128, 64), 3.0, dtype=torch.bfloat16, device="cuda")
+        db = torch.full((6, 128), 3.0, dtype=torch.bfloat16, device="cuda")
+        d.op_linear(X, W, guard[1:65], groups=e)
+        d.op_linear_backward(guard[1:65], X, W, dW=dW[1:5], dbias=db[1:5], groups=e)
+        assert (guard[[0, 65]] == 3).all() and (dW[[0, 5]] == 3).all() and (db[[0, 5]] == 3).all()
+
+
+def test_same_bits_again_and_on_another_stream():
+    X, W = rand((500, 1000), "bf16", 1), rand((300, 1000), "bf16", 2)
+    Y = [torch.zeros(500, 300, dtype=torch.bfloat16, device="cuda") for _ in range(3)]
+    d.op_linear(X, W, Y[0], act="gelu")
+    d.op_linear(X, W, Y[1], act="gelu")
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        slow = torch.randn(2000, 2000, device="cuda")
+        for _ in range(10):
+            slow = slow @ slow * 1e-3
+        X2 = X + slow[:500, :1000].to(X.dtype) * 0  # ready only after the work before it
+        d.op_linear(X2, W, Y[2], act="gelu")
+    side.synchronize()
+    assert torch.equal(Y[0], Y[1]) and torch.equal(Y[0], Y[2])
+
+
+def test_graph_capture_with_a_workspace_of_the_callers():
+    X, W = rand((100, 4096), "bf16", 1), rand((64, 4096), "bf16", 2)
+    Y = torch.zeros(100, 64, dtype=torch.bfloat16, device="cuda")
+    ws = torch.empty(max(1, d.linear_workspace(100, 4096, 64, "torch.bfloat16")[0]), dtype=torch.uint8, device="cuda")
+    d.op_linear(X, W, Y, workspace=ws)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        d.op_linear(X, W, Y, workspace=ws)
+    for k in range(3):
+        X.copy_(rand((100, 4096), "bf16", 10 + k))
+        want = torch.zeros_like(Y)
+        g.replay()
+        torch.cuda.synchronize()
+        d.op_linear(X, W, want, workspace=torch.empty_like(ws))
+        torch.cuda.synchronize()
+        assert torch.equal(Y, want)
+
+
+def test_device_arrays():
+    rng = np.random.default_rng(0)
+    x, w = rng.standard_normal((33, 40), dtype=np.float32), rng.standard_normal((20, 40), dtype=np.float32)
+    X, W, Y = d.DeviceArray.from_numpy(x), d.DeviceArray.from_numpy(w), d.DeviceArray((33, 20))
+    d.op_linear(X, W, Y, act="relu")
+    d.sync()
+    want = np.maximum(x.astype(np.float64) @ w.T.astype(np.float64), 0)
+    assert np.abs(Y.numpy() - want).max() <= 80 * EPS32 * (np.abs(x) @ np.abs(w).T).max()
+    bits = d.DeviceArray.from_numpy((x.view(np.uint32) >> 16).astype(np.uint16), dtype=np.uint16)
+    wb = d.DeviceArray.from_numpy((w.view(np.uint32) >> 16).astype(np.uint16), dtype=np.uint16)
+    ends = d.DeviceArray.from_numpy(np.array([0, 10, 10, 33]), dtype=np.int64)
+    out, dY = d.DeviceArray((3, 40, 40)), bits
+    d.op_example_grads(dY, bits, ends, out)
+    d.sync()
+    xb = ((x.view(np.uint32) >> 16) << 16).view(np.float32).astype(np.float64)
+    for e, (i, j) in enumerate(((0, 10), (10, 10), (10, 33))):
+        assert np.abs(out.numpy()[e] - xb[i:j].T @ xb[i:j]).max() <= 1e-4
+    del wb
+
+
+def test_refusals():
+    X, W, Y = torch.zeros(8, 16, device="cuda"), torch.zeros(4, 16, device="cuda"), torch.zeros(8, 4, device="cuda")
+
+    def refused(*a, **k):
+        with pytest.raises(d.DnpeffError):
+            d.op_linear(*a, **k)
+
+    refused(X, W.half(), Y)
+    refused(X.double(), W.double(), Y.double())
+    refused(X, W[:, :8], Y)
+    refused(X, W, Y[:7])
+    refused(X.T.contiguous().T, W, Y)
+    refused(X[:1].expand(8, 16), W, Y)
+    refused(X, W, Y, act="tanh")
+    refused(X, W, Y, bias=torch.zeros(5, device="cuda"))
+    refused(X, W, Y, residual=torch.zeros(8, 4))
+    refused(X, W, Y, groups=ends_of([8]))
+    refused(X, W[None], Y, groups=ends_of([4, 4]))
+    refused(X, W[None], Y, groups=ends_of([8]).int())
+    refused(X, d.DeviceArray((4, 16)), Y)
+    with pytest.raises(d.DnpeffError):
+        d.op_linear_backward(Y, X, W, act="silu", dX=torch.zeros_like(X))  # without pre
+    big = torch.zeros(100, 5000, device="cuda"), torch.zeros(96, 5000, device="cuda"), torch.zeros(100, 96, device="cuda")
+    with pytest.raises(d.DnpeffError, match="workspace"):
+        d.op_linear(*big, workspace=torch.zeros(16, dtype=torch.uint8, device="cuda"))
+    z = C.c_void_p(0)
+    assert d.lib.dnpeff_linear(z, 9, 1, 1, 1, z, 1, z, 1, 1, z, 0, z, 0, z, 1, z, 0, 0, z, z, 0) != 0
+    assert b"type" in d.lib.dnpeff_last_error()
+    assert d.lib.dnpeff_linear(z, 0, 1, 1, 1, z, 1, z, 1, 1, z, 0, z, 0, z, 1, z, 0, 0, z, z, 0) != 0
+    assert b"no X" in d.lib.dnpeff_last_error()
+    assert d.lib.dnpeff_linear(z, 0, -1, 1, 1, z, 1, z, 1, 1, z, 0, z, 0, z, 1, z, 0, 0, z, z, 0) != 0
+    torch.cuda.synchronize()
