@@ -563,13 +563,14 @@ int dnpeff_op_init_uniform(int matrix_id, int64_t logical_rows, int64_t logical_
  * All arrays are device memory, row-major with the last index contiguous; ld* are elements from one row to
  * the next (>= the row's width).  `type` is that of every array not declared with one of its own; sums, softmax
  * statistics and losses are fp32.  fp32 products run on the fp32 matrix cores, 16-bit ones on theirs; results are
- * rounded once.  Any size and any alignment of whole elements is taken; rows that begin on 16 bytes (pointer and ld)
- * are the fast ones.  Outputs must not overlap inputs, except Y and residual, which may be one array.
+ * rounded once.  Any size and any alignment of whole elements is taken; operands of the products whose rows do not
+ * begin and end on 16 bytes (pointer, ld and width) are copied to such rows in the workspace first.  Outputs must not overlap inputs, except Y and residual, which may be one array.
  *
  * Calls are queued on `stream`, a hipStream_t of the caller's (NULL: HIP's null stream) or dnpeff_stream(),
  * and allocate nothing and wait for nothing, so they can be captured in a HIP graph.  The workspace belongs to the
- * caller, at least as large as the *_workspace call says for the same sizes, aligned to 16 bytes, and is free for
- * other use once the stream has passed the call.  Every sum is taken in an order that the sizes alone decide. */
+ * caller, aligned to 16 bytes and at least as large as the *_workspace call says for the same sizes (aligned: 1 where the
+ * inputs' pointers and ld are multiples of 16 bytes; 0 serves any), and is free for other use once the stream has passed the
+ * call; with 0 bytes asked for it may be NULL.  Every sum is taken in an order that the sizes alone decide. */
 enum { DNPEFF_F32 = 0, DNPEFF_F16 = 1, DNPEFF_BF16 = 2 };
 /* GELU: z (1 + erf(z / sqrt 2)) / 2;  GELU_TANH: z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2;  SILU: z / (1 + exp(-z)) */
 enum { DNPEFF_ACT_NONE = 0, DNPEFF_ACT_RELU = 1, DNPEFF_ACT_GELU = 2, DNPEFF_ACT_GELU_TANH = 3, DNPEFF_ACT_SILU = 4 };
@@ -584,8 +585,8 @@ enum { DNPEFF_ACT_NONE = 0, DNPEFF_ACT_RELU = 1, DNPEFF_ACT_GELU = 2, DNPEFF_ACT
  * to the next one's, bias [n_groups, n_out].  Groups may be empty.  Rows past the last end belong to none: their product is
  * zero, without bias and activation (Y = residual or 0, pre = 0).  The ends are only read on the device; values that break these
  * rules give undefined results but no access outside the arrays. */
-int dnpeff_linear_workspace(int type, int64_t rows, int64_t n_in, int64_t n_out, int n_groups, int64_t* forward_bytes,
-                            int64_t* backward_bytes);
+int dnpeff_linear_workspace(int type, int64_t rows, int64_t n_in, int64_t n_out, int n_groups, int aligned, int64_t* forward_bytes,
+                            int64_t* backward_bytes, int64_t* example_bytes);
 int dnpeff_linear(void* stream, int type, int64_t rows, int64_t n_in, int64_t n_out, const void* X, int64_t ldx,
                   const void* W, int64_t ldw, int64_t w_group, const void* bias, int act, const void* residual, int64_t ldr,
                   void* Y, int64_t ldy, void* pre, int64_t ldp, int n_groups, const int64_t* ends, void* workspace,
@@ -606,12 +607,13 @@ int dnpeff_linear_backward(void* stream, int type, int64_t rows, int64_t n_in, i
  * output of a linear layer this is the example's gradient of the layer's weight, squared its row of the diagonal Fisher.
  * ends as above (n_examples + 1 of them); an example without rows gives zeros. */
 int dnpeff_example_grads(void* stream, int type, int64_t rows, int64_t n_in, int64_t n_out, const void* dY, int64_t lddy,
-                         const void* X, int64_t ldx, int n_examples, const int64_t* ends, float* out, int square);
+                         const void* X, int64_t ldx, int n_examples, const int64_t* ends, float* out, int square, void* workspace,
+                         int64_t workspace_bytes);
 
 /* Softmax cross entropy of hidden states X [rows, n_in] over a vocabulary with embeddings E [n_words, n_in], without
  * an array of logits: lse[t] = log sum over v of exp(x_t . e_v), loss[t] = lse[t] - x_t . e_label.  labels [rows]; a negative
  * one means that the token has no loss (0), one of n_words and more gives NaN.  loss and lse may be NULL. */
-int dnpeff_vocab_loss_workspace(int type, int64_t rows, int64_t n_in, int64_t n_words, int64_t* forward_bytes,
+int dnpeff_vocab_loss_workspace(int type, int64_t rows, int64_t n_in, int64_t n_words, int aligned, int64_t* forward_bytes,
                                 int64_t* backward_bytes);
 int dnpeff_vocab_loss(void* stream, int type, int64_t rows, int64_t n_in, int64_t n_words, const void* X, int64_t ldx,
                       const void* E, int64_t lde, const int32_t* labels, float* loss, float* lse, void* workspace,

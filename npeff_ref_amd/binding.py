@@ -137,7 +137,10 @@ SIGNATURES = {
     "dnpeff_op_spsp_dense": (C.c_int, [_p, _p, _p]),
     "dnpeff_op_copy": (C.c_int, [_i64, _p, _p]),
     "dnpeff_op_init_uniform": (C.c_int, [C.c_int, _i64, _i64, _u64, _p]),
-    "dnpeff_linear_workspace": (C.c_int, [C.c_int, _i64, _i64, _i64, C.c_int, C.POINTER(_i64), C.POINTER(_i64)]),
+    "dnpeff_linear_workspace": (
+        C.c_int,
+        [C.c_int, _i64, _i64, _i64, C.c_int, C.c_int, C.POINTER(_i64), C.POINTER(_i64), C.POINTER(_i64)],
+    ),
     "dnpeff_linear": (
         C.c_int,
         [_p, C.c_int, _i64, _i64, _i64, _p, _i64, _p, _i64, _i64, _p, C.c_int, _p, _i64, _p, _i64, _p, _i64, C.c_int, _p,
@@ -150,9 +153,9 @@ SIGNATURES = {
     ),
     "dnpeff_example_grads": (
         C.c_int,
-        [_p, C.c_int, _i64, _i64, _i64, _p, _i64, _p, _i64, C.c_int, _p, _p, C.c_int],
+        [_p, C.c_int, _i64, _i64, _i64, _p, _i64, _p, _i64, C.c_int, _p, _p, C.c_int, _p, _i64],
     ),
-    "dnpeff_vocab_loss_workspace": (C.c_int, [C.c_int, _i64, _i64, _i64, C.POINTER(_i64), C.POINTER(_i64)]),
+    "dnpeff_vocab_loss_workspace": (C.c_int, [C.c_int, _i64, _i64, _i64, C.c_int, C.POINTER(_i64), C.POINTER(_i64)]),
     "dnpeff_vocab_loss": (
         C.c_int,
         [_p, C.c_int, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _p, _p, _p, _i64],
@@ -530,25 +533,32 @@ _BYTES = {}  # sizes of workspaces asked for so far
 
 
 def _bytes(fn, *sizes):
-    """(forward, backward) bytes of a workspace."""
+    """Bytes of the workspaces that a library call tells."""
     got = _BYTES.get((fn, sizes))
     if got is None:
-        f, b = _i64(0), _i64(0)
-        _check(getattr(lib, fn)(*sizes, C.byref(f), C.byref(b)))
+        out = [_i64(0) for _ in range(3 if fn == "dnpeff_linear_workspace" else 2)]
+        _check(getattr(lib, fn)(*sizes, *(C.byref(v) for v in out)))
         if len(_BYTES) > 4096:
             _BYTES.clear()
-        got = _BYTES[fn, sizes] = f.value, b.value
+        got = _BYTES[fn, sizes] = tuple(v.value for v in out)
     return got
 
 
-def linear_workspace(rows, n_in, n_out, dtype="float32", n_groups=0):
-    """(forward, backward) bytes of workspace that op_linear and op_linear_backward take."""
-    return _bytes("dnpeff_linear_workspace", _KINDS[str(dtype)], rows, n_in, n_out, n_groups)
+def _on16(c, *places):
+    """Whether arrays at (address, ld, group) begin all their rows on 16 bytes."""
+    mask = 3 if c.type == F32 else 7
+    return int(all(p is None or not (p & 15 or ld & mask or group & mask) for p, ld, group in places))
 
 
-def vocab_loss_workspace(rows, n_in, n_words, dtype="float32"):
+def linear_workspace(rows, n_in, n_out, dtype="float32", n_groups=0, aligned=False):
+    """Bytes of workspace that op_linear, op_linear_backward and op_example_grads take; aligned: for inputs whose rows all
+    begin on 16 bytes."""
+    return _bytes("dnpeff_linear_workspace", _KINDS[str(dtype)], rows, n_in, n_out, n_groups, int(aligned))
+
+
+def vocab_loss_workspace(rows, n_in, n_words, dtype="float32", aligned=False):
     """The same of op_vocab_loss and op_vocab_loss_backward."""
-    return _bytes("dnpeff_vocab_loss_workspace", _KINDS[str(dtype)], rows, n_in, n_words)
+    return _bytes("dnpeff_vocab_loss_workspace", _KINDS[str(dtype)], rows, n_in, n_words, int(aligned))
 
 
 def _layer(c, X_rows, W, groups):
@@ -579,7 +589,9 @@ def op_linear(X, W, Y, bias=None, act="none", residual=None, pre=None, groups=No
     b = c.dense("bias", bias, lead + (n_out,))
     r, ldr, _ = c.array("residual", residual, (rows, n_out))
     p, ldp, _ = c.array("pre", pre, (rows, n_out))
-    need = 0 if workspace is not None else _bytes("dnpeff_linear_workspace", c.type, rows, n_in, n_out, n)[0]
+    need = 0
+    if workspace is None:
+        need = _bytes("dnpeff_linear_workspace", c.type, rows, n_in, n_out, n, _on16(c, (x, ldx, 0), (w, ldw, w_group)))[0]
     c.run(lib.dnpeff_linear, (c.type, rows, n_in, n_out, x, ldx, w, ldw, w_group, b, ACTS[act], r, ldr, y, ldy, p, ldp, n,
                               ends), need, workspace, stream)
 
@@ -601,12 +613,15 @@ def op_linear_backward(dY, X, W, pre=None, act="none", dX=None, dW=None, dbias=N
     gx, lddx, _ = c.array("dX", dX, (rows, n_in))
     gw, lddw, dw_group = c.array("dW", dW, lead + (n_out, n_in))
     b = c.dense("dbias", dbias, lead + (n_out,))
-    need = 0 if workspace is not None else _bytes("dnpeff_linear_workspace", c.type, rows, n_in, n_out, n)[1]
+    need = 0
+    if workspace is None:
+        on16 = _on16(c, (g, lddy, 0), (x, ldx, 0), (w, ldw, w_group))
+        need = _bytes("dnpeff_linear_workspace", c.type, rows, n_in, n_out, n, on16)[1]
     c.run(lib.dnpeff_linear_backward, (c.type, rows, n_in, n_out, g, lddy, x, ldx, w, ldw, w_group, p, ldp, ACTS[act], gx,
                                        lddx, gw, lddw, dw_group, b, n, ends), need, workspace, stream)
 
 
-def op_example_grads(dY, X, examples, out, square=False, stream=None):
+def op_example_grads(dY, X, examples, out, square=False, workspace=None, stream=None):
     """out[e] = dY_e^T X_e (float32 [examples, n_out, n_in]), squared where asked for: with dY the gradient of the log
     likelihood, rows of the diagonal Fisher.  examples: the ends of their rows (dnpeff_example_grads)."""
     c = _Call("op_example_grads", dY)
@@ -618,7 +633,11 @@ def op_example_grads(dY, X, examples, out, square=False, stream=None):
     x, ldx, _ = c.array("X", X, (rows, n_in))
     ends = c.dense("examples", examples, (n + 1,), "i8")
     o = c.dense("out", out, (n, n_out, n_in), F32)
-    _check(lib.dnpeff_example_grads(c.stream(stream), c.type, rows, n_in, n_out, g, lddy, x, ldx, n, ends, o, 1 if square else 0))
+    need = 0
+    if workspace is None and n > 0:
+        need = _bytes("dnpeff_linear_workspace", c.type, rows, n_in, n_out, n, _on16(c, (g, lddy, 0), (x, ldx, 0)))[2]
+    c.run(lib.dnpeff_example_grads, (c.type, rows, n_in, n_out, g, lddy, x, ldx, n, ends, o, 1 if square else 0), need,
+          workspace, stream)
 
 
 def op_vocab_loss(X, E, labels, loss=None, lse=None, workspace=None, stream=None):
@@ -629,7 +648,9 @@ def op_vocab_loss(X, E, labels, loss=None, lse=None, workspace=None, stream=None
     (rows, n_in), words = X.shape, E.shape[0]
     x, ldx, _ = c.array("X", X, (rows, n_in))
     e, lde, _ = c.array("E", E, (words, n_in))
-    need = 0 if workspace is not None else _bytes("dnpeff_vocab_loss_workspace", c.type, rows, n_in, words)[0]
+    need = 0
+    if workspace is None:
+        need = _bytes("dnpeff_vocab_loss_workspace", c.type, rows, n_in, words, _on16(c, (x, ldx, 0), (e, lde, 0)))[0]
     c.run(lib.dnpeff_vocab_loss, (c.type, rows, n_in, words, x, ldx, e, lde, c.dense("labels", labels, (rows,), "i4"),
                                   c.dense("loss", loss, (rows,), F32), c.dense("lse", lse, (rows,), F32)),
           need, workspace, stream)
@@ -645,7 +666,9 @@ def op_vocab_loss_backward(X, E, labels, lse, dloss, dX=None, dE=None, workspace
     e, lde, _ = c.array("E", E, (words, n_in))
     gx, lddx, _ = c.array("dX", dX, (rows, n_in))
     ge, ldde, _ = c.array("dE", dE, (words, n_in))
-    need = 0 if workspace is not None else _bytes("dnpeff_vocab_loss_workspace", c.type, rows, n_in, words)[1]
+    need = 0
+    if workspace is None:
+        need = _bytes("dnpeff_vocab_loss_workspace", c.type, rows, n_in, words, _on16(c, (x, ldx, 0), (e, lde, 0)))[1]
     c.run(lib.dnpeff_vocab_loss_backward,
           (c.type, rows, n_in, words, x, ldx, e, lde, c.dense("labels", labels, (rows,), "i4"),
            c.dense("lse", lse, (rows,), F32), c.dense("dloss", dloss, (rows,), F32), gx, lddx, ge, ldde),

@@ -108,104 +108,167 @@ int check_act(const char* what, int act) {
 }
 group_rows rows_of(const layer& l) { return group_rows{l.ends, l.grouped() ? l.groups : 1, l.rows}; }
 
-template <class T>
-int64_t forward_ws(const layer& l) {
-  return l.grouped() ? 0 : round256(4 * split_floats<T>(l.rows, l.n_out, l.n_in));
+matrix rows_matrix(const layer& l, const void* p, int64_t ld, int64_t width) { return matrix{p, ld, l.rows, width, 1, 0}; }
+matrix weight_matrix(const layer& l, const void* p, int64_t ld, int64_t sheet) {
+  return matrix{p, ld, l.n_out, l.n_in, l.grouped() ? l.groups : 1, sheet};
 }
+
+// Parts of a workspace: copies of operands that do not lie well, then the rest.
 template <class T>
-struct backward_ws {
-  int64_t dz, sums, parts, all;
-  backward_ws(const layer& l) {
-    dz = round256(l.rows * ((l.n_out + 7) / 8 * 8) * (int64_t)sizeof(T));
-    sums = round256(slope_tiles(l.rows, l.grouped() ? l.groups : 1) * l.n_out * 4);
-    const int64_t x = l.grouped() ? 0 : split_floats<T>(l.rows, l.n_in, l.n_out), w = l.grouped() ? 0 : split_floats<T>(l.n_out, l.n_in, l.rows);
-    parts = round256(4 * (x > w ? x : w));
-    all = dz + sums + parts;
+struct forward_room {
+  int64_t packs = 0, parts, all;
+  matrix m[2];
+  forward_room(const layer& l, const void* X, int64_t ldx, const void* W, int64_t ldw, int64_t w_group)
+      : m{rows_matrix(l, X, ldx, l.n_in), weight_matrix(l, W, ldw, w_group)} {
+    for (const matrix& q : m) packs += packed_bytes<T>(q);
+    parts = l.grouped() ? 0 : round256(4 * split_floats<T>(l.rows, l.n_out, l.n_in));
+    all = packs + parts;
+  }
+};
+template <class T>
+struct backward_room {
+  int64_t packs = 0, dz = 0, sums = 0, parts = 0, all;
+  int n = 0;
+  matrix m[3];
+  int x = -1, w = -1, y = -1;  // which of m
+  backward_room(const layer& l, const void* dY, int64_t lddy, const void* X, int64_t ldx, const void* W, int64_t ldw, int64_t w_group, int act,
+                bool dX, bool dW, bool dbias) {
+    if (act != DNPEFF_ACT_NONE && (dX || dW))
+      dz = round256(l.rows * packed_ld<T>(l.n_out) * (int64_t)sizeof(T));
+    else if (dX || dW)
+      m[y = n++] = rows_matrix(l, dY, lddy, l.n_out);
+    if (dW) m[x = n++] = rows_matrix(l, X, ldx, l.n_in);
+    if (dX) m[w = n++] = weight_matrix(l, W, ldw, w_group);
+    for (int i = 0; i < n; i++) packs += packed_bytes<T>(m[i]);
+    if (dbias) sums = round256(slope_tiles(l.rows, l.grouped() ? l.groups : 1) * l.n_out * 4);
+    if (!l.grouped()) {
+      const int64_t a = dX ? split_floats<T>(l.rows, l.n_in, l.n_out) : 0, b = dW ? split_floats<T>(l.n_out, l.n_in, l.rows) : 0;
+      parts = round256(4 * (a > b ? a : b));
+    }
+    all = packs + dz + sums + parts;
+  }
+};
+template <class T>
+struct example_room {
+  int64_t packs = 0;
+  matrix m[2];
+  example_room(const layer& l, const void* dY, int64_t lddy, const void* X, int64_t ldx)
+      : m{rows_matrix(l, dY, lddy, l.n_out), rows_matrix(l, X, ldx, l.n_in)} {
+    for (const matrix& q : m) packs += packed_bytes<T>(q);
   }
 };
 
+int check_room(const char* what, int64_t need, const void* ws, int64_t bytes) {
+  DN_CHECK(need == 0 || (ws != nullptr && bytes >= need && (uintptr_t)ws % 16 == 0),
+           "%s: a workspace of %lld bytes, aligned to 16, is needed", what, (long long)need);
+  return 0;
+}
+
 template <class T>
 int forward(hipStream_t st, const layer& l, const void* X, int64_t ldx, const void* W, int64_t ldw, int64_t w_group, const void* bias, int act,
-            const void* residual, int64_t ldr, void* Y, int64_t ldy, void* pre, int64_t ldp, void* ws) {
+            const void* residual, int64_t ldr, void* Y, int64_t ldy, void* pre, int64_t ldp, char* ws, int64_t ws_bytes) {
+  forward_room<T> room(l, X, ldx, W, ldw, w_group);
+  DN_TRY(check_room("dnpeff_linear", room.all, ws, ws_bytes));
+  DN_TRY(pack<T>(room.m, 2, ws, st));
   args p{};
-  p.A = X, p.lda = ldx, p.B = W, p.ldb = ldw, p.b_group = w_group;
+  p.A = room.m[0].p, p.lda = room.m[0].ld, p.B = room.m[1].p, p.ldb = room.m[1].ld, p.b_group = room.m[1].sheet;
   p.M = l.rows, p.N = l.n_out, p.K = l.n_in;
   p.mode = l.grouped() ? BY_ROWS : ONE;
   p.G = rows_of(l);
   p.out = Y, p.ldc = ldy, p.pre = pre, p.ldp = ldp, p.residual = residual, p.ldr = ldr, p.bias = bias, p.act = act;
   p.wide = fours<T>(Y, ldy) && fours<T>(pre, ldp) && fours<T>(residual, ldr) && fours<T>(bias, l.n_out);
-  return launch_product<T, true, true, E_LINEAR>(p, false, false, (float*)ws, st);
+  return launch_product<T, true, true, E_LINEAR>(p, room.parts ? (float*)(ws + room.packs) : nullptr, st);
 }
 
 template <class T>
 int backward(hipStream_t st, const layer& l, const void* dY, int64_t lddy, const void* X, int64_t ldx, const void* W, int64_t ldw,
              int64_t w_group, const void* pre, int64_t ldp, int act, void* dX, int64_t lddx, void* dW, int64_t lddw, int64_t dw_group,
-             void* dbias, char* ws) {
-  const backward_ws<T> room(l);
+             void* dbias, char* ws, int64_t ws_bytes) {
+  backward_room<T> room(l, dY, lddy, X, ldx, W, ldw, w_group, act, dX, dW, dbias);
+  DN_TRY(check_room("dnpeff_linear_backward", room.all, ws, ws_bytes));
   const group_rows G = rows_of(l);
-  const void* dz = dY;
-  int64_t ldz = lddy;
-  float* sums = dbias ? (float*)(ws + room.dz) : nullptr;
-  float* parts = room.parts > 0 ? (float*)(ws + room.dz + room.sums) : nullptr;
-  const bool slopes = act != DNPEFF_ACT_NONE && (dX || dW);
-  if (slopes) {  // (rows of whole 16 bytes, whatever those of dY are)
-    dz = ws;
-    ldz = (l.n_out + 7) / 8 * 8;
-  }
-  if ((slopes || dbias) && l.rows > 0) {
+  DN_TRY(pack<T>(room.m, room.n, ws, st));
+  char* at = ws + room.packs;
+  T* dz = room.dz ? (T*)at : nullptr;
+  at += room.dz;
+  float* sums = dbias ? (float*)at : nullptr;
+  at += room.sums;
+  float* parts = room.parts ? (float*)at : nullptr;
+  if ((dz || dbias) && l.rows > 0) {
     const bool wide = fours<T>(dY, lddy) && (act == DNPEFF_ACT_NONE || fours<T>(pre, ldp));
     const dim3 grid((unsigned)slope_tiles(l.rows, G.groups), (unsigned)ceil_div(l.n_out, DZ_COLS));
     DN_CHECK(grid.y <= 65535, "dnpeff_linear_backward: n_out = %lld is too wide for one launch", (long long)l.n_out);
-    k_slopes<T><<<grid, 256, 0, st>>>(G, l.n_out, (const T*)dY, lddy, (const T*)pre, ldp, act, slopes ? (T*)ws : nullptr, ldz, sums, wide);
+    k_slopes<T><<<grid, 256, 0, st>>>(G, l.n_out, (const T*)dY, lddy, (const T*)pre, ldp, act, dz, packed_ld<T>(l.n_out), sums, wide);
     DN_LAUNCH_CHECK();
   }
   if (dbias) {
-    k_bias_sums<T><<<dim3((unsigned)ceil_div(l.n_out, 256), (unsigned)G.groups), 256, 0, st>>>(G, l.n_out, sums, (int)slope_tiles(l.rows, G.groups), (T*)dbias);
+    k_bias_sums<T><<<dim3((unsigned)ceil_div(l.n_out, 256), (unsigned)G.groups), 256, 0, st>>>(G, l.n_out, sums,
+                                                                                               (int)slope_tiles(l.rows, G.groups), (T*)dbias);
     DN_LAUNCH_CHECK();
   }
+  const void* g = dz ? dz : room.y >= 0 ? room.m[room.y].p : nullptr;
+  const int64_t ldg = dz ? packed_ld<T>(l.n_out) : room.y >= 0 ? room.m[room.y].ld : 0;
   if (dX) {
     args p{};
-    p.A = dz, p.lda = ldz, p.B = W, p.ldb = ldw, p.b_group = w_group;
+    p.A = g, p.lda = ldg, p.B = room.m[room.w].p, p.ldb = room.m[room.w].ld, p.b_group = room.m[room.w].sheet;
     p.M = l.rows, p.N = l.n_in, p.K = l.n_out;
     p.mode = l.grouped() ? BY_ROWS : ONE;
     p.G = G;
     p.out = dX, p.ldo = lddx, p.wide = fours<T>(dX, lddx);
-    DN_TRY((launch_product<T, true, false, E_STORE>(p, slopes, false, parts, st)));
+    DN_TRY((launch_product<T, true, false, E_STORE>(p, parts, st)));
   }
   if (dW) {
     args p{};
-    p.A = dz, p.lda = ldz, p.B = X, p.ldb = ldx;
+    p.A = g, p.lda = ldg, p.B = room.m[room.x].p, p.ldb = room.m[room.x].ld;
     p.M = l.n_out, p.N = l.n_in, p.K = l.rows;
     p.mode = l.grouped() ? BY_REDUCTION : ONE;
     p.G = G;
     p.out = dW, p.ldo = lddw, p.c_group = dw_group, p.wide = fours<T>(dW, lddw) && dw_group % 4 == 0;
-    DN_TRY((launch_product<T, false, false, E_STORE>(p, slopes, false, parts, st)));
+    DN_TRY((launch_product<T, false, false, E_STORE>(p, parts, st)));
   }
   return 0;
 }
 
 template <class T>
-int example_grads(hipStream_t st, const layer& l, const void* dY, int64_t lddy, const void* X, int64_t ldx, float* out, int square) {
+int example_grads(hipStream_t st, const layer& l, const void* dY, int64_t lddy, const void* X, int64_t ldx, float* out, int square, char* ws,
+                  int64_t ws_bytes) {
+  example_room<T> room(l, dY, lddy, X, ldx);
+  DN_TRY(check_room("dnpeff_example_grads", room.packs, ws, ws_bytes));
+  DN_TRY(pack<T>(room.m, 2, ws, st));
   args p{};
-  p.A = dY, p.lda = lddy, p.B = X, p.ldb = ldx;
+  p.A = room.m[0].p, p.lda = room.m[0].ld, p.B = room.m[1].p, p.ldb = room.m[1].ld;
   p.M = l.n_out, p.N = l.n_in, p.K = l.rows;
   p.mode = BY_REDUCTION;
   p.G = rows_of(l);
   p.out = out, p.out_f32 = 1, p.square = square, p.ldo = l.n_in, p.c_group = l.n_out * l.n_in;
   p.wide = fours<float>(out, l.n_in);
-  return launch_product<T, false, false, E_STORE>(p, false, false, nullptr, st);
+  return launch_product<T, false, false, E_STORE>(p, nullptr, st);
 }
+
+// Operands as a workspace is asked for: of whole rows, on 16 bytes or (not aligned) on none.
+struct as_if {
+  const void* p;
+  int64_t in, out;
+  as_if(bool aligned, int64_t n_in, int64_t n_out) : p((const void*)(uintptr_t)(aligned ? 16 : 1)), in(n_in), out(n_out) {}
+};
 
 }  // namespace
 
-DN_API int dnpeff_linear_workspace(int type, int64_t rows, int64_t n_in, int64_t n_out, int n_groups, int64_t* forward_bytes,
-                                   int64_t* backward_bytes) {
+DN_API int dnpeff_linear_workspace(int type, int64_t rows, int64_t n_in, int64_t n_out, int n_groups, int aligned, int64_t* forward_bytes,
+                                   int64_t* backward_bytes, int64_t* example_bytes) {
   clear_error();
   static const int64_t some = 0;
   const layer l{rows, n_in, n_out, n_groups, n_groups > 0 ? &some : nullptr};
   DN_TRY(check_layer("dnpeff_linear_workspace", type, l));
-  if (forward_bytes) *forward_bytes = DN_BY_TYPE(type, forward_ws<T>(l));
-  if (backward_bytes) *backward_bytes = DN_BY_TYPE(type, backward_ws<T>(l).all);
+  const as_if a(aligned, n_in, n_out);
+  const int64_t sheet = n_in * n_out;
+  if (forward_bytes) *forward_bytes = DN_BY_TYPE(type, (forward_room<T>(l, a.p, a.in, a.p, a.in, sheet).all));
+  if (backward_bytes) {  // the larger of the two ways that dZ comes
+    const int64_t y = DN_BY_TYPE(type, (backward_room<T>(l, a.p, a.out, a.p, a.in, a.p, a.in, sheet, DNPEFF_ACT_NONE, true, true, true).all));
+    const int64_t z = DN_BY_TYPE(type, (backward_room<T>(l, a.p, a.out, a.p, a.in, a.p, a.in, sheet, DNPEFF_ACT_SILU, true, true, true).all));
+    *backward_bytes = y > z ? y : z;
+  }
+  if (example_bytes) *example_bytes = DN_BY_TYPE(type, (example_room<T>(l, a.p, a.out, a.p, a.in).packs));
   return 0;
 }
 
@@ -224,11 +287,8 @@ DN_API int dnpeff_linear(void* stream, int type, int64_t rows, int64_t n_in, int
   DN_TRY(check_array(me, "bias", bias, n_out, n_out, type, true));
   DN_TRY(check_array(me, "residual", residual, ldr, n_out, type, true));
   DN_TRY(check_array(me, "pre", pre, ldp, n_out, type, true));
-  const int64_t need = DN_BY_TYPE(type, forward_ws<T>(l));
-  DN_CHECK(need == 0 || (workspace != nullptr && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0),
-           "%s: a workspace of %lld bytes, aligned to 16, is needed", me, (long long)need);
   return DN_BY_TYPE(type, forward<T>((hipStream_t)stream, l, X, ldx, W, ldw, w_group, bias, act, residual, ldr, Y, ldy, pre, ldp,
-                                     need ? workspace : nullptr));
+                                     (char*)workspace, workspace_bytes));
 }
 
 DN_API int dnpeff_linear_backward(void* stream, int type, int64_t rows, int64_t n_in, int64_t n_out, const void* dY, int64_t lddy,
@@ -247,15 +307,13 @@ DN_API int dnpeff_linear_backward(void* stream, int type, int64_t rows, int64_t 
   DN_TRY(check_array(me, "dX", dX, lddx, n_in, type, true));
   DN_TRY(check_array(me, "dW", dW, lddw, n_in, type, true));
   DN_TRY(check_array(me, "dbias", dbias, n_out, n_out, type, true));
-  const int64_t need = DN_BY_TYPE(type, backward_ws<T>(l).all);
-  DN_CHECK(need == 0 || (workspace != nullptr && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0),
-           "%s: a workspace of %lld bytes, aligned to 16, is needed", me, (long long)need);
   return DN_BY_TYPE(type, backward<T>((hipStream_t)stream, l, dY, lddy, X, ldx, W, ldw, w_group, pre, ldp, act, dX, lddx, dW, lddw,
-                                      dw_group, dbias, (char*)workspace));
+                                      dw_group, dbias, (char*)workspace, workspace_bytes));
 }
 
 DN_API int dnpeff_example_grads(void* stream, int type, int64_t rows, int64_t n_in, int64_t n_out, const void* dY, int64_t lddy,
-                                const void* X, int64_t ldx, int n_examples, const int64_t* ends, float* out, int square) {
+                                const void* X, int64_t ldx, int n_examples, const int64_t* ends, float* out, int square, void* workspace,
+                                int64_t workspace_bytes) {
   clear_error();
   const char* me = "dnpeff_example_grads";
   const layer l{rows, n_in, n_out, n_examples, ends};
@@ -265,5 +323,5 @@ DN_API int dnpeff_example_grads(void* stream, int type, int64_t rows, int64_t n_
   DN_TRY(check_array(me, "dY", dY, lddy, n_out, type, rows == 0));
   DN_TRY(check_array(me, "X", X, ldx, n_in, type, rows == 0));
   DN_TRY(check_array(me, "out", out, n_in, n_in, DNPEFF_F32, false));
-  return DN_BY_TYPE(type, example_grads<T>((hipStream_t)stream, l, dY, lddy, X, ldx, out, square));
+  return DN_BY_TYPE(type, example_grads<T>((hipStream_t)stream, l, dY, lddy, X, ldx, out, square, (char*)workspace, workspace_bytes));
 }

@@ -7,8 +7,8 @@
 // gradient of its input one of each, the gradient of its weight two of the second.  A workgroup forms a
 // tile of BM x BN, 128 bytes of the reduction at a time, from two LDS stages: while the matrix cores
 // work on one, the other is filled past the registers (buffer loads to LDS), whose lanes outside the
-// operand are given an offset past the buffer's end and so arrive as zeros.  Operands whose rows do not
-// begin on 16 bytes go through registers instead, in 16-byte loads from any address.
+// operand lie past the buffer's end and so arrive as zeros.  Operands whose rows do not
+// begin and end on 16 bytes are copied to such rows first.
 //
 // In LDS the 16-byte pieces of a row are permuted by its index, so that the 64 lanes of a read meet all banks:
 //   rows of k:   piece c of row i sits at c ^ ((i >> 1) & 7); a lane reads its 16 bytes of k at once
@@ -229,14 +229,18 @@ struct args {
   int64_t word0, words;
 };
 
-// The result for four consecutive n of one m.
 template <class T>
-__device__ __forceinline__ void finish_linear(const args& p, int64_t m, int64_t n, v4f v, int group, bool held) {
+__device__ __forceinline__ v4f bias4(const args& p, int64_t n, int group) {
+  const int there = (int)(p.N - n < 4 ? p.N - n : 4);
+  return load4((const T*)p.bias + (int64_t)group * p.N + n, p.wide && there == 4, there);
+}
+// The result for four consecutive n of one m, from the product with the bias added.
+template <class T>
+__device__ __forceinline__ void finish_linear(const args& p, int64_t m, int64_t n, v4f v, bool held) {
   constexpr bool EXACT = sizeof(T) == 4;
   const int there = (int)(p.N - n < 4 ? p.N - n : 4);
   const bool whole = p.wide && there == 4;
   if (held) {
-    if (p.bias) v += load4((const T*)p.bias + (int64_t)group * p.N + n, whole, there);
     if (p.pre) store4((T*)p.pre + m * p.ldp + n, v, whole, there);
     if (p.act != DNPEFF_ACT_NONE) {
 #pragma unroll
@@ -270,131 +274,122 @@ __device__ __forceinline__ void finish_store(const args& p, int64_t sheet, int64
 
 // A buffer load of 16 bytes per lane to LDS: lane l's go to lds + 16 l.
 __device__ __forceinline__ void to_lds(v4i buffer, unsigned lds, int offset) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer) : "memory");
 }
-__device__ __forceinline__ v4i buffer_at(const char* p) {
-  const uint64_t a = (uint64_t)p;
-  return v4i{(int)(unsigned)a, (int)(unsigned)((a >> 32) & 0xffff), (int)0x80000000u, 0x00020000};
-}
-
 __device__ __forceinline__ int64_t uniform(int64_t v) {
   const unsigned lo = __builtin_amdgcn_readfirstlane((int)(unsigned)v), hi = __builtin_amdgcn_readfirstlane((int)((uint64_t)v >> 32));
   return (int64_t)(((uint64_t)hi << 32) | lo);
 }
 
-// One operand's part of a tile: R of its own index, 128 bytes of the reduction.
-template <class T, int R, int THREADS, bool ROWS_OF_K, bool DIRECT>
+// One operand's part of a tile: R of its own index, 128 bytes of the reduction, in N loads of 1 KB by each wave.  A load's
+// buffer begins at its first row and ends with the operand: what lies past that arrives as zeros, as do pieces of a row
+// past the reduction's end (their offset is past any buffer's).  What is read of the own index between its end and a row's
+// makes results that nobody takes.  So a lane keeps two offsets: the permutation of the pieces repeats after two loads.
+template <class T, int R, int THREADS, bool ROWS_OF_K>
 struct operand {
   static constexpr int S = sizeof(T), CH = 16 / S, BK = 128 / S;
   static constexpr int PER_ROW = ROWS_OF_K ? 8 : R * S / 16;  // pieces in a row
-  static constexpr int N = R * 8 / THREADS;                   // pieces of a lane
-  static constexpr int BYTES = R * 128;
-  const char* at;   // first row's first piece of the next tile
+  static constexpr int N = R * 8 / THREADS, ROWS = 64 / PER_ROW;
+  static_assert(N == 4, "two offsets serve four loads");
+  static constexpr bool ODD = ROWS_OF_K || ROWS == 2 && S == 2;  // loads 0, 2 and 1, 3 are alike (else 0, 1 and 2, 3)
+  static constexpr int NOWHERE = (int)0x80000000u;
+  int64_t at, end;  // addresses: this wave's first row of the next tile, the operand's end
   int64_t step;     // bytes from a tile to the next
-  int64_t ld;
-  int offset[DIRECT ? N : 1];
-  int r0, c0;       // (not DIRECT) the lane's first row; rows come THREADS / PER_ROW apart
-  int there;        // pieces' own index that exists: rows (rows of k), columns
-  v4i held[DIRECT ? 1 : N];
+  int next;         // bytes from a load to the next
+  int offset[2], k[2];  // k: (rows of k) a lane's place in the reduction
 
   __device__ static __forceinline__ int swizzle(int row) {
     if (ROWS_OF_K) return (row >> 1) & 7;
     if (S == 4) return ((row >> 2) & 3) << 2;
     return (((row & 3) | ((row >> 1) & 4)) << 1) & (PER_ROW - 1);
   }
-  __device__ __forceinline__ void start(const T* p, int64_t ld_, int64_t own0, int64_t k0, int there_, int tid) {
-    ld = ld_ * S;
-    there = there_;
-    at = (const char*)uniform((int64_t)p + (ROWS_OF_K ? own0 * ld + k0 * S : k0 * ld + own0 * S));
-    step = ROWS_OF_K ? 128 : BK * ld;
-    if (DIRECT) {
+  // there: how many of the operand's own index exist from own0 on; k_end: the reduction's end.
+  __device__ __forceinline__ void start(const T* p, int64_t ld, int64_t own0, int64_t k0, int64_t k_end, int there, int tid) {
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    ld *= S;
+    const int64_t first = (int64_t)p + (ROWS_OF_K ? own0 * ld : own0 * S);
+    at = uniform(first + (ROWS_OF_K ? k0 * S : k0 * ld) + wave * N * ROWS * ld);
+    end = uniform(first + (ROWS_OF_K ? (there - 1) * ld + (k_end + CH - 1) / CH * 16 : (k_end - 1) * ld + (int64_t)(there + CH - 1) / CH * 16));
+    step = uniform(ROWS_OF_K ? 128 : BK * ld);
+    next = __builtin_amdgcn_readfirstlane((int)(ROWS * ld));
 #pragma unroll
-      for (int e = 0; e < N; e++) {
-        const int piece = (tid / 64 * N + e) * 64 + tid % 64, row = piece / PER_ROW, c = (piece % PER_ROW) ^ swizzle(row);
-        const bool in = ROWS_OF_K ? row < there : c * CH < there;
-        offset[e] = in ? (int)(row * ld) + c * 16 : (int)0x80000000u;
-      }
+    for (int h = 0; h < 2; h++) {
+      const int row = (wave * N + (ODD ? h : 2 * h)) * ROWS + lane / PER_ROW, c = (lane % PER_ROW) ^ swizzle(row);
+      offset[h] = (int)(lane / PER_ROW * ld) + c * 16;
+      k[h] = c * CH;
     }
   }
   // left: what is left of the reduction.
   __device__ __forceinline__ void fill(unsigned lds, int64_t left, int tid) {
-    const int k_there = left < BK ? (int)left : BK;
-    if (DIRECT) {
-      const v4i buffer = buffer_at(at);
+    const unsigned to = lds + __builtin_amdgcn_readfirstlane(tid >> 6) * (N * 1024);
+    int64_t room = end - at;
+    room = room < 0 ? 0 : room > 0x7fffffff ? 0x7fffffff : room;
+    int o[2] = {offset[0], offset[1]};
+    if (ROWS_OF_K && left < BK) {
 #pragma unroll
-      for (int e = 0; e < N; e++) {
-        const int first = (tid / 64 * N + e) * 64, piece = first + tid % 64, row = piece / PER_ROW;
-        const bool in = ROWS_OF_K ? (((piece % 8) ^ swizzle(row)) * CH < k_there) : row < k_there;
-        to_lds(buffer, lds + __builtin_amdgcn_readfirstlane(first) * 16, in ? offset[e] : (int)0x80000000u);
-      }
-    } else {
+      for (int h = 0; h < 2; h++) o[h] = k[h] < (int)left ? o[h] : NOWHERE;
+    }
+    asm volatile("s_nop 4");  // (between a lane's write of an address and the loads)
 #pragma unroll
-      for (int e = 0; e < N; e++) {
-        const int piece = e * THREADS + tid, row = piece / PER_ROW, c = (piece % PER_ROW) ^ swizzle(row);
-        const int rows = ROWS_OF_K ? there : k_there, cols = ROWS_OF_K ? k_there : there;
-        v4i v = {0, 0, 0, 0};
-        if (row < rows && c * CH < cols) {
-          const char* src = at + row * ld + c * 16;
-          if ((c + 1) * CH <= cols) {
-            struct __attribute__((packed, aligned(S))) loose {
-              v4i v;
-            };
-            v = ((const loose*)src)->v;
-          } else {  // the row ends within the piece
-            union {
-              T t[CH];
-              v4i v;
-            } u;
-#pragma unroll
-            for (int i = 0; i < CH; i++) u.t[i] = c * CH + i < cols ? ((const T*)src)[i] : (T)0.f;
-            v = u.v;
-          }
-        }
-        held[e] = v;
-      }
+    for (int e = 0; e < N; e++) {
+      const uint64_t from = (uint64_t)at + (uint64_t)(unsigned)(e * next);
+      const int size = (int)room - e * next;
+      const v4i buffer = {(int)(unsigned)from, (int)(unsigned)((from >> 32) & 0xffff), size < 0 ? 0 : size, 0x00020000};
+      to_lds(buffer, to + e * 1024, o[ODD ? e & 1 : e >> 1]);
     }
     at += step;
   }
-  // (not DIRECT) what fill() left in registers to its place
-  __device__ __forceinline__ void put(unsigned lds, int tid) {
-    if (DIRECT) return;
+};
+
+// How a lane reads an operand's part of a tile: 16 of its index, `own` + 16 i .. + 15, for 64 bytes of the reduction (the s-th half).
+template <class T, int R, bool ROWS_OF_K>
+struct reader {
+  typedef typename num<T>::piece piece;
+  unsigned lane_at[2];  // rows of k: by half
+  __device__ __forceinline__ void start(int own, int lane) {
+    const int q = lane >> 4, i = lane & 15;
+    if (ROWS_OF_K) {
+      lane_at[0] = (own + i) * 128 + ((q ^ (i >> 1)) << 4);
+      lane_at[1] = lane_at[0] ^ 64;
+    } else if (sizeof(T) == 4) {
+      lane_at[0] = q * 4 * (R * 4) + (i & 3) * 4 + ((((own + i) >> 2) ^ (q << 2)) << 4);
+    } else {
+      const int r = i >> 2, col = own + (i & 3) * 4, swz = ((r | ((q & 1) << 2)) << 1) & (R / 8 - 1);
+      lane_at[0] = (q * 8 + r) * (R * 2) + (((col >> 3) ^ swz) << 4) + (col & 4) * 2;
+    }
+  }
+  __device__ __forceinline__ piece read(unsigned lds, int i, int s) const {
+    if (ROWS_OF_K) {
+      return *(const DN_LDS piece*)(lds_at<const char>(lds + lane_at[s]) + i * 2048);
+    } else if constexpr (sizeof(T) == 4) {
+      const DN_LDS char* p = lds_at<const char>(lds + (lane_at[0] ^ (i << 6)));
+      piece v;
 #pragma unroll
-    for (int e = 0; e < N; e++) *lds_at<v4i>(lds + (e * THREADS + tid) * 16) = held[e];
+      for (int e = 0; e < 4; e++) v[e] = *(const DN_LDS float*)(p + (s * 16 + e) * (R * 4));
+      return v;
+    } else {
+      DN_LDS char* p = lds_at<char>(lds + (lane_at[0] ^ (i << 5)));
+      union {
+        v4s h[2];
+        piece p;
+      } u;
+      u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DN_LDS v4s*)(p + s * 32 * (R * 2)));
+      u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DN_LDS v4s*)(p + (s * 32 + 4) * (R * 2)));
+      return u.p;
+    }
   }
 };
 
-// What a lane reads of 16 of an operand's index, `own` .. + 15, for 64 bytes of the reduction (s-th half).
-template <class T, int R, bool ROWS_OF_K>
-__device__ __forceinline__ typename num<T>::piece read_piece(unsigned lds, int own, int s, int lane) {
-  typedef typename num<T>::piece piece;
-  const int q = lane >> 4, i = lane & 15;
-  if (ROWS_OF_K) {
-    return *lds_at<piece>(lds + (own + i) * 128 + (((q + 4 * s) ^ (i >> 1)) << 4));
-  } else if constexpr (sizeof(T) == 4) {
-    piece v;
-    const int col = own + i;
-#pragma unroll
-    for (int e = 0; e < 4; e++)
-      v[e] = *lds_at<float>(lds + (s * 16 + q * 4 + e) * (R * 4) + (((col >> 2) ^ (q << 2)) << 4) + (col & 3) * 4);
-    return v;
-  } else {
-    const int r = i >> 2, col = own + (i & 3) * 4;
-    const int swz = ((r | ((q & 1) << 2)) << 1) & (R / 8 - 1);
-    const unsigned a = lds + (s * 32 + q * 8 + r) * (R * 2) + (((col >> 3) ^ swz) << 4) + (col & 4) * 2;
-    union {
-      v4s h[2];
-      piece p;
-    } u;
-    u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<v4s>(a));
-    u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<v4s>(a + 4 * R * 2));
-    return u.p;
-  }
+// Everything of this wave's but the last N loads to LDS has arrived, all its LDS reads are done, and so for every wave.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-template <class T, int BM, int BN, int WM, int WN, bool A_ROWS, bool B_ROWS, bool DIRECT, int E>
+template <class T, int BM, int BN, int WM, int WN, bool A_ROWS, bool B_ROWS, int E>
 __global__ __launch_bounds__(WM* WN * 64, 2) void k_tiles(args p) {
   constexpr int THREADS = WM * WN * 64, BK = 128 / sizeof(T);
-  constexpr int FM = BM / WM / 16, FN = BN / WN / 16, STAGE = (BM + BN) * 128;
+  constexpr int FM = BM / WM / 16, FN = BN / WN / 16, STAGE = (BM + BN) * 128, N_LOADS = STAGE / 16 / THREADS;
   __shared__ __align__(16) char smem[2 * STAGE];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
@@ -453,61 +448,91 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_tiles(args p) {
 #pragma unroll
     for (int j = 0; j < FN; j++) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
   const unsigned base = (unsigned)(uintptr_t)(DN_LDS char*)smem;
-  operand<T, BM, THREADS, A_ROWS, DIRECT> a;
-  operand<T, BN, THREADS, B_ROWS, DIRECT> b;
-  a.start(A, p.lda, m0, k0, m_there, tid);
-  b.start(B, p.ldb, n0, k0, n_there, tid);
+  operand<T, BM, THREADS, A_ROWS> a;
+  operand<T, BN, THREADS, B_ROWS> b;
+  a.start(A, p.lda, m0, k0, k_end, m_there, tid);
+  b.start(B, p.ldb, n0, k0, k_end, n_there, tid);
+  // Two stages of 128 bytes of the reduction each.  A lane's operands of one half of a stage are read while the matrix
+  // cores work on the other half's; once the second half's are read a stage is free, and takes the tile after the next.
   int64_t left = uniform(k_end - k0);
-  unsigned stage = 0;
   if (left > 0) {
     a.fill(base, left, tid);
     b.fill(base + BM * 128, left, tid);
-    a.put(base, tid);
-    b.put(base + BM * 128, tid);
-  }
-  while (left > 0) {
-    // the loads of this stage have arrived, and everyone has read the other one
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    left -= BK;
-    const unsigned here = base + stage, next = base + (STAGE - stage);
-    if (left > 0) {
-      a.fill(next, left, tid);
-      b.fill(next + BM * 128, left, tid);
+    if (left > BK) {
+      a.fill(base + STAGE, left - BK, tid);
+      b.fill(base + STAGE + BM * 128, left - BK, tid);
+      wait_loads<N_LOADS>();
+    } else {
+      wait_loads<0>();
     }
+    typename num<T>::piece fa[2][FM], fb[2][FN];
+    unsigned here = base, there = base + STAGE;
+    reader<T, BM, A_ROWS> ra;
+    reader<T, BN, B_ROWS> rb;
+    ra.start(wm * (BM / WM), lane);
+    rb.start(wn * (BN / WN), lane);
+    auto read = [&](unsigned stage, int s) {
 #pragma unroll
-    for (int s = 0; s < 2; s++) {
-      typename num<T>::piece fb[FN], fa[FM];
+      for (int j = 0; j < FN; j++) fb[s][j] = rb.read(stage + BM * 128, j, s);
 #pragma unroll
-      for (int j = 0; j < FN; j++) fb[j] = read_piece<T, BN, B_ROWS>(here + BM * 128, wn * (BN / WN) + j * 16, s, lane);
-#pragma unroll
-      for (int i = 0; i < FM; i++) fa[i] = read_piece<T, BM, A_ROWS>(here, wm * (BM / WM) + i * 16, s, lane);
+      for (int i = 0; i < FM; i++) fa[s][i] = ra.read(stage, i, s);
+    };
+    auto multiply = [&](int s) {
 #pragma unroll
       for (int i = 0; i < FM; i++)
 #pragma unroll
-        for (int j = 0; j < FN; j++) acc[i][j] = mma(fb[j], fa[i], acc[i][j]);
+        for (int j = 0; j < FN; j++) acc[i][j] = mma(fb[s][j], fa[s][i], acc[i][j]);
+    };
+    // (reads of the other half between the products, a few ahead: no more registers than that takes)
+    auto mix = [&]() {
+      constexpr int RA = A_ROWS ? 1 : sizeof(T) == 4 ? 4 : 2, RB = B_ROWS ? 1 : sizeof(T) == 4 ? 4 : 2, ONE_MMA = sizeof(T) == 4 ? 4 : 1;
+      constexpr int AHEAD = FM < 3 ? FM : 3;
+      __builtin_amdgcn_sched_group_barrier(0x100, FN * RB + AHEAD * RA, 0);
+#pragma unroll
+      for (int i = 0; i < FM; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x008, FN * ONE_MMA, 0);
+        if (i + AHEAD < FM) __builtin_amdgcn_sched_group_barrier(0x100, RA, 0);
+      }
+    };
+    read(here, 0);
+    while (true) {
+      read(here, 1);
+      multiply(0);
+      mix();
+      __builtin_amdgcn_sched_barrier(0);
+      // the next stage has arrived, and everyone has read this one
+      wait_loads<0>();
+      left -= BK;
+      if (left > BK) {
+        a.fill(here, left - BK, tid);
+        b.fill(here + BM * 128, left - BK, tid);
+      }
+      read(there, 0);  // (after the last stage: of what is there, for nothing)
+      multiply(1);
+      mix();
+      __builtin_amdgcn_sched_barrier(0);
+      if (left <= 0) break;
+      const unsigned t = here;
+      here = there;
+      there = t;
     }
-    if (left > 0) {
-      a.put(next, tid);
-      b.put(next + BM * 128, tid);
-    }
-    stage = STAGE - stage;
   }
 
   // -- what becomes of it --
   const int64_t mw = m0 + wm * (BM / WM) + (lane & 15), nw = n0 + wn * (BN / WN) + q * 4;
   if constexpr (E == E_LINEAR || E == E_STORE) {
 #pragma unroll
-    for (int i = 0; i < FM; i++) {
-      const int64_t m = mw + i * 16;
-      if (m >= m_end) continue;
+    for (int j = 0; j < FN; j++) {
+      const int64_t n = nw + j * 16;
+      if (n >= p.N) continue;
+      v4f b4 = {0.f, 0.f, 0.f, 0.f};
+      if (E == E_LINEAR && p.bias && held) b4 = bias4<T>(p, n, group);
 #pragma unroll
-      for (int j = 0; j < FN; j++) {
-        const int64_t n = nw + j * 16;
-        if (n >= p.N) continue;
+      for (int i = 0; i < FM; i++) {
+        const int64_t m = mw + i * 16;
+        if (m >= m_end) continue;
         if constexpr (E == E_LINEAR)
-          finish_linear<T>(p, m, n, acc[i][j], group, held);
+          finish_linear<T>(p, m, n, acc[i][j] + b4, held);
         else
           finish_store<T>(p, sheet, m, n, acc[i][j]);
       }
@@ -582,6 +607,8 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_tiles(args p) {
   }
 }
 
+inline int64_t round256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+
 // ---- host --------------------------------------------------------------------------------------------------------
 // Partial sums of a split reduction, added in their order, then as the tiles' own epilogue.
 template <class T, int E>
@@ -592,7 +619,7 @@ __global__ void k_join(args p, const float* parts, int splits) {
   v4f v = {0.f, 0.f, 0.f, 0.f};
   for (int s = 0; s < splits; s++) v += *(const v4f*)(parts + ((int64_t)s * p.M + m) * row + n);
   if constexpr (E == E_LINEAR)
-    finish_linear<T>(p, m, n, v, 0, true);
+    finish_linear<T>(p, m, n, p.bias ? v + bias4<T>(p, n, 0) : v, true);
   else
     finish_store<T>(p, 0, m, n, v);
 }
@@ -626,9 +653,84 @@ inline int64_t split_floats(int64_t M, int64_t N, int64_t K) {
   return r.splits > 1 ? r.splits * M * (ceil_div(N, 4) * 4) : 0;
 }
 
-inline bool fits16(const void* p, int64_t ld, int64_t size) { return (uintptr_t)p % 16 == 0 && ld * size % 16 == 0; }
+// ---- operands that tiles can be loaded from -----------------------------------------------------------------------
+// A matrix whose rows begin on 16 bytes and end on them is loaded as it lies; any other is first copied to rows that do,
+// with zeros behind their ends (k_pack): once, where a tile's loads would come from any address again and again.
+struct matrix {
+  const void* p;
+  int64_t ld, rows, width;
+  int64_t sheets, sheet;  // and so many such, so far apart
+};
+template <class T>
+inline bool lies_well(const matrix& m) {
+  constexpr int64_t S = sizeof(T), NEAR = (int64_t)1 << 31;
+  return (uintptr_t)m.p % 16 == 0 && m.ld * S % 16 == 0 && m.width * S % 16 == 0 && (m.sheets < 2 || m.sheet * S % 16 == 0) &&
+         256 * m.ld * S < NEAR;
+}
+template <class T>
+inline int64_t packed_ld(int64_t width) {
+  return ceil_div(width, 64) * 64;
+}
+template <class T>
+inline int64_t packed_bytes(const matrix& m) {
+  return lies_well<T>(m) ? 0 : round256(m.sheets * m.rows * packed_ld<T>(m.width) * (int64_t)sizeof(T));
+}
+struct pack_args {
+  matrix m[3];
+  void* to[3];
+  int64_t first[4];  // workgroups before each
+};
+// A lane makes 16 bytes of a packed row.
+template <class T>
+__global__ __launch_bounds__(256) void k_pack(pack_args p) {
+  constexpr int S = sizeof(T), CH = 16 / S;
+  const int w = blockIdx.x < p.first[1] ? 0 : blockIdx.x < p.first[2] ? 1 : 2;
+  const matrix m = p.m[w];
+  const int64_t ld = (m.width + 63) / 64 * 64, per_row = ld / CH;
+  const int64_t at = ((int64_t)blockIdx.x - p.first[w]) * 256 + threadIdx.x, row = at / per_row;
+  if (row >= m.rows * m.sheets) return;
+  const int c = (int)(at - row * per_row) * CH, there = (int)(m.width - c);
+  const T* src = (const T*)m.p + (m.sheets > 1 ? row / m.rows * m.sheet + row % m.rows * m.ld : row * m.ld) + c;
+  union {
+    T t[CH];
+    v4i v;
+  } u;
+  if (there >= CH) {
+    struct __attribute__((packed, aligned(S))) loose {
+      v4i v;
+    };
+    u.v = ((const loose*)src)->v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < CH; i++) u.t[i] = i < there ? src[i] : (T)0.f;
+  }
+  *(v4i*)((T*)p.to[w] + row * ld + c) = u.v;
+}
+// Packs those of n matrices (at most 3) that do not lie well into `room`, and makes them the copies.  Returns what it took of it.
+template <class T>
+inline int pack(matrix* m, int n, char* room, hipStream_t st) {
+  pack_args p{};
+  int64_t blocks = 0;
+  int k = 0;
+  for (int i = 0; i < n; i++) {
+    const int64_t bytes = packed_bytes<T>(m[i]);
+    if (bytes == 0) continue;
+    const int64_t ld = packed_ld<T>(m[i].width);
+    p.m[k] = m[i], p.to[k] = room, p.first[k] = blocks;
+    blocks += ceil_div(m[i].sheets * m[i].rows * (ld * (int64_t)sizeof(T) / 16), 256);
+    m[i].p = room, m[i].ld = ld, m[i].sheet = m[i].rows * ld;
+    room += bytes;
+    k++;
+  }
+  if (blocks == 0) return 0;
+  for (int i = k; i < 4; i++) p.first[i] = blocks;
+  DN_CHECK(blocks < (int64_t)1 << 31, "operands of %lld MB that are not aligned to 16 bytes", (long long)(blocks >> 8));
+  k_pack<T><<<(unsigned)blocks, 256, 0, st>>>(p);
+  DN_LAUNCH_CHECK();
+  return 0;
+}
 
-template <class T, int BM, int BN, int WM, int WN, bool A_ROWS, bool B_ROWS, bool DIRECT, int E>
+template <class T, int BM, int BN, int WM, int WN, bool A_ROWS, bool B_ROWS, int E>
 int launch_tiles(const args& p, hipStream_t st) {
   const int64_t nt = ceil_div(p.N, BN);
   int64_t mt = ceil_div(p.M, BM), sheets = 1;
@@ -639,23 +741,18 @@ int launch_tiles(const args& p, hipStream_t st) {
   const int64_t many = mt * nt * sheets;
   if (many == 0) return 0;
   DN_CHECK(many < (int64_t)1 << 31, "product of %lld x %lld: too many tiles for one launch", (long long)p.M, (long long)p.N);
-  k_tiles<T, BM, BN, WM, WN, A_ROWS, B_ROWS, DIRECT, E><<<(unsigned)many, WM * WN * 64, 0, st>>>(p);
+  k_tiles<T, BM, BN, WM, WN, A_ROWS, B_ROWS, E><<<(unsigned)many, WM * WN * 64, 0, st>>>(p);
   DN_LAUNCH_CHECK();
   return 0;
 }
 
-// A product whose args are complete but for splits.  ws: room for split_floats (NULL: the reduction is not split).  *_pad:
-// the operand's rows may be read up to the next 16 bytes past their end.  *tile (or NULL): the tiles' width.
+// A product whose args are complete but for splits; its operands lie well, or are packed.  ws: room for split_floats (NULL: the
+// reduction is not split).  *tile (or NULL): the tiles' width.
 template <class T, bool A_ROWS, bool B_ROWS, int E>
-int launch_product(args p, bool a_pad, bool b_pad, float* ws, hipStream_t st, int* tile = nullptr) {
-  constexpr int64_t S = sizeof(T), CH = 16 / S, BK = 128 / S, NEAR = (int64_t)1 << 31;
+int launch_product(args p, float* ws, hipStream_t st, int* tile = nullptr) {
   p.splits = 1;
   p.split_k = p.K;
   p.c_split = 0;
-  const int64_t a_width = A_ROWS ? p.K : p.M, b_width = B_ROWS ? p.K : p.N;
-  const bool direct = fits16(p.A, p.lda, S) && fits16(p.B, p.ldb, S) && (a_pad || a_width % CH == 0) && (b_pad || b_width % CH == 0) &&
-                      (A_ROWS ? 256 : BK) * p.lda * S < NEAR && (B_ROWS ? 256 : BK) * p.ldb * S < NEAR &&
-                      (p.mode != BY_ROWS || p.b_group * S % 16 == 0);
   if constexpr (E == E_LINEAR || E == E_STORE) {
     const plan r = plan_for<T>(p.M, p.N, p.K, ws != nullptr && p.mode == ONE);
     if (r.splits > 1) {
@@ -667,10 +764,7 @@ int launch_product(args p, bool a_pad, bool b_pad, float* ws, hipStream_t st, in
       q.add_sums = 0;
       q.ldc = ceil_div(p.N, 4) * 4;
       q.c_split = p.M * q.ldc;
-      if (direct)
-        DN_TRY((launch_tiles<T, 128, 128, 2, 2, A_ROWS, B_ROWS, true, E_STORE>(q, st)));
-      else
-        DN_TRY((launch_tiles<T, 128, 128, 2, 2, A_ROWS, B_ROWS, false, E_STORE>(q, st)));
+      DN_TRY((launch_tiles<T, 128, 128, 2, 2, A_ROWS, B_ROWS, E_STORE>(q, st)));
       const int64_t many = p.M * ceil_div(p.N, 4);
       k_join<T, E><<<(unsigned)ceil_div(many, 256), 256, 0, st>>>(p, ws, r.splits);
       DN_LAUNCH_CHECK();
@@ -678,21 +772,20 @@ int launch_product(args p, bool a_pad, bool b_pad, float* ws, hipStream_t st, in
     }
   }
   if (tile) *tile = 128;
-  if (!direct) return launch_tiles<T, 128, 128, 2, 2, A_ROWS, B_ROWS, false, E>(p, st);
   if constexpr (sizeof(T) == 2) {
     const int64_t sheets = p.mode == BY_REDUCTION ? p.G.groups : 1;
     if (ceil_div(p.M, 256) * ceil_div(p.N, 256) * sheets >= 200) {
       if (tile) *tile = 256;
-      return launch_tiles<T, 256, 256, 2, 4, A_ROWS, B_ROWS, true, E>(p, st);
+      return launch_tiles<T, 256, 256, 2, 4, A_ROWS, B_ROWS, E>(p, st);
     }
   }
-  return launch_tiles<T, 128, 128, 2, 2, A_ROWS, B_ROWS, true, E>(p, st);
+  return launch_tiles<T, 128, 128, 2, 2, A_ROWS, B_ROWS, E>(p, st);
 }
 
 // (their kernels are in linear.hip)
 #define DN_STORE_PRODUCTS(X, T)                                                              \
-  X template int launch_product<T, true, false, E_STORE>(args, bool, bool, float*, hipStream_t, int*); \
-  X template int launch_product<T, false, false, E_STORE>(args, bool, bool, float*, hipStream_t, int*);
+  X template int launch_product<T, true, false, E_STORE>(args, float*, hipStream_t, int*); \
+  X template int launch_product<T, false, false, E_STORE>(args, float*, hipStream_t, int*);
 
 // Whether rows of `ld` elements from p on can be accessed four values at once.
 template <class T>
@@ -715,8 +808,6 @@ inline int check_array(const char* what, const char* name, const void* p, int64_
   ((type) == DNPEFF_F32   ? [&] { typedef float T; return call; }()     \
    : (type) == DNPEFF_F16 ? [&] { typedef _Float16 T; return call; }()  \
                           : [&] { typedef __bf16 T; return call; }())
-
-inline int64_t round256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
 }  // namespace tl
 }  // namespace dn

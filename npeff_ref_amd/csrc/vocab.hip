@@ -86,36 +86,55 @@ int64_t piece_words(int64_t rows, int64_t words, int size) {
 int64_t padded(int64_t words) { return ceil_div(words, 64) * 64; }
 
 template <class T>
-struct room {
-  int64_t piece, g, sums, parts, all;
-  room(int64_t rows, int64_t n_in, int64_t words) {
+struct loss_room {  // of the forward pass
+  int64_t packs = 0, parts, all;
+  matrix m[2];
+  loss_room(int64_t rows, int64_t n_in, int64_t words, const void* X, int64_t ldx, const void* E, int64_t lde)
+      : m{{X, ldx, rows, n_in, 1, 0}, {E, lde, words, n_in, 1, 0}} {
+    for (const matrix& q : m) packs += packed_bytes<T>(q);
+    parts = round256(rows * ceil_div(words, 128) * 8);
+    all = packs + parts + round256(rows * 4);
+  }
+};
+template <class T>
+struct grad_room {
+  int64_t packs = 0, piece, g, sums, parts, all;
+  matrix m[2];
+  grad_room(int64_t rows, int64_t n_in, int64_t words, const void* X, int64_t ldx, const void* E, int64_t lde)
+      : m{{X, ldx, rows, n_in, 1, 0}, {E, lde, words, n_in, 1, 0}} {
+    for (const matrix& q : m) packs += packed_bytes<T>(q);
     piece = piece_words(rows, words, sizeof(T));
     g = round256(rows * padded(piece) * (int64_t)sizeof(T));
     sums = piece < words ? round256(rows * (ceil_div(n_in, 4) * 4) * 4) : 0;
-    const int64_t x = split_floats<T>(rows, n_in, piece), e = split_floats<T>(piece, n_in, rows);
     const int64_t last = words - (ceil_div(words, piece) - 1) * piece;
-    const int64_t x1 = split_floats<T>(rows, n_in, last), e1 = split_floats<T>(last, n_in, rows);
-    int64_t most = x > e ? x : e;
-    if (x1 > most) most = x1;
-    if (e1 > most) most = e1;
-    parts = round256(4 * most);
-    all = 256 + g + sums + parts;
+    parts = 0;
+    for (int64_t n : {piece, last})
+      for (int64_t f : {split_floats<T>(rows, n_in, n), split_floats<T>(n, n_in, rows)})
+        if (round256(4 * f) > parts) parts = round256(4 * f);
+    all = 256 + packs + g + sums + parts;
   }
 };
-int64_t forward_bytes_of(int64_t rows, int64_t words) { return round256(rows * ceil_div(words, 128) * 8) + round256(rows * 4); }
+int check_room(const char* what, int64_t need, const void* ws, int64_t bytes) {
+  DN_CHECK(ws != nullptr && bytes >= need && (uintptr_t)ws % 16 == 0, "%s: a workspace of %lld bytes, aligned to 16, is needed", what,
+           (long long)need);
+  return 0;
+}
 
 template <class T>
 int loss_forward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, const void* X, int64_t ldx, const void* E, int64_t lde,
-                 const int32_t* labels, float* loss, float* lse, char* ws) {
+                 const int32_t* labels, float* loss, float* lse, char* ws, int64_t ws_bytes) {
+  loss_room<T> room(rows, n_in, words, X, ldx, E, lde);
+  DN_TRY(check_room("dnpeff_vocab_loss", room.all, ws, ws_bytes));
+  DN_TRY(pack<T>(room.m, 2, ws, st));
   args p{};
-  p.A = X, p.lda = ldx, p.B = E, p.ldb = lde;
+  p.A = room.m[0].p, p.lda = room.m[0].ld, p.B = room.m[1].p, p.ldb = room.m[1].ld;
   p.M = rows, p.N = words, p.K = n_in;
   p.mode = ONE;
   p.labels = labels, p.words = words, p.word0 = 0;
-  p.parts = (float2*)ws;
-  p.hit = (float*)(ws + round256(rows * ceil_div(words, 128) * 8));
+  p.parts = (float2*)(ws + room.packs);
+  p.hit = (float*)(ws + room.packs + room.parts);
   int tile = 0;
-  DN_TRY((launch_product<T, true, true, E_LOSS>(p, false, false, nullptr, st, &tile)));
+  DN_TRY((launch_product<T, true, true, E_LOSS>(p, nullptr, st, &tile)));
   k_join_loss<<<(unsigned)ceil_div(rows, 4), 256, 0, st>>>(rows, (int)ceil_div(words, tile), p.parts, p.hit, labels, words, loss, lse);
   DN_LAUNCH_CHECK();
   return 0;
@@ -123,10 +142,14 @@ int loss_forward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, cons
 
 template <class T>
 int loss_backward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, const void* X, int64_t ldx, const void* E, int64_t lde,
-                  const int32_t* labels, const float* lse, const float* dloss, void* dX, int64_t lddx, void* dE, int64_t ldde, char* ws) {
-  const room<T> r(rows, n_in, words);
+                  const int32_t* labels, const float* lse, const float* dloss, void* dX, int64_t lddx, void* dE, int64_t ldde, char* ws,
+                  int64_t ws_bytes) {
+  grad_room<T> r(rows, n_in, words, X, ldx, E, lde);
+  DN_TRY(check_room("dnpeff_vocab_loss_backward", r.all, ws, ws_bytes));
   float* both = (float*)ws;
-  char* g = ws + 256;
+  ws += 256;
+  DN_TRY(pack<T>(r.m, 2, ws, st));
+  char* g = ws + r.packs;
   float* sums = (float*)(g + r.g);
   float* parts = r.parts ? (float*)(g + r.g + r.sums) : nullptr;
   const float *shrink = nullptr, *grow = nullptr;
@@ -137,33 +160,33 @@ int loss_backward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, con
   }
   for (int64_t w0 = 0; w0 < words; w0 += r.piece) {
     const int64_t n = words - w0 < r.piece ? words - w0 : r.piece;
-    const T* Ep = (const T*)E + w0 * lde;
+    const T* Ep = (const T*)r.m[1].p + w0 * r.m[1].ld;
     const bool first = w0 == 0, last = w0 + n == words;
     args p{};
-    p.A = X, p.lda = ldx, p.B = Ep, p.ldb = lde;
+    p.A = r.m[0].p, p.lda = r.m[0].ld, p.B = Ep, p.ldb = r.m[1].ld;
     p.M = rows, p.N = n, p.K = n_in;
     p.mode = ONE;
     p.labels = labels, p.lse = lse, p.dloss = dloss, p.shrink = shrink, p.word0 = w0, p.words = words;
     p.out = g, p.ldc = padded(n);
-    DN_TRY((launch_product<T, true, true, E_LOSS_GRAD>(p, false, false, nullptr, st)));
+    DN_TRY((launch_product<T, true, true, E_LOSS_GRAD>(p, nullptr, st)));
     if (dX) {
       args q{};
-      q.A = g, q.lda = padded(n), q.B = Ep, q.ldb = lde;
+      q.A = g, q.lda = padded(n), q.B = Ep, q.ldb = r.m[1].ld;
       q.M = rows, q.N = n_in, q.K = n;
       q.mode = ONE;
       q.sums = first && last ? nullptr : sums, q.add_sums = !first;
       q.ldc = ceil_div(n_in, 4) * 4;
       if (last) q.out = dX, q.ldo = lddx, q.wide = fours<T>(dX, lddx), q.scale = grow;
-      DN_TRY((launch_product<T, true, false, E_STORE>(q, true, false, parts, st)));
+      DN_TRY((launch_product<T, true, false, E_STORE>(q, parts, st)));
     }
     if (dE) {
       args q{};
-      q.A = g, q.lda = padded(n), q.B = X, q.ldb = ldx;
+      q.A = g, q.lda = padded(n), q.B = r.m[0].p, q.ldb = r.m[0].ld;
       q.M = n, q.N = n_in, q.K = rows;
       q.mode = ONE;
       T* to = (T*)dE + w0 * ldde;
       q.out = to, q.ldo = ldde, q.wide = fours<T>(to, ldde), q.scale = grow;
-      DN_TRY((launch_product<T, false, false, E_STORE>(q, true, false, parts, st)));
+      DN_TRY((launch_product<T, false, false, E_STORE>(q, parts, st)));
     }
   }
   return 0;
@@ -178,11 +201,13 @@ int check_head(const char* me, int type, int64_t rows, int64_t n_in, int64_t wor
 
 }  // namespace
 
-DN_API int dnpeff_vocab_loss_workspace(int type, int64_t rows, int64_t n_in, int64_t n_words, int64_t* forward_bytes, int64_t* backward_bytes) {
+DN_API int dnpeff_vocab_loss_workspace(int type, int64_t rows, int64_t n_in, int64_t n_words, int aligned, int64_t* forward_bytes,
+                                       int64_t* backward_bytes) {
   clear_error();
   DN_TRY(check_head("dnpeff_vocab_loss_workspace", type, rows, n_in, n_words));
-  if (forward_bytes) *forward_bytes = forward_bytes_of(rows, n_words);
-  if (backward_bytes) *backward_bytes = DN_BY_TYPE(type, (room<T>(rows, n_in, n_words).all));
+  const void* p = (const void*)(uintptr_t)(aligned ? 16 : 1);
+  if (forward_bytes) *forward_bytes = DN_BY_TYPE(type, (loss_room<T>(rows, n_in, n_words, p, n_in, p, n_in).all));
+  if (backward_bytes) *backward_bytes = DN_BY_TYPE(type, (grad_room<T>(rows, n_in, n_words, p, n_in, p, n_in).all));
   return 0;
 }
 
@@ -197,10 +222,8 @@ DN_API int dnpeff_vocab_loss(void* stream, int type, int64_t rows, int64_t n_in,
   DN_TRY(check_array(me, "labels", labels, 1, 1, DNPEFF_F32, false));
   DN_TRY(check_array(me, "loss", loss, 1, 1, DNPEFF_F32, true));
   DN_TRY(check_array(me, "lse", lse, 1, 1, DNPEFF_F32, true));
-  const int64_t need = forward_bytes_of(rows, n_words);
-  DN_CHECK(workspace != nullptr && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0,
-           "%s: a workspace of %lld bytes, aligned to 16, is needed", me, (long long)need);
-  return DN_BY_TYPE(type, loss_forward<T>((hipStream_t)stream, rows, n_in, n_words, X, ldx, E, lde, labels, loss, lse, (char*)workspace));
+  return DN_BY_TYPE(type, loss_forward<T>((hipStream_t)stream, rows, n_in, n_words, X, ldx, E, lde, labels, loss, lse, (char*)workspace,
+                                          workspace_bytes));
 }
 
 DN_API int dnpeff_vocab_loss_backward(void* stream, int type, int64_t rows, int64_t n_in, int64_t n_words, const void* X, int64_t ldx,
@@ -216,9 +239,6 @@ DN_API int dnpeff_vocab_loss_backward(void* stream, int type, int64_t rows, int6
   DN_TRY(check_array(me, "dloss", dloss, 1, 1, DNPEFF_F32, rows == 0));
   DN_TRY(check_array(me, "dX", dX, lddx, n_in, type, true));
   DN_TRY(check_array(me, "dE", dE, ldde, n_in, type, true));
-  const int64_t need = DN_BY_TYPE(type, (room<T>(rows, n_in, n_words).all));
-  DN_CHECK(workspace != nullptr && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0,
-           "%s: a workspace of %lld bytes, aligned to 16, is needed", me, (long long)need);
   return DN_BY_TYPE(type, loss_backward<T>((hipStream_t)stream, rows, n_in, n_words, X, ldx, E, lde, labels, lse, dloss, dX, lddx, dE,
-                                           ldde, (char*)workspace));
+                                           ldde, (char*)workspace, workspace_bytes));
 }
