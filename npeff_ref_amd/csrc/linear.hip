@@ -19,49 +19,69 @@ DN_STORE_PRODUCTS(, __bf16)
 
 namespace {
 
-constexpr int DZ_ROWS = 128;  // rows of a group that one workgroup of k_slopes takes
-constexpr int DZ_COLS = 256;  // (a lane: four columns; a wave: every fourth row)
+constexpr int DZ_ROWS = 64;  // rows of a group that one workgroup of k_slopes takes: a wave every fourth of them
 
-// dZ = dY act'(Z), and the column sums of each tile of rows.
+// dZ = dY act'(Z), and the column sums of each tile of rows.  A lane has 16 bytes of each row where the rows allow it
+// (wide), else as many values 64 columns apart.
 template <class T>
 __global__ __launch_bounds__(256) void k_slopes(group_rows G, int64_t N, const T* dY, int64_t ldy, const T* Z, int64_t ldz, int act, T* dZ,
                                                 int64_t ldd, float* sums, int wide) {
   constexpr bool EXACT = sizeof(T) == 4;
+  constexpr int W = 16 / sizeof(T);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int group, within;
   group_of_tile(G, DZ_ROWS, lane, blockIdx.x, &group, &within);
   if (group < 0) return;
   const int64_t m0 = G.first(group) + (int64_t)within * DZ_ROWS, m_end = G.last(group);
   const bool held = group < G.groups;
-  const int64_t n = (int64_t)blockIdx.y * DZ_COLS + lane * 4;
-  const int there = n < N ? (int)(N - n < 4 ? N - n : 4) : 0;
-  const bool whole = wide && there == 4;
-  v4f sum = {0.f, 0.f, 0.f, 0.f};
-  if (there > 0 || (dZ && n < ldd)) {  // (columns of dZ past the last of dY: zero)
-#pragma unroll 4
-    for (int r = wave; r < DZ_ROWS; r += 4) {
-      const int64_t m = m0 + r;
-      if (m >= m_end) break;
-      v4f g = {0.f, 0.f, 0.f, 0.f};
-      if (held) {
-        g = load4(dY + m * ldy + n, whole, there);
-        if (act != DNPEFF_ACT_NONE) {
-          const v4f z = load4(Z + m * ldz + n, whole, there);
+  const int64_t n0 = (int64_t)blockIdx.y * (64 * W) + (wide ? lane * W : lane);
+  const int step = wide ? 1 : 64;  // (columns of dZ past the last of dY: zero)
+  float sum[W];
 #pragma unroll
-          for (int t = 0; t < 4; t++) g[t] *= slope_of<EXACT>(z[t], act);
-        }
+  for (int t = 0; t < W; t++) sum[t] = 0.f;
+#pragma unroll 4
+  for (int r = wave; r < DZ_ROWS; r += 4) {
+    const int64_t m = m0 + r;
+    if (m >= m_end) break;
+    float g[W], z[W];
+#pragma unroll
+    for (int t = 0; t < W; t++) g[t] = z[t] = 0.f;
+    if (held && wide) {
+      if (n0 < N) {
+        load_row<T, W>(dY + m * ldy + n0, g);
+        if (act != DNPEFF_ACT_NONE) load_row<T, W>(Z + m * ldz + n0, z);
       }
-      if (dZ) store4(dZ + m * ldd + n, g, true, 4);
-      sum += g;
+    } else if (held) {
+#pragma unroll
+      for (int t = 0; t < W; t++)
+        if (n0 + t * 64 < N) {
+          g[t] = (float)dY[m * ldy + n0 + t * 64];
+          if (act != DNPEFF_ACT_NONE) z[t] = (float)Z[m * ldz + n0 + t * 64];
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < W; t++) {
+      g[t] *= slope_of<EXACT>(z[t], act);
+      sum[t] += g[t];
+    }
+    if (dZ && wide) {
+      if (n0 < ldd) store_row<T, W>(dZ + m * ldd + n0, g);
+    } else if (dZ) {
+#pragma unroll
+      for (int t = 0; t < W; t++)
+        if (n0 + t * 64 < ldd) dZ[m * ldd + n0 + t * 64] = (T)g[t];
     }
   }
   if (!sums) return;
-  __shared__ v4f side[4][64];
-  side[wave][lane] = sum;
+  __shared__ float side[4][W][64];
+#pragma unroll
+  for (int t = 0; t < W; t++) side[wave][t][lane] = sum[t];
   __syncthreads();
-  if (wave == 0 && there > 0) {
-    const v4f s = (side[0][lane] + side[1][lane]) + (side[2][lane] + side[3][lane]);
-    store4(sums + blockIdx.x * N + n, s, N % 4 == 0, there);
+  if (wave == 0) {
+#pragma unroll
+    for (int t = 0; t < W; t++)
+      if (n0 + t * step < N)
+        sums[blockIdx.x * N + n0 + t * step] = (side[0][t][lane] + side[1][t][lane]) + (side[2][t][lane] + side[3][t][lane]);
   }
 }
 
@@ -79,6 +99,7 @@ __global__ __launch_bounds__(256) void k_bias_sums(group_rows G, int64_t N, cons
   const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (n >= N) return;
   float s = 0.f;
+#pragma unroll 8
   for (int t = 0; t < tiles; t++) s += sums[(int64_t)(before + t) * N + n];
   db[g * N + n] = (T)s;
 }
@@ -176,7 +197,7 @@ int forward(hipStream_t st, const layer& l, const void* X, int64_t ldx, const vo
   p.mode = l.grouped() ? BY_ROWS : ONE;
   p.G = rows_of(l);
   p.out = Y, p.ldc = ldy, p.pre = pre, p.ldp = ldp, p.residual = residual, p.ldr = ldr, p.bias = bias, p.act = act;
-  p.wide = fours<T>(Y, ldy) && fours<T>(pre, ldp) && fours<T>(residual, ldr) && fours<T>(bias, l.n_out);
+  p.wide = wide<T>(Y, ldy) && wide<T>(pre, ldp) && wide<T>(residual, ldr) && wide<T>(bias, l.n_out);
   return launch_product<T, true, true, E_LINEAR>(p, room.parts ? (float*)(ws + room.packs) : nullptr, st);
 }
 
@@ -195,10 +216,11 @@ int backward(hipStream_t st, const layer& l, const void* dY, int64_t lddy, const
   at += room.sums;
   float* parts = room.parts ? (float*)at : nullptr;
   if ((dz || dbias) && l.rows > 0) {
-    const bool wide = fours<T>(dY, lddy) && (act == DNPEFF_ACT_NONE || fours<T>(pre, ldp));
-    const dim3 grid((unsigned)slope_tiles(l.rows, G.groups), (unsigned)ceil_div(l.n_out, DZ_COLS));
+    constexpr int W = 16 / sizeof(T);
+    const bool whole = l.n_out % W == 0 && wide<T>(dY, lddy) && (act == DNPEFF_ACT_NONE || wide<T>(pre, ldp));
+    const dim3 grid((unsigned)slope_tiles(l.rows, G.groups), (unsigned)ceil_div(l.n_out, 64 * W));
     DN_CHECK(grid.y <= 65535, "dnpeff_linear_backward: n_out = %lld is too wide for one launch", (long long)l.n_out);
-    k_slopes<T><<<grid, 256, 0, st>>>(G, l.n_out, (const T*)dY, lddy, (const T*)pre, ldp, act, dz, packed_ld<T>(l.n_out), sums, wide);
+    k_slopes<T><<<grid, 256, 0, st>>>(G, l.n_out, (const T*)dY, lddy, (const T*)pre, ldp, act, dz, packed_ld<T>(l.n_out), sums, whole);
     DN_LAUNCH_CHECK();
   }
   if (dbias) {
@@ -214,7 +236,7 @@ int backward(hipStream_t st, const layer& l, const void* dY, int64_t lddy, const
     p.M = l.rows, p.N = l.n_in, p.K = l.n_out;
     p.mode = l.grouped() ? BY_ROWS : ONE;
     p.G = G;
-    p.out = dX, p.ldo = lddx, p.wide = fours<T>(dX, lddx);
+    p.out = dX, p.ldo = lddx, p.wide = wide<T>(dX, lddx);
     DN_TRY((launch_product<T, true, false, E_STORE>(p, parts, st)));
   }
   if (dW) {
@@ -223,7 +245,7 @@ int backward(hipStream_t st, const layer& l, const void* dY, int64_t lddy, const
     p.M = l.n_out, p.N = l.n_in, p.K = l.rows;
     p.mode = l.grouped() ? BY_REDUCTION : ONE;
     p.G = G;
-    p.out = dW, p.ldo = lddw, p.c_group = dw_group, p.wide = fours<T>(dW, lddw) && dw_group % 4 == 0;
+    p.out = dW, p.ldo = lddw, p.c_group = dw_group, p.wide = wide<T>(dW, lddw) && dw_group * (int64_t)sizeof(T) % 16 == 0;
     DN_TRY((launch_product<T, false, false, E_STORE>(p, parts, st)));
   }
   return 0;
@@ -241,7 +263,7 @@ int example_grads(hipStream_t st, const layer& l, const void* dY, int64_t lddy, 
   p.mode = BY_REDUCTION;
   p.G = rows_of(l);
   p.out = out, p.out_f32 = 1, p.square = square, p.ldo = l.n_in, p.c_group = l.n_out * l.n_in;
-  p.wide = fours<float>(out, l.n_in);
+  p.wide = wide<float>(out, l.n_in);
   return launch_product<T, false, false, E_STORE>(p, nullptr, st);
 }
 

@@ -26,9 +26,7 @@ namespace tl {
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
-typedef __bf16 v4b __attribute__((ext_vector_type(4)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-typedef _Float16 v4h __attribute__((ext_vector_type(4)));
 typedef short v4s __attribute__((ext_vector_type(4)));
 
 #define DN_LDS __attribute__((address_space(3)))
@@ -43,17 +41,14 @@ struct num;
 template <>
 struct num<float> {
   typedef v4f piece;  // 16 bytes of the reduction index of one row, as a lane holds them
-  typedef v4f four;
 };
 template <>
 struct num<_Float16> {
   typedef v8h piece;
-  typedef v4h four;
 };
 template <>
 struct num<__bf16> {
   typedef v8b piece;
-  typedef v4b four;
 };
 
 __device__ __forceinline__ v4f mma(v8b a, v8b b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -63,35 +58,6 @@ __device__ __forceinline__ v4f mma(v4f a, v4f b, v4f c) {
 #pragma unroll
   for (int e = 0; e < 4; e++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
   return c;
-}
-
-// Four consecutive values of a row; those from `there` on are not touched (read as zero).
-template <class T>
-__device__ __forceinline__ v4f load4(const T* p, bool whole, int there) {
-  v4f v = {0.f, 0.f, 0.f, 0.f};
-  if (whole) {
-    const typename num<T>::four q = *(const typename num<T>::four*)p;
-#pragma unroll
-    for (int t = 0; t < 4; t++) v[t] = (float)q[t];
-  } else {
-#pragma unroll
-    for (int t = 0; t < 4; t++)
-      if (t < there) v[t] = (float)p[t];
-  }
-  return v;
-}
-template <class T>
-__device__ __forceinline__ void store4(T* p, v4f v, bool whole, int there) {
-  if (whole) {
-    typename num<T>::four q;
-#pragma unroll
-    for (int t = 0; t < 4; t++) q[t] = (T)v[t];
-    *(typename num<T>::four*)p = q;
-  } else {
-#pragma unroll
-    for (int t = 0; t < 4; t++)
-      if (t < there) p[t] = (T)v[t];
-  }
 }
 
 // ---- activations and their slopes, in fp32 -----------------------------------------------------------------------
@@ -214,7 +180,7 @@ struct args {
   void* out;
   int64_t ldc, ldo;
   const float* scale;
-  int add_sums, out_f32, square, wide;  // wide: the rows of the epilogue's arrays can be accessed four values at once
+  int add_sums, out_f32, square, wide;  // wide: the rows of the epilogue's arrays can be accessed 16 bytes at once
   // E_LINEAR
   const void *bias, *residual;
   void* pre;
@@ -229,47 +195,86 @@ struct args {
   int64_t word0, words;
 };
 
-template <class T>
-__device__ __forceinline__ v4f bias4(const args& p, int64_t n, int group) {
-  const int there = (int)(p.N - n < 4 ? p.N - n : 4);
-  return load4((const T*)p.bias + (int64_t)group * p.N + n, p.wide && there == 4, there);
-}
-// The result for four consecutive n of one m, from the product with the bias added.
-template <class T>
-__device__ __forceinline__ void finish_linear(const args& p, int64_t m, int64_t n, v4f v, bool held) {
-  constexpr bool EXACT = sizeof(T) == 4;
-  const int there = (int)(p.N - n < 4 ? p.N - n : 4);
-  const bool whole = p.wide && there == 4;
-  if (held) {
-    if (p.pre) store4((T*)p.pre + m * p.ldp + n, v, whole, there);
-    if (p.act != DNPEFF_ACT_NONE) {
+// W consecutive values of a row at once, where all of them are there and aligned.
+template <class T, int W>
+__device__ __forceinline__ void load_row(const T* p, float* v) {
+  typedef T piece __attribute__((ext_vector_type(W)));
+  const piece q = *(const piece*)p;
 #pragma unroll
-      for (int t = 0; t < 4; t++) v[t] = act_of<EXACT>(v[t], p.act);
-    }
-  } else {
-    v = v4f{0.f, 0.f, 0.f, 0.f};
-    if (p.pre) store4((T*)p.pre + m * p.ldp + n, v, whole, there);
-  }
-  if (p.residual) v += load4((const T*)p.residual + m * p.ldr + n, whole, there);
-  store4((T*)p.out + m * p.ldc + n, v, whole, there);
+  for (int t = 0; t < W; t++) v[t] = (float)q[t];
 }
-template <class T>
-__device__ __forceinline__ void finish_store(const args& p, int64_t sheet, int64_t m, int64_t n, v4f v) {
-  const int there = (int)(p.N - n < 4 ? p.N - n : 4);
+template <class T, int W>
+__device__ __forceinline__ void store_row(T* p, const float* v) {
+  typedef T piece __attribute__((ext_vector_type(W)));
+  piece q;
+#pragma unroll
+  for (int t = 0; t < W; t++) q[t] = (T)v[t];
+  *(piece*)p = q;
+}
+
+// What becomes of W consecutive values of row m from column n on (all of them there, and aligned for W at once).
+// held: the row belongs to a group (its product counts); bias: of these columns.
+template <class T, int W>
+__device__ __forceinline__ void finish_linear(const args& p, int64_t m, int64_t n, float* v, const float* bias, bool held) {
+  constexpr bool EXACT = sizeof(T) == 4;
+#pragma unroll
+  for (int t = 0; t < W; t++) v[t] = held ? v[t] + bias[t] : 0.f;
+  if (p.pre) store_row<T, W>((T*)p.pre + m * p.ldp + n, v);
+  if (held && p.act != DNPEFF_ACT_NONE) {
+#pragma unroll
+    for (int t = 0; t < W; t++) v[t] = act_of<EXACT>(v[t], p.act);
+  }
+  if (p.residual) {
+    float r[W];
+    load_row<T, W>((const T*)p.residual + m * p.ldr + n, r);
+#pragma unroll
+    for (int t = 0; t < W; t++) v[t] += r[t];
+  }
+  store_row<T, W>((T*)p.out + m * p.ldc + n, v);
+}
+template <class T, int W>
+__device__ __forceinline__ void finish_store(const args& p, int64_t sheet, int64_t m, int64_t n, float* v) {
   const int64_t at = sheet * p.c_split + m * p.ldc + n;
-  if (p.add_sums) v += load4(p.sums + at, true, 4);
+  if (p.add_sums) {
+    float r[W];
+    load_row<float, W>(p.sums + at, r);
+#pragma unroll
+    for (int t = 0; t < W; t++) v[t] += r[t];
+  }
   if (!p.out) {
-    store4(p.sums + at, v, true, 4);
+    store_row<float, W>(p.sums + at, v);
     return;
   }
-  const bool whole = p.wide && there == 4;
   const int64_t to = sheet * p.c_group + m * p.ldo + n;
-  if (p.scale) v *= *p.scale;
-  if (p.square) v *= v;
+  const float s = p.scale ? *p.scale : 1.f;
+#pragma unroll
+  for (int t = 0; t < W; t++) {
+    v[t] *= s;
+    if (p.square) v[t] *= v[t];
+  }
   if (p.out_f32)
-    store4((float*)p.out + to, v, whole, there);
+    store_row<float, W>((float*)p.out + to, v);
   else
-    store4((T*)p.out + to, v, whole, there);
+    store_row<T, W>((T*)p.out + to, v);
+}
+// (softmax - label) times the token's weight; the piece's columns past the last word are zero
+template <class T, int W>
+__device__ __forceinline__ void finish_grad(const args& p, int64_t m, int64_t n, float* v, float shrink) {
+  const int32_t label = p.labels[m];
+  const float lse = p.lse[m], w = label >= p.words ? __builtin_nanf("") : p.dloss[m] * shrink;
+  const int64_t word = p.word0 + n;
+#pragma unroll
+  for (int t = 0; t < W; t++) {
+    const float g = (__expf(v[t] - lse) - (word + t == label ? 1.f : 0.f)) * w;
+    v[t] = n + t < p.N && label >= 0 ? g : 0.f;
+  }
+  store_row<T, W>((T*)p.out + m * p.ldc + n, v);
+}
+template <class T, int W>
+__device__ __forceinline__ void bias_of(const args& p, int64_t n, int group, bool held, float* b) {
+#pragma unroll
+  for (int t = 0; t < W; t++) b[t] = 0.f;
+  if (p.bias && held) load_row<T, W>((const T*)p.bias + (int64_t)group * p.N + n, b);
 }
 
 // A buffer load of 16 bytes per lane to LDS: lane l's go to lds + 16 l.
@@ -520,22 +525,66 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_tiles(args p) {
 
   // -- what becomes of it --
   const int64_t mw = m0 + wm * (BM / WM) + (lane & 15), nw = n0 + wn * (BN / WN) + q * 4;
-  if constexpr (E == E_LINEAR || E == E_STORE) {
+  if constexpr (E != E_LOSS) {
+    // Each wave by itself, 32 of its rows at a time: through LDS, so that its lanes take consecutive values of a row, and
+    // whole lines go out.  Piece c of row r at c ^ (r & 15).
+    constexpr int COLS = BN / WN, W = 16 / sizeof(T);
+    static_assert(COLS == 64, "a row of a wave's part is 16 pieces of 16 bytes");
+    const unsigned mine = base + wave * 8192;
+    const int64_t m_wave = m0 + wm * (BM / WM), n_wave = n0 + wn * COLS;
+    const int64_t n_end = E == E_LOSS_GRAD ? p.ldc : p.N;
+    const bool wide = p.wide && n_wave + COLS <= n_end;
+    const float shrink = E == E_LOSS_GRAD && p.shrink ? *p.shrink : 1.f;
+    float bias[W];
+    if (E == E_LINEAR) {
+      if (wide)
+        bias_of<T, W>(p, n_wave + lane % (COLS / W) * W, group, held, bias);
+      else
+        bias_of<T, 1>(p, n_wave + lane < p.N ? n_wave + lane : p.N - 1, group, held, bias);
+    }
 #pragma unroll
-    for (int j = 0; j < FN; j++) {
-      const int64_t n = nw + j * 16;
-      if (n >= p.N) continue;
-      v4f b4 = {0.f, 0.f, 0.f, 0.f};
-      if (E == E_LINEAR && p.bias && held) b4 = bias4<T>(p, n, group);
+    for (int i0 = 0; i0 < FM; i0 += 2) {
 #pragma unroll
-      for (int i = 0; i < FM; i++) {
-        const int64_t m = mw + i * 16;
-        if (m >= m_end) continue;
-        if constexpr (E == E_LINEAR)
-          finish_linear<T>(p, m, n, acc[i][j] + b4, held);
-        else
-          finish_store<T>(p, sheet, m, n, acc[i][j]);
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int j = 0; j < FN; j++) *lds_at<v4f>(mine + (i * 16 + (lane & 15)) * 256 + (((j * 4 + q) ^ (lane & 15)) << 4)) = acc[i0 + i][j];
+      asm volatile("" ::: "memory");  // (a wave's LDS accesses happen in their order: the compiler is to keep it too)
+      const int64_t m_top = m_wave + i0 * 16;
+      if (wide) {
+        constexpr int PER_ROW = COLS / W, STEP = 64 / PER_ROW;
+#pragma unroll
+        for (int r0 = 0; r0 < 32; r0 += STEP) {
+          const int r = r0 + lane / PER_ROW, c = lane % PER_ROW * (W / 4);
+          float v[W];
+#pragma unroll
+          for (int h = 0; h < W / 4; h++) {
+            const v4f x = *lds_at<v4f>(mine + r * 256 + (((c + h) ^ (r & 15)) << 4));
+#pragma unroll
+            for (int t = 0; t < 4; t++) v[h * 4 + t] = x[t];
+          }
+          if (m_top + r < m_end) {
+            if constexpr (E == E_LINEAR)
+              finish_linear<T, W>(p, m_top + r, n_wave + c * 4, v, bias, held);
+            else if constexpr (E == E_LOSS_GRAD)
+              finish_grad<T, W>(p, m_top + r, n_wave + c * 4, v, shrink);
+            else
+              finish_store<T, W>(p, sheet, m_top + r, n_wave + c * 4, v);
+          }
+        }
+      } else if (E != E_LOSS_GRAD) {  // (a row of g is whole waves' parts)
+        const int64_t n = n_wave + lane;
+#pragma unroll 4
+        for (int r = 0; r < 32; r++) {
+          float v = *lds_at<float>(mine + r * 256 + (((lane >> 2) ^ (r & 15)) << 4) + (lane & 3) * 4);
+          if (m_top + r < m_end && n < p.N) {
+            if constexpr (E == E_LINEAR)
+              finish_linear<T, 1>(p, m_top + r, n, &v, bias, held);
+            else if constexpr (E == E_STORE)
+              finish_store<T, 1>(p, sheet, m_top + r, n, &v);
+          }
+        }
       }
+      asm volatile("" ::: "memory");
     }
   } else if constexpr (E == E_LOSS) {
     // The maximum and the sum of exponentials of the tile's words for every row: over the lane's own, the four
@@ -581,48 +630,42 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_tiles(args p) {
       }
       p.parts[(m0 + m) * nt + tn] = float2{top, sum};
     }
+  }
+}
+
+// ---- host --------------------------------------------------------------------------------------------------------
+// Partial sums of a split reduction, added in their order, then as the tiles' own epilogue.
+template <class T, int E>
+__global__ __launch_bounds__(256) void k_join(args p, const float* parts, int splits) {
+  const int64_t row = (p.N + 3) / 4 * 4, per_row = row / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= p.M * per_row) return;
+  const int64_t m = i / per_row, n = i % per_row * 4;
+  v4f v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < splits; s++) v += *(const v4f*)(parts + ((int64_t)s * p.M + m) * row + n);
+  float x[4] = {v[0], v[1], v[2], v[3]}, b[4];
+  if (p.wide && n + 4 <= p.N) {
+    if constexpr (E == E_LINEAR) {
+      bias_of<T, 4>(p, n, 0, true, b);
+      finish_linear<T, 4>(p, m, n, x, b, true);
+    } else {
+      finish_store<T, 4>(p, 0, m, n, x);
+    }
   } else {
-    // (softmax - label) times the token's weight; the piece's columns past the last word are zero
-    const float shrink = p.shrink ? *p.shrink : 1.f;
 #pragma unroll
-    for (int i = 0; i < FM; i++) {
-      const int64_t m = mw + i * 16;
-      if (m >= m_end) continue;
-      const int32_t label = p.labels[m];
-      const float lse = p.lse[m];
-      const float w = label < 0 ? 0.f : label >= p.words ? __builtin_nanf("") : p.dloss[m] * shrink;
-#pragma unroll
-      for (int j = 0; j < FN; j++) {
-        const int64_t n = nw + j * 16;
-        if (n >= p.ldc) continue;
-        v4f g;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          float v = __expf(acc[i][j][e] - lse) - (p.word0 + n + e == label ? 1.f : 0.f);
-          g[e] = n + e < p.N && label >= 0 ? v * w : 0.f;
-        }
-        store4((T*)p.out + m * p.ldc + n, g, true, 4);
+    for (int t = 0; t < 4; t++) {
+      if (n + t >= p.N) break;
+      if constexpr (E == E_LINEAR) {
+        bias_of<T, 1>(p, n + t, 0, true, b);
+        finish_linear<T, 1>(p, m, n + t, x + t, b, true);
+      } else {
+        finish_store<T, 1>(p, 0, m, n + t, x + t);
       }
     }
   }
 }
 
 inline int64_t round256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
-
-// ---- host --------------------------------------------------------------------------------------------------------
-// Partial sums of a split reduction, added in their order, then as the tiles' own epilogue.
-template <class T, int E>
-__global__ void k_join(args p, const float* parts, int splits) {
-  const int64_t n4 = (p.N + 3) / 4, i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= p.M * n4) return;
-  const int64_t m = i / n4, n = i % n4 * 4, row = n4 * 4;
-  v4f v = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < splits; s++) v += *(const v4f*)(parts + ((int64_t)s * p.M + m) * row + n);
-  if constexpr (E == E_LINEAR)
-    finish_linear<T>(p, m, n, p.bias ? v + bias4<T>(p, n, 0) : v, true);
-  else
-    finish_store<T>(p, 0, m, n, v);
-}
 
 // How a product is run.  Tiles of 256 x 256 (eight waves, one workgroup per CU) where they fill the chip, else of
 // 128 x 128 (four waves, two per CU), the reduction of those split over workgroups where they are few.
@@ -764,6 +807,7 @@ int launch_product(args p, float* ws, hipStream_t st, int* tile = nullptr) {
       q.add_sums = 0;
       q.ldc = ceil_div(p.N, 4) * 4;
       q.c_split = p.M * q.ldc;
+      q.wide = 1;
       DN_TRY((launch_tiles<T, 128, 128, 2, 2, A_ROWS, B_ROWS, E_STORE>(q, st)));
       const int64_t many = p.M * ceil_div(p.N, 4);
       k_join<T, E><<<(unsigned)ceil_div(many, 256), 256, 0, st>>>(p, ws, r.splits);
@@ -787,10 +831,10 @@ int launch_product(args p, float* ws, hipStream_t st, int* tile = nullptr) {
   X template int launch_product<T, true, false, E_STORE>(args, float*, hipStream_t, int*); \
   X template int launch_product<T, false, false, E_STORE>(args, float*, hipStream_t, int*);
 
-// Whether rows of `ld` elements from p on can be accessed four values at once.
+// Whether rows of `ld` elements from p on can be accessed 16 bytes at once (T of 16 bits: eight values).
 template <class T>
-inline bool fours(const void* p, int64_t ld) {
-  return p == nullptr || ((uintptr_t)p % (4 * sizeof(T)) == 0 && ld % 4 == 0);
+inline bool wide(const void* p, int64_t ld) {
+  return p == nullptr || ((uintptr_t)p % 16 == 0 && ld * (int64_t)sizeof(T) % 16 == 0);
 }
 
 // ---- checks of arguments -----------------------------------------------------------------------------------------
