@@ -295,13 +295,14 @@ struct operand {
   static constexpr int S = sizeof(T), CH = 16 / S, BK = 128 / S;
   static constexpr int PER_ROW = ROWS_OF_K ? 8 : R * S / 16;  // pieces in a row
   static constexpr int N = R * 8 / THREADS, ROWS = 64 / PER_ROW;
-  static_assert(N == 4, "two offsets serve four loads");
+  static_assert(N == 2 || N == 4, "two offsets serve all loads");
   static constexpr bool ODD = ROWS_OF_K || ROWS == 2 && S == 2;  // loads 0, 2 and 1, 3 are alike (else 0, 1 and 2, 3)
   static constexpr int NOWHERE = (int)0x80000000u;
   int64_t at, end;  // addresses: this wave's first row of the next tile, the operand's end
   int64_t step;     // bytes from a tile to the next
   int next;         // bytes from a load to the next
   int offset[2], k[2];  // k: (rows of k) a lane's place in the reduction
+  int room, now[2];
 
   __device__ static __forceinline__ int swizzle(int row) {
     if (ROWS_OF_K) return (row >> 1) & 7;
@@ -319,31 +320,26 @@ struct operand {
     next = __builtin_amdgcn_readfirstlane((int)(ROWS * ld));
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-      const int row = (wave * N + (ODD ? h : 2 * h)) * ROWS + lane / PER_ROW, c = (lane % PER_ROW) ^ swizzle(row);
+      const int row = (wave * N + (N == 2 || ODD ? h : 2 * h)) * ROWS + lane / PER_ROW, c = (lane % PER_ROW) ^ swizzle(row);
       offset[h] = (int)(lane / PER_ROW * ld) + c * 16;
       k[h] = c * CH;
     }
   }
-  // left: what is left of the reduction.
-  __device__ __forceinline__ void fill(unsigned lds, int64_t left, int tid) {
-    const unsigned to = lds + __builtin_amdgcn_readfirstlane(tid >> 6) * (N * 1024);
-    int64_t room = end - at;
-    room = room < 0 ? 0 : room > 0x7fffffff ? 0x7fffffff : room;
-    int o[2] = {offset[0], offset[1]};
-    if (ROWS_OF_K && left < BK) {
+  // A stage's loads, one by one: begin() says how much of the reduction is left (or nothing: zeros), load() makes the e-th
+  // of N, end_stage() goes on to the next.
+  __device__ __forceinline__ void begin(int left) {
+    int64_t r = end - at;
+    room = r < 0 ? 0 : r > 0x7fffffff ? 0x7fffffff : (int)r;
 #pragma unroll
-      for (int h = 0; h < 2; h++) o[h] = k[h] < (int)left ? o[h] : NOWHERE;
-    }
-    asm volatile("s_nop 4");  // (between a lane's write of an address and the loads)
-#pragma unroll
-    for (int e = 0; e < N; e++) {
-      const uint64_t from = (uint64_t)at + (uint64_t)(unsigned)(e * next);
-      const int size = (int)room - e * next;
-      const v4i buffer = {(int)(unsigned)from, (int)(unsigned)((from >> 32) & 0xffff), size < 0 ? 0 : size, 0x00020000};
-      to_lds(buffer, to + e * 1024, o[ODD ? e & 1 : e >> 1]);
-    }
-    at += step;
+    for (int h = 0; h < 2; h++) now[h] = ROWS_OF_K && k[h] >= left ? NOWHERE : offset[h];
   }
+  __device__ __forceinline__ void load(unsigned to, int e) const {
+    const uint64_t from = (uint64_t)at + (uint64_t)(unsigned)(e * next);
+    const int size = room - e * next;
+    const v4i buffer = {(int)(unsigned)from, (int)(unsigned)((from >> 32) & 0xffff), size < 0 ? 0 : size, 0x00020000};
+    to_lds(buffer, to + e * 1024, now[N == 2 || ODD ? e & 1 : e >> 1]);
+  }
+  __device__ __forceinline__ void end_stage() { at += step; }
 };
 
 // How a lane reads an operand's part of a tile: 16 of its index, `own` + 16 i .. + 15, for 64 bytes of the reduction (the s-th half).
@@ -457,70 +453,80 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_tiles(args p) {
   operand<T, BN, THREADS, B_ROWS> b;
   a.start(A, p.lda, m0, k0, k_end, m_there, tid);
   b.start(B, p.ldb, n0, k0, k_end, n_there, tid);
-  // Two stages of 128 bytes of the reduction each.  A lane's operands of one half of a stage are read while the matrix
-  // cores work on the other half's; once the second half's are read a stage is free, and takes the tile after the next.
+  // Two stages of 128 bytes of the reduction each, in two halves.  A lane's operands of one half are read while the matrix
+  // cores work on the other's; once everyone has read the second half, the stage takes the one after the next, load by load
+  // between products: nothing but the barrier keeps the matrix cores waiting.  Stages past the end are zeros.
   int64_t left = uniform(k_end - k0);
   if (left > 0) {
-    a.fill(base, left, tid);
-    b.fill(base + BM * 128, left, tid);
-    if (left > BK) {
-      a.fill(base + STAGE, left - BK, tid);
-      b.fill(base + STAGE + BM * 128, left - BK, tid);
-      wait_loads<N_LOADS>();
-    } else {
-      wait_loads<0>();
-    }
-    typename num<T>::piece fa[2][FM], fb[2][FN];
-    unsigned here = base, there = base + STAGE;
     reader<T, BM, A_ROWS> ra;
     reader<T, BN, B_ROWS> rb;
     ra.start(wm * (BM / WM), lane);
     rb.start(wn * (BN / WN), lane);
-    auto read = [&](unsigned stage, int s) {
-#pragma unroll
-      for (int j = 0; j < FN; j++) fb[s][j] = rb.read(stage + BM * 128, j, s);
-#pragma unroll
-      for (int i = 0; i < FM; i++) fa[s][i] = ra.read(stage, i, s);
+    constexpr int LA = operand<T, BM, THREADS, A_ROWS>::N, LB = operand<T, BN, THREADS, B_ROWS>::N;
+    auto begin = [&](int64_t l) {
+      const int to_go = l < 0 ? 0 : l > BK ? BK : (int)l;
+      a.begin(to_go);
+      b.begin(to_go);
     };
-    auto multiply = [&](int s) {
-#pragma unroll
-      for (int i = 0; i < FM; i++)
-#pragma unroll
-        for (int j = 0; j < FN; j++) acc[i][j] = mma(fb[s][j], fa[s][i], acc[i][j]);
+    auto load = [&](unsigned stage, int e) {
+      if (e < LA)
+        a.load(stage + wave * (LA * 1024), e);
+      else if (e < LA + LB)
+        b.load(stage + BM * 128 + wave * (LB * 1024), e - LA);
     };
-    // (reads of the other half between the products, a few ahead: no more registers than that takes)
-    auto mix = [&]() {
-      constexpr int RA = A_ROWS ? 1 : sizeof(T) == 4 ? 4 : 2, RB = B_ROWS ? 1 : sizeof(T) == 4 ? 4 : 2, ONE_MMA = sizeof(T) == 4 ? 4 : 1;
-      constexpr int AHEAD = FM < 3 ? FM : 3;
-      __builtin_amdgcn_sched_group_barrier(0x100, FN * RB + AHEAD * RA, 0);
+    auto end_stage = [&]() {
+      a.end_stage();
+      b.end_stage();
+    };
+#pragma unroll
+    for (int s = 0; s < 2; s++) {
+      begin(left - s * BK);
+      asm volatile("s_nop 4");  // (between a lane's write of an address and the loads)
+#pragma unroll
+      for (int e = 0; e < LA + LB; e++) load(base + s * STAGE, e);
+      end_stage();
+    }
+    wait_loads<N_LOADS>();
+    typename num<T>::piece fa[2][FM], fb[2][FN];
+    auto read = [&](unsigned stage, int s, int r) {
+      if (r < FN)
+        fb[s][r] = rb.read(stage + BM * 128, r, s);
+      else if (r < FN + FM)
+        fa[s][r - FN] = ra.read(stage, r - FN, s);
+    };
+    // The products of half s, row by row, with the reads of the other half in the first rows' company.
+    constexpr int READS = (FN + FM + FM - 3) / (FM - 2), LOADS = (LA + LB + FM - 1) / FM;
+    auto products = [&](unsigned stage, int s, bool loads, unsigned free) {
 #pragma unroll
       for (int i = 0; i < FM; i++) {
-        __builtin_amdgcn_sched_group_barrier(0x008, FN * ONE_MMA, 0);
-        if (i + AHEAD < FM) __builtin_amdgcn_sched_group_barrier(0x100, RA, 0);
+#pragma unroll
+        for (int r = i * READS; r < i * READS + READS; r++) read(stage, 1 - s, r);
+        if (loads) {
+#pragma unroll
+          for (int e = i * LOADS; e < i * LOADS + LOADS; e++) load(free, e);
+        }
+#pragma unroll
+        for (int j = 0; j < FN; j++) acc[i][j] = mma(fb[s][j], fa[s][i], acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
       }
     };
-    read(here, 0);
+    unsigned here = base, there = base + STAGE;
+#pragma unroll
+    for (int r = 0; r < FN + FM; r++) read(here, 0, r);
     while (true) {
-      read(here, 1);
-      multiply(0);
-      mix();
-      __builtin_amdgcn_sched_barrier(0);
+      products(here, 0, false, 0);
       // the next stage has arrived, and everyone has read this one
       wait_loads<0>();
       left -= BK;
-      if (left > BK) {
-        a.fill(here, left - BK, tid);
-        b.fill(here + BM * 128, left - BK, tid);
-      }
-      read(there, 0);  // (after the last stage: of what is there, for nothing)
-      multiply(1);
-      mix();
-      __builtin_amdgcn_sched_barrier(0);
+      begin(left - BK);
+      products(there, 1, true, here);
+      end_stage();
       if (left <= 0) break;
       const unsigned t = here;
       here = there;
       there = t;
     }
+    wait_loads<0>();  // (of zeros)
   }
 
   // -- what becomes of it --
