@@ -59,11 +59,9 @@ __global__ __launch_bounds__(256) void k_slopes(group_rows G, int64_t N, const T
           if (act != DNPEFF_ACT_NONE) z[t] = (float)Z[m * ldz + n0 + t * 64];
         }
     }
+    slopes_of<EXACT, W>(g, z, act);
 #pragma unroll
-    for (int t = 0; t < W; t++) {
-      g[t] *= slope_of<EXACT>(z[t], act);
-      sum[t] += g[t];
-    }
+    for (int t = 0; t < W; t++) sum[t] += g[t];
     if (dZ && wide) {
       if (n0 < ldd) store_row<T, W>(dZ + m * ldd + n0, g);
     } else if (dZ) {

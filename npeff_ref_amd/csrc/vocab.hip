@@ -9,8 +9,6 @@
 // products run on the matrix cores of that type, and the rounding (2^-9 of a value in bf16) is that of the results.
 #include "tiles.hpp"
 
-#include <type_traits>
-
 using namespace dn;
 using namespace dn::tl;
 
