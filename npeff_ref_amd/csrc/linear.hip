@@ -19,56 +19,49 @@ DN_STORE_PRODUCTS(, __bf16)
 
 namespace {
 
-constexpr int DZ_ROWS = 64;  // rows of a group that one workgroup of k_slopes takes: a wave every fourth of them
+// Rows of a group that one workgroup of k_slopes takes (a wave every fourth of them): 64, or 16 where those would leave
+// CUs without work (777 x 515 in fp32: 20 -> SLOPES us).
+int slope_rows(int64_t rows, int64_t n_out, int size) { return ceil_div(rows, 64) * ceil_div(n_out * size, 1024) >= 1024 ? 64 : 16; }
 
-// dZ = dY act'(Z), and the column sums of each tile of rows.  A lane has 16 bytes of each row where the rows allow it
-// (wide), else as many values 64 columns apart.
+// dZ = dY act'(Z), and the column sums of each tile of rows.  A lane has 16 bytes of each row.
 template <class T>
 __global__ __launch_bounds__(256) void k_slopes(group_rows G, int64_t N, const T* dY, int64_t ldy, const T* Z, int64_t ldz, int act, T* dZ,
-                                                int64_t ldd, float* sums, int wide) {
+                                                int64_t ldd, float* sums, int tall) {
   constexpr bool EXACT = sizeof(T) == 4;
   constexpr int W = 16 / sizeof(T);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int group, within;
-  group_of_tile(G, DZ_ROWS, lane, blockIdx.x, &group, &within);
+  group_of_tile(G, tall, lane, blockIdx.x, &group, &within);
   if (group < 0) return;
-  const int64_t m0 = G.first(group) + (int64_t)within * DZ_ROWS, m_end = G.last(group);
+  const int64_t m0 = G.first(group) + (int64_t)within * tall, m_end = G.last(group);
   const bool held = group < G.groups;
-  const int64_t n0 = (int64_t)blockIdx.y * (64 * W) + (wide ? lane * W : lane);
-  const int step = wide ? 1 : 64;  // (columns of dZ past the last of dY: zero)
+  const int64_t n = ((int64_t)blockIdx.y * 64 + lane) * W;
+  const int there = n < N ? (N - n < W ? (int)(N - n) : W) : 0;
   float sum[W];
 #pragma unroll
   for (int t = 0; t < W; t++) sum[t] = 0.f;
 #pragma unroll 4
-  for (int r = wave; r < DZ_ROWS; r += 4) {
+  for (int r = wave; r < tall; r += 4) {
     const int64_t m = m0 + r;
     if (m >= m_end) break;
     float g[W], z[W];
 #pragma unroll
     for (int t = 0; t < W; t++) g[t] = z[t] = 0.f;
-    if (held && wide) {
-      if (n0 < N) {
-        load_row<T, W>(dY + m * ldy + n0, g);
-        if (act != DNPEFF_ACT_NONE) load_row<T, W>(Z + m * ldz + n0, z);
-      }
+    if (held && there == W) {
+      load_row<T, W>(dY + m * ldy + n, g);
+      if (act != DNPEFF_ACT_NONE) load_row<T, W>(Z + m * ldz + n, z);
     } else if (held) {
 #pragma unroll
       for (int t = 0; t < W; t++)
-        if (n0 + t * 64 < N) {
-          g[t] = (float)dY[m * ldy + n0 + t * 64];
-          if (act != DNPEFF_ACT_NONE) z[t] = (float)Z[m * ldz + n0 + t * 64];
+        if (t < there) {
+          g[t] = (float)dY[m * ldy + n + t];
+          if (act != DNPEFF_ACT_NONE) z[t] = (float)Z[m * ldz + n + t];
         }
     }
     slopes_of<EXACT, W>(g, z, act);
 #pragma unroll
     for (int t = 0; t < W; t++) sum[t] += g[t];
-    if (dZ && wide) {
-      if (n0 < ldd) store_row<T, W>(dZ + m * ldd + n0, g);
-    } else if (dZ) {
-#pragma unroll
-      for (int t = 0; t < W; t++)
-        if (n0 + t * 64 < ldd) dZ[m * ldd + n0 + t * 64] = (T)g[t];
-    }
+    if (dZ && n < ldd) store_row<T, W>(dZ + m * ldd + n, g);  // (past the last column: zeros)
   }
   if (!sums) return;
   __shared__ float side[4][W][64];
@@ -78,21 +71,20 @@ __global__ __launch_bounds__(256) void k_slopes(group_rows G, int64_t N, const T
   if (wave == 0) {
 #pragma unroll
     for (int t = 0; t < W; t++)
-      if (n0 + t * step < N)
-        sums[blockIdx.x * N + n0 + t * step] = (side[0][t][lane] + side[1][t][lane]) + (side[2][t][lane] + side[3][t][lane]);
+      if (t < there) sums[blockIdx.x * N + n + t] = (side[0][t][lane] + side[1][t][lane]) + (side[2][t][lane] + side[3][t][lane]);
   }
 }
 
 // db[g] = the sums of the group's tiles, in their order.
 template <class T>
-__global__ __launch_bounds__(256) void k_bias_sums(group_rows G, int64_t N, const float* sums, int tiles_most, T* db) {
+__global__ __launch_bounds__(256) void k_bias_sums(group_rows G, int64_t N, const float* sums, int tall, int tiles_most, T* db) {
   const int lane = threadIdx.x & 63, g = blockIdx.y;
   int before = 0;
   for (int b = 0; b < g; b += 64) {
-    const int t = b + lane < g ? (int)((G.count(b + lane) + DZ_ROWS - 1) / DZ_ROWS) : 0;
+    const int t = b + lane < g ? (int)((G.count(b + lane) + tall - 1) / tall) : 0;
     before += __shfl(wave_scan(t, lane), 63, 64);
   }
-  int tiles = (int)((G.count(g) + DZ_ROWS - 1) / DZ_ROWS);
+  int tiles = (int)((G.count(g) + tall - 1) / tall);
   if (tiles > tiles_most - before) tiles = tiles_most - before;  // (groups that overlap: no more than there were)
   const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (n >= N) return;
@@ -102,7 +94,7 @@ __global__ __launch_bounds__(256) void k_bias_sums(group_rows G, int64_t N, cons
   db[g * N + n] = (T)s;
 }
 
-int64_t slope_tiles(int64_t rows, int groups) { return rows / DZ_ROWS + (groups + 1 < rows ? groups + 1 : rows); }
+int64_t slope_tiles(int64_t rows, int groups, int tall) { return rows / tall + (groups + 1 < rows ? groups + 1 : rows); }
 
 struct layer {
   int64_t rows, n_in, n_out;
@@ -159,7 +151,7 @@ struct backward_room {
     if (dW) m[x = n++] = rows_matrix(l, X, ldx, l.n_in);
     if (dX) m[w = n++] = weight_matrix(l, W, ldw, w_group);
     for (int i = 0; i < n; i++) packs += packed_bytes<T>(m[i]);
-    if (dbias) sums = round256(slope_tiles(l.rows, l.grouped() ? l.groups : 1) * l.n_out * 4);
+    if (dbias) sums = round256(slope_tiles(l.rows, l.grouped() ? l.groups : 1, slope_rows(l.rows, l.n_out, sizeof(T))) * l.n_out * 4);
     if (!l.grouped()) {
       const int64_t a = dX ? split_floats<T>(l.rows, l.n_in, l.n_out) : 0, b = dW ? split_floats<T>(l.n_out, l.n_in, l.rows) : 0;
       parts = round256(4 * (a > b ? a : b));
@@ -195,7 +187,6 @@ int forward(hipStream_t st, const layer& l, const void* X, int64_t ldx, const vo
   p.mode = l.grouped() ? BY_ROWS : ONE;
   p.G = rows_of(l);
   p.out = Y, p.ldc = ldy, p.pre = pre, p.ldp = ldp, p.residual = residual, p.ldr = ldr, p.bias = bias, p.act = act;
-  p.wide = wide<T>(Y, ldy) && wide<T>(pre, ldp) && wide<T>(residual, ldr) && wide<T>(bias, l.n_out);
   return launch_product<T, true, true, E_LINEAR>(p, room.parts ? (float*)(ws + room.packs) : nullptr, st);
 }
 
@@ -213,17 +204,17 @@ int backward(hipStream_t st, const layer& l, const void* dY, int64_t lddy, const
   float* sums = dbias ? (float*)at : nullptr;
   at += room.sums;
   float* parts = room.parts ? (float*)at : nullptr;
+  constexpr int PIECE = 16 / sizeof(T);
+  const int tall = slope_rows(l.rows, l.n_out, sizeof(T));
   if ((dz || dbias) && l.rows > 0) {
-    constexpr int W = 16 / sizeof(T);
-    const bool whole = l.n_out % W == 0 && wide<T>(dY, lddy) && (act == DNPEFF_ACT_NONE || wide<T>(pre, ldp));
-    const dim3 grid((unsigned)slope_tiles(l.rows, G.groups), (unsigned)ceil_div(l.n_out, 64 * W));
+    const dim3 grid((unsigned)slope_tiles(l.rows, G.groups, tall), (unsigned)ceil_div(l.n_out, 64 * PIECE));
     DN_CHECK(grid.y <= 65535, "dnpeff_linear_backward: n_out = %lld is too wide for one launch", (long long)l.n_out);
-    k_slopes<T><<<grid, 256, 0, st>>>(G, l.n_out, (const T*)dY, lddy, (const T*)pre, ldp, act, dz, packed_ld<T>(l.n_out), sums, whole);
+    k_slopes<T><<<grid, 256, 0, st>>>(G, l.n_out, (const T*)dY, lddy, (const T*)pre, ldp, act, dz, packed_ld<T>(l.n_out), sums, tall);
     DN_LAUNCH_CHECK();
   }
   if (dbias) {
-    k_bias_sums<T><<<dim3((unsigned)ceil_div(l.n_out, 256), (unsigned)G.groups), 256, 0, st>>>(G, l.n_out, sums,
-                                                                                               (int)slope_tiles(l.rows, G.groups), (T*)dbias);
+    k_bias_sums<T><<<dim3((unsigned)ceil_div(l.n_out, 256), (unsigned)G.groups), 256, 0, st>>>(G, l.n_out, sums, tall,
+                                                                                               (int)slope_tiles(l.rows, G.groups, tall), (T*)dbias);
     DN_LAUNCH_CHECK();
   }
   const void* g = dz ? dz : room.y >= 0 ? room.m[room.y].p : nullptr;
@@ -234,7 +225,7 @@ int backward(hipStream_t st, const layer& l, const void* dY, int64_t lddy, const
     p.M = l.rows, p.N = l.n_in, p.K = l.n_out;
     p.mode = l.grouped() ? BY_ROWS : ONE;
     p.G = G;
-    p.out = dX, p.ldo = lddx, p.wide = wide<T>(dX, lddx);
+    p.out = dX, p.ldo = lddx;
     DN_TRY((launch_product<T, true, false, E_STORE>(p, parts, st)));
   }
   if (dW) {
@@ -243,7 +234,7 @@ int backward(hipStream_t st, const layer& l, const void* dY, int64_t lddy, const
     p.M = l.n_out, p.N = l.n_in, p.K = l.rows;
     p.mode = l.grouped() ? BY_REDUCTION : ONE;
     p.G = G;
-    p.out = dW, p.ldo = lddw, p.c_group = dw_group, p.wide = wide<T>(dW, lddw) && dw_group * (int64_t)sizeof(T) % 16 == 0;
+    p.out = dW, p.ldo = lddw, p.c_group = dw_group;
     DN_TRY((launch_product<T, false, false, E_STORE>(p, parts, st)));
   }
   return 0;
@@ -261,7 +252,6 @@ int example_grads(hipStream_t st, const layer& l, const void* dY, int64_t lddy, 
   p.mode = BY_REDUCTION;
   p.G = rows_of(l);
   p.out = out, p.out_f32 = 1, p.square = square, p.ldo = l.n_in, p.c_group = l.n_out * l.n_in;
-  p.wide = wide<float>(out, l.n_in);
   return launch_product<T, false, false, E_STORE>(p, nullptr, st);
 }
 

@@ -223,7 +223,7 @@ struct args {
   int64_t ldc, ldo;
   const float* scale;
   int past;  // out is larger than the caches: past them
-  int add_sums, out_f32, square, wide;  // wide: the rows of the epilogue's arrays can be accessed 16 bytes at once
+  int add_sums, out_f32, square;
   // E_LINEAR
   const void *bias, *residual;
   void* pre;
@@ -246,27 +246,28 @@ __device__ __forceinline__ kargs& again() {
   return *p;
 }
 
-// W consecutive values of a row at once, where all of them are there and aligned.
+// W consecutive values of a row at once, wherever they begin: the memory pipe takes any alignment of whole elements
+// (results of 1999 x 4101 in fp16: 68 us value by value, ODDSTORE so).
+template <class T, int W>
+using loose = T __attribute__((ext_vector_type(W), aligned(sizeof(T))));
 template <class T, int W>
 __device__ __forceinline__ void load_row(const T* p, float* v) {
-  typedef T piece __attribute__((ext_vector_type(W)));
-  const piece q = *(const piece*)p;
+  const loose<T, W> q = *(const loose<T, W>*)p;
 #pragma unroll
   for (int t = 0; t < W; t++) v[t] = (float)q[t];
 }
 template <class T, int W>
 __device__ __forceinline__ void store_row(T* p, const float* v, bool past = false) {
-  typedef T piece __attribute__((ext_vector_type(W)));
-  piece q;
+  loose<T, W> q;
 #pragma unroll
   for (int t = 0; t < W; t++) q[t] = (T)v[t];
   if (past)
-    __builtin_nontemporal_store(q, (piece*)p);
+    __builtin_nontemporal_store(q, (loose<T, W>*)p);
   else
-    *(piece*)p = q;
+    *(loose<T, W>*)p = q;
 }
 
-// What becomes of W consecutive values of row m from column n on (all of them there, and aligned for W at once).
+// What becomes of W consecutive values of row m from column n on (all of them there).
 // held: the row belongs to a group (its product counts); bias, residual: of these values (0 where there is none).
 template <class T, int W, class P>
 __device__ __forceinline__ void finish_linear(const P& p, int64_t m, int64_t n, float* v, const float* bias, const float* residual, bool held) {
@@ -468,17 +469,19 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
     const unsigned mine = room + wave * (BLOCKS * 4096);
     const int64_t n_end = E == E_LOSS_GRAD ? p.ldc : p.N;
     if (n_wave >= n_end) return;
-    const bool wide = p.wide && n_wave + COLS <= n_end;  // (a row of g is whole waves' parts: always)
     const float shrink = E == E_LOSS_GRAD && p.shrink ? *p.shrink : 1.f;
-    // rows m_top .. of 64, W values a lane
-    auto rows_out = [&](auto width, int64_t m_top) {
-      constexpr int W = decltype(width)::value, PER_ROW = W == 1 ? 64 : COLS / W, STEP = 64 / PER_ROW, AT_ONCE = W == 1 ? 8 : 4;
-      const int r_lane = lane / PER_ROW, c = lane % PER_ROW * (W / 4);
-      int64_t n = n_wave + lane % PER_ROW * W;
-      const bool in = W > 1 || n < p.N;
-      if (!in) n = p.N - 1;
+    // Rows m_top .. of 64: W values a lane, `lanes` side by side.  Where the columns end within a wave's part (tail) the last
+    // lane begins as much earlier as makes its values whole: both lanes have the same for what they share.
+    const int cols = n_end - n_wave < COLS ? (int)(n_end - n_wave) : COLS;
+    auto rows_out = [&](auto width, auto lanes, auto tail, int64_t m_top) {
+      constexpr int W = decltype(width)::value, PER_ROW = decltype(lanes)::value, STEP = 64 / PER_ROW;
+      constexpr int AT_ONCE = STEP >= 16 ? 64 / STEP : 4;
+      const int r_lane = lane / PER_ROW, l = lane % PER_ROW * W;
+      const bool in = !tail || l < cols;
+      const int c = !tail || l + W <= cols ? l : cols - W;
+      const int64_t n = n_wave + c;
       const int last = (int)(m_end - m_top - 1);
-      typedef T piece __attribute__((ext_vector_type(W)));
+      typedef loose<T, W> piece;
       float bias[W];
       piece more[AT_ONCE], next[AT_ONCE];  // the residual of a turn's rows, and of the next turn's
       auto fetch = [&](int r0) {
@@ -503,12 +506,14 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
         for (int u = 0; u < AT_ONCE; u++) {
           const int r = r0 + u * STEP + r_lane;
           float v[W];
-          if constexpr (W == 1) {
-            v[0] = *lds_at<float>(mine + r * 256 + (((lane >> 2) ^ (r & 15)) << 4) + (lane & 3) * 4);
+          if constexpr (tail) {
+#pragma unroll
+            for (int e = 0; e < W; e++)
+              v[e] = *lds_at<float>(mine + r * 256 + ((((c + e) >> 2) ^ (r & 15)) << 4) + ((c + e) & 3) * 4);
           } else {
 #pragma unroll
             for (int k = 0; k < W / 4; k++) {
-              const v4f x = *lds_at<v4f>(mine + r * 256 + (((c + k) ^ (r & 15)) << 4));
+              const v4f x = *lds_at<v4f>(mine + r * 256 + (((c / 4 + k) ^ (r & 15)) << 4));
 #pragma unroll
               for (int e = 0; e < 4; e++) v[k * 4 + e] = x[e];
             }
@@ -540,12 +545,26 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
         for (int j = 0; j < FN; j++)
           *lds_at<v4f>(mine + (i * 16 + (lane & 15)) * 256 + (((j * 4 + q) ^ (lane & 15)) << 4)) = acc[i0 + i][j];
       asm volatile("" ::: "memory");
-      if (!wide)
-        rows_out(std::integral_constant<int, 1>(), m_top);
-      else if (E == E_STORE && sizeof(T) == 2 && (!p.out || p.out_f32))  // (16 bytes of fp32)
-        rows_out(std::integral_constant<int, 4>(), m_top);
-      else
-        rows_out(std::integral_constant<int, 16 / sizeof(T)>(), m_top);
+      constexpr int W = 16 / sizeof(T);
+      typedef std::integral_constant<int, 1> one;
+      typedef std::integral_constant<int, 2> two;
+      typedef std::integral_constant<int, 4> four;
+      typedef std::integral_constant<int, W> full;
+      if (cols == COLS) {
+        if (E == E_STORE && W != 4 && (!p.out || p.out_f32))  // (16 bytes of fp32)
+          rows_out(four(), std::integral_constant<int, 16>(), std::false_type(), m_top);
+        else
+          rows_out(full(), std::integral_constant<int, 64 / W>(), std::false_type(), m_top);
+      } else if (E != E_LOSS_GRAD) {  // (a row of g is whole waves' parts)
+        if (cols >= W)
+          rows_out(full(), std::integral_constant<int, 64 / W>(), std::true_type(), m_top);
+        else if (cols >= 4)
+          rows_out(four(), two(), std::true_type(), m_top);
+        else if (cols >= 2)
+          rows_out(two(), two(), std::true_type(), m_top);
+        else
+          rows_out(one(), one(), std::true_type(), m_top);
+      }
     }
   } else {
     // The maximum and the sum of exponentials of the tile's words for every row: over the lane's own, the four
@@ -760,7 +779,7 @@ __global__ __launch_bounds__(256) void k_join(args p, const float* parts, int sp
 #pragma unroll 4
   for (int s = 0; s < splits; s++) v += *(const v4f*)(parts + ((int64_t)s * p.M + m) * row + n);
   float x[4] = {v[0], v[1], v[2], v[3]}, b[4], r[4];
-  if (p.wide && n + 4 <= p.N) {
+  if (n + 4 <= p.N) {
     if constexpr (E == E_LINEAR) {
       bias_of<T, 4>(p, n, 0, true, b);
       residual_of<T, 4>(p, m, n, r);
@@ -785,9 +804,13 @@ __global__ __launch_bounds__(256) void k_join(args p, const float* parts, int sp
 
 inline int64_t round256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
-// How a product is run.  Tiles of 256 x 256 (eight waves, one workgroup per CU) where they fill the chip, else of
-// 128 x 128 (four waves, two per CU), the reduction of those split over workgroups where they are few.
+// How a product is run: with tiles of 256 x 256 (16-bit types; eight waves, one workgroup per CU) or of 128 x 128 (four
+// waves, two per CU), and with the reduction split over workgroups where tiles are few.  What is least by these times, in us,
+// measured on products of 1 to 8192 rows: a stage of a round of large tiles (256 at once) 0.80, of small ones (512 at once)
+// 0.51, fp32 3.8 (with a CU each 0.40 and 1.9); what a round costs besides 8, 5 and 12; a join 5 and its bytes at 4 TB/s.  8192 x 4096 x 16384 in bf16
+// is 927 us in large tiles, 1186 in small ones; 1999 x 4101 x 1030 in 136 large or 528 small ones 50 and 68.
 struct plan {
+  bool big;
   int splits;
   int64_t split_k;
 };
@@ -795,20 +818,31 @@ constexpr int64_t MOST_SPLITS = 32;
 // Results of more bytes than this are stored past the caches: they would not be found there again, and push out what the
 // product reads (64 experts' dW, 1 GB: 755 -> 715 us; 64 examples' squares, 268 MB: 84 -> 75).
 constexpr int64_t PAST_BYTES = (int64_t)128 << 20;
+inline double rounds_of(double tiles, double at_once) { return tiles <= at_once ? 1.0 : (double)(int64_t)((tiles + at_once - 1) / at_once); }
+// half_tiles: tiles of rows that groups leave half empty (BY_ROWS); sheets: products of this size in one launch.
 template <class T>
-inline plan plan_for(int64_t M, int64_t N, int64_t K, bool may_split) {
+inline plan plan_for(int64_t M, int64_t N, int64_t K, bool may_split, int64_t half_tiles = 0, int64_t sheets = 1) {
   constexpr int64_t BK = 128 / sizeof(T);
-  plan r{1, K};
-  const int64_t tiles = ceil_div(M, 128) * ceil_div(N, 128);
-  if (!may_split || tiles == 0 || tiles >= 256 || K < 8 * BK) return r;
-  int64_t s = 512 / tiles;
-  if (s > K / (4 * BK)) s = K / (4 * BK);
-  if (s > MOST_SPLITS) s = MOST_SPLITS;
-  if (s < 2) return r;
-  r.split_k = ceil_div(ceil_div(K, s), BK) * BK;
-  r.splits = (int)ceil_div(K, r.split_k);
-  if (r.splits < 2) r = plan{1, K};
-  return r;
+  plan best{false, 1, K};
+  double least = 1e300;
+  for (int big = 0; big < (sizeof(T) == 2 ? 2 : 1); big++) {
+    const int64_t side = big ? 256 : 128;
+    const double tiles = (double)(ceil_div(M, side) + half_tiles / 2) * ceil_div(N, side) * sheets, at_once = big ? 256 : 512;
+    const double round = sizeof(T) == 4 ? 12.0 : big ? 8.0 : 5.0;
+    for (int64_t s = 1; s <= (may_split ? MOST_SPLITS : 1); s++) {
+      const int64_t split_k = ceil_div(ceil_div(K, s), BK) * BK;
+      if (s > 1 && (split_k < 2 * BK || (s - 1) * split_k >= K)) break;
+      const bool one = tiles * s <= 256;  // workgroup on a CU
+      const double stage = sizeof(T) == 4 ? (one ? 1.9 : 3.8) : big ? 0.80 : one ? 0.40 : 0.51;
+      double us = rounds_of(tiles * s, at_once) * ((double)ceil_div(split_k, BK) * stage + round);
+      if (s > 1) us += 5.0 + (double)s * M * N * 8.0 / 4e6;
+      if (us < least) {
+        least = us;
+        best = plan{big != 0, (int)s, s > 1 ? split_k : K};
+      }
+    }
+  }
+  return best;
 }
 // Floats that the partial sums of a split product take (0: it is not split).
 template <class T>
@@ -860,10 +894,9 @@ __global__ __launch_bounds__(256) void k_pack(pack_args p) {
     v4i v;
   } u;
   if (there >= CH) {
-    struct __attribute__((packed, aligned(S))) loose {
-      v4i v;
-    };
-    u.v = ((const loose*)src)->v;
+    const loose<T, CH> q = *(const loose<T, CH>*)src;
+#pragma unroll
+    for (int i = 0; i < CH; i++) u.t[i] = q[i];
   } else {
 #pragma unroll
     for (int i = 0; i < CH; i++) u.t[i] = i < there ? src[i] : (T)0.f;
@@ -910,6 +943,14 @@ int launch_tiles(const args& p, hipStream_t st) {
   return 0;
 }
 
+template <class T, bool A_ROWS, bool B_ROWS, int E>
+int launch_size(const args& p, bool big, hipStream_t st) {
+  if constexpr (sizeof(T) == 2) {
+    if (big) return launch_tiles<T, 256, 256, 2, 4, A_ROWS, B_ROWS, E>(p, st);
+  }
+  return launch_tiles<T, 128, 128, 2, 2, A_ROWS, B_ROWS, E>(p, st);
+}
+
 // A product whose args are complete but for splits; its operands lie well, or are packed.  ws: room for split_floats (NULL: the
 // reduction is not split).  *tile (or NULL): the tiles' width.
 template <class T, bool A_ROWS, bool B_ROWS, int E>
@@ -918,8 +959,12 @@ int launch_product(args p, float* ws, hipStream_t st, int* tile = nullptr) {
   p.split_k = p.K;
   p.c_split = 0;
   p.past = (p.mode == BY_REDUCTION ? p.G.groups : 1) * p.M * p.N * (p.out_f32 ? 4 : (int64_t)sizeof(T)) > PAST_BYTES;
+  const int64_t groups = p.G.groups > 0 ? p.G.groups : 1;
+  const plan r = p.mode == BY_ROWS        ? plan_for<T>(p.M, p.N, p.K, false, groups < p.M ? groups : p.M)
+                 : p.mode == BY_REDUCTION ? plan_for<T>(p.M, p.N, ceil_div(p.K, groups), false, 0, groups)
+                                          : plan_for<T>(p.M, p.N, p.K, ws != nullptr);
+  if (tile) *tile = r.big ? 256 : 128;
   if constexpr (E == E_LINEAR || E == E_STORE) {
-    const plan r = plan_for<T>(p.M, p.N, p.K, ws != nullptr && p.mode == ONE);
     if (r.splits > 1) {
       args q = p;
       q.splits = r.splits;
@@ -929,35 +974,20 @@ int launch_product(args p, float* ws, hipStream_t st, int* tile = nullptr) {
       q.add_sums = 0;
       q.ldc = ceil_div(p.N, 4) * 4;
       q.c_split = p.M * q.ldc;
-      q.wide = 1;
-      DN_TRY((launch_tiles<T, 128, 128, 2, 2, A_ROWS, B_ROWS, E_STORE>(q, st)));
+      DN_TRY((launch_size<T, A_ROWS, B_ROWS, E_STORE>(q, r.big, st)));
       const int64_t many = p.M * ceil_div(p.N, 4);
       k_join<T, E><<<(unsigned)ceil_div(many, 256), 256, 0, st>>>(p, ws, r.splits);
       DN_LAUNCH_CHECK();
       return 0;
     }
   }
-  if (tile) *tile = 128;
-  if constexpr (sizeof(T) == 2) {
-    const int64_t sheets = p.mode == BY_REDUCTION ? p.G.groups : 1;
-    if (ceil_div(p.M, 256) * ceil_div(p.N, 256) * sheets >= 200) {
-      if (tile) *tile = 256;
-      return launch_tiles<T, 256, 256, 2, 4, A_ROWS, B_ROWS, E>(p, st);
-    }
-  }
-  return launch_tiles<T, 128, 128, 2, 2, A_ROWS, B_ROWS, E>(p, st);
+  return launch_size<T, A_ROWS, B_ROWS, E>(p, r.big, st);
 }
 
 // (their kernels are in linear.hip)
 #define DN_STORE_PRODUCTS(X, T)                                                              \
   X template int launch_product<T, true, false, E_STORE>(args, float*, hipStream_t, int*); \
   X template int launch_product<T, false, false, E_STORE>(args, float*, hipStream_t, int*);
-
-// Whether rows of `ld` elements from p on can be accessed 16 bytes at once (T of 16 bits: eight values).
-template <class T>
-inline bool wide(const void* p, int64_t ld) {
-  return p == nullptr || ((uintptr_t)p % 16 == 0 && ld * (int64_t)sizeof(T) % 16 == 0);
-}
 
 // ---- checks of arguments -----------------------------------------------------------------------------------------
 inline int check_array(const char* what, const char* name, const void* p, int64_t ld, int64_t width, int type, bool may_lack) {

@@ -165,7 +165,7 @@ int loss_backward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, con
     p.M = rows, p.N = n, p.K = n_in;
     p.mode = ONE;
     p.labels = labels, p.lse = lse, p.dloss = dloss, p.shrink = shrink, p.word0 = w0, p.words = words;
-    p.out = g, p.ldc = padded(n), p.wide = 1;
+    p.out = g, p.ldc = padded(n);
     DN_TRY((launch_product<T, true, true, E_LOSS_GRAD>(p, nullptr, st)));
     if (dX) {
       args q{};
@@ -174,8 +174,7 @@ int loss_backward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, con
       q.mode = ONE;
       q.sums = first && last ? nullptr : sums, q.add_sums = !first;
       q.ldc = ceil_div(n_in, 4) * 4;
-      q.wide = 1;
-      if (last) q.out = dX, q.ldo = lddx, q.wide = wide<T>(dX, lddx), q.scale = grow;
+      if (last) q.out = dX, q.ldo = lddx, q.scale = grow;
       DN_TRY((launch_product<T, true, false, E_STORE>(q, parts, st)));
     }
     if (dE) {
@@ -184,7 +183,7 @@ int loss_backward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, con
       q.M = n, q.N = n_in, q.K = rows;
       q.mode = ONE;
       T* to = (T*)dE + w0 * ldde;
-      q.out = to, q.ldo = ldde, q.wide = wide<T>(to, ldde), q.scale = grow;
+      q.out = to, q.ldo = ldde, q.scale = grow;
       DN_TRY((launch_product<T, false, false, E_STORE>(q, parts, st)));
     }
   }
