@@ -432,9 +432,9 @@ def op_threshold_compact(x: "DeviceArray", divisor: float, threshold: float):
 
 
 # ---- operators of a language model whose Fishers are wanted ----------------------------------------------------
-# Operands are DeviceArrays (float32, float16, or uint16 holding the bits of bfloat16) or tensors of a library with
-# torch's interface on the GPU, all of one kind in a call.  Calls are queued on `stream` (a stream's handle): by default the
-# library's for DeviceArrays, the tensors' library's current one for tensors.
+# Operands are DeviceArrays (float32, float16, or uint16 holding the bits of bfloat16) or torch's tensors on the current
+# device, all of one kind in a call.  Calls are queued on `stream` (a stream's handle): by default the library's for
+# DeviceArrays, torch's current one for tensors.
 
 F32, F16, BF16 = 0, 1, 2
 ACTS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
@@ -443,58 +443,65 @@ _KINDS = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16, "t
 _KIND_OF = {}  # dtype objects seen so far
 
 
+def _kind(dtype):
+    k = _KIND_OF.get(dtype)
+    if k is None:
+        k = _KIND_OF[dtype] = _KINDS.get(str(dtype), str(dtype))
+    return k
+
+
+def _refuse(what, why):
+    raise DnpeffError(f"{what}: {why}")
+
+
 class _Call:
     """The operands of one call: checks of their kind, shape and layout; pointers, and where to queue it."""
 
+    __slots__ = ("what", "own", "first", "type", "place")
+
     def __init__(self, what, first):
-        self.what = what
+        self.what, self.first = what, first
         self.own = isinstance(first, DeviceArray)
-        self.first = first
-        self.type = self.kind(first)
-        if self.type not in (F32, F16, BF16):
-            self.refuse(f"operands of {first.dtype}: float32, float16 or bfloat16 is wanted")
-
-    def refuse(self, why):
-        raise DnpeffError(f"{self.what}: {why}")
-
-    def kind(self, a):
-        k = _KIND_OF.get(a.dtype)
-        if k is None:
-            k = _KIND_OF[a.dtype] = _KINDS.get(str(a.dtype), str(a.dtype))
-        return k
+        self.place = -2 if self.own else first.get_device()
+        self.type = _kind(first.dtype)
+        if self.type.__class__ is not int:
+            _refuse(what, f"operands of {first.dtype}: float32, float16 or bfloat16 is wanted")
 
     def array(self, name, a, shape, kind=None):
         """(address, elements from one row to the next, ... from one matrix to the next); None: a NULL."""
         if a is None:
             return None, 0, 0
-        if isinstance(a, DeviceArray) != self.own:
-            self.refuse(f"{name}: DeviceArrays and tensors do not mix in a call")
-        if self.kind(a) != (self.type if kind is None else kind):
-            self.refuse(f"{name} is of {a.dtype}")
-        if tuple(a.shape) != shape:
-            self.refuse(f"{name} is {tuple(a.shape)}, not {shape}")
+        if (a.__class__ is DeviceArray) != self.own:
+            _refuse(self.what, f"{name}: DeviceArrays and tensors do not mix in a call")
+        if _kind(a.dtype) != (self.type if kind is None else kind):
+            _refuse(self.what, f"{name} is of {a.dtype}")
+        if a.shape != shape:
+            _refuse(self.what, f"{name} is {tuple(a.shape)}, not {shape}")
+        n = len(shape)
         width = shape[-1]
         if self.own:
-            return a.ptr.value, width, (shape[-2] * width if len(shape) > 2 else 0)
-        if not a.is_cuda or a.device != self.first.device:
-            self.refuse(f"{name} is on {a.device}")
+            return a.ptr.value, width, (shape[-2] * width if n > 2 else 0)
+        if a.get_device() != self.place or self.place < 0:
+            _refuse(self.what, f"{name} is on {a.device}")
         st = a.stride()
         if st[-1] != 1 and width > 1:
-            self.refuse(f"{name}: elements of a row have to be next to each other")
-        ld = st[-2] if len(shape) > 1 and shape[-2] > 1 else width
-        if len(shape) > 1 and ld < width:
-            self.refuse(f"{name}: rows overlap")
-        group = 0
-        if len(shape) > 2:
-            group = st[-3] if shape[-3] > 1 else shape[-2] * ld
-            if group < (shape[-2] - 1) * ld + width:
-                self.refuse(f"{name}: matrices overlap")
+            _refuse(self.what, f"{name}: elements of a row have to be next to each other")
+        if n == 1:
+            return a.data_ptr(), width, 0
+        ld = st[-2] if shape[-2] > 1 else width
+        if ld < width:
+            _refuse(self.what, f"{name}: rows overlap")
+        if n == 2:
+            return a.data_ptr(), ld, 0
+        group = st[-3] if shape[-3] > 1 else shape[-2] * ld
+        if group < (shape[-2] - 1) * ld + width:
+            _refuse(self.what, f"{name}: matrices overlap")
         return a.data_ptr(), ld, group
 
     def dense(self, name, a, shape, kind=None):
         p, ld, group = self.array(name, a, shape, kind)
         if len(shape) > 1 and p is not None and (ld != shape[-1] or (len(shape) > 2 and group != shape[-2] * shape[-1])):
-            self.refuse(f"{name} has to be dense")
+            _refuse(self.what, f"{name} has to be dense")
         return p
 
     def stream(self, stream):
@@ -502,31 +509,36 @@ class _Call:
             return stream
         if self.own:
             return lib.dnpeff_stream()
-        return sys.modules[type(self.first).__module__.split(".")[0]].cuda.current_stream(self.first.device).cuda_stream
+        torch = sys.modules["torch"]
+        if torch.cuda.current_device() != self.place:
+            _refuse(self.what, f"tensors on device {self.place}, and another one is the current device")
+        return torch.cuda.current_stream(self.place).cuda_stream
 
     def run(self, fn, args, bytes_needed, workspace, stream):
         """fn(stream, *args, workspace, bytes), with a workspace of the call's own where none is given."""
         st = self.stream(stream)
-        if workspace is not None:
-            p, _, _ = (workspace.ptr.value, 0, 0) if isinstance(workspace, DeviceArray) else (workspace.data_ptr(), 0, 0)
-            n = workspace.nbytes if isinstance(workspace, DeviceArray) else workspace.numel() * workspace.element_size()
-            return _check(fn(st, *args, p, n))
-        if bytes_needed == 0:
-            return _check(fn(st, *args, None, 0))
-        if not self.own:
-            if stream is not None:
-                self.refuse("a workspace has to be given with a stream")
-            torch = sys.modules[type(self.first).__module__.split(".")[0]]
+        if workspace is None and bytes_needed == 0:
+            status = fn(st, *args, None, 0)
+        elif workspace is not None:
+            if isinstance(workspace, DeviceArray):
+                status = fn(st, *args, workspace.ptr.value, workspace.nbytes)
+            else:
+                status = fn(st, *args, workspace.data_ptr(), workspace.numel() * workspace.element_size())
+        elif stream is not None and not (self.own and stream == lib.dnpeff_stream()):
+            _refuse(self.what, "a workspace has to be given with a stream")
+        elif not self.own:
+            torch = sys.modules["torch"]
             w = torch.empty(bytes_needed, dtype=torch.uint8, device=self.first.device)
-            return _check(fn(st, *args, w.data_ptr(), bytes_needed))
-        if stream is not None and stream != lib.dnpeff_stream():
-            self.refuse("a workspace has to be given with a stream")
-        w = C.c_void_p()
-        _check(lib.dnpeff_scratch_malloc(bytes_needed, C.byref(w)))
-        try:
-            _check(fn(st, *args, w, bytes_needed))
-        finally:
-            lib.dnpeff_scratch_free(w)
+            status = fn(st, *args, w.data_ptr(), bytes_needed)
+        else:
+            w = C.c_void_p()
+            _check(lib.dnpeff_scratch_malloc(bytes_needed, C.byref(w)))
+            try:
+                status = fn(st, *args, w, bytes_needed)
+            finally:
+                lib.dnpeff_scratch_free(w)
+        if status:
+            _check(status)
 
 
 _BYTES = {}  # sizes of workspaces asked for so far
@@ -565,10 +577,10 @@ def _layer(c, X_rows, W, groups):
     """rows, n_in, n_out, leading shape of weights, number of groups, their ends' address."""
     if groups is None:
         if len(W.shape) != 2:
-            c.refuse(f"W is {tuple(W.shape)}: one weight is a matrix")
+            _refuse(c.what, f"W is {tuple(W.shape)}: one weight is a matrix")
         return W.shape[1], W.shape[0], (), 0, None
     if len(W.shape) != 3:
-        c.refuse(f"W is {tuple(W.shape)}: the weights of groups have three dimensions")
+        _refuse(c.what, f"W is {tuple(W.shape)}: the weights of groups have three dimensions")
     n = W.shape[0]
     return W.shape[2], W.shape[1], (n,), n, c.dense("groups", groups, (n + 1,), "i8")
 
@@ -578,9 +590,9 @@ def op_linear(X, W, Y, bias=None, act="none", residual=None, pre=None, groups=No
     W's matrices (include/dnpeff.h, dnpeff_linear)."""
     c = _Call("op_linear", X)
     if act not in ACTS:
-        c.refuse(f"unknown activation {act!r}")
+        _refuse(c.what, f"unknown activation {act!r}")
     if len(X.shape) != 2:
-        c.refuse(f"X is {tuple(X.shape)}")
+        _refuse(c.what, f"X is {tuple(X.shape)}")
     rows = X.shape[0]
     n_in, n_out, lead, n, ends = _layer(c, rows, W, groups)
     x, ldx, _ = c.array("X", X, (rows, n_in))
@@ -601,9 +613,9 @@ def op_linear_backward(dY, X, W, pre=None, act="none", dX=None, dW=None, dbias=N
     """The gradients of op_linear for dY, into those of dX, dW and dbias that are given (dnpeff_linear_backward)."""
     c = _Call("op_linear_backward", dY)
     if act not in ACTS:
-        c.refuse(f"unknown activation {act!r}")
+        _refuse(c.what, f"unknown activation {act!r}")
     if len(dY.shape) != 2:
-        c.refuse(f"dY is {tuple(dY.shape)}")
+        _refuse(c.what, f"dY is {tuple(dY.shape)}")
     rows = dY.shape[0]
     n_in, n_out, lead, n, ends = _layer(c, rows, W, groups)
     g, lddy, _ = c.array("dY", dY, (rows, n_out))
@@ -626,7 +638,7 @@ def op_example_grads(dY, X, examples, out, square=False, workspace=None, stream=
     likelihood, rows of the diagonal Fisher.  examples: the ends of their rows (dnpeff_example_grads)."""
     c = _Call("op_example_grads", dY)
     if len(dY.shape) != 2 or len(X.shape) != 2:
-        c.refuse(f"dY is {tuple(dY.shape)}, X {tuple(X.shape)}")
+        _refuse(c.what, f"dY is {tuple(dY.shape)}, X {tuple(X.shape)}")
     rows, n_out = dY.shape
     n_in, n = X.shape[1], examples.shape[0] - 1
     g, lddy, _ = c.array("dY", dY, (rows, n_out))
@@ -644,7 +656,7 @@ def op_vocab_loss(X, E, labels, loss=None, lse=None, workspace=None, stream=None
     """Token losses lse - x . e_label and lse = log sum exp over the vocabulary E (dnpeff_vocab_loss)."""
     c = _Call("op_vocab_loss", X)
     if len(X.shape) != 2 or len(E.shape) != 2:
-        c.refuse(f"X is {tuple(X.shape)}, E {tuple(E.shape)}")
+        _refuse(c.what, f"X is {tuple(X.shape)}, E {tuple(E.shape)}")
     (rows, n_in), words = X.shape, E.shape[0]
     x, ldx, _ = c.array("X", X, (rows, n_in))
     e, lde, _ = c.array("E", E, (words, n_in))
@@ -660,7 +672,7 @@ def op_vocab_loss_backward(X, E, labels, lse, dloss, dX=None, dE=None, workspace
     """The gradients of op_vocab_loss for dloss, into those of dX and dE that are given (dnpeff_vocab_loss_backward)."""
     c = _Call("op_vocab_loss_backward", X)
     if len(X.shape) != 2 or len(E.shape) != 2:
-        c.refuse(f"X is {tuple(X.shape)}, E {tuple(E.shape)}")
+        _refuse(c.what, f"X is {tuple(X.shape)}, E {tuple(E.shape)}")
     (rows, n_in), words = X.shape, E.shape[0]
     x, ldx, _ = c.array("X", X, (rows, n_in))
     e, lde, _ = c.array("E", E, (words, n_in))

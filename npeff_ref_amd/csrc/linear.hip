@@ -127,10 +127,11 @@ matrix weight_matrix(const layer& l, const void* p, int64_t ld, int64_t sheet) {
 // Parts of a workspace: copies of operands that do not lie well, then the rest.
 template <class T>
 struct forward_room {
-  int64_t packs = 0, parts, all;
+  int64_t packs = 0, parts = 0, all = 0;
   matrix m[2];
   forward_room(const layer& l, const void* X, int64_t ldx, const void* W, int64_t ldw, int64_t w_group)
       : m{rows_matrix(l, X, ldx, l.n_in), weight_matrix(l, W, ldw, w_group)} {
+    if (is_few(l.rows, l.groups)) return;
     for (const matrix& q : m) packs += packed_bytes<T>(q);
     parts = l.grouped() ? 0 : round256(4 * split_floats<T>(l.rows, l.n_out, l.n_in));
     all = packs + parts;
@@ -180,13 +181,15 @@ int forward(hipStream_t st, const layer& l, const void* X, int64_t ldx, const vo
             const void* residual, int64_t ldr, void* Y, int64_t ldy, void* pre, int64_t ldp, char* ws, int64_t ws_bytes) {
   forward_room<T> room(l, X, ldx, W, ldw, w_group);
   DN_TRY(check_room("dnpeff_linear", room.all, ws, ws_bytes));
-  DN_TRY(pack<T>(room.m, 2, ws, st));
+  const bool few = is_few(l.rows, l.groups);
+  if (!few) DN_TRY(pack<T>(room.m, 2, ws, st));
   args p{};
   p.A = room.m[0].p, p.lda = room.m[0].ld, p.B = room.m[1].p, p.ldb = room.m[1].ld, p.b_group = room.m[1].sheet;
   p.M = l.rows, p.N = l.n_out, p.K = l.n_in;
   p.mode = l.grouped() ? BY_ROWS : ONE;
   p.G = rows_of(l);
   p.out = Y, p.ldc = ldy, p.pre = pre, p.ldp = ldp, p.residual = residual, p.ldr = ldr, p.bias = bias, p.act = act;
+  if (few) return launch_few<T, E_LINEAR>(p, st);
   return launch_product<T, true, true, E_LINEAR>(p, room.parts ? (float*)(ws + room.packs) : nullptr, st);
 }
 

@@ -768,6 +768,160 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_tiles(args p) {
   finish_tile<T, BM, BN, WM, WN, E>(again(), w, acc, base, nt, tid, wave);
 }
 
+// ---- few rows ----------------------------------------------------------------------------------------------------
+// Products of at most 16 rows at a time with rows of k, bound by the one read of B: no LDS stages, every wave streams 16
+// COLS rows of B from memory straight to the matrix cores, eight loads of 1 KB ahead.  A workgroup's eight waves are `parts` of the
+// reduction times 8 / parts blocks of 16 COLS columns; parts so that the chip has enough waves to keep its memory busy.  Groups
+// (BY_ROWS): blockIdx.y counts those that hold rows; a group of more than 16 rows reads its B again for every 16.
+template <class T, int COLS, int E>
+__global__ __launch_bounds__(512, 2) void k_few(args p, int parts) {
+  typedef typename num<T>::piece piece;
+  constexpr int CH = 16 / sizeof(T), STEP = 4 * CH, AHEAD = 8 / COLS;
+  __shared__ v4f sums[COLS][8][64];
+  __shared__ float2 stats[8][16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int q = lane >> 4, part = wave % parts;
+  const int64_t n0 = ((int64_t)blockIdx.x * (8 / parts) + wave / parts) * (16 * COLS);
+  const T* B = (const T*)p.B;
+  int64_t m0 = 0, m_end = p.M;
+  int group = 0;
+  bool held = true;
+  if (p.mode == BY_ROWS) {
+    int seen = 0;
+    group = -1;
+    for (int b = 0; b <= p.G.groups && group < 0; b += 64) {
+      const int g = b + lane;
+      const unsigned long long some = __ballot(g <= p.G.groups && p.G.count(g) > 0);
+      const int before = __popcll(some & ((1ull << lane) - 1));
+      const unsigned long long hit = __ballot(((some >> lane) & 1) && seen + before == (int)blockIdx.y);
+      if (hit) group = b + __ffsll(hit) - 1;
+      seen += __popcll(some);
+    }
+    group = __builtin_amdgcn_readfirstlane(group);
+    if (group < 0) return;
+    m0 = p.G.one_first(group);
+    m_end = p.G.one_last(group);
+    held = group < p.G.groups;
+    if (held) B += group * p.b_group;
+  }
+  const T* b_row[COLS];
+#pragma unroll
+  for (int h = 0; h < COLS; h++) {
+    const int64_t n = n0 + h * 16 + (lane & 15);
+    b_row[h] = B + (n < p.N ? n : p.N - 1) * p.ldb + q * CH;
+  }
+  const int64_t steps = (p.K + STEP - 1) / STEP, each = (steps + parts - 1) / parts;
+  const int64_t k_from = part * each * STEP, k_to = k_from + each * STEP < p.K ? k_from + each * STEP : p.K;
+  for (; m0 < m_end; m0 += 16) {
+    const T* a_row = (const T*)p.A + (m0 + (lane & 15) < m_end ? m0 + (lane & 15) : m_end - 1) * p.lda + q * CH;
+    v4f acc[COLS];
+#pragma unroll
+    for (int h = 0; h < COLS; h++) acc[h] = v4f{0.f, 0.f, 0.f, 0.f};
+    if (held && n0 < p.N) {
+      int64_t k = k_from;
+      for (; k + AHEAD * STEP <= k_to; k += AHEAD * STEP) {
+        loose<T, CH> fb[AHEAD][COLS], fa[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++)
+#pragma unroll
+          for (int h = 0; h < COLS; h++) fb[u][h] = *(const loose<T, CH>*)(b_row[h] + k + u * STEP);
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++) fa[u] = *(const loose<T, CH>*)(a_row + k + u * STEP);
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++)
+#pragma unroll
+          for (int h = 0; h < COLS; h++) acc[h] = mma((piece)fb[u][h], (piece)fa[u], acc[h]);
+      }
+      for (; k < k_to; k += STEP) {
+        piece fb[COLS], fa;
+        const int there = p.K - k - q * CH < CH ? (int)(p.K - k - q * CH) : CH;
+        if (there == CH) {
+#pragma unroll
+          for (int h = 0; h < COLS; h++) fb[h] = *(const loose<T, CH>*)(b_row[h] + k);
+          fa = *(const loose<T, CH>*)(a_row + k);
+        } else {
+#pragma unroll
+          for (int e = 0; e < CH; e++) {
+#pragma unroll
+            for (int h = 0; h < COLS; h++) fb[h][e] = e < there ? b_row[h][k + e] : (T)0.f;
+            fa[e] = e < there ? a_row[k + e] : (T)0.f;
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < COLS; h++) acc[h] = mma(fb[h], fa, acc[h]);
+      }
+    }
+    if (parts > 1) {
+      __syncthreads();  // (of the rows before)
+#pragma unroll
+      for (int h = 0; h < COLS; h++) sums[h][wave][lane] = acc[h];
+      __syncthreads();
+      if (part == 0)
+        for (int w = 1; w < parts; w++)
+#pragma unroll
+          for (int h = 0; h < COLS; h++) acc[h] += sums[h][wave + w][lane];
+    }
+    const int64_t m = m0 + (lane & 15);
+    if constexpr (E == E_LINEAR) {
+#pragma unroll
+      for (int h = 0; h < COLS; h++) {
+        const int64_t n = n0 + h * 16 + q * 4;
+        if (part != 0 || m >= m_end || n >= p.N) continue;
+        float v[4] = {acc[h][0], acc[h][1], acc[h][2], acc[h][3]}, b[4], r[4];
+        if (n + 4 <= p.N) {
+          bias_of<T, 4>(p, n, group, held, b);
+          residual_of<T, 4>(p, m, n, r);
+          finish_linear<T, 4>(p, m, n, v, b, r, held);
+        } else {
+#pragma unroll
+          for (int t = 0; t < 3; t++) {
+            if (n + t >= p.N) break;
+            bias_of<T, 1>(p, n + t, group, held, b);
+            residual_of<T, 1>(p, m, n + t, r);
+            finish_linear<T, 1>(p, m, n + t, v + t, b, r, held);
+          }
+        }
+      }
+    } else {
+      if (part == 0) {
+        const int64_t label = m < m_end ? (int64_t)p.labels[m] : -1;
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int h = 0; h < COLS; h++)
+#pragma unroll
+          for (int t = 0; t < 4; t++) {
+            const int64_t n = n0 + h * 16 + q * 4 + t;
+            if (n < p.N) top = fmaxf(top, acc[h][t]);
+            if (n == label && n < p.N) p.hit[m] = acc[h][t];
+          }
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float from = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int h = 0; h < COLS; h++)
+#pragma unroll
+          for (int t = 0; t < 4; t++)
+            if (n0 + h * 16 + q * 4 + t < p.N) sum += __expf(acc[h][t] - from);
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        if (q == 0) stats[wave][lane] = float2{top, sum};
+      }
+      __syncthreads();
+      if (threadIdx.x < 16 && m0 + threadIdx.x < m_end) {
+        float top = -INFINITY, sum = 0.f;
+        for (int w = 0; w < 8; w += parts) top = fmaxf(top, stats[w][threadIdx.x].x);
+        const float from = top == -INFINITY ? 0.f : top;
+        for (int w = 0; w < 8; w += parts) {
+          const float2 s = stats[w][threadIdx.x];
+          if (s.x != -INFINITY || s.y != 0.f) sum += s.y * __expf(s.x - from);
+        }
+        p.parts[(m0 + threadIdx.x) * gridDim.x + blockIdx.x] = float2{top, sum};
+      }
+      __syncthreads();
+    }
+  }
+}
+
 // ---- host --------------------------------------------------------------------------------------------------------
 // Partial sums of a split reduction, added in their order, then as the tiles' own epilogue.
 template <class T, int E>
@@ -815,6 +969,7 @@ struct plan {
   int64_t split_k;
 };
 constexpr int64_t MOST_SPLITS = 32;
+constexpr int64_t FEW_WAVES = 2048;  // eight on every CU: more parts than that cost more than they bring
 // Results of more bytes than this are stored past the caches: they would not be found there again, and push out what the
 // product reads (64 experts' dW, 1 GB: 755 -> 715 us; 64 examples' squares, 268 MB: 84 -> 75).
 constexpr int64_t PAST_BYTES = (int64_t)128 << 20;
@@ -988,6 +1143,31 @@ int launch_product(args p, float* ws, hipStream_t st, int* tile = nullptr) {
 #define DN_STORE_PRODUCTS(X, T)                                                              \
   X template int launch_product<T, true, false, E_STORE>(args, float*, hipStream_t, int*); \
   X template int launch_product<T, false, false, E_STORE>(args, float*, hipStream_t, int*);
+
+// Few rows: how many, and a product of them (which takes its operands as they lie).  *tile: columns of a workgroup.
+inline bool is_few(int64_t rows, int64_t groups) { return rows <= 16 || rows <= 4 * groups; }
+inline int few_parts(int64_t blocks) {
+  int parts = 1;
+  while (parts < 8 && blocks * parts < FEW_WAVES) parts *= 2;
+  return parts;
+}
+template <class T, int E>
+int launch_few(const args& p, hipStream_t st, int* tile = nullptr) {
+  const int64_t slots = p.mode == BY_ROWS ? (p.G.groups + 1 < p.M ? p.G.groups + 1 : p.M) : 1;
+  DN_CHECK(slots <= 65535, "product of %lld rows in %d groups: too many for one launch", (long long)p.M, p.G.groups);
+  // 32 columns a wave where they are enough (one token of 32000 words of 4096: 44 -> 41 us), else 16 (one of 4096 of 1024: 4.6
+  // against 6.1)
+  const int wide = ceil_div(p.N, 32) * slots >= FEW_WAVES / 2 ? 32 : 16;
+  const int parts = few_parts(ceil_div(p.N, wide) * slots), cols = wide * 8 / parts;
+  if (tile) *tile = cols;
+  const dim3 grid((unsigned)ceil_div(p.N, cols), (unsigned)slots);
+  if (wide == 32)
+    k_few<T, 2, E><<<grid, 512, 0, st>>>(p, parts);
+  else
+    k_few<T, 1, E><<<grid, 512, 0, st>>>(p, parts);
+  DN_LAUNCH_CHECK();
+  return 0;
+}
 
 // ---- checks of arguments -----------------------------------------------------------------------------------------
 inline int check_array(const char* what, const char* name, const void* p, int64_t ld, int64_t width, int type, bool may_lack) {

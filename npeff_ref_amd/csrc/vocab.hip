@@ -89,8 +89,9 @@ struct loss_room {  // of the forward pass
   matrix m[2];
   loss_room(int64_t rows, int64_t n_in, int64_t words, const void* X, int64_t ldx, const void* E, int64_t lde)
       : m{{X, ldx, rows, n_in, 1, 0}, {E, lde, words, n_in, 1, 0}} {
-    for (const matrix& q : m) packs += packed_bytes<T>(q);
-    parts = round256(rows * ceil_div(words, 128) * 8);
+    if (!is_few(rows, 0))
+      for (const matrix& q : m) packs += packed_bytes<T>(q);
+    parts = round256(rows * ceil_div(words, is_few(rows, 0) ? 16 : 128) * 8);
     all = packs + parts + round256(rows * 4);
   }
 };
@@ -123,7 +124,8 @@ int loss_forward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, cons
                  const int32_t* labels, float* loss, float* lse, char* ws, int64_t ws_bytes) {
   loss_room<T> room(rows, n_in, words, X, ldx, E, lde);
   DN_TRY(check_room("dnpeff_vocab_loss", room.all, ws, ws_bytes));
-  DN_TRY(pack<T>(room.m, 2, ws, st));
+  const bool few = is_few(rows, 0);
+  if (!few) DN_TRY(pack<T>(room.m, 2, ws, st));
   args p{};
   p.A = room.m[0].p, p.lda = room.m[0].ld, p.B = room.m[1].p, p.ldb = room.m[1].ld;
   p.M = rows, p.N = words, p.K = n_in;
@@ -132,7 +134,10 @@ int loss_forward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, cons
   p.parts = (float2*)(ws + room.packs);
   p.hit = (float*)(ws + room.packs + room.parts);
   int tile = 0;
-  DN_TRY((launch_product<T, true, true, E_LOSS>(p, nullptr, st, &tile)));
+  if (few)
+    DN_TRY((launch_few<T, E_LOSS>(p, st, &tile)));
+  else
+    DN_TRY((launch_product<T, true, true, E_LOSS>(p, nullptr, st, &tile)));
   k_join_loss<<<(unsigned)ceil_div(rows, 4), 256, 0, st>>>(rows, (int)ceil_div(words, tile), p.parts, p.hit, labels, words, loss, lse);
   DN_LAUNCH_CHECK();
   return 0;
