@@ -25,8 +25,8 @@ int slope_rows(int64_t rows, int64_t n_out, int size) { return ceil_div(rows, 64
 
 // dZ = dY act'(Z), and the column sums of each tile of rows.  A lane has 16 bytes of each row.
 template <class T>
-__global__ __launch_bounds__(256) void k_slopes(group_rows G, int64_t N, const T* dY, int64_t ldy, const T* Z, int64_t ldz, int act, T* dZ,
-                                                int64_t ldd, float* sums, int tall) {
+__global__ __launch_bounds__(256) void k_slopes(group_rows G, int64_t N, const T* dY, int64_t ldy, const T* Z, int64_t ldz, int act,
+                                                typename num<T>::op* dZ, int64_t ldd, float* sums, int tall) {
   constexpr bool EXACT = sizeof(T) == 4;
   constexpr int W = 16 / sizeof(T);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -61,7 +61,7 @@ __global__ __launch_bounds__(256) void k_slopes(group_rows G, int64_t N, const T
     slopes_of<EXACT, W>(g, z, act);
 #pragma unroll
     for (int t = 0; t < W; t++) sum[t] += g[t];
-    if (dZ && n < ldd) store_row<T, W>(dZ + m * ldd + n, g);  // (past the last column: zeros)
+    if (dZ && n < ldd) store_op<T, W>(dZ + m * ldd + n, G.rows * ldd, g);  // (past the last column: zeros)
   }
   if (!sums) return;
   __shared__ float side[4][W][64];
@@ -119,9 +119,9 @@ int check_act(const char* what, int act) {
 }
 group_rows rows_of(const layer& l) { return group_rows{l.ends, l.grouped() ? l.groups : 1, l.rows}; }
 
-matrix rows_matrix(const layer& l, const void* p, int64_t ld, int64_t width) { return matrix{p, ld, l.rows, width, 1, 0}; }
+matrix rows_matrix(const layer& l, const void* p, int64_t ld, int64_t width) { return matrix{p, ld, l.rows, width, 1, 0, 0}; }
 matrix weight_matrix(const layer& l, const void* p, int64_t ld, int64_t sheet) {
-  return matrix{p, ld, l.n_out, l.n_in, l.grouped() ? l.groups : 1, sheet};
+  return matrix{p, ld, l.n_out, l.n_in, l.grouped() ? l.groups : 1, sheet, 0};
 }
 
 // Parts of a workspace: copies of operands that do not lie well, then the rest.
@@ -146,7 +146,7 @@ struct backward_room {
   backward_room(const layer& l, const void* dY, int64_t lddy, const void* X, int64_t ldx, const void* W, int64_t ldw, int64_t w_group, int act,
                 bool dX, bool dW, bool dbias) {
     if (act != DNPEFF_ACT_NONE && (dX || dW))
-      dz = round256(l.rows * packed_ld<T>(l.n_out) * (int64_t)sizeof(T));
+      dz = round256(num<T>::PLANES * l.rows * packed_ld(l.n_out) * 2);
     else if (dX || dW)
       m[y = n++] = rows_matrix(l, dY, lddy, l.n_out);
     if (dW) m[x = n++] = rows_matrix(l, X, ldx, l.n_in);
@@ -185,6 +185,7 @@ int forward(hipStream_t st, const layer& l, const void* X, int64_t ldx, const vo
   if (!few) DN_TRY(pack<T>(room.m, 2, ws, st));
   args p{};
   p.A = room.m[0].p, p.lda = room.m[0].ld, p.B = room.m[1].p, p.ldb = room.m[1].ld, p.b_group = room.m[1].sheet;
+  p.a_plane = room.m[0].plane, p.b_plane = room.m[1].plane;
   p.M = l.rows, p.N = l.n_out, p.K = l.n_in;
   p.mode = l.grouped() ? BY_ROWS : ONE;
   p.G = rows_of(l);
@@ -202,7 +203,8 @@ int backward(hipStream_t st, const layer& l, const void* dY, int64_t lddy, const
   const group_rows G = rows_of(l);
   DN_TRY(pack<T>(room.m, room.n, ws, st));
   char* at = ws + room.packs;
-  T* dz = room.dz ? (T*)at : nullptr;
+  typedef typename num<T>::op O;
+  O* dz = room.dz ? (O*)at : nullptr;
   at += room.dz;
   float* sums = dbias ? (float*)at : nullptr;
   at += room.sums;
@@ -212,7 +214,7 @@ int backward(hipStream_t st, const layer& l, const void* dY, int64_t lddy, const
   if ((dz || dbias) && l.rows > 0) {
     const dim3 grid((unsigned)slope_tiles(l.rows, G.groups, tall), (unsigned)ceil_div(l.n_out, 64 * PIECE));
     DN_CHECK(grid.y <= 65535, "dnpeff_linear_backward: n_out = %lld is too wide for one launch", (long long)l.n_out);
-    k_slopes<T><<<grid, 256, 0, st>>>(G, l.n_out, (const T*)dY, lddy, (const T*)pre, ldp, act, dz, packed_ld<T>(l.n_out), sums, tall);
+    k_slopes<T><<<grid, 256, 0, st>>>(G, l.n_out, (const T*)dY, lddy, (const T*)pre, ldp, act, dz, packed_ld(l.n_out), sums, tall);
     DN_LAUNCH_CHECK();
   }
   if (dbias) {
@@ -221,10 +223,12 @@ int backward(hipStream_t st, const layer& l, const void* dY, int64_t lddy, const
     DN_LAUNCH_CHECK();
   }
   const void* g = dz ? dz : room.y >= 0 ? room.m[room.y].p : nullptr;
-  const int64_t ldg = dz ? packed_ld<T>(l.n_out) : room.y >= 0 ? room.m[room.y].ld : 0;
+  const int64_t ldg = dz ? packed_ld(l.n_out) : room.y >= 0 ? room.m[room.y].ld : 0;
+  const int64_t plane = dz ? l.rows * ldg : room.y >= 0 ? room.m[room.y].plane : 0;
   if (dX) {
     args p{};
     p.A = g, p.lda = ldg, p.B = room.m[room.w].p, p.ldb = room.m[room.w].ld, p.b_group = room.m[room.w].sheet;
+    p.a_plane = plane, p.b_plane = room.m[room.w].plane;
     p.M = l.rows, p.N = l.n_in, p.K = l.n_out;
     p.mode = l.grouped() ? BY_ROWS : ONE;
     p.G = G;
@@ -234,6 +238,7 @@ int backward(hipStream_t st, const layer& l, const void* dY, int64_t lddy, const
   if (dW) {
     args p{};
     p.A = g, p.lda = ldg, p.B = room.m[room.x].p, p.ldb = room.m[room.x].ld;
+    p.a_plane = plane, p.b_plane = room.m[room.x].plane;
     p.M = l.n_out, p.N = l.n_in, p.K = l.rows;
     p.mode = l.grouped() ? BY_REDUCTION : ONE;
     p.G = G;
@@ -251,6 +256,7 @@ int example_grads(hipStream_t st, const layer& l, const void* dY, int64_t lddy, 
   DN_TRY(pack<T>(room.m, 2, ws, st));
   args p{};
   p.A = room.m[0].p, p.lda = room.m[0].ld, p.B = room.m[1].p, p.ldb = room.m[1].ld;
+  p.a_plane = room.m[0].plane, p.b_plane = room.m[1].plane;
   p.M = l.n_out, p.N = l.n_in, p.K = l.rows;
   p.mode = BY_REDUCTION;
   p.G = rows_of(l);

@@ -40,18 +40,32 @@ __device__ __forceinline__ DN_LDS V* lds_at(unsigned address) {
 
 template <class T>
 struct num;
+// piece: 16 bytes of the reduction index of one row, as a lane holds them; op: the type that tiles multiply; TERMS: products of
+// it that a product takes.  fp32 goes as three bf16 numbers that add up to it, in the six products that matter next to fp32 (the
+// matrix cores multiply fp32 itself at a sixteenth of bf16's rate).
 template <>
 struct num<float> {
-  typedef v4f piece;  // 16 bytes of the reduction index of one row, as a lane holds them
+  typedef v4f piece;
+  typedef __bf16 op;
+  static constexpr int TERMS = 6, PLANES = 3;
 };
 template <>
 struct num<_Float16> {
   typedef v8h piece;
+  typedef _Float16 op;
+  static constexpr int TERMS = 1, PLANES = 1;
 };
 template <>
 struct num<__bf16> {
   typedef v8b piece;
+  typedef __bf16 op;
+  static constexpr int TERMS = 1, PLANES = 1;
 };
+// The planes of the t-th term, the smallest first: low high, high low, middle middle, middle high, high middle, high high.
+__device__ __forceinline__ int plane_a(int t) { return (0x0052 >> (2 * t)) & 3; }
+__device__ __forceinline__ int plane_b(int t) { return (0x0118 >> (2 * t)) & 3; }
+// W consecutive values as an operand holds them: as they are, or in planes so far apart.
+
 
 __device__ __forceinline__ v4f mma(v8b a, v8b b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ v4f mma(v8h a, v8h b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
@@ -208,8 +222,9 @@ enum { ONE = 0, BY_ROWS = 1, BY_REDUCTION = 2 };                      // groups:
 enum { E_LINEAR = 0, E_STORE = 1, E_LOSS = 2, E_LOSS_GRAD = 3 };     // what becomes of a tile
 
 struct args {
-  const void *A, *B;
+  const void *A, *B;        // (of num<T>::op)
   int64_t lda, ldb;         // elements from one row to the next
+  int64_t a_plane, b_plane; // ... from a plane of fp32 to the next
   int64_t M, N, K;          // BY_REDUCTION: K = rows of both operands
   int64_t b_group;          // BY_ROWS: elements from a group's B to the next one's
   group_rows G;
@@ -267,6 +282,28 @@ __device__ __forceinline__ void store_row(T* p, const float* v, bool past = fals
     *(loose<T, W>*)p = q;
 }
 
+// W consecutive values as an operand of tiles: as they are, or as planes so far apart.
+template <class T, int W>
+__device__ __forceinline__ void store_op(typename num<T>::op* p, int64_t plane, const float* v) {
+  if constexpr (num<T>::PLANES == 1) {
+    store_row<T, W>(p, v);
+  } else {
+    float rest[W];
+#pragma unroll
+    for (int t = 0; t < W; t++) rest[t] = v[t];
+#pragma unroll
+    for (int h = 0; h < 3; h++) {
+      loose<__bf16, W> q;
+#pragma unroll
+      for (int t = 0; t < W; t++) {
+        q[t] = (__bf16)rest[t];
+        rest[t] -= (float)q[t];
+      }
+      *(loose<__bf16, W>*)(p + h * plane) = q;
+    }
+  }
+}
+
 // What becomes of W consecutive values of row m from column n on (all of them there).
 // held: the row belongs to a group (its product counts); bias, residual: of these values (0 where there is none).
 template <class T, int W, class P>
@@ -316,7 +353,7 @@ __device__ __forceinline__ void finish_grad(const P& p, int64_t m, int64_t n, fl
     const float g = (__expf(v[t] - lse) - (word + t == label ? 1.f : 0.f)) * w;
     v[t] = n + t < p.N && label >= 0 ? g : 0.f;
   }
-  store_row<T, W>((T*)p.out + m * p.ldc + n, v);
+  store_op<T, W>((typename num<T>::op*)p.out + m * p.ldc + n, p.M * p.ldc, v);
 }
 template <class T, int W, class P>
 __device__ __forceinline__ void bias_of(const P& p, int64_t n, int group, bool held, float* b) {
@@ -341,27 +378,27 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
   return (int64_t)(((uint64_t)hi << 32) | lo);
 }
 
-// One operand's part of a tile: R of its own index, 128 bytes of the reduction, in N loads of 1 KB by each wave.  A load's
-// buffer begins at its first row and ends with the operand: what lies past that arrives as zeros, as do pieces of a row
+// One operand's part of a stage: R of its own index, 128 bytes of the reduction, in N loads of 1 KB by each wave.  A stage's
+// buffer begins at the wave's first row and ends with the operand: what lies past that arrives as zeros, as do pieces of a row
 // past the reduction's end (their offset is past any buffer's).  What is read of the own index between its end and a row's
-// makes results that nobody takes.  So a lane keeps two offsets: the permutation of the pieces repeats after two loads.
+// makes results that nobody takes.
 template <class T, int R, int THREADS, bool ROWS_OF_K>
 struct operand {
-  static constexpr int S = sizeof(T), CH = 16 / S, BK = 128 / S;
-  static constexpr int PER_ROW = ROWS_OF_K ? 8 : R * S / 16;  // pieces in a row
+  static constexpr int S = 2, CH = 8, BK = 64;
+  static_assert(sizeof(T) == 2, "operands are of 16 bits");
+  static constexpr int PER_ROW = ROWS_OF_K ? 8 : R / 8;  // pieces in a row
   static constexpr int N = R * 8 / THREADS, ROWS = 64 / PER_ROW;
-  static_assert(N == 2 || N == 4, "two offsets serve all loads");
-  static constexpr bool ODD = ROWS_OF_K || ROWS == 2 && S == 2;  // loads 0, 2 and 1, 3 are alike (else 0, 1 and 2, 3)
   static constexpr int NOWHERE = (int)0x80000000u;
-  int64_t at, end;  // addresses: this wave's first row of the next tile, the operand's end
-  int64_t step;     // bytes from a tile to the next
-  int next;         // bytes from a load to the next
-  int offset[2], k[2];  // k: (rows of k) a lane's place in the reduction
-  int room, now[2];
+  int64_t at, end;  // addresses: this wave's first row of the next stage, the operand's end
+  int64_t at0, end0;
+  int64_t step;     // bytes from a stage to the next
+  int offset[N];
+  int k[2];         // (rows of k) a lane's place in the reduction, in even and odd loads
+  v4i buffer;
+  bool in[2];
 
   __device__ static __forceinline__ int swizzle(int row) {
     if (ROWS_OF_K) return (row >> 1) & 7;
-    if (S == 4) return ((row >> 2) & 3) << 2;
     return (((row & 3) | ((row >> 1) & 4)) << 1) & (PER_ROW - 1);
   }
   // there: how many of the operand's own index exist from own0 on; k_end: the reduction's end.
@@ -371,30 +408,29 @@ struct operand {
     const int64_t first = (int64_t)p + (ROWS_OF_K ? own0 * ld : own0 * S);
     at = uniform(first + (ROWS_OF_K ? k0 * S : k0 * ld) + wave * N * ROWS * ld);
     end = uniform(first + (ROWS_OF_K ? (there - 1) * ld + (k_end + CH - 1) / CH * 16 : (k_end - 1) * ld + (int64_t)(there + CH - 1) / CH * 16));
+    at0 = at, end0 = end;
     step = uniform(ROWS_OF_K ? 128 : BK * ld);
-    next = __builtin_amdgcn_readfirstlane((int)(ROWS * ld));
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const int row = (wave * N + (N == 2 || ODD ? h : 2 * h)) * ROWS + lane / PER_ROW, c = (lane % PER_ROW) ^ swizzle(row);
-      offset[h] = (int)(lane / PER_ROW * ld) + c * 16;
-      k[h] = c * CH;
+    for (int e = 0; e < N; e++) {
+      const int row = (wave * N + e) * ROWS + lane / PER_ROW, c = (lane % PER_ROW) ^ swizzle(row);
+      offset[e] = (int)((e * ROWS + lane / PER_ROW) * ld) + c * 16;
+      if (e < 2) k[e] = c * CH;
     }
   }
   // A stage's loads, one by one: begin() says how much of the reduction is left (or nothing: zeros), load() makes the e-th
   // of N, end_stage() goes on to the next.
   __device__ __forceinline__ void begin(int left) {
-    int64_t r = end - at;
-    room = r < 0 ? 0 : r > 0x7fffffff ? 0x7fffffff : (int)r;
+    const int64_t r = end - at;
+    buffer = v4i{(int)(unsigned)(uint64_t)at, (int)(((uint64_t)at >> 32) & 0xffff), r < 0 ? 0 : r > 0x7fffffff ? 0x7fffffff : (int)r, 0x00020000};
 #pragma unroll
-    for (int h = 0; h < 2; h++) now[h] = ROWS_OF_K && k[h] >= left ? NOWHERE : offset[h];
+    for (int h = 0; h < 2; h++) in[h] = !ROWS_OF_K || k[h] < left;
   }
-  __device__ __forceinline__ void load(unsigned to, int e) const {
-    const uint64_t from = (uint64_t)at + (uint64_t)(unsigned)(e * next);
-    const int size = room - e * next;
-    const v4i buffer = {(int)(unsigned)from, (int)(unsigned)((from >> 32) & 0xffff), size < 0 ? 0 : size, 0x00020000};
-    to_lds(buffer, to + e * 1024, now[N == 2 || ODD ? e & 1 : e >> 1]);
-  }
+  __device__ __forceinline__ void load(unsigned to, int e) const { to_lds(buffer, to + e * 1024, in[e & 1] ? offset[e] : NOWHERE); }
   __device__ __forceinline__ void end_stage() { at += step; }
+  __device__ __forceinline__ void to_plane(int64_t elements) {  // back to the first stage, of another plane
+    at = at0 + elements * S;
+    end = end0 + elements * S;
+  }
 };
 
 // How a lane reads an operand's part of a tile: 16 of its index, `own` + 16 i .. + 15, for 64 bytes of the reduction (the s-th half).
@@ -407,8 +443,6 @@ struct reader {
     if (ROWS_OF_K) {
       lane_at[0] = (own + i) * 128 + ((q ^ (i >> 1)) << 4);
       lane_at[1] = lane_at[0] ^ 64;
-    } else if (sizeof(T) == 4) {
-      lane_at[0] = q * 4 * (R * 4) + (i & 3) * 4 + ((((own + i) >> 2) ^ (q << 2)) << 4);
     } else {
       const int r = i >> 2, col = own + (i & 3) * 4, swz = ((r | ((q & 1) << 2)) << 1) & (R / 8 - 1);
       lane_at[0] = (q * 8 + r) * (R * 2) + (((col >> 3) ^ swz) << 4) + (col & 4) * 2;
@@ -417,12 +451,6 @@ struct reader {
   __device__ __forceinline__ piece read(unsigned lds, int i, int s) const {
     if (ROWS_OF_K) {
       return *(const DN_LDS piece*)(lds_at<const char>(lds + lane_at[s]) + i * 2048);
-    } else if constexpr (sizeof(T) == 4) {
-      const DN_LDS char* p = lds_at<const char>(lds + (lane_at[0] ^ (i << 6)));
-      piece v;
-#pragma unroll
-      for (int e = 0; e < 4; e++) v[e] = *(const DN_LDS float*)(p + (s * 16 + e) * (R * 4));
-      return v;
     } else {
       DN_LDS char* p = lds_at<char>(lds + (lane_at[0] ^ (i << 5)));
       union {
@@ -445,7 +473,7 @@ __device__ __forceinline__ void wait_loads() {
 // A workgroup's tile: sums over k0 .. k_end of rows m0 .. m_end and columns from n0 on.
 template <class T>
 struct place {
-  const T *A, *B;
+  const typename num<T>::op *A, *B;
   int64_t m0, m_end, n0, k0, k_end;
   int sheet, tn, group;
   bool held;  // (BY_ROWS) the rows belong to a group
@@ -619,7 +647,8 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
 
 template <class T, int BM, int BN, int WM, int WN, bool A_ROWS, bool B_ROWS, int E>
 __global__ __launch_bounds__(WM* WN * 64, 2) void k_tiles(args p) {
-  constexpr int THREADS = WM * WN * 64, BK = 128 / sizeof(T);
+  typedef typename num<T>::op O;
+  constexpr int THREADS = WM * WN * 64, BK = 64, TERMS = num<T>::TERMS;
   constexpr int FM = BM / WM / 16, FN = BN / WN / 16, STAGE = (BM + BN) * 128, N_LOADS = STAGE / 16 / THREADS;
   __shared__ __align__(16) char smem[2 * STAGE];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -637,7 +666,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_tiles(args p) {
   if ((int)blockIdx.x >= many) return;
   const int tile = xcd * share + (xcd < more ? xcd : more) + blockIdx.x / 8;
   place<T> w;
-  w.A = (const T*)p.A, w.B = (const T*)p.B;
+  w.A = (const O*)p.A, w.B = (const O*)p.B;
   w.sheet = tile / plane;
   const int on = tile % plane;
   constexpr int HIGH = BM >= 256 ? 4 : 8;
@@ -672,15 +701,18 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_tiles(args p) {
     }
   }
 
-  operand<T, BM, THREADS, A_ROWS> a;
-  operand<T, BN, THREADS, B_ROWS> b;
-  reader<T, BM, A_ROWS> ra;
-  reader<T, BN, B_ROWS> rb;
+  operand<O, BM, THREADS, A_ROWS> a;
+  operand<O, BN, THREADS, B_ROWS> b;
+  reader<O, BM, A_ROWS> ra;
+  reader<O, BN, B_ROWS> rb;
   ra.start(wm * (BM / WM), lane);
   rb.start(wn * (BN / WN), lane);
-  constexpr int LA = operand<T, BM, THREADS, A_ROWS>::N, LB = operand<T, BN, THREADS, B_ROWS>::N;
-  auto begin = [&](int64_t l) {
-    const int to_go = l < 0 ? 0 : l > BK ? BK : (int)l;
+  constexpr int LA = operand<O, BM, THREADS, A_ROWS>::N, LB = operand<O, BN, THREADS, B_ROWS>::N;
+  const int64_t length = uniform(w.k_end - w.k0);
+  int64_t to_load = length;  // of the term that is being loaded
+  int term = 0;
+  auto begin = [&]() {
+    const int to_go = to_load < 0 ? 0 : to_load > BK ? BK : (int)to_load;
     a.begin(to_go);
     b.begin(to_go);
   };
@@ -693,34 +725,46 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_tiles(args p) {
   auto end_stage = [&]() {
     a.end_stage();
     b.end_stage();
+    to_load -= BK;
+    if (TERMS > 1 && to_load <= 0 && term + 1 < TERMS) {
+      term++;
+      to_load = length;
+      a.to_plane(plane_a(term) * p.a_plane);
+      b.to_plane(plane_b(term) * p.b_plane);
+    }
   };
   v4f acc[FM][FN];
 #pragma unroll
   for (int i = 0; i < FM; i++)
 #pragma unroll
     for (int j = 0; j < FN; j++) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
-  // Two stages of 128 bytes of the reduction each, in two halves.  A lane's operands of one half are read while the
-  // matrix cores work on the other's; once everyone has read the second half, the stage takes the one after the next,
-  // load by load between products: nothing but the barrier keeps the matrix cores waiting.
-  int64_t left = uniform(w.k_end - w.k0);
+  // Two stages of 128 bytes of the reduction each, in two halves.  A lane's operands of one half are read while the matrix
+  // cores work on the other's; once everyone has read the second half, the stage takes the one after the next, load by load
+  // between products: nothing but the barrier keeps the matrix cores waiting.  (Four stages of the small tiles where a CU has
+  // one: 333 x 10007 x 515 in fp32 49 us instead of 43.)
+  int64_t left = length > 0 ? (length + BK - 1) / BK * TERMS : 0;  // stages
   if (left > 0) {
     a.start(w.A, p.lda, w.m0, w.k0, w.k_end, (int)(w.m_end - w.m0 < BM ? w.m_end - w.m0 : BM), tid);
     b.start(w.B, p.ldb, w.n0, w.k0, w.k_end, (int)(p.N - w.n0 < BN ? p.N - w.n0 : BN), tid);
-    auto whole_stage = [&](unsigned stage, int64_t l) {
-      begin(l);
+    if (TERMS > 1) {
+      a.to_plane(plane_a(0) * p.a_plane);
+      b.to_plane(plane_b(0) * p.b_plane);
+    }
+    auto whole_stage = [&](unsigned stage) {
+      begin();
       asm volatile("s_nop 4");  // (between a lane's write of an address and the loads)
 #pragma unroll
       for (int e = 0; e < LA + LB; e++) load(stage, e);
       end_stage();
     };
-    whole_stage(base, left);
-    if (left > BK) {
-      whole_stage(base + STAGE, left - BK);
+    whole_stage(base);
+    if (left > 1) {
+      whole_stage(base + STAGE);
       wait_loads<N_LOADS>();
     } else {
       wait_loads<0>();
     }
-    typename num<T>::piece fa[2][FM], fb[2][FN];
+    typename num<O>::piece fa[2][FM], fb[2][FN];
     auto read = [&](unsigned stage, int s, int r) {
       if (r < FN)
         fb[s][r] = rb.read(stage + BM * 128, r, s);
@@ -748,12 +792,12 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_tiles(args p) {
     unsigned here = base, there = base + STAGE;
 #pragma unroll
     for (int r = 0; r < FN + FM; r++) read(here, 0, r);
-    while (left > BK) {
+    while (left > 1) {
       products(here, 0, true, false, 0);
       // the next stage has arrived, and everyone has read this one
       wait_loads<0>();
-      left -= BK;
-      begin(left - BK);
+      left--;
+      begin();
       products(there, 1, true, true, here);
       end_stage();
       const unsigned x = here;
@@ -958,10 +1002,10 @@ __global__ __launch_bounds__(256) void k_join(args p, const float* parts, int sp
 
 inline int64_t round256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
-// How a product is run: with tiles of 256 x 256 (16-bit types; eight waves, one workgroup per CU) or of 128 x 128 (four
+// How a product is run: with tiles of 256 x 256 (eight waves, one workgroup per CU) or of 128 x 128 (four
 // waves, two per CU), and with the reduction split over workgroups where tiles are few.  What is least by these times, in us,
-// measured on products of 1 to 8192 rows: a stage of a round of large tiles (256 at once) 0.80, of small ones (512 at once)
-// 0.51, fp32 3.8 (with a CU each 0.40 and 1.9); what a round costs besides 8, 5 and 12; a join 5 and its bytes at 4 TB/s.  8192 x 4096 x 16384 in bf16
+// measured on products of 1 to 8192 rows: a stage of a round of large tiles (256 at once) 1.6, of small ones (512 at once)
+// 1.0 (with a CU each 0.7), fp32 six times that; what a round costs besides 8 and 5; a join 5 and its bytes at 4 TB/s.  8192 x 4096 x 16384 in bf16
 // is 927 us in large tiles, 1186 in small ones; 1999 x 4101 x 1030 in 136 large or 528 small ones 50 and 68.
 struct plan {
   bool big;
@@ -977,18 +1021,18 @@ inline double rounds_of(double tiles, double at_once) { return tiles <= at_once 
 // half_tiles: tiles of rows that groups leave half empty (BY_ROWS); sheets: products of this size in one launch.
 template <class T>
 inline plan plan_for(int64_t M, int64_t N, int64_t K, bool may_split, int64_t half_tiles = 0, int64_t sheets = 1) {
-  constexpr int64_t BK = 128 / sizeof(T);
+  constexpr int64_t BK = 64;
   plan best{false, 1, K};
   double least = 1e300;
-  for (int big = 0; big < (sizeof(T) == 2 ? 2 : 1); big++) {
+  for (int big = 0; big < 2; big++) {
     const int64_t side = big ? 256 : 128;
     const double tiles = (double)(ceil_div(M, side) + half_tiles / 2) * ceil_div(N, side) * sheets, at_once = big ? 256 : 512;
-    const double round = sizeof(T) == 4 ? 12.0 : big ? 8.0 : 5.0;
+    const double round = big ? 8.0 : 5.0;
     for (int64_t s = 1; s <= (may_split ? MOST_SPLITS : 1); s++) {
       const int64_t split_k = ceil_div(ceil_div(K, s), BK) * BK;
       if (s > 1 && (split_k < 2 * BK || (s - 1) * split_k >= K)) break;
       const bool one = tiles * s <= 256;  // workgroup on a CU
-      const double stage = sizeof(T) == 4 ? (one ? 1.9 : 3.8) : big ? 0.80 : one ? 0.40 : 0.51;
+      const double stage = num<T>::TERMS * (big ? 1.6 : one ? 0.7 : 1.0);
       double us = rounds_of(tiles * s, at_once) * ((double)ceil_div(split_k, BK) * stage + round);
       if (s > 1) us += 5.0 + (double)s * M * N * 8.0 / 4e6;
       if (us < least) {
@@ -1007,36 +1051,35 @@ inline int64_t split_floats(int64_t M, int64_t N, int64_t K) {
 }
 
 // ---- operands that tiles can be loaded from -----------------------------------------------------------------------
-// A matrix whose rows begin on 16 bytes and end on them is loaded as it lies; any other is first copied to rows that do,
-// with zeros behind their ends (k_pack): once, where a tile's loads would come from any address again and again.
+// A matrix of 16-bit values whose rows begin on 16 bytes and end on them is loaded as it lies; any other is first copied to rows
+// that do, with zeros behind their ends (k_pack): once, where a tile's loads would come from any address again and again.  fp32
+// is copied to its three planes.
 struct matrix {
   const void* p;
   int64_t ld, rows, width;
   int64_t sheets, sheet;  // and so many such, so far apart
+  int64_t plane;          // (packed fp32) and its planes
 };
 template <class T>
 inline bool lies_well(const matrix& m) {
   constexpr int64_t S = sizeof(T), NEAR = (int64_t)1 << 31;
-  return (uintptr_t)m.p % 16 == 0 && m.ld * S % 16 == 0 && m.width * S % 16 == 0 && (m.sheets < 2 || m.sheet * S % 16 == 0) &&
+  return S == 2 && (uintptr_t)m.p % 16 == 0 && m.ld * S % 16 == 0 && m.width * S % 16 == 0 && (m.sheets < 2 || m.sheet * S % 16 == 0) &&
          256 * m.ld * S < NEAR;
 }
-template <class T>
-inline int64_t packed_ld(int64_t width) {
-  return ceil_div(width, 64) * 64;
-}
+inline int64_t packed_ld(int64_t width) { return ceil_div(width, 64) * 64; }
 template <class T>
 inline int64_t packed_bytes(const matrix& m) {
-  return lies_well<T>(m) ? 0 : round256(m.sheets * m.rows * packed_ld<T>(m.width) * (int64_t)sizeof(T));
+  return lies_well<T>(m) ? 0 : round256(num<T>::PLANES * m.sheets * m.rows * packed_ld(m.width) * 2);
 }
 struct pack_args {
   matrix m[3];
   void* to[3];
   int64_t first[4];  // workgroups before each
 };
-// A lane makes 16 bytes of a packed row.
+// A lane makes eight values of a packed row.
 template <class T>
 __global__ __launch_bounds__(256) void k_pack(pack_args p) {
-  constexpr int S = sizeof(T), CH = 16 / S;
+  constexpr int CH = 8;
   const int w = blockIdx.x < p.first[1] ? 0 : blockIdx.x < p.first[2] ? 1 : 2;
   const matrix m = p.m[w];
   const int64_t ld = (m.width + 63) / 64 * 64, per_row = ld / CH;
@@ -1044,21 +1087,16 @@ __global__ __launch_bounds__(256) void k_pack(pack_args p) {
   if (row >= m.rows * m.sheets) return;
   const int c = (int)(at - row * per_row) * CH, there = (int)(m.width - c);
   const T* src = (const T*)m.p + (m.sheets > 1 ? row / m.rows * m.sheet + row % m.rows * m.ld : row * m.ld) + c;
-  union {
-    T t[CH];
-    v4i v;
-  } u;
+  float v[CH];
   if (there >= CH) {
-    const loose<T, CH> q = *(const loose<T, CH>*)src;
-#pragma unroll
-    for (int i = 0; i < CH; i++) u.t[i] = q[i];
+    load_row<T, CH>(src, v);
   } else {
 #pragma unroll
-    for (int i = 0; i < CH; i++) u.t[i] = i < there ? src[i] : (T)0.f;
+    for (int i = 0; i < CH; i++) v[i] = i < there ? (float)src[i] : 0.f;
   }
-  *(v4i*)((T*)p.to[w] + row * ld + c) = u.v;
+  store_op<T, CH>((typename num<T>::op*)p.to[w] + row * ld + c, m.sheets * m.rows * ld, v);
 }
-// Packs those of n matrices (at most 3) that do not lie well into `room`, and makes them the copies.  Returns what it took of it.
+// Packs those of n matrices (at most 3) that do not lie well into `room`, and makes them the copies.
 template <class T>
 inline int pack(matrix* m, int n, char* room, hipStream_t st) {
   pack_args p{};
@@ -1067,16 +1105,16 @@ inline int pack(matrix* m, int n, char* room, hipStream_t st) {
   for (int i = 0; i < n; i++) {
     const int64_t bytes = packed_bytes<T>(m[i]);
     if (bytes == 0) continue;
-    const int64_t ld = packed_ld<T>(m[i].width);
+    const int64_t ld = packed_ld(m[i].width);
     p.m[k] = m[i], p.to[k] = room, p.first[k] = blocks;
-    blocks += ceil_div(m[i].sheets * m[i].rows * (ld * (int64_t)sizeof(T) / 16), 256);
-    m[i].p = room, m[i].ld = ld, m[i].sheet = m[i].rows * ld;
+    blocks += ceil_div(m[i].sheets * m[i].rows * (ld / 8), 256);
+    m[i].p = room, m[i].ld = ld, m[i].sheet = m[i].rows * ld, m[i].plane = m[i].sheets * m[i].sheet;
     room += bytes;
     k++;
   }
   if (blocks == 0) return 0;
   for (int i = k; i < 4; i++) p.first[i] = blocks;
-  DN_CHECK(blocks < (int64_t)1 << 31, "operands of %lld MB that are not aligned to 16 bytes", (long long)(blocks >> 8));
+  DN_CHECK(blocks < (int64_t)1 << 31, "operands of %lld MB that have to be copied", (long long)(blocks >> 8));
   k_pack<T><<<(unsigned)blocks, 256, 0, st>>>(p);
   DN_LAUNCH_CHECK();
   return 0;
@@ -1099,10 +1137,8 @@ int launch_tiles(const args& p, hipStream_t st) {
 }
 
 template <class T, bool A_ROWS, bool B_ROWS, int E>
-int launch_size(const args& p, bool big, hipStream_t st) {
-  if constexpr (sizeof(T) == 2) {
-    if (big) return launch_tiles<T, 256, 256, 2, 4, A_ROWS, B_ROWS, E>(p, st);
-  }
+int launch_size(const args& p, const plan& r, hipStream_t st) {
+  if (r.big) return launch_tiles<T, 256, 256, 2, 4, A_ROWS, B_ROWS, E>(p, st);
   return launch_tiles<T, 128, 128, 2, 2, A_ROWS, B_ROWS, E>(p, st);
 }
 
@@ -1129,14 +1165,14 @@ int launch_product(args p, float* ws, hipStream_t st, int* tile = nullptr) {
       q.add_sums = 0;
       q.ldc = ceil_div(p.N, 4) * 4;
       q.c_split = p.M * q.ldc;
-      DN_TRY((launch_size<T, A_ROWS, B_ROWS, E_STORE>(q, r.big, st)));
+      DN_TRY((launch_size<T, A_ROWS, B_ROWS, E_STORE>(q, r, st)));
       const int64_t many = p.M * ceil_div(p.N, 4);
       k_join<T, E><<<(unsigned)ceil_div(many, 256), 256, 0, st>>>(p, ws, r.splits);
       DN_LAUNCH_CHECK();
       return 0;
     }
   }
-  return launch_size<T, A_ROWS, B_ROWS, E>(p, r.big, st);
+  return launch_size<T, A_ROWS, B_ROWS, E>(p, r, st);
 }
 
 // (their kernels are in linear.hip)

@@ -88,7 +88,7 @@ struct loss_room {  // of the forward pass
   int64_t packs = 0, parts, all;
   matrix m[2];
   loss_room(int64_t rows, int64_t n_in, int64_t words, const void* X, int64_t ldx, const void* E, int64_t lde)
-      : m{{X, ldx, rows, n_in, 1, 0}, {E, lde, words, n_in, 1, 0}} {
+      : m{{X, ldx, rows, n_in, 1, 0, 0}, {E, lde, words, n_in, 1, 0, 0}} {
     if (!is_few(rows, 0))
       for (const matrix& q : m) packs += packed_bytes<T>(q);
     parts = round256(rows * ceil_div(words, is_few(rows, 0) ? 16 : 128) * 8);
@@ -100,10 +100,10 @@ struct grad_room {
   int64_t packs = 0, piece, g, sums, parts, all;
   matrix m[2];
   grad_room(int64_t rows, int64_t n_in, int64_t words, const void* X, int64_t ldx, const void* E, int64_t lde)
-      : m{{X, ldx, rows, n_in, 1, 0}, {E, lde, words, n_in, 1, 0}} {
+      : m{{X, ldx, rows, n_in, 1, 0, 0}, {E, lde, words, n_in, 1, 0, 0}} {
     for (const matrix& q : m) packs += packed_bytes<T>(q);
-    piece = piece_words(rows, words, sizeof(T));
-    g = round256(rows * padded(piece) * (int64_t)sizeof(T));
+    piece = piece_words(rows, words, num<T>::PLANES * 2);
+    g = round256(num<T>::PLANES * rows * padded(piece) * 2);
     sums = piece < words ? round256(rows * (ceil_div(n_in, 4) * 4) * 4) : 0;
     const int64_t last = words - (ceil_div(words, piece) - 1) * piece;
     parts = 0;
@@ -128,6 +128,7 @@ int loss_forward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, cons
   if (!few) DN_TRY(pack<T>(room.m, 2, ws, st));
   args p{};
   p.A = room.m[0].p, p.lda = room.m[0].ld, p.B = room.m[1].p, p.ldb = room.m[1].ld;
+  p.a_plane = room.m[0].plane, p.b_plane = room.m[1].plane;
   p.M = rows, p.N = words, p.K = n_in;
   p.mode = ONE;
   p.labels = labels, p.words = words, p.word0 = 0;
@@ -163,10 +164,11 @@ int loss_backward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, con
   }
   for (int64_t w0 = 0; w0 < words; w0 += r.piece) {
     const int64_t n = words - w0 < r.piece ? words - w0 : r.piece;
-    const T* Ep = (const T*)r.m[1].p + w0 * r.m[1].ld;
+    const void* Ep = (const typename num<T>::op*)r.m[1].p + w0 * r.m[1].ld;
     const bool first = w0 == 0, last = w0 + n == words;
     args p{};
     p.A = r.m[0].p, p.lda = r.m[0].ld, p.B = Ep, p.ldb = r.m[1].ld;
+    p.a_plane = r.m[0].plane, p.b_plane = r.m[1].plane;
     p.M = rows, p.N = n, p.K = n_in;
     p.mode = ONE;
     p.labels = labels, p.lse = lse, p.dloss = dloss, p.shrink = shrink, p.word0 = w0, p.words = words;
@@ -175,6 +177,7 @@ int loss_backward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, con
     if (dX) {
       args q{};
       q.A = g, q.lda = padded(n), q.B = Ep, q.ldb = r.m[1].ld;
+      q.a_plane = rows * padded(n), q.b_plane = r.m[1].plane;
       q.M = rows, q.N = n_in, q.K = n;
       q.mode = ONE;
       q.sums = first && last ? nullptr : sums, q.add_sums = !first;
@@ -185,6 +188,7 @@ int loss_backward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, con
     if (dE) {
       args q{};
       q.A = g, q.lda = padded(n), q.B = r.m[0].p, q.ldb = r.m[0].ld;
+      q.a_plane = rows * padded(n), q.b_plane = r.m[0].plane;
       q.M = n, q.N = n_in, q.K = rows;
       q.mode = ONE;
       T* to = (T*)dE + w0 * ldde;
