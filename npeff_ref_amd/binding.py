@@ -20,16 +20,32 @@ class DnpeffError(RuntimeError):
     """A C-ABI call returned a non-zero status."""
 
 
-def _load():
-    if not os.path.exists(LIB_PATH):
-        raise ImportError(
-            f"{LIB_PATH} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'` "
-            "(or `make -C npeff_ref_amd/csrc`). There is no CPU fallback."
-        )
-    return C.CDLL(LIB_PATH)
+if not os.path.exists(LIB_PATH):
+    raise ImportError(
+        f"{LIB_PATH} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'` "
+        "(or `make -C npeff_ref_amd/csrc`). There is no CPU fallback."
+    )
 
 
-lib = _load()
+class _Library:
+    """The library, loaded by its first call.  torch brings a HIP runtime of its own, and a process has to have one: what is
+    loaded first decides, so a program that hands tensors to the op_* calls imports torch before the first of any."""
+
+    without_torch = False  # loaded in a process without torch
+
+    def __getattr__(self, name):
+        if name not in SIGNATURES:
+            raise AttributeError(name)
+        loaded = C.CDLL(LIB_PATH)
+        for n, (res, args) in SIGNATURES.items():
+            fn = getattr(loaded, n)
+            fn.restype, fn.argtypes = res, args
+            setattr(self, n, fn)
+        self.without_torch = "torch" not in sys.modules
+        return self.__dict__[name]
+
+
+lib = _Library()
 
 _i64 = C.c_int64
 _i32 = C.c_int32
@@ -166,11 +182,6 @@ SIGNATURES = {
     ),
 }
 
-for _name, (_res, _args) in SIGNATURES.items():
-    _fn = getattr(lib, _name)
-    _fn.restype = _res
-    _fn.argtypes = _args
-
 KERNEL_CLASSES = ["spmm_n", "spmm_n_reduce", "gram_H", "xg_mu_W", "spmm_t", "gram_W", "xg_mu_H"]
 
 
@@ -295,8 +306,15 @@ def gather_rows(dev_ptr, r: int, rows) -> np.ndarray:
     return res
 
 
+# a tensor's type as numpy has it (bfloat16: its bits)
+_VIEWED = {"torch.float32": "float32", "torch.float16": "float16", "torch.bfloat16": "uint16", "torch.int32": "int32",
+           "torch.int64": "int64"}
+
+
 class DeviceArray:
     """A plain device buffer holding a numpy array (for the dnpeff_op_* entry points)."""
+
+    _owner = None  # of the memory, where it is not the array itself
 
     def __init__(self, shape, dtype=np.float32):
         self.shape = tuple(int(x) for x in np.atleast_1d(shape))
@@ -313,6 +331,18 @@ class DeviceArray:
         _check(lib.dnpeff_dev_upload(d.ptr, _ptr(a), d.nbytes))
         return d
 
+    @staticmethod
+    def view(t) -> "DeviceArray":
+        """The memory of a dense tensor on the GPU as a DeviceArray, for the calls that take one; the tensor stays alive with
+        it.  Its own work has to be finished, or ordered before the library's stream."""
+        if not t.is_cuda or not t.is_contiguous() or str(t.dtype) not in _VIEWED:
+            raise DnpeffError(f"a view of {tuple(t.shape)} {t.dtype} on {t.device}: a dense tensor on the GPU is wanted")
+        d = object.__new__(DeviceArray)
+        d.shape, d.dtype, d._owner = tuple(t.shape), np.dtype(_VIEWED[str(t.dtype)]), t
+        d.nbytes = t.numel() * t.element_size()
+        d.ptr = C.c_void_p(t.data_ptr())
+        return d
+
     def numpy(self) -> np.ndarray:
         out = np.empty(self.shape, dtype=self.dtype)
         _check(lib.dnpeff_dev_download(_ptr(out), self.ptr, self.nbytes))
@@ -326,8 +356,9 @@ class DeviceArray:
 
     def free(self):
         if self.ptr is not None:
-            lib.dnpeff_dev_free(self.ptr)
-            self.ptr = None
+            if self._owner is None:
+                lib.dnpeff_dev_free(self.ptr)
+            self.ptr = self._owner = None
 
     def __del__(self):  # pragma: no cover
         try:
@@ -462,6 +493,8 @@ class _Call:
     def __init__(self, what, first):
         self.what, self.first = what, first
         self.own = isinstance(first, DeviceArray)
+        if not self.own and lib.without_torch:
+            _refuse(what, "torch was imported after the library's first call, with a HIP runtime of its own: import it before")
         self.place = -2 if self.own else first.get_device()
         self.type = _kind(first.dtype)
         if self.type.__class__ is not int:
