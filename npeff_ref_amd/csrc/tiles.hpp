@@ -343,15 +343,20 @@ __device__ __forceinline__ void finish_store(const P& p, int64_t sheet, int64_t 
     store_row<T, W>((T*)p.out + to, v, p.past);
 }
 // (softmax - label) times the token's weight; the piece's columns past the last word are zero
+struct token {
+  int label;
+  float lse, dloss;
+};
 template <class T, int W, class P>
-__device__ __forceinline__ void finish_grad(const P& p, int64_t m, int64_t n, float* v, float shrink) {
-  const int32_t label = p.labels[m];
-  const float lse = p.lse[m], w = label >= p.words ? __builtin_nanf("") : p.dloss[m] * shrink;
-  const int64_t word = p.word0 + n;
+__device__ __forceinline__ void finish_grad(const P& p, int64_t m, int64_t n, float* v, const token& t, float shrink) {
+  const int32_t label = t.label;
+  const float lse = t.lse, w = label >= p.words ? __builtin_nanf("") : t.dloss * shrink;
+  const int64_t place = label - (p.word0 + n);
+  const int mine = place >= 0 && place < W ? (int)place : -1, there = label < 0 || n >= p.N ? 0 : p.N - n < W ? (int)(p.N - n) : W;
 #pragma unroll
   for (int t = 0; t < W; t++) {
-    const float g = (__expf(v[t] - lse) - (word + t == label ? 1.f : 0.f)) * w;
-    v[t] = n + t < p.N && label >= 0 ? g : 0.f;
+    const float g = (__expf(v[t] - lse) - (t == mine ? 1.f : 0.f)) * w;
+    v[t] = t < there ? g : 0.f;
   }
   store_op<T, W>((typename num<T>::op*)p.out + m * p.ldc + n, p.M * p.ldc, v);
 }
@@ -512,22 +517,33 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
       typedef loose<T, W> piece;
       float bias[W];
       piece more[AT_ONCE], next[AT_ONCE];  // the residual of a turn's rows, and of the next turn's
+      token these[AT_ONCE], those[AT_ONCE];  // what the loss needs of them
       auto fetch = [&](int r0) {
 #pragma unroll
         for (int u = 0; u < AT_ONCE; u++) {
           const int r = r0 + u * STEP + r_lane;
-          next[u] = *(const piece*)((const T*)p.residual + (m_top + (r < last ? r : last)) * p.ldr + n);
+          const int64_t m = m_top + (r < last ? r : last);
+          if constexpr (E == E_LOSS_GRAD)
+            those[u] = token{p.labels[m], p.lse[m], p.dloss[m]};
+          else
+            next[u] = *(const piece*)((const T*)p.residual + m * p.ldr + n);
         }
       };
       if constexpr (E == E_LINEAR) {
         bias_of<T, W>(p, n, w.group, w.held, bias);
         if (p.residual) fetch(0);
       }
+      if constexpr (E == E_LOSS_GRAD) fetch(0);
 #pragma unroll 1
       for (int r0 = 0; r0 < 16 * BLOCKS && r0 <= last; r0 += STEP * AT_ONCE) {
         if (E == E_LINEAR && p.residual) {
 #pragma unroll
           for (int u = 0; u < AT_ONCE; u++) more[u] = next[u];
+          fetch(r0 + STEP * AT_ONCE);
+        }
+        if constexpr (E == E_LOSS_GRAD) {
+#pragma unroll
+          for (int u = 0; u < AT_ONCE; u++) these[u] = those[u];
           fetch(r0 + STEP * AT_ONCE);
         }
 #pragma unroll
@@ -554,7 +570,7 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
               for (int e = 0; e < W; e++) res[e] = p.residual ? (float)more[u][e] : 0.f;
               finish_linear<T, W>(p, m, n, v, bias, res, w.held);
             } else if constexpr (E == E_LOSS_GRAD) {
-              finish_grad<T, W>(p, m, n, v, shrink);
+              finish_grad<T, W>(p, m, n, v, these[u], shrink);
             } else {
               finish_store<T, W>(p, w.sheet, m, n, v);
             }
@@ -600,19 +616,40 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
     __syncthreads();
     DN_LDS float2* side = lds_at<float2>(room);  // [WN][BM]
     const int m_there = (int)(m_end - w.m0 < BM ? m_end - w.m0 : BM);
+    const bool whole = n_wave + FN * 16 <= p.N;
+    const int there = whole ? FN * 16 : (int)(p.N - n_wave < 0 ? 0 : p.N - n_wave) - q * 4;
+    int labels[FM];  // (asked for together)
 #pragma unroll
     for (int i = 0; i < FM; i++) {
       const int64_t m = m_wave + i * 16 + (lane & 15);
-      const int64_t label = m < m_end ? (int64_t)p.labels[m] - p.word0 : -1;
-      float top = -INFINITY;
+      labels[i] = p.labels[m < m_end ? m : m_end - 1];
+    }
+#pragma unroll
+    for (int i = 0; i < FM; i++) {
+      const int64_t m = m_wave + i * 16 + (lane & 15);
+      // (the label's column among the lane's, or none)
+      const int64_t place = m < m_end ? labels[i] - (n_wave + q * 4) : -1;
+      const int mine = place >= 0 && place < 64 && labels[i] < p.N ? (int)place : -1;
+      float top = -INFINITY, hit = 0.f;
+      if (whole) {
+#pragma unroll
+        for (int j = 0; j < FN; j++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) top = fmaxf(top, acc[i][j][e]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < FN; j++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            if (j * 16 + e >= there) acc[i][j][e] = -INFINITY;
+            top = fmaxf(top, acc[i][j][e]);
+          }
+      }
 #pragma unroll
       for (int j = 0; j < FN; j++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const int64_t n = n_wave + q * 4 + j * 16 + e;
-          if (n < p.N) top = fmaxf(top, acc[i][j][e]);
-          if (n == label && label >= 0 && n < p.N) p.hit[m] = acc[i][j][e];
-        }
+        for (int e = 0; e < 4; e++) hit = j * 16 + e == mine ? acc[i][j][e] : hit;
+      if (mine >= 0 && (mine & 15) < 4) p.hit[m] = hit;
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
       const float from = top == -INFINITY ? 0.f : top;
@@ -620,8 +657,7 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
 #pragma unroll
       for (int j = 0; j < FN; j++)
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-          if (n_wave + q * 4 + j * 16 + e < p.N) sum += __expf(acc[i][j][e] - from);
+        for (int e = 0; e < 4; e++) sum += __expf(acc[i][j][e] - from);
       sum += __shfl_xor(sum, 16, 64);
       sum += __shfl_xor(sum, 32, 64);
       if (q == 0) {
