@@ -560,31 +560,35 @@ int dnpeff_op_init_uniform(int matrix_id, int64_t logical_rows, int64_t logical_
  * gradients that dnpeff_topk_rows then takes (in the reference this is TensorFlow's work, above
  * npeff/fishers/d_pefs_computer.py:126-145, on the host's side of the PEF file).
  *
- * All arrays are device memory, row-major with the last index contiguous; ld* are elements from one row to
- * the next (>= the row's width).  `type` is that of every array not declared with one of its own; sums, softmax
- * statistics and losses are fp32.  fp32 products run on the fp32 matrix cores, 16-bit ones on theirs; results are
- * rounded once.  Any size and any alignment of whole elements is taken; operands of the products whose rows do not
- * begin and end on 16 bytes (pointer, ld and width) are copied to such rows in the workspace first.  Outputs must not overlap inputs, except Y and residual, which may be one array.
+ * All arrays are device memory, row-major with the last index contiguous; ld* are elements from one row to the next
+ * (>= the row's width).  `type` is that of every array not declared with one of its own; sums, softmax statistics
+ * and losses are fp32, results are rounded once.  16-bit operands are multiplied as they are, fp32 ones as three
+ * bf16 numbers that add up to them, in the six products that matter next to fp32 (an operand that is not finite
+ * makes NaN of what it reaches), but for few rows, which go through the fp32 matrix cores.  Any size (widths up to
+ * 2^24) and any alignment of whole elements is taken; 16-bit operands of the products whose rows do not begin and
+ * end on 16 bytes (pointer, ld and width) are copied to such rows in the workspace first, fp32 ones always.  Outputs
+ * must not overlap inputs, except Y and residual, which may be one array.
  *
- * Calls are queued on `stream`, a hipStream_t of the caller's (NULL: HIP's null stream) or dnpeff_stream(),
- * and allocate nothing and wait for nothing, so they can be captured in a HIP graph.  The workspace belongs to the
- * caller, aligned to 16 bytes and at least as large as the *_workspace call says for the same sizes (aligned: 1 where the
- * inputs' pointers and ld are multiples of 16 bytes; 0 serves any), and is free for other use once the stream has passed the
- * call; with 0 bytes asked for it may be NULL.  Every sum is taken in an order that the sizes alone decide. */
+ * Calls are queued on `stream`, a hipStream_t of the caller's (NULL: HIP's null stream) or dnpeff_stream(), and
+ * allocate nothing and wait for nothing, so they can be captured in a HIP graph.  The workspace belongs to the
+ * caller, aligned to 16 bytes and at least as large as the *_workspace call says for the same sizes (aligned: 1
+ * where the inputs' pointers and ld are multiples of 16 bytes and ld below 2^25; 0 serves any), and is free for
+ * other use once the stream has passed the call; with 0 bytes asked for it may be NULL.  Every sum is taken in an
+ * order that the sizes alone decide. */
 enum { DNPEFF_F32 = 0, DNPEFF_F16 = 1, DNPEFF_BF16 = 2 };
 /* GELU: z (1 + erf(z / sqrt 2)) / 2;  GELU_TANH: z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2;  SILU: z / (1 + exp(-z)) */
 enum { DNPEFF_ACT_NONE = 0, DNPEFF_ACT_RELU = 1, DNPEFF_ACT_GELU = 2, DNPEFF_ACT_GELU_TANH = 3, DNPEFF_ACT_SILU = 4 };
 
 /* Y = act(X W^T + bias) + residual: X [rows, n_in], W [n_out, n_in], bias [n_out], Y and residual [rows, n_out];
- * bias and residual may be NULL.  pre (or NULL) receives X W^T + bias, which the backward pass of an
- * activation takes.
+ * bias and residual may be NULL.  pre (or NULL) receives X W^T + bias, which the backward pass of an activation
+ * takes.
  *
  * With n_groups > 0 (at most 65535; else 0 and ends NULL) the rows are in groups with a weight each, as a router
- * leaves the tokens of its experts: group g holds rows ends[g] .. ends[g + 1] - 1 (n_groups + 1 device
- * words, ends[0] = 0, not falling, the last at most `rows`), W is [n_groups, n_out, n_in] with w_group elements from a group's
- * to the next one's, bias [n_groups, n_out].  Groups may be empty.  Rows past the last end belong to none: their product is
- * zero, without bias and activation (Y = residual or 0, pre = 0).  The ends are only read on the device; values that break these
- * rules give undefined results but no access outside the arrays. */
+ * leaves the tokens of its experts: group g holds rows ends[g] .. ends[g + 1] - 1 (n_groups + 1 device words,
+ * ends[0] = 0, not falling, the last at most `rows`), W is [n_groups, n_out, n_in] with w_group elements from a
+ * group's to the next one's, bias [n_groups, n_out].  Groups may be empty.  Rows past the last end belong to none:
+ * their product is zero, without bias and activation (Y = residual or 0, pre = 0).  The ends are only read on the
+ * device; values that break these rules give undefined results but no access outside the arrays. */
 int dnpeff_linear_workspace(int type, int64_t rows, int64_t n_in, int64_t n_out, int n_groups, int aligned, int64_t* forward_bytes,
                             int64_t* backward_bytes, int64_t* example_bytes);
 int dnpeff_linear(void* stream, int type, int64_t rows, int64_t n_in, int64_t n_out, const void* X, int64_t ldx,
@@ -593,35 +597,36 @@ int dnpeff_linear(void* stream, int type, int64_t rows, int64_t n_in, int64_t n_
                   int64_t workspace_bytes);
 
 /* Its gradients, from dY [rows, n_out]: with dZ = dY * act'(pre), rounded to `type` once for the products,
- * dX = dZ W, dW = dZ^T X, dbias = column sums of dZ (before that rounding), per group where there are groups (dW [n_groups, n_out,
- * n_in] with dw_group elements from one to the next, zero for an empty group; dX zero for rows of no group).  Each of
- * the three may be NULL.  The residual's gradient is dY itself.  pre is not read for ACT_NONE, X not
- * without dW, W not without dX. */
+ * dX = dZ W, dW = dZ^T X, dbias = column sums of dZ (before that rounding), per group where there are groups (dW [n_groups,
+ * n_out, n_in] with dw_group elements from one to the next, zero for an empty group; dX zero for rows of no group).
+ * Each of the three may be NULL.  The residual's gradient is dY itself.  pre is not read for ACT_NONE, X not without
+ * dW, W not without dX. */
 int dnpeff_linear_backward(void* stream, int type, int64_t rows, int64_t n_in, int64_t n_out, const void* dY, int64_t lddy,
                            const void* X, int64_t ldx, const void* W, int64_t ldw, int64_t w_group, const void* pre, int64_t ldp,
                            int act, void* dX, int64_t lddx, void* dW, int64_t lddw, int64_t dw_group, void* dbias, int n_groups,
                            const int64_t* ends, void* workspace, int64_t workspace_bytes);
 
-/* out[e] = sum over the rows t of example e of dY[t]^T X[t], e < n_examples, squared element by element
- * where `square` is not 0: fp32 [n_examples, n_out, n_in], dense.  With dY the gradient of an example's log likelihood by the
- * output of a linear layer this is the example's gradient of the layer's weight, squared its row of the diagonal Fisher.
- * ends as above (n_examples + 1 of them); an example without rows gives zeros. */
+/* out[e] = sum over the rows t of example e of dY[t]^T X[t], e < n_examples, squared element by element where
+ * `square` is not 0: fp32 [n_examples, n_out, n_in], dense.  With dY the gradient of an example's log likelihood by
+ * the output of a linear layer this is the example's gradient of the layer's weight, squared its row of the diagonal
+ * Fisher. ends as above (n_examples + 1 of them); an example without rows gives zeros. */
 int dnpeff_example_grads(void* stream, int type, int64_t rows, int64_t n_in, int64_t n_out, const void* dY, int64_t lddy,
                          const void* X, int64_t ldx, int n_examples, const int64_t* ends, float* out, int square, void* workspace,
                          int64_t workspace_bytes);
 
 /* Softmax cross entropy of hidden states X [rows, n_in] over a vocabulary with embeddings E [n_words, n_in], without
- * an array of logits: lse[t] = log sum over v of exp(x_t . e_v), loss[t] = lse[t] - x_t . e_label.  labels [rows]; a negative
- * one means that the token has no loss (0), one of n_words and more gives NaN.  loss and lse may be NULL. */
+ * an array of logits: lse[t] = log sum over v of exp(x_t . e_v), loss[t] = lse[t] - x_t . e_label.  labels [rows]; a
+ * negative one means that the token has no loss (0), one of n_words and more gives NaN.  loss and lse may be NULL. */
 int dnpeff_vocab_loss_workspace(int type, int64_t rows, int64_t n_in, int64_t n_words, int aligned, int64_t* forward_bytes,
                                 int64_t* backward_bytes);
 int dnpeff_vocab_loss(void* stream, int type, int64_t rows, int64_t n_in, int64_t n_words, const void* X, int64_t ldx,
                       const void* E, int64_t lde, const int32_t* labels, float* loss, float* lse, void* workspace,
                       int64_t workspace_bytes);
-/* Its gradients for dloss [rows], the gradients of the tokens' losses, from the lse of the forward call: dX [rows, n_in] and dE
- * [n_words, n_in], either may be NULL.  The vocabulary goes by in pieces whose logits are formed again; (softmax - label) dloss is
- * rounded to `type` once for the products (16-bit types: after dividing by the largest |dloss|, which fp32 puts back).
- * Tokens without a label contribute nothing; a label of n_words and more makes dX's row and dE NaN. */
+/* Its gradients for dloss [rows], the gradients of the tokens' losses, from the lse of the forward call: dX [rows,
+ * n_in] and dE [n_words, n_in], either may be NULL.  The vocabulary goes by in pieces whose logits are formed again;
+ * (softmax - label) dloss is rounded to `type` once for the products (16-bit types: after dividing by the largest
+ * |dloss|, which fp32 puts back). Tokens without a label contribute nothing; a label of n_words and more makes dX's
+ * row and dE NaN. */
 int dnpeff_vocab_loss_backward(void* stream, int type, int64_t rows, int64_t n_in, int64_t n_words, const void* X, int64_t ldx,
                                const void* E, int64_t lde, const int32_t* labels, const float* lse, const float* dloss, void* dX,
                                int64_t lddx, void* dE, int64_t ldde, void* workspace, int64_t workspace_bytes);

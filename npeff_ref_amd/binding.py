@@ -592,7 +592,7 @@ def _bytes(fn, *sizes):
 def _on16(c, *places):
     """Whether arrays at (address, ld, group) begin all their rows on 16 bytes."""
     mask = 3 if c.type == F32 else 7
-    return int(all(p is None or not (p & 15 or ld & mask or group & mask) for p, ld, group in places))
+    return int(all(p is None or not (p & 15 or ld & mask or group & mask or ld >= 1 << 25) for p, ld, group in places))
 
 
 def linear_workspace(rows, n_in, n_out, dtype="float32", n_groups=0, aligned=False):

@@ -5,17 +5,21 @@
 // Each operand lies in memory either with its reduction index contiguous (rows of k) or with its own
 // index contiguous (rows of m or n, one per k): a layer's forward product has two of the first kind, the
 // gradient of its input one of each, the gradient of its weight two of the second.  A workgroup forms a
-// tile of BM x BN, 128 bytes of the reduction at a time, from two LDS stages: while the matrix cores
-// work on one, the other is filled past the registers (buffer loads to LDS), whose lanes outside the
-// operand lie past the buffer's end and so arrive as zeros.  Operands whose rows do not
-// begin and end on 16 bytes are copied to such rows first.
+// tile of 256 x 256 or 128 x 128, 128 bytes of the reduction at a time, from two LDS stages that are
+// filled past the registers (buffer loads to LDS); what lies outside the operand lies past the buffer's end
+// and so arrives as zeros.  16-bit operands whose rows do not begin and end on 16 bytes are copied to
+// such rows first, and fp32 ones to three planes of bf16.
 //
-// In LDS the 16-byte pieces of a row are permuted by its index, so that the 64 lanes of a read meet all banks:
+// In LDS the 16-byte pieces of a row are permuted by its index, so that the 64 lanes of a read meet all banks
+// (SQ_LDS_BANK_CONFLICT is 0):
 //   rows of k:   piece c of row i sits at c ^ ((i >> 1) & 7); a lane reads its 16 bytes of k at once
-//   rows of m/n: piece c of row k sits at c ^ swz(k); 16-bit values are transposed by the LDS read itself
-//                (ds_read_b64_tr_b16: lane i of 16 gets element i of four rows), 32-bit ones read one by one
-// The products run as B A, so that a lane ends with four consecutive n of one m: one store.
-// All sums are fp32.
+//   rows of m/n: piece c of row k sits at c ^ swizzle(k); values are transposed by the LDS read itself
+//                (ds_read_b64_tr_b16: lane i of 16 gets element i of four rows)
+// The products run as B A, so that a lane ends with four consecutive n of one m.  All sums are fp32.
+//
+// What bounds it: the matrix cores and the power they take.  The four products of 8192 tokens, 32768 words and a width of
+// 4096 in bf16 run at 1264 (with the softmax in its epilogue) to 1388 TFLOP/s, where the library's reach 1489, 1214 and
+// 1068 in the three layouts; they are busy 55 % of the cycles of a clock that falls to 1.9 GHz.
 #pragma once
 
 #include "dnpeff_internal.hpp"
@@ -99,7 +103,8 @@ __device__ __forceinline__ float normal(float z, float* e) {
   }
   const float x = fabsf(z) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(1.f + 0.45f * x);
   *e = __expf(-x * x);
-  float y = fmaf(fmaf(fmaf(fmaf(fmaf(fmaf(fmaf(0.0682241097f, t, -0.246025205f), t, 0.218937039f), t, 0.0308285784f), t, 0.193743601f), t, 0.226509377f), t, 0.253890544f), t, 0.253892303f);
+  float y = fmaf(fmaf(fmaf(0.0682241097f, t, -0.246025205f), t, 0.218937039f), t, 0.0308285784f);
+  y = fmaf(fmaf(fmaf(fmaf(y, t, 0.193743601f), t, 0.226509377f), t, 0.253890544f), t, 0.253892303f);
   y = 0.5f * *e * t * y;
   return z < 0.f ? y : 1.f - y;
 }
@@ -262,7 +267,7 @@ __device__ __forceinline__ kargs& again() {
 }
 
 // W consecutive values of a row at once, wherever they begin: the memory pipe takes any alignment of whole elements
-// (results of 1999 x 4101 in fp16: 68 us value by value, ODDSTORE so).
+// (products of 1999 x 4101 in fp16 68 us with their results value by value, 46 so).
 template <class T, int W>
 using loose = T __attribute__((ext_vector_type(W), aligned(sizeof(T))));
 template <class T, int W>
@@ -1041,17 +1046,17 @@ inline int64_t round256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 // How a product is run: with tiles of 256 x 256 (eight waves, one workgroup per CU) or of 128 x 128 (four
 // waves, two per CU), and with the reduction split over workgroups where tiles are few.  What is least by these times, in us,
 // measured on products of 1 to 8192 rows: a stage of a round of large tiles (256 at once) 1.6, of small ones (512 at once)
-// 1.0 (with a CU each 0.7), fp32 six times that; what a round costs besides 8 and 5; a join 5 and its bytes at 4 TB/s.  8192 x 4096 x 16384 in bf16
-// is 927 us in large tiles, 1186 in small ones; 1999 x 4101 x 1030 in 136 large or 528 small ones 50 and 68.
+// 1.0 (with a CU each 0.7), fp32 six times that; what a round costs besides 8 and 5; a join 5 and its bytes at 4 TB/s.
+// 8192 x 4096 x 16384 in bf16 is 927 us in large tiles, 1186 in small ones.
 struct plan {
   bool big;
   int splits;
   int64_t split_k;
 };
 constexpr int64_t MOST_SPLITS = 32;
-constexpr int64_t FEW_WAVES = 2048;  // eight on every CU: more parts than that cost more than they bring
+constexpr int64_t FEW_WAVES = 2048;  // eight on every CU
 // Results of more bytes than this are stored past the caches: they would not be found there again, and push out what the
-// product reads (64 experts' dW, 1 GB: 755 -> 715 us; 64 examples' squares, 268 MB: 84 -> 75).
+// product reads (64 experts' dW, 1 GB: 755 -> 715 us).
 constexpr int64_t PAST_BYTES = (int64_t)128 << 20;
 inline double rounds_of(double tiles, double at_once) { return tiles <= at_once ? 1.0 : (double)(int64_t)((tiles + at_once - 1) / at_once); }
 // half_tiles: tiles of rows that groups leave half empty (BY_ROWS); sheets: products of this size in one launch.
@@ -1100,7 +1105,7 @@ template <class T>
 inline bool lies_well(const matrix& m) {
   constexpr int64_t S = sizeof(T), NEAR = (int64_t)1 << 31;
   return S == 2 && (uintptr_t)m.p % 16 == 0 && m.ld * S % 16 == 0 && m.width * S % 16 == 0 && (m.sheets < 2 || m.sheet * S % 16 == 0) &&
-         256 * m.ld * S < NEAR;
+         32 * m.ld * S < NEAR;
 }
 inline int64_t packed_ld(int64_t width) { return ceil_div(width, 64) * 64; }
 template <class T>
@@ -1227,9 +1232,9 @@ template <class T, int E>
 int launch_few(const args& p, hipStream_t st, int* tile = nullptr) {
   const int64_t slots = p.mode == BY_ROWS ? (p.G.groups + 1 < p.M ? p.G.groups + 1 : p.M) : 1;
   DN_CHECK(slots <= 65535, "product of %lld rows in %d groups: too many for one launch", (long long)p.M, p.G.groups);
-  // 32 columns a wave where they are enough (one token of 32000 words of 4096: 44 -> 41 us), else 16 (one of 4096 of 1024: 4.6
-  // against 6.1)
-  const int wide = ceil_div(p.N, 32) * slots >= FEW_WAVES / 2 ? 32 : 16;
+  // 32 columns a wave where they are enough for three on every CU (one token of 32000 words of 4096: 43.5 us at 16, 41.1 at 32;
+  // of 24576: 40.7 and 38.2), else 16 (one of 4096 of 1024: 4.6 us at 16, 6.1 at 32)
+  const int wide = ceil_div(p.N, 32) * slots >= FEW_WAVES * 3 / 8 ? 32 : 16;
   const int parts = few_parts(ceil_div(p.N, wide) * slots), cols = wide * 8 / parts;
   if (tile) *tile = cols;
   const dim3 grid((unsigned)ceil_div(p.N, cols), (unsigned)slots);

@@ -74,10 +74,12 @@ __global__ __launch_bounds__(1024) void k_shrink(int64_t rows, const int32_t* la
 }
 
 constexpr int64_t PIECE_BYTES = (int64_t)512 << 20;  // of g at a time
+constexpr int64_t MOST_WORDS = (int64_t)1 << 24;       // (offsets within a tile are of 32 bits)
 // Words per piece: even pieces, whole tiles.
 int64_t piece_words(int64_t rows, int64_t words, int size) {
   int64_t most = PIECE_BYTES / (size * (rows > 0 ? rows : 1)) / 256 * 256;
   if (most < 1024) most = 1024;
+  if (most > MOST_WORDS) most = MOST_WORDS;
   if (most >= words) return words;
   return ceil_div(ceil_div(words, ceil_div(words, most)), 256) * 256;
 }
@@ -201,8 +203,8 @@ int loss_backward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, con
 
 int check_head(const char* me, int type, int64_t rows, int64_t n_in, int64_t words) {
   DN_CHECK(type == DNPEFF_F32 || type == DNPEFF_F16 || type == DNPEFF_BF16, "%s: unknown type %d", me, type);
-  DN_CHECK(rows >= 0 && n_in >= 1 && words >= 1 && rows < ((int64_t)1 << 31) && n_in < ((int64_t)1 << 31) && words < ((int64_t)1 << 31),
-           "%s: rows = %lld, n_in = %lld, n_words = %lld", me, (long long)rows, (long long)n_in, (long long)words);
+  DN_CHECK(rows >= 0 && n_in >= 1 && words >= 1 && rows < ((int64_t)1 << 31) && n_in <= ((int64_t)1 << 24) && words < ((int64_t)1 << 31),
+           "%s: rows = %lld, n_in = %lld (at most 2^24), n_words = %lld", me, (long long)rows, (long long)n_in, (long long)words);
   return 0;
 }
 

@@ -327,6 +327,28 @@ def test_device_arrays():
     del wb
 
 
+def test_offsets_past_32_bits():
+    """70,000 rows that are 40,000 elements apart: more than 2^31 of them, and 5.6 GB, between the first and the last."""
+    big = torch.empty(70_000 * 40_000, dtype=torch.bfloat16, device="cuda").view(70_000, 40_000)
+    X, Y = big[:, 8:72], big[:, 128:192]
+    X.copy_(torch.randn(70_000, 64, device="cuda"))
+    W = rand((64, 64), "bf16", 2)
+    d.op_linear(X, W, Y, act="relu")
+    for rows in (slice(0, 300), slice(53_600, 53_800), slice(69_700, 70_000)):
+        x = X[rows].double().cpu()
+        close(Y[rows], (x @ W.double().cpu().T).clamp(min=0), x.abs() @ W.double().cpu().abs().T, 64, "bf16")
+    dW, dX = torch.zeros_like(W), big[:, 256:320]
+    ends = ends_of([69_000, 0, 1_000])
+    d.op_linear_backward(Y, X, W, dW=dW, dX=dX)
+    a, b = Y.double(), X.double()
+    close(dW, a.T @ b, a.T.abs() @ b.abs(), 70_000, "bf16")
+    close(dX[-500:], (a[-500:] @ W.double()), a[-500:].abs() @ W.double().abs(), 64, "bf16")
+    out = torch.zeros(3, 64, 64, device="cuda")
+    d.op_example_grads(Y, X, ends, out)
+    close(out[2], a[-1000:].T @ b[-1000:], a[-1000:].T.abs() @ b[-1000:].abs(), 1000, "f32")
+    assert not out[1].any()
+
+
 def test_refusals():
     X, W, Y = torch.zeros(8, 16, device="cuda"), torch.zeros(4, 16, device="cuda"), torch.zeros(8, 4, device="cuda")
 

@@ -136,6 +136,24 @@ def test_pieces_of_the_vocabulary_give_the_whole():
         assert (err.norm(dim=1) <= 3 * HALF["bf16"] * exact.norm(dim=1) + 1e-6).all()
 
 
+@pytest.mark.parametrize("rows", [3, 40])
+def test_a_vocabulary_past_32_bits(rows):
+    """600,000 words of 4096: 4.9 GB, its last words past 2^31 elements."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    E = torch.empty(600_000, 4096, dtype=torch.bfloat16, device="cuda")
+    for i in range(0, 600_000, 100_000):
+        E[i : i + 100_000] = torch.randn(100_000, 4096, generator=g, device="cuda") * 0.03
+    X = rand((rows, 4096), "bf16", 2)
+    y = torch.randint(560_000, 600_000, (rows,), generator=torch.Generator().manual_seed(3), dtype=torch.int32).cuda()
+    loss, lse = torch.zeros(rows, device="cuda"), torch.zeros(rows, device="cuda")
+    d.op_vocab_loss(X, E, y, loss, lse)
+    z = torch.cat([X.double() @ E[i : i + 100_000].double().T for i in range(0, 600_000, 100_000)], 1)
+    want = torch.logsumexp(z, 1)
+    size = 4104 * EPS32 * (X.abs().double().sum(1) * E.abs().max().double())
+    assert ((lse - want).abs() <= 2 * size + 600_064 * EPS32).all()
+    assert ((loss - (want - z.gather(1, y.long()[:, None])[:, 0])).abs() <= 4 * size + 600_064 * EPS32).all()
+
+
 def test_all_masked_and_labels_outside():
     X, E = rand((70, 64), "bf16", 1), rand((900, 64), "bf16", 2)
     y = torch.full((70,), -1, dtype=torch.int32, device="cuda")
