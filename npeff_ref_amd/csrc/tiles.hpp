@@ -231,6 +231,7 @@ struct args {
   int64_t lda, ldb;         // elements from one row to the next
   int64_t a_plane, b_plane; // ... from a plane of fp32 to the next
   int64_t M, N, K;          // BY_REDUCTION: K = rows of both operands
+  int tm_first, tn_first;   // (ONE) the launch's first tile in either direction
   int64_t b_group;          // BY_ROWS: elements from a group's B to the next one's
   group_rows G;
   int mode, splits;         // splits: of the reduction, for E_STORE to fp32 partial sums
@@ -253,7 +254,8 @@ struct args {
   const int32_t* labels;
   const float *lse, *dloss;
   const float* shrink;      // (dloss is multiplied by this; NULL: by 1)
-  float2* parts;            // [M][tiles of words]: maximum and sum of the tile's words
+  float2* parts;            // [M][parts_n]: maximum and sum of each tile's words, this launch's from part0 on
+  int parts_n, part0;
   float* hit;               // [M] the label's logit
   int64_t word0, words;
 };
@@ -491,7 +493,7 @@ struct place {
 
 // What becomes of a tile's sums.
 template <class T, int BM, int BN, int WM, int WN, int E>
-__device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&acc)[BM / WM / 16][BN / WN / 16], unsigned room, int nt, int tid,
+__device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&acc)[BM / WM / 16][BN / WN / 16], unsigned room, int tid,
                                             int wave) {
   constexpr int FM = BM / WM / 16, FN = BN / WN / 16, THREADS = WM * WN * 64;
   asm volatile("" : "+v"(tid));  // (what follows from it is worked out here, not kept over the products)
@@ -681,7 +683,7 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
         const float x = side[v * BM + m].x, y = side[v * BM + m].y;
         if (x != -INFINITY || y != 0.f) sum += y * __expf(x - from);
       }
-      p.parts[(w.m0 + m) * nt + w.tn] = float2{top, sum};
+      p.parts[(w.m0 + m) * p.parts_n + p.part0 + w.tn] = float2{top, sum};
     }
   }
 }
@@ -698,8 +700,8 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_tiles(args p) {
   const unsigned base = (unsigned)(uintptr_t)(DN_LDS char*)smem;
 
   // -- which tiles --
-  const int nt = (int)((p.N + BN - 1) / BN);
-  const int mt = __builtin_amdgcn_readfirstlane(p.mode == BY_ROWS ? group_tiles(p.G, BM, lane) : (int)((p.M + BM - 1) / BM));
+  const int nt = (int)((p.N + BN - 1) / BN) - p.tn_first;
+  const int mt = __builtin_amdgcn_readfirstlane(p.mode == BY_ROWS ? group_tiles(p.G, BM, lane) : (int)((p.M + BM - 1) / BM) - p.tm_first);
   const int plane = mt * nt, many = plane * (p.mode == BY_REDUCTION ? p.G.groups : p.splits);
   // Workgroups go to the XCDs round-robin: each XCD gets a run of tiles, in blocks of a few tiles of m by all of n, so
   // that what its workgroups read at one time is shared in its L2.
@@ -715,7 +717,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_tiles(args p) {
   const int high = mt - block * HIGH < HIGH ? mt - block * HIGH : HIGH;
   const int tm = block * HIGH + in_block % high;
   w.tn = in_block / high;
-  w.n0 = (int64_t)w.tn * BN;
+  w.n0 = (int64_t)(w.tn + p.tn_first) * BN;
   w.k0 = 0, w.k_end = p.K;
   w.group = 0, w.held = true;
   if (p.mode == BY_ROWS) {
@@ -730,7 +732,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_tiles(args p) {
     else
       w.k_end = 0;
   } else {
-    w.m0 = (int64_t)tm * BM;
+    w.m0 = (int64_t)(tm + p.tm_first) * BM;
     w.m_end = p.M;
     if (p.mode == BY_REDUCTION) {
       w.group = w.sheet;
@@ -850,7 +852,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_tiles(args p) {
     wait_loads<0>();  // (of zeros, and for everyone's reads)
   }
 
-  finish_tile<T, BM, BN, WM, WN, E>(again(), w, acc, base, nt, tid, wave);
+  finish_tile<T, BM, BN, WM, WN, E>(again(), w, acc, base, tid, wave);
 }
 
 // ---- few rows ----------------------------------------------------------------------------------------------------
@@ -1000,7 +1002,7 @@ __global__ __launch_bounds__(512, 2) void k_few(args p, int parts) {
           const float2 s = stats[w][threadIdx.x];
           if (s.x != -INFINITY || s.y != 0.f) sum += s.y * __expf(s.x - from);
         }
-        p.parts[(m0 + threadIdx.x) * gridDim.x + blockIdx.x] = float2{top, sum};
+        p.parts[(m0 + threadIdx.x) * p.parts_n + blockIdx.x] = float2{top, sum};
       }
       __syncthreads();
     }
@@ -1048,11 +1050,17 @@ inline int64_t round256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 // measured on products of 1 to 8192 rows: a stage of a round of large tiles (256 at once) 1.6, of small ones (512 at once)
 // 1.0 (with a CU each 0.7), fp32 six times that; what a round costs besides 8 and 5; a join 5 and its bytes at 4 TB/s.
 // 8192 x 4096 x 16384 in bf16 is 927 us in large tiles, 1186 in small ones.
+// Large tiles that leave the last round partly empty are cut: as many strips of columns (or of rows) as make whole rounds, and
+// small tiles in a launch of their own for the rest.  Uncut and cut, in us: 2048 x 17880 x 4096 276 and 242, 3000 x 21976 x 768 131
+// and 122, 1000 x 134360 x 512 with the loss 154 and 149.  Not after a single round of less than 32 stages, where small
+// tiles alone are as fast or faster (2048 x 8920 x 1024: 52 against 56; with 4096 in place of 1024 152 and 145).
 struct plan {
   bool big;
   int splits;
   int64_t split_k;
+  int64_t m_cut, n_cut;  // rows or columns of the large tiles (0: all)
 };
+enum { NO_CUT = 0, CUT_N = 1, CUT_BOTH = 2 };
 constexpr int64_t MOST_SPLITS = 32;
 constexpr int64_t FEW_WAVES = 2048;  // eight on every CU
 // Results of more bytes than this are stored past the caches: they would not be found there again, and push out what the
@@ -1061,9 +1069,9 @@ constexpr int64_t PAST_BYTES = (int64_t)128 << 20;
 inline double rounds_of(double tiles, double at_once) { return tiles <= at_once ? 1.0 : (double)(int64_t)((tiles + at_once - 1) / at_once); }
 // half_tiles: tiles of rows that groups leave half empty (BY_ROWS); sheets: products of this size in one launch.
 template <class T>
-inline plan plan_for(int64_t M, int64_t N, int64_t K, bool may_split, int64_t half_tiles = 0, int64_t sheets = 1) {
+inline plan plan_for(int64_t M, int64_t N, int64_t K, bool may_split, int cut, int64_t half_tiles = 0, int64_t sheets = 1) {
   constexpr int64_t BK = 64;
-  plan best{false, 1, K};
+  plan best{false, 1, K, 0, 0};
   double least = 1e300;
   for (int big = 0; big < 2; big++) {
     const int64_t side = big ? 256 : 128;
@@ -1078,8 +1086,23 @@ inline plan plan_for(int64_t M, int64_t N, int64_t K, bool may_split, int64_t ha
       if (s > 1) us += 5.0 + (double)s * M * N * 8.0 / 4e6;
       if (us < least) {
         least = us;
-        best = plan{big != 0, (int)s, s > 1 ? split_k : K};
+        best = plan{big != 0, (int)s, s > 1 ? split_k : K, 0, 0};
       }
+    }
+  }
+  const int64_t tall = ceil_div(M, 256), wide = ceil_div(N, 256), rounds = tall * wide / 256;
+  const double stages = (double)num<T>::TERMS * ceil_div(K, BK);
+  const bool worth = rounds > 1 || (rounds == 1 && stages >= 32);
+  for (int way = CUT_N; worth && way <= cut; way++) {
+    const int64_t strip = way == CUT_N ? tall : wide, strips = rounds * 256 / strip;
+    if (strips == 0 || strips >= (way == CUT_N ? wide : tall)) continue;
+    const int64_t m_rest = way == CUT_N ? M : M - strips * 256, n_rest = way == CUT_N ? N - strips * 256 : N;
+    const double rest = (double)ceil_div(m_rest, 128) * ceil_div(n_rest, 128);
+    const double us = (double)ceil_div(strips * strip, 256) * (stages * 1.6 + 8.0) +
+                      rounds_of(rest, 512) * (stages * (rest <= 256 ? 0.7 : 1.0) + 5.0) + 4.0;
+    if (us < least) {
+      least = us;
+      best = plan{true, 1, K, way == CUT_N ? 0 : strips * 256, way == CUT_N ? strips * 256 : 0};
     }
   }
   return best;
@@ -1087,7 +1110,7 @@ inline plan plan_for(int64_t M, int64_t N, int64_t K, bool may_split, int64_t ha
 // Floats that the partial sums of a split product take (0: it is not split).
 template <class T>
 inline int64_t split_floats(int64_t M, int64_t N, int64_t K) {
-  const plan r = plan_for<T>(M, N, K, true);
+  const plan r = plan_for<T>(M, N, K, true, CUT_BOTH);
   return r.splits > 1 ? r.splits * M * (ceil_div(N, 4) * 4) : 0;
 }
 
@@ -1163,8 +1186,8 @@ inline int pack(matrix* m, int n, char* room, hipStream_t st) {
 
 template <class T, int BM, int BN, int WM, int WN, bool A_ROWS, bool B_ROWS, int E>
 int launch_tiles(const args& p, hipStream_t st) {
-  const int64_t nt = ceil_div(p.N, BN);
-  int64_t mt = ceil_div(p.M, BM), sheets = 1;
+  const int64_t nt = ceil_div(p.N, BN) - p.tn_first;
+  int64_t mt = ceil_div(p.M, BM) - p.tm_first, sheets = 1;
   if (p.mode == BY_ROWS)
     mt = p.G.rows / BM + (p.G.groups + 1 < p.G.rows ? p.G.groups + 1 : p.G.rows);
   else
@@ -1184,18 +1207,29 @@ int launch_size(const args& p, const plan& r, hipStream_t st) {
 }
 
 // A product whose args are complete but for splits; its operands lie well, or are packed.  ws: room for split_floats (NULL: the
-// reduction is not split).  *tile (or NULL): the tiles' width.
+// reduction is not split).  *parts_n (or NULL): the parts of a row that it leaves (E_LOSS).
 template <class T, bool A_ROWS, bool B_ROWS, int E>
-int launch_product(args p, float* ws, hipStream_t st, int* tile = nullptr) {
+int launch_product(args p, float* ws, hipStream_t st, int* parts_n = nullptr) {
   p.splits = 1;
   p.split_k = p.K;
   p.c_split = 0;
   p.past = (p.mode == BY_REDUCTION ? p.G.groups : 1) * p.M * p.N * (p.out_f32 ? 4 : (int64_t)sizeof(T)) > PAST_BYTES;
   const int64_t groups = p.G.groups > 0 ? p.G.groups : 1;
-  const plan r = p.mode == BY_ROWS        ? plan_for<T>(p.M, p.N, p.K, false, groups < p.M ? groups : p.M)
-                 : p.mode == BY_REDUCTION ? plan_for<T>(p.M, p.N, ceil_div(p.K, groups), false, 0, groups)
-                                          : plan_for<T>(p.M, p.N, p.K, ws != nullptr);
-  if (tile) *tile = r.big ? 256 : 128;
+  const int cut = E == E_LINEAR || E == E_STORE ? CUT_BOTH : CUT_N;
+  const plan r = p.mode == BY_ROWS        ? plan_for<T>(p.M, p.N, p.K, false, NO_CUT, groups < p.M ? groups : p.M)
+                 : p.mode == BY_REDUCTION ? plan_for<T>(p.M, p.N, ceil_div(p.K, groups), false, NO_CUT, 0, groups)
+                                          : plan_for<T>(p.M, p.N, p.K, ws != nullptr, cut);
+  const int64_t whole = r.n_cut / 256;
+  p.parts_n = (int)(r.n_cut ? whole + ceil_div(p.N - r.n_cut, 128) : ceil_div(p.N, r.big ? 256 : 128));
+  if (parts_n) *parts_n = p.parts_n;
+  if (r.m_cut || r.n_cut) {
+    args q = p;
+    if (r.m_cut) q.M = r.m_cut, p.tm_first = (int)(r.m_cut / 128);
+    if (r.n_cut) q.N = r.n_cut, p.tn_first = (int)(r.n_cut / 128);
+    p.part0 = (int)whole;
+    DN_TRY((launch_tiles<T, 256, 256, 2, 4, A_ROWS, B_ROWS, E>(q, st)));
+    return launch_tiles<T, 128, 128, 2, 2, A_ROWS, B_ROWS, E>(p, st);
+  }
   if constexpr (E == E_LINEAR || E == E_STORE) {
     if (r.splits > 1) {
       args q = p;
@@ -1221,7 +1255,7 @@ int launch_product(args p, float* ws, hipStream_t st, int* tile = nullptr) {
   X template int launch_product<T, true, false, E_STORE>(args, float*, hipStream_t, int*); \
   X template int launch_product<T, false, false, E_STORE>(args, float*, hipStream_t, int*);
 
-// Few rows: how many, and a product of them (which takes its operands as they lie).  *tile: columns of a workgroup.
+// Few rows: how many, and a product of them (which takes its operands as they lie).  *parts_n as above.
 inline bool is_few(int64_t rows, int64_t groups) { return rows <= 16 || rows <= 4 * groups; }
 inline int few_parts(int64_t blocks) {
   int parts = 1;
@@ -1229,14 +1263,15 @@ inline int few_parts(int64_t blocks) {
   return parts;
 }
 template <class T, int E>
-int launch_few(const args& p, hipStream_t st, int* tile = nullptr) {
+int launch_few(args p, hipStream_t st, int* parts_n = nullptr) {
   const int64_t slots = p.mode == BY_ROWS ? (p.G.groups + 1 < p.M ? p.G.groups + 1 : p.M) : 1;
   DN_CHECK(slots <= 65535, "product of %lld rows in %d groups: too many for one launch", (long long)p.M, p.G.groups);
   // 32 columns a wave where they are enough for three on every CU (one token of 32000 words of 4096: 43.5 us at 16, 41.1 at 32;
   // of 24576: 40.7 and 38.2), else 16 (one of 4096 of 1024: 4.6 us at 16, 6.1 at 32)
   const int wide = ceil_div(p.N, 32) * slots >= FEW_WAVES * 3 / 8 ? 32 : 16;
   const int parts = few_parts(ceil_div(p.N, wide) * slots), cols = wide * 8 / parts;
-  if (tile) *tile = cols;
+  p.parts_n = (int)ceil_div(p.N, cols);
+  if (parts_n) *parts_n = p.parts_n;
   const dim3 grid((unsigned)ceil_div(p.N, cols), (unsigned)slots);
   if (wide == 32)
     k_few<T, 2, E><<<grid, 512, 0, st>>>(p, parts);

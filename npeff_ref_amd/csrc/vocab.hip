@@ -136,12 +136,12 @@ int loss_forward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, cons
   p.labels = labels, p.words = words, p.word0 = 0;
   p.parts = (float2*)(ws + room.packs);
   p.hit = (float*)(ws + room.packs + room.parts);
-  int tile = 0;
+  int parts_n = 0;
   if (few)
-    DN_TRY((launch_few<T, E_LOSS>(p, st, &tile)));
+    DN_TRY((launch_few<T, E_LOSS>(p, st, &parts_n)));
   else
-    DN_TRY((launch_product<T, true, true, E_LOSS>(p, nullptr, st, &tile)));
-  k_join_loss<<<(unsigned)ceil_div(rows, 4), 256, 0, st>>>(rows, (int)ceil_div(words, tile), p.parts, p.hit, labels, words, loss, lse);
+    DN_TRY((launch_product<T, true, true, E_LOSS>(p, nullptr, st, &parts_n)));
+  k_join_loss<<<(unsigned)ceil_div(rows, 4), 256, 0, st>>>(rows, parts_n, p.parts, p.hit, labels, words, loss, lse);
   DN_LAUNCH_CHECK();
   return 0;
 }

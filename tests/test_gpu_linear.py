@@ -327,6 +327,16 @@ def test_device_arrays():
     del wb
 
 
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("rows, n_out", [(4200, 4203), (17_000, 1000), (1000, 17_001)])
+def test_whole_rounds_of_large_tiles_and_a_rest(rows, n_out, dt):
+    """A little more than 256 tiles of 256 x 256, in either direction, in products of all three layouts."""
+    check_forward(rows, 200, n_out, dt, act="silu", bias=True, residual=True, seed=1)
+    if dt != "f32":
+        check_backward(rows, n_out, 200, dt, act="silu", seed=2)  # dX [rows, n_out]
+        check_backward(200, rows, n_out, dt, seed=3)              # dW [n_out, rows]
+
+
 def test_offsets_past_32_bits():
     """70,000 rows that are 40,000 elements apart: more than 2^31 of them, and 5.6 GB, between the first and the last."""
     big = torch.empty(70_000 * 40_000, dtype=torch.bfloat16, device="cuda").view(70_000, 40_000)

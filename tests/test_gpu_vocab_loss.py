@@ -99,6 +99,12 @@ def test_large_tiles(dt):
     check(1500, 72, 9001, dt)
 
 
+@pytest.mark.parametrize("rows, n_in, words", [(4200, 200, 4203), (1000, 264, 17_001), (300, 1024, 17_000)])
+@pytest.mark.parametrize("dt", list(DTYPES))
+def test_whole_rounds_of_large_tiles_and_a_rest(rows, n_in, words, dt):
+    check(rows, n_in, words, dt)
+
+
 @pytest.mark.parametrize("dt", list(DTYPES))
 @pytest.mark.parametrize("weight", [1e-7, 1e4])
 def test_weights_of_any_size(weight, dt):
