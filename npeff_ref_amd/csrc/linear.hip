@@ -132,7 +132,7 @@ struct forward_room {
   matrix m[2];
   forward_room(const layer& l, const void* X, int64_t ldx, const void* W, int64_t ldw, int64_t w_group)
       : m{rows_matrix(l, X, ldx, l.n_in), weight_matrix(l, W, ldw, w_group)} {
-    if (is_few(l.rows, l.groups)) return;
+    if (is_few<T>(l.rows, l.groups, l.n_out, l.n_in)) return;
     for (const matrix& q : m) packs += packed_bytes<T>(q);
     parts = l.grouped() ? 0 : round256(4 * split_floats<T>(l.rows, l.n_out, l.n_in));
     all = packs + parts;
@@ -182,7 +182,7 @@ int forward(hipStream_t st, const layer& l, const void* X, int64_t ldx, const vo
             const void* residual, int64_t ldr, void* Y, int64_t ldy, void* pre, int64_t ldp, char* ws, int64_t ws_bytes) {
   forward_room<T> room(l, X, ldx, W, ldw, w_group);
   DN_TRY(check_room("dnpeff_linear", room.all, ws, ws_bytes));
-  const bool few = is_few(l.rows, l.groups);
+  const bool few = is_few<T>(l.rows, l.groups, l.n_out, l.n_in);
   if (!few) DN_TRY(pack<T>(room.m, 2, ws, st));
   args p{};
   p.A = room.m[0].p, p.lda = room.m[0].ld, p.B = room.m[1].p, p.ldb = room.m[1].ld, p.b_group = room.m[1].sheet;

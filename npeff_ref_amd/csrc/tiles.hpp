@@ -969,6 +969,20 @@ __global__ __launch_bounds__(512, 2) void k_few(args p, int parts) {
           }
         }
       }
+    } else if constexpr (E == E_LOSS_GRAD) {
+      // (at most 16 rows) out: fp32, [words][16]
+      if (part == 0) {
+        const int64_t label = m < m_end ? (int64_t)p.labels[m] : -1;
+        const float lse = label < 0 ? 0.f : p.lse[m], w = label < 0 ? 0.f : label >= p.words ? __builtin_nanf("") : p.dloss[m];
+#pragma unroll
+        for (int h = 0; h < COLS; h++)
+#pragma unroll
+          for (int t = 0; t < 4; t++) {
+            const int64_t n = n0 + h * 16 + q * 4 + t;
+            const float g = label < 0 ? 0.f : (__expf(acc[h][t] - lse) - (n == label ? 1.f : 0.f)) * w;
+            if (n < p.N) ((float*)p.out)[n * 16 + (lane & 15)] = g;
+          }
+      }
     } else {
       if (part == 0) {
         const int64_t label = m < m_end ? (int64_t)p.labels[m] : -1;
@@ -1255,8 +1269,21 @@ int launch_product(args p, float* ws, hipStream_t st, int* parts_n = nullptr) {
   X template int launch_product<T, true, false, E_STORE>(args, float*, hipStream_t, int*); \
   X template int launch_product<T, false, false, E_STORE>(args, float*, hipStream_t, int*);
 
-// Few rows: how many, and a product of them (which takes its operands as they lie).  *parts_n as above.
-inline bool is_few(int64_t rows, int64_t groups) { return rows <= 16 || rows <= 4 * groups; }
+// Few rows: how many, and a product of them (which takes its operands as they lie).  *parts_n as above.  fp32 has its packing to gain,
+// and so more rows (us in tiles and here): 16384 x 4096 of 32 rows 254 and 140, of 48 259 and 199, of 64 263 and 265; 61 groups of
+// 1005 x 2048 with 32 rows each 580 and 463, 48 each 583 and 656; the loss of 64000 x 2048 of 64 rows 594 and 445, of 96 594 and 653.
+// The loss's tiles cannot split the reduction: where they are few, more rows (3220 x 2296 of 192 rows, fp32: 146 and 96; 48 in bf16 26
+// and 19, 16384 x 1024 in bf16 of 17 18 and 20).  Small layers save the launch that joins a split (1024 x 1024 of 48 rows in bf16 13
+// and 9, 4096 x 1024 13 and 9, 1024 x 4096 13 and 15).  16-bit groups of two rows each: 32 of 2048 x 1024 20 and 23, 61 of 1005 x
+// 2048 32 and 41.
+template <class T>
+inline bool is_few(int64_t rows, int64_t groups, int64_t N, int64_t K, bool loss = false) {
+  if (rows <= 16) return true;
+  const int64_t tiles = ceil_div(rows, 128) * ceil_div(N, 128);
+  if (sizeof(T) == 4) return rows <= (loss ? (tiles <= 64 ? 192 : 64) : groups > 0 ? 32 * groups : 48);
+  if (loss) return rows <= 48 && tiles <= 32;
+  return groups > 0 ? rows <= groups : rows <= 48 && tiles <= 32 && K <= 2048;
+}
 inline int few_parts(int64_t blocks) {
   int parts = 1;
   while (parts < 8 && blocks * parts < FEW_WAVES) parts *= 2;

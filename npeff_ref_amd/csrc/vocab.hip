@@ -73,6 +73,126 @@ __global__ __launch_bounds__(1024) void k_shrink(int64_t rows, const int32_t* la
   }
 }
 
+// Both gradients of at most R <= 16 tokens from g [words][16], in one pass over E: a wave has 256 columns of a run of words, four a
+// lane with the tokens' X and dX in registers, g's values lane by lane; eight words are loaded ahead.  A workgroup's eight
+// waves add their dX, k_join adds the workgroups'.  What bounds it: E read and dE written, 4.3 TB/s at 65536 words of 4096 in
+// fp32 (500 us, 16 tokens); in 16 bits the vector units from 8 tokens on.
+constexpr int BACK_AHEAD = 8, BACK_SPLITS = 64;
+struct back_args {
+  int rows;
+  int64_t n_in, words, run;  // words of a wave
+  const void *X, *E;
+  int64_t ldx, lde, ldde;
+  const float* g;
+  void* dE;      // (or NULL)
+  float* parts;  // [workgroups of words][rows][n_in, to a multiple of 4] (or NULL)
+};
+template <class T, int R>
+__global__ __launch_bounds__(512, 2) void k_few_back(back_args p) {
+  __shared__ float4 sums[4][R][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // (the last lane of a row begins as much earlier as makes its four whole: what both have is the same)
+  const int64_t n = (int64_t)blockIdx.x * 256 + lane * 4, c = n + 4 <= p.n_in ? n : p.n_in - 4;
+  const bool in = n < p.n_in;
+  float x[R][4], acc[R][4];
+#pragma unroll
+  for (int m = 0; m < R; m++) {
+#pragma unroll
+    for (int t = 0; t < 4; t++) x[m][t] = acc[m][t] = 0.f;
+    if (p.dE && m < p.rows) load_row<T, 4>((const T*)p.X + m * p.ldx + c, x[m]);
+  }
+  const int64_t v0 = ((int64_t)blockIdx.y * 8 + wave) * p.run, v_end = v0 + p.run < p.words ? v0 + p.run : p.words;
+  const T* e_row = (const T*)p.E + c;
+  T* de_row = (T*)p.dE + c;
+  typedef loose<T, 4> four;
+  auto word = [&](int64_t v, four e, const float* w) {
+    float de[4] = {0.f, 0.f, 0.f, 0.f};
+    if (p.parts) {
+#pragma unroll
+      for (int m = 0; m < R; m++)
+#pragma unroll
+        for (int t = 0; t < 4; t++) acc[m][t] = fmaf(w[m], (float)e[t], acc[m][t]);
+    }
+    if (p.dE) {
+#pragma unroll
+      for (int m = 0; m < R; m++)
+#pragma unroll
+        for (int t = 0; t < 4; t++) de[t] = fmaf(w[m], x[m][t], de[t]);
+      if (in) store_row<T, 4>(de_row + v * p.ldde, de);
+    }
+  };
+  // Eight words ahead, and their g: 128 values, two a lane.
+  auto load = [&](int64_t v, four* e, float* g) {
+    if (p.parts) {
+#pragma unroll
+      for (int u = 0; u < BACK_AHEAD; u++) e[u] = *(const four*)(e_row + (v + u) * p.lde);
+    }
+#pragma unroll
+    for (int h = 0; h < BACK_AHEAD / 4; h++) g[h] = p.g[v * 16 + h * 64 + lane];
+  };
+  four e[BACK_AHEAD] = {}, e_next[BACK_AHEAD] = {};
+  float g[BACK_AHEAD / 4] = {}, g_next[BACK_AHEAD / 4] = {};
+  int64_t v = v0;
+  if (v + BACK_AHEAD <= v_end) load(v, e, g);
+  while (v + BACK_AHEAD <= v_end) {
+    if (v + 2 * BACK_AHEAD <= v_end) load(v + BACK_AHEAD, e_next, g_next);
+#pragma unroll
+    for (int u = 0; u < BACK_AHEAD; u++) {
+      float w[R];
+#pragma unroll
+      for (int m = 0; m < R; m++) w[m] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(g[u / 4]), u % 4 * 16 + m));
+      word(v + u, e[u], w);
+    }
+#pragma unroll
+    for (int u = 0; u < BACK_AHEAD; u++) e[u] = e_next[u];
+#pragma unroll
+    for (int h = 0; h < BACK_AHEAD / 4; h++) g[h] = g_next[h];
+    v += BACK_AHEAD;
+  }
+  for (; v < v_end; v++) {
+    float w[R];
+#pragma unroll
+    for (int m = 0; m < R; m++) w[m] = p.g[v * 16 + m];
+    word(v, p.parts ? *(const four*)(e_row + v * p.lde) : four{}, w);
+  }
+  if (!p.parts) return;
+#pragma unroll
+  for (int half = 4; half >= 1; half /= 2) {
+    __syncthreads();
+    if (wave >= half && wave < 2 * half) {
+#pragma unroll
+      for (int m = 0; m < R; m++) sums[wave - half][m][lane] = float4{acc[m][0], acc[m][1], acc[m][2], acc[m][3]};
+    }
+    __syncthreads();
+    if (wave < half) {
+#pragma unroll
+      for (int m = 0; m < R; m++) {
+        const float4 s = sums[wave][m][lane];
+        acc[m][0] += s.x, acc[m][1] += s.y, acc[m][2] += s.z, acc[m][3] += s.w;
+      }
+    }
+  }
+  if (wave == 0 && in) {
+    const int64_t ld = (p.n_in + 3) / 4 * 4;
+#pragma unroll
+    for (int m = 0; m < R; m++)
+      if (m < p.rows) store_row<float, 4>(p.parts + ((int64_t)blockIdx.y * p.rows + m) * ld + c, acc[m]);
+  }
+}
+// Both gradients of so many tokens go through k_few_back, others through tiles (us there and here, logits included): 65536 words of 4096 in
+// fp32, 16 tokens 2008 and 678; in bf16 1 token 431 and 358, 8 tokens 430 and 410, 12 tokens 431 and 502 (the products of 12 take the
+// vector units longer than E takes memory); 91355 of 3683, whose rows lie anywhere, 8 tokens 774 and 891; 10007 of 515 43 and 33.
+template <class T>
+bool back_is_few(int64_t rows, int64_t n_in) {
+  return rows >= 1 && rows <= (sizeof(T) == 4 ? 16 : 8) && n_in >= 4;
+}
+// Workgroups of words: eight waves on every CU, and no more than k_join should add.
+int64_t back_splits(int64_t n_in, int64_t words) {
+  int64_t s = ceil_div(256, ceil_div(n_in, 256));
+  if (s > BACK_SPLITS) s = BACK_SPLITS;
+  return s < ceil_div(words, 64) ? s : ceil_div(words, 64);
+}
+
 constexpr int64_t PIECE_BYTES = (int64_t)512 << 20;  // of g at a time
 constexpr int64_t MOST_WORDS = (int64_t)1 << 24;       // (offsets within a tile are of 32 bits)
 // Words per piece: even pieces, whole tiles.
@@ -91,9 +211,9 @@ struct loss_room {  // of the forward pass
   matrix m[2];
   loss_room(int64_t rows, int64_t n_in, int64_t words, const void* X, int64_t ldx, const void* E, int64_t lde)
       : m{{X, ldx, rows, n_in, 1, 0, 0}, {E, lde, words, n_in, 1, 0, 0}} {
-    if (!is_few(rows, 0))
+    if (!is_few<T>(rows, 0, words, n_in, true))
       for (const matrix& q : m) packs += packed_bytes<T>(q);
-    parts = round256(rows * ceil_div(words, is_few(rows, 0) ? 16 : 128) * 8);
+    parts = round256(rows * ceil_div(words, is_few<T>(rows, 0, words, n_in, true) ? 16 : 128) * 8);
     all = packs + parts + round256(rows * 4);
   }
 };
@@ -103,6 +223,14 @@ struct grad_room {
   matrix m[2];
   grad_room(int64_t rows, int64_t n_in, int64_t words, const void* X, int64_t ldx, const void* E, int64_t lde)
       : m{{X, ldx, rows, n_in, 1, 0, 0}, {E, lde, words, n_in, 1, 0, 0}} {
+    if (back_is_few<T>(rows, n_in)) {
+      piece = words;
+      sums = 0;
+      g = round256(words * 64);
+      parts = round256(back_splits(n_in, words) * rows * (ceil_div(n_in, 4) * 4) * 4);
+      all = 256 + g + parts;
+      return;
+    }
     for (const matrix& q : m) packs += packed_bytes<T>(q);
     piece = piece_words(rows, words, num<T>::PLANES * 2);
     g = round256(num<T>::PLANES * rows * padded(piece) * 2);
@@ -126,7 +254,7 @@ int loss_forward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, cons
                  const int32_t* labels, float* loss, float* lse, char* ws, int64_t ws_bytes) {
   loss_room<T> room(rows, n_in, words, X, ldx, E, lde);
   DN_TRY(check_room("dnpeff_vocab_loss", room.all, ws, ws_bytes));
-  const bool few = is_few(rows, 0);
+  const bool few = is_few<T>(rows, 0, words, n_in, true);
   if (!few) DN_TRY(pack<T>(room.m, 2, ws, st));
   args p{};
   p.A = room.m[0].p, p.lda = room.m[0].ld, p.B = room.m[1].p, p.ldb = room.m[1].ld;
@@ -146,12 +274,46 @@ int loss_forward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, cons
   return 0;
 }
 
+// (back_is_few)
+template <class T>
+int few_backward(hipStream_t st, const args& logits, char* g, float* parts, void* dX, int64_t lddx, void* dE, int64_t ldde) {
+  args p = logits;
+  p.out = g;
+  DN_TRY((launch_few<T, E_LOSS_GRAD>(p, st)));
+  const int64_t splits = back_splits(p.K, p.N);
+  back_args b{};
+  b.rows = (int)p.M, b.n_in = p.K, b.words = p.N, b.run = ceil_div(p.N, splits * 8);
+  b.X = p.A, b.ldx = p.lda, b.E = p.B, b.lde = p.ldb, b.g = (const float*)g, b.dE = dE, b.ldde = ldde, b.parts = dX ? parts : nullptr;
+  const dim3 grid((unsigned)ceil_div(p.K, 256), (unsigned)splits);
+  if (p.M <= 4)
+    k_few_back<T, 4><<<grid, 512, 0, st>>>(b);
+  else if (p.M <= 8)
+    k_few_back<T, 8><<<grid, 512, 0, st>>>(b);
+  else if constexpr (sizeof(T) == 4)
+    k_few_back<T, 16><<<grid, 512, 0, st>>>(b);
+  DN_LAUNCH_CHECK();
+  if (!dX) return 0;
+  args q{};
+  q.M = p.M, q.N = p.K, q.mode = ONE, q.out = dX, q.ldo = lddx;
+  k_join<T, E_STORE><<<(unsigned)ceil_div(q.M * ceil_div(q.N, 4), 256), 256, 0, st>>>(q, parts, (int)splits);
+  DN_LAUNCH_CHECK();
+  return 0;
+}
 template <class T>
 int loss_backward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, const void* X, int64_t ldx, const void* E, int64_t lde,
                   const int32_t* labels, const float* lse, const float* dloss, void* dX, int64_t lddx, void* dE, int64_t ldde, char* ws,
                   int64_t ws_bytes) {
   grad_room<T> r(rows, n_in, words, X, ldx, E, lde);
   DN_TRY(check_room("dnpeff_vocab_loss_backward", r.all, ws, ws_bytes));
+  if (back_is_few<T>(rows, n_in)) {
+    if (!dX && !dE) return 0;
+    args p{};
+    p.A = X, p.lda = ldx, p.B = E, p.ldb = lde;
+    p.M = rows, p.N = words, p.K = n_in;
+    p.mode = ONE;
+    p.labels = labels, p.lse = lse, p.dloss = dloss, p.words = words;
+    return few_backward<T>(st, p, ws + 256, (float*)(ws + 256 + r.g), dX, lddx, dE, ldde);
+  }
   float* both = (float*)ws;
   ws += 256;
   DN_TRY(pack<T>(r.m, 2, ws, st));

@@ -94,6 +94,28 @@ def test_strides(extra, dt):
     check(90, 136, 700, dt, extra=extra)
 
 
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("rows, n_in, words, extra", [(1, 4, 700, 0), (3, 257, 9001, 1), (4, 1030, 513, 3), (5, 3, 300, 0), (9, 515, 20_000, 8),
+                                                      (16, 1003, 65, 5), (16, 5, 7, 0), (33, 130, 3000, 1), (64, 72, 1000, 0)])
+def test_few_tokens(rows, n_in, words, extra, dt):
+    check(rows, n_in, words, dt, extra=extra, seed=rows)
+
+
+@pytest.mark.parametrize("rows", [0, 3, 40])
+def test_one_gradient_alone(rows):
+    X, E = rand((rows, 100), "bf16", 1), rand((900, 100), "bf16", 2, 0.3)
+    y = labels_of(rows, 900, 3)
+    loss, lse, dl = torch.zeros(rows, device="cuda"), torch.zeros(rows, device="cuda"), torch.ones(rows, device="cuda")
+    d.op_vocab_loss(X, E, y, loss, lse)
+    both, alone = [[torch.full_like(t, 3.0) for t in (X, E)] for _ in range(2)]
+    d.op_vocab_loss_backward(X, E, y, lse, dl, dX=both[0], dE=both[1])
+    d.op_vocab_loss_backward(X, E, y, lse, dl, dX=alone[0])
+    d.op_vocab_loss_backward(X, E, y, lse, dl, dE=alone[1])
+    assert torch.equal(both[0], alone[0]) and torch.equal(both[1], alone[1])
+    if rows == 0:
+        assert not both[1].any()
+
+
 @pytest.mark.parametrize("dt", ["f16", "bf16"])
 def test_large_tiles(dt):
     check(1500, 72, 9001, dt)
