@@ -1279,6 +1279,7 @@ int launch_product(args p, float* ws, hipStream_t st, int* parts_n = nullptr) {
 template <class T>
 inline bool is_few(int64_t rows, int64_t groups, int64_t N, int64_t K, bool loss = false) {
   if (rows <= 16) return true;
+  if (groups >= 65535) return false;  // (a launch's second dimension)
   const int64_t tiles = ceil_div(rows, 128) * ceil_div(N, 128);
   if (sizeof(T) == 4) return rows <= (loss ? (tiles <= 64 ? 192 : 64) : groups > 0 ? 32 * groups : 48);
   if (loss) return rows <= 48 && tiles <= 32;
