@@ -856,11 +856,11 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_tiles(args p) {
 }
 
 // ---- few rows ----------------------------------------------------------------------------------------------------
-// Products of at most 16 rows at a time with rows of k, bound by the one read of B: no LDS stages, every wave streams 16
-// COLS rows of B from memory straight to the matrix cores, eight loads of 1 KB ahead.  A workgroup's eight waves are `parts` of the
+// Products of at most 16 ROWS rows at a time with rows of k, bound by the one read of B: no LDS stages, every wave streams
+// 16 COLS rows of B from memory straight to the matrix cores, eight loads of 1 KB ahead.  A workgroup's eight waves are `parts` of the
 // reduction times 8 / parts blocks of 16 COLS columns; parts so that the chip has enough waves to keep its memory busy.  Groups
-// (BY_ROWS): blockIdx.y counts those that hold rows; a group of more than 16 rows reads its B again for every 16.
-template <class T, int COLS, int E>
+// (BY_ROWS): blockIdx.y counts those that hold rows; a group of more rows reads its B again for every 16 ROWS.
+template <class T, int COLS, int ROWS, int E>
 __global__ __launch_bounds__(512, 2) void k_few(args p, int parts) {
   typedef typename num<T>::piece piece;
   constexpr int CH = 16 / sizeof(T), STEP = 4 * CH, AHEAD = 8 / COLS;
@@ -899,126 +899,147 @@ __global__ __launch_bounds__(512, 2) void k_few(args p, int parts) {
   }
   const int64_t steps = (p.K + STEP - 1) / STEP, each = (steps + parts - 1) / parts;
   const int64_t k_from = part * each * STEP, k_to = k_from + each * STEP < p.K ? k_from + each * STEP : p.K;
-  for (; m0 < m_end; m0 += 16) {
-    const T* a_row = (const T*)p.A + (m0 + (lane & 15) < m_end ? m0 + (lane & 15) : m_end - 1) * p.lda + q * CH;
-    v4f acc[COLS];
+  for (; m0 < m_end; m0 += 16 * ROWS) {
+    const T* a_row[ROWS];
+    v4f sum[ROWS][COLS];
 #pragma unroll
-    for (int h = 0; h < COLS; h++) acc[h] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int r = 0; r < ROWS; r++) {
+      const int64_t m = m0 + r * 16 + (lane & 15);
+      a_row[r] = (const T*)p.A + (m < m_end ? m : m_end - 1) * p.lda + q * CH;
+#pragma unroll
+      for (int h = 0; h < COLS; h++) sum[r][h] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
     if (held && n0 < p.N) {
       int64_t k = k_from;
       for (; k + AHEAD * STEP <= k_to; k += AHEAD * STEP) {
-        loose<T, CH> fb[AHEAD][COLS], fa[AHEAD];
+        loose<T, CH> fb[AHEAD][COLS], fa[AHEAD][ROWS];
 #pragma unroll
         for (int u = 0; u < AHEAD; u++)
 #pragma unroll
           for (int h = 0; h < COLS; h++) fb[u][h] = *(const loose<T, CH>*)(b_row[h] + k + u * STEP);
 #pragma unroll
-        for (int u = 0; u < AHEAD; u++) fa[u] = *(const loose<T, CH>*)(a_row + k + u * STEP);
+        for (int u = 0; u < AHEAD; u++)
+#pragma unroll
+          for (int r = 0; r < ROWS; r++) fa[u][r] = *(const loose<T, CH>*)(a_row[r] + k + u * STEP);
 #pragma unroll
         for (int u = 0; u < AHEAD; u++)
 #pragma unroll
-          for (int h = 0; h < COLS; h++) acc[h] = mma((piece)fb[u][h], (piece)fa[u], acc[h]);
+          for (int r = 0; r < ROWS; r++)
+#pragma unroll
+            for (int h = 0; h < COLS; h++) sum[r][h] = mma((piece)fb[u][h], (piece)fa[u][r], sum[r][h]);
       }
       for (; k < k_to; k += STEP) {
-        piece fb[COLS], fa;
+        piece fb[COLS], fa[ROWS];
         const int there = p.K - k - q * CH < CH ? (int)(p.K - k - q * CH) : CH;
         if (there == CH) {
 #pragma unroll
           for (int h = 0; h < COLS; h++) fb[h] = *(const loose<T, CH>*)(b_row[h] + k);
-          fa = *(const loose<T, CH>*)(a_row + k);
+#pragma unroll
+          for (int r = 0; r < ROWS; r++) fa[r] = *(const loose<T, CH>*)(a_row[r] + k);
         } else {
 #pragma unroll
           for (int e = 0; e < CH; e++) {
 #pragma unroll
             for (int h = 0; h < COLS; h++) fb[h][e] = e < there ? b_row[h][k + e] : (T)0.f;
-            fa[e] = e < there ? a_row[k + e] : (T)0.f;
+#pragma unroll
+            for (int r = 0; r < ROWS; r++) fa[r][e] = e < there ? a_row[r][k + e] : (T)0.f;
           }
         }
 #pragma unroll
-        for (int h = 0; h < COLS; h++) acc[h] = mma(fb[h], fa, acc[h]);
+        for (int r = 0; r < ROWS; r++)
+#pragma unroll
+          for (int h = 0; h < COLS; h++) sum[r][h] = mma(fb[h], fa[r], sum[r][h]);
       }
     }
-    if (parts > 1) {
-      __syncthreads();  // (of the rows before)
 #pragma unroll
-      for (int h = 0; h < COLS; h++) sums[h][wave][lane] = acc[h];
-      __syncthreads();
-      if (part == 0)
-        for (int w = 1; w < parts; w++)
+    for (int r = 0; r < ROWS; r++) {
+      const int64_t m_top = m0 + r * 16;
+      if (m_top >= m_end) break;
+      v4f acc[COLS];
 #pragma unroll
-          for (int h = 0; h < COLS; h++) acc[h] += sums[h][wave + w][lane];
-    }
-    const int64_t m = m0 + (lane & 15);
-    if constexpr (E == E_LINEAR) {
+      for (int h = 0; h < COLS; h++) acc[h] = sum[r][h];
+      if (parts > 1) {
+        __syncthreads();  // (of the rows before)
 #pragma unroll
-      for (int h = 0; h < COLS; h++) {
-        const int64_t n = n0 + h * 16 + q * 4;
-        if (part != 0 || m >= m_end || n >= p.N) continue;
-        float v[4] = {acc[h][0], acc[h][1], acc[h][2], acc[h][3]}, b[4], r[4];
-        if (n + 4 <= p.N) {
-          bias_of<T, 4>(p, n, group, held, b);
-          residual_of<T, 4>(p, m, n, r);
-          finish_linear<T, 4>(p, m, n, v, b, r, held);
-        } else {
+        for (int h = 0; h < COLS; h++) sums[h][wave][lane] = acc[h];
+        __syncthreads();
+        if (part == 0)
+          for (int w = 1; w < parts; w++)
 #pragma unroll
-          for (int t = 0; t < 3; t++) {
-            if (n + t >= p.N) break;
-            bias_of<T, 1>(p, n + t, group, held, b);
-            residual_of<T, 1>(p, m, n + t, r);
-            finish_linear<T, 1>(p, m, n + t, v + t, b, r, held);
+            for (int h = 0; h < COLS; h++) acc[h] += sums[h][wave + w][lane];
+      }
+      const int64_t m = m_top + (lane & 15);
+      if constexpr (E == E_LINEAR) {
+#pragma unroll
+        for (int h = 0; h < COLS; h++) {
+          const int64_t n = n0 + h * 16 + q * 4;
+          if (part != 0 || m >= m_end || n >= p.N) continue;
+          float v[4] = {acc[h][0], acc[h][1], acc[h][2], acc[h][3]}, b[4], add[4];
+          if (n + 4 <= p.N) {
+            bias_of<T, 4>(p, n, group, held, b);
+            residual_of<T, 4>(p, m, n, add);
+            finish_linear<T, 4>(p, m, n, v, b, add, held);
+          } else {
+#pragma unroll
+            for (int t = 0; t < 3; t++) {
+              if (n + t >= p.N) break;
+              bias_of<T, 1>(p, n + t, group, held, b);
+              residual_of<T, 1>(p, m, n + t, add);
+              finish_linear<T, 1>(p, m, n + t, v + t, b, add, held);
+            }
           }
         }
-      }
-    } else if constexpr (E == E_LOSS_GRAD) {
-      // (at most 16 rows) out: fp32, [words][16]
-      if (part == 0) {
-        const int64_t label = m < m_end ? (int64_t)p.labels[m] : -1;
-        const float lse = label < 0 ? 0.f : p.lse[m], w = label < 0 ? 0.f : label >= p.words ? __builtin_nanf("") : p.dloss[m];
+      } else if constexpr (E == E_LOSS_GRAD) {
+        // (at most 16 rows) out: fp32, [words][16]
+        if (part == 0) {
+          const int64_t label = m < m_end ? (int64_t)p.labels[m] : -1;
+          const float lse = label < 0 ? 0.f : p.lse[m], w = label < 0 ? 0.f : label >= p.words ? __builtin_nanf("") : p.dloss[m];
 #pragma unroll
-        for (int h = 0; h < COLS; h++)
+          for (int h = 0; h < COLS; h++)
 #pragma unroll
-          for (int t = 0; t < 4; t++) {
-            const int64_t n = n0 + h * 16 + q * 4 + t;
-            const float g = label < 0 ? 0.f : (__expf(acc[h][t] - lse) - (n == label ? 1.f : 0.f)) * w;
-            if (n < p.N) ((float*)p.out)[n * 16 + (lane & 15)] = g;
-          }
-      }
-    } else {
-      if (part == 0) {
-        const int64_t label = m < m_end ? (int64_t)p.labels[m] : -1;
-        float top = -INFINITY, sum = 0.f;
-#pragma unroll
-        for (int h = 0; h < COLS; h++)
-#pragma unroll
-          for (int t = 0; t < 4; t++) {
-            const int64_t n = n0 + h * 16 + q * 4 + t;
-            if (n < p.N) top = fmaxf(top, acc[h][t]);
-            if (n == label && n < p.N) p.hit[m] = acc[h][t];
-          }
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float from = top == -INFINITY ? 0.f : top;
-#pragma unroll
-        for (int h = 0; h < COLS; h++)
-#pragma unroll
-          for (int t = 0; t < 4; t++)
-            if (n0 + h * 16 + q * 4 + t < p.N) sum += __expf(acc[h][t] - from);
-        sum += __shfl_xor(sum, 16, 64);
-        sum += __shfl_xor(sum, 32, 64);
-        if (q == 0) stats[wave][lane] = float2{top, sum};
-      }
-      __syncthreads();
-      if (threadIdx.x < 16 && m0 + threadIdx.x < m_end) {
-        float top = -INFINITY, sum = 0.f;
-        for (int w = 0; w < 8; w += parts) top = fmaxf(top, stats[w][threadIdx.x].x);
-        const float from = top == -INFINITY ? 0.f : top;
-        for (int w = 0; w < 8; w += parts) {
-          const float2 s = stats[w][threadIdx.x];
-          if (s.x != -INFINITY || s.y != 0.f) sum += s.y * __expf(s.x - from);
+            for (int t = 0; t < 4; t++) {
+              const int64_t n = n0 + h * 16 + q * 4 + t;
+              const float g = label < 0 ? 0.f : (__expf(acc[h][t] - lse) - (n == label ? 1.f : 0.f)) * w;
+              if (n < p.N) ((float*)p.out)[n * 16 + (lane & 15)] = g;
+            }
         }
-        p.parts[(m0 + threadIdx.x) * p.parts_n + blockIdx.x] = float2{top, sum};
+      } else {
+        if (part == 0) {
+          const int64_t label = m < m_end ? (int64_t)p.labels[m] : -1;
+          float top = -INFINITY, sum = 0.f;
+#pragma unroll
+          for (int h = 0; h < COLS; h++)
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+              const int64_t n = n0 + h * 16 + q * 4 + t;
+              if (n < p.N) top = fmaxf(top, acc[h][t]);
+              if (n == label && n < p.N) p.hit[m] = acc[h][t];
+            }
+          top = fmaxf(top, __shfl_xor(top, 16, 64));
+          top = fmaxf(top, __shfl_xor(top, 32, 64));
+          const float from = top == -INFINITY ? 0.f : top;
+#pragma unroll
+          for (int h = 0; h < COLS; h++)
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+              if (n0 + h * 16 + q * 4 + t < p.N) sum += __expf(acc[h][t] - from);
+          sum += __shfl_xor(sum, 16, 64);
+          sum += __shfl_xor(sum, 32, 64);
+          if (q == 0) stats[wave][lane] = float2{top, sum};
+        }
+        __syncthreads();
+        if (threadIdx.x < 16 && m_top + threadIdx.x < m_end) {
+          float top = -INFINITY, sum = 0.f;
+          for (int w = 0; w < 8; w += parts) top = fmaxf(top, stats[w][threadIdx.x].x);
+          const float from = top == -INFINITY ? 0.f : top;
+          for (int w = 0; w < 8; w += parts) {
+            const float2 s = stats[w][threadIdx.x];
+            if (s.x != -INFINITY || s.y != 0.f) sum += s.y * __expf(s.x - from);
+          }
+          p.parts[(m_top + threadIdx.x) * p.parts_n + blockIdx.x] = float2{top, sum};
+        }
+        __syncthreads();
       }
-      __syncthreads();
     }
   }
 }
@@ -1270,18 +1291,18 @@ int launch_product(args p, float* ws, hipStream_t st, int* parts_n = nullptr) {
   X template int launch_product<T, false, false, E_STORE>(args, float*, hipStream_t, int*);
 
 // Few rows: how many, and a product of them (which takes its operands as they lie).  *parts_n as above.  fp32 has its packing to gain,
-// and so more rows (us in tiles and here): 16384 x 4096 of 32 rows 254 and 140, of 48 259 and 199, of 64 263 and 265; 61 groups of
-// 1005 x 2048 with 32 rows each 580 and 463, 48 each 583 and 656; the loss of 64000 x 2048 of 64 rows 594 and 445, of 96 594 and 653.
-// The loss's tiles cannot split the reduction: where they are few, more rows (3220 x 2296 of 192 rows, fp32: 146 and 96; 48 in bf16 26
-// and 19, 16384 x 1024 in bf16 of 17 18 and 20).  Small layers save the launch that joins a split (1024 x 1024 of 48 rows in bf16 13
-// and 9, 4096 x 1024 13 and 9, 1024 x 4096 13 and 15).  16-bit groups of two rows each: 32 of 2048 x 1024 20 and 23, 61 of 1005 x
-// 2048 32 and 41.
+// and so more rows (us in tiles and here): 16384 x 4096 of 32 rows 254 and 95, of 64 262 and 147, of 96 267 and 251, 4096 x 1024 of 64 45
+// and 40, of 96 45 and 67; 61 groups of 1005 x 2048 with 64 rows each 698 and 536; the loss of 64000 x 2048 of 128 rows 592 and 470.
+// The loss's tiles cannot split the reduction: where they are few, more rows (3220 x 2296 of 256 rows, fp32: 152
+// and 89; 48 in bf16 26 and 16, 16384 x 1024 in bf16 of 17 18 and 20).  Small layers save the launch that joins a split (1024 x 1024
+// of 48 rows in bf16 13 and 9, 4096 x 1024 13 and 9, 1024 x 4096 13 and 15).  16-bit groups of two rows each: 32 of 2048 x 1024 20 and
+// 23, 61 of 1005 x 2048 32 and 41.
 template <class T>
 inline bool is_few(int64_t rows, int64_t groups, int64_t N, int64_t K, bool loss = false) {
   if (rows <= 16) return true;
   if (groups >= 65535) return false;  // (a launch's second dimension)
   const int64_t tiles = ceil_div(rows, 128) * ceil_div(N, 128);
-  if (sizeof(T) == 4) return rows <= (loss ? (tiles <= 64 ? 192 : 64) : groups > 0 ? 32 * groups : 48);
+  if (sizeof(T) == 4) return rows <= (loss ? (tiles <= 64 ? 256 : 128) : groups > 0 ? 64 * groups : 64);
   if (loss) return rows <= 48 && tiles <= 32;
   return groups > 0 ? rows <= groups : rows <= 48 && tiles <= 32 && K <= 2048;
 }
@@ -1301,10 +1322,22 @@ int launch_few(args p, hipStream_t st, int* parts_n = nullptr) {
   p.parts_n = (int)ceil_div(p.N, cols);
   if (parts_n) *parts_n = p.parts_n;
   const dim3 grid((unsigned)ceil_div(p.N, cols), (unsigned)slots);
-  if (wide == 32)
-    k_few<T, 2, E><<<grid, 512, 0, st>>>(p, parts);
-  else
-    k_few<T, 1, E><<<grid, 512, 0, st>>>(p, parts);
+  // 16, 32 or 64 rows for each reading of B (fp32 products of 64000 x 2048, 16 at a time and so: 32 rows 266 and 164 us, 48 391 and
+  // 233, the loss of 64 rows 449 and 253)
+  const int64_t each = p.mode == BY_ROWS ? ceil_div(p.M, p.G.groups) : p.M;
+  const int rows = E == E_LOSS_GRAD || each <= 16 ? 1 : each <= 32 ? 2 : 4;
+  auto launch = [&](auto cols_of, auto rows_of) { k_few<T, decltype(cols_of)::value, decltype(rows_of)::value, E><<<grid, 512, 0, st>>>(p, parts); };
+  auto launch_cols = [&](auto rows_of) {
+    if (wide == 32)
+      launch(std::integral_constant<int, 2>(), rows_of);
+    else
+      launch(std::integral_constant<int, 1>(), rows_of);
+  };
+  if constexpr (E != E_LOSS_GRAD) {
+    if (rows == 4) launch_cols(std::integral_constant<int, 4>());
+    if (rows == 2) launch_cols(std::integral_constant<int, 2>());
+  }
+  if (rows == 1) launch_cols(std::integral_constant<int, 1>());
   DN_LAUNCH_CHECK();
   return 0;
 }

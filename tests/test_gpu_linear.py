@@ -337,6 +337,18 @@ def test_whole_rounds_of_large_tiles_and_a_rest(rows, n_out, dt):
         check_backward(200, rows, n_out, dt, seed=3)              # dW [n_out, rows]
 
 
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("rows, n_in, n_out", [(33, 129, 1001), (48, 70, 33), (64, 515, 2000), (65, 515, 300)])
+def test_a_few_dozen_rows(rows, n_in, n_out, dt):
+    check_forward(rows, n_in, n_out, dt, act="gelu_tanh", bias=True, residual=True, lay=(3, 1), seed=rows)
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("sizes", [[0, 70, 3, 33, 0, 129], [20, 0, 40, 1], [5, 16, 17, 15]])
+def test_groups_of_a_few_dozen_rows(sizes, dt):
+    check_forward(sum(sizes), 100, 130, dt, act="silu", bias=True, sizes=sizes, seed=4)
+
+
 def test_offsets_past_32_bits():
     """70,000 rows that are 40,000 elements apart: more than 2^31 of them, and 5.6 GB, between the first and the last."""
     big = torch.empty(70_000 * 40_000, dtype=torch.bfloat16, device="cuda").view(70_000, 40_000)

@@ -96,7 +96,8 @@ def test_strides(extra, dt):
 
 @pytest.mark.parametrize("dt", list(DTYPES))
 @pytest.mark.parametrize("rows, n_in, words, extra", [(1, 4, 700, 0), (3, 257, 9001, 1), (4, 1030, 513, 3), (5, 3, 300, 0), (9, 515, 20_000, 8),
-                                                      (16, 1003, 65, 5), (16, 5, 7, 0), (33, 130, 3000, 1), (64, 72, 1000, 0)])
+                                                      (16, 1003, 65, 5), (16, 5, 7, 0), (33, 130, 3000, 1), (64, 72, 1000, 0),
+                                                      (128, 100, 20_000, 0), (250, 66, 901, 1)])
 def test_few_tokens(rows, n_in, words, extra, dt):
     check(rows, n_in, words, dt, extra=extra, seed=rows)
 
