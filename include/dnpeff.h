@@ -626,8 +626,8 @@ int dnpeff_vocab_loss(void* stream, int type, int64_t rows, int64_t n_in, int64_
 /* Its gradients for dloss [rows], the gradients of the tokens' losses, from the lse of the forward call: dX [rows,
  * n_in] and dE [n_words, n_in], either may be NULL.  The vocabulary goes by in pieces whose logits are formed again;
  * (softmax - label) dloss is rounded to `type` once for the products (16-bit types: after dividing by the largest
- * |dloss|, which fp32 puts back; of few tokens it stays fp32 and whole). Tokens without a label contribute nothing; a label of n_words and more makes dX's
- * row and dE NaN. */
+ * |dloss|, which fp32 puts back; of few tokens it stays fp32 and whole). Tokens without a label contribute nothing, whatever
+ * their rows of X hold (for dE, X is copied without them); a label of n_words and more makes dX's row and dE NaN. */
 int dnpeff_vocab_loss_backward(void* stream, int type, int64_t rows, int64_t n_in, int64_t n_words, const void* X, int64_t ldx,
                                const void* E, int64_t lde, const int32_t* labels, const float* lse, const float* dloss, void* dX,
                                int64_t lddx, void* dE, int64_t ldde, void* workspace, int64_t workspace_bytes);

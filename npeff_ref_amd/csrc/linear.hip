@@ -120,9 +120,9 @@ int check_act(const char* what, int act) {
 }
 group_rows rows_of(const layer& l) { return group_rows{l.ends, l.grouped() ? l.groups : 1, l.rows}; }
 
-matrix rows_matrix(const layer& l, const void* p, int64_t ld, int64_t width) { return matrix{p, ld, l.rows, width, 1, 0, 0}; }
+matrix rows_matrix(const layer& l, const void* p, int64_t ld, int64_t width) { return matrix{p, ld, l.rows, width, 1, 0, 0, nullptr}; }
 matrix weight_matrix(const layer& l, const void* p, int64_t ld, int64_t sheet) {
-  return matrix{p, ld, l.n_out, l.n_in, l.grouped() ? l.groups : 1, sheet, 0};
+  return matrix{p, ld, l.n_out, l.n_in, l.grouped() ? l.groups : 1, sheet, 0, nullptr};
 }
 
 // Parts of a workspace: copies of operands that do not lie well, then the rest.

@@ -1152,17 +1152,19 @@ inline int64_t split_floats(int64_t M, int64_t N, int64_t K) {
 // ---- operands that tiles can be loaded from -----------------------------------------------------------------------
 // A matrix of 16-bit values whose rows begin on 16 bytes and end on them is loaded as it lies; any other is first copied to rows
 // that do, with zeros behind their ends (k_pack): once, where a tile's loads would come from any address again and again.  fp32
-// is copied to its three planes.
+// is copied to its three planes, and a matrix whose rows do not all count to one where the others are zero (a product of zeros
+// with them would not be: they may hold infinities or NaN).
 struct matrix {
   const void* p;
   int64_t ld, rows, width;
   int64_t sheets, sheet;  // and so many such, so far apart
   int64_t plane;          // (packed fp32) and its planes
+  const int32_t* keep;    // (NULL: all) rows of a negative word are copied as zeros, whatever they hold
 };
 template <class T>
 inline bool lies_well(const matrix& m) {
   constexpr int64_t S = sizeof(T), NEAR = (int64_t)1 << 31;
-  return S == 2 && (uintptr_t)m.p % 16 == 0 && m.ld * S % 16 == 0 && m.width * S % 16 == 0 && (m.sheets < 2 || m.sheet * S % 16 == 0) &&
+  return S == 2 && m.keep == nullptr && (uintptr_t)m.p % 16 == 0 && m.ld * S % 16 == 0 && m.width * S % 16 == 0 && (m.sheets < 2 || m.sheet * S % 16 == 0) &&
          32 * m.ld * S < NEAR;
 }
 inline int64_t packed_ld(int64_t width) { return ceil_div(width, 64) * 64; }
@@ -1184,7 +1186,7 @@ __global__ __launch_bounds__(256) void k_pack(pack_args p) {
   const int64_t ld = (m.width + 63) / 64 * 64, per_row = ld / CH;
   const int64_t at = ((int64_t)blockIdx.x - p.first[w]) * 256 + threadIdx.x, row = at / per_row;
   if (row >= m.rows * m.sheets) return;
-  const int c = (int)(at - row * per_row) * CH, there = (int)(m.width - c);
+  const int c = (int)(at - row * per_row) * CH, there = m.keep && m.keep[row] < 0 ? 0 : (int)(m.width - c);
   const T* src = (const T*)m.p + (m.sheets > 1 ? row / m.rows * m.sheet + row % m.rows * m.ld : row * m.ld) + c;
   float v[CH];
   if (there >= CH) {

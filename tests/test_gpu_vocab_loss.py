@@ -217,6 +217,30 @@ def test_masked_rows_may_hold_anything():
     assert all(torch.equal(a, b) for a, b in zip(out[0], out[1])) and all(torch.equal(a, b) for a, b in zip(out[0], out[2]))
 
 
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("rows, extra", [(3, 0), (8, 1), (12, 0), (70, 0), (70, 1), (300, 8)])
+def test_masked_rows_do_not_reach_the_embeddings(rows, extra, dt):
+    """The same bits in all gradients whatever the state of a row without a label holds: infinities and NaN too."""
+    X, E = rand((rows, 72), dt, 1), rand((900, 72), dt, 2, 0.3)
+    y = labels_of(rows, 900, 3)
+    y[1], y[2] = -1, 17
+    dl, out = torch.ones(rows, device="cuda"), []
+    for bad in (0.0, float("inf"), float("nan")):
+        X[1] = 0
+        X[1, ::5] = bad
+        x, e = padded(X, extra), padded(E, extra)
+        loss, lse = torch.zeros(rows, device="cuda"), torch.zeros(rows, device="cuda")
+        d.op_vocab_loss(x, e, y, loss, lse)
+        gx, ge, alone = torch.ones_like(X), torch.ones_like(E), torch.ones_like(E)
+        d.op_vocab_loss_backward(x, e, y, lse, dl, dX=gx, dE=ge)
+        d.op_vocab_loss_backward(x, e, y, lse, dl, dE=alone)
+        assert torch.isfinite(ge).all() and not gx[1].any() and loss[1] == 0
+        assert torch.equal(ge, alone)
+        out.append((loss, gx, ge))
+    for other in out[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(out[0], other))
+
+
 def test_gradient_against_differences():
     rows, n_in, words = 5, 7, 11
     X, E, y = rand((rows, n_in), "f32", 1), rand((words, n_in), "f32", 2), labels_of(rows, words, 3)
