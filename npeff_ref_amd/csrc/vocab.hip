@@ -67,7 +67,7 @@ __global__ __launch_bounds__(1024) void k_shrink(int64_t rows, const int32_t* la
   if (threadIdx.x == 0) {
     for (int i = 1; i < 16; i++) most = fmaxf(most, side[i]);
     const float top = std::is_same<T, _Float16>::value ? 16384.f : 1.f;
-    most = most > 0.f ? fmaxf(most, 1e-36f) : 1.f;
+    most = most > 0.f ? fmaxf(most, top * 1e-36f) : 1.f;  // (top / most stays finite)
     both[0] = top / most;
     both[1] = most / top;
   }

@@ -139,6 +139,25 @@ def test_weights_of_any_size(weight, dt):
 
 
 @pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("rows", [3, 64])
+@pytest.mark.parametrize("weights", [(1e-36,), (1e-36, 0.0), (4e-35, 0.0, -1e-38), (1e-42, 0.0)])
+def test_weights_next_to_nothing(weights, rows, dt):
+    """Gradients are at most a weight times the sum of 2 for each row and the size of X or E: zero in fp16, and never more than that."""
+    X, E, y = rand((rows, 40), dt, 1), rand((300, 40), dt, 2, 0.3), labels_of(rows, 300, 3, masked=0.0)
+    dl = torch.tensor([weights[i % len(weights)] for i in range(rows)]).cuda()
+    loss, lse = torch.zeros(rows, device="cuda"), torch.zeros(rows, device="cuda")
+    d.op_vocab_loss(X, E, y, loss, lse)
+    gx, ge = torch.ones_like(X), torch.ones_like(E)
+    d.op_vocab_loss_backward(X, E, y, lse, dl, dX=gx, dE=ge)
+    most = 2 * dl.abs().max().item() * 1.01
+    assert gx.abs().max().item() <= most * E.abs().max().item() and ge.abs().max().item() <= most * rows * X.abs().max().item()
+    if dt == "f16":
+        assert not gx.any() and not ge.any()
+    elif max(weights) > 1e-36:
+        assert gx.any() and ge.any()
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
 def test_large_logits(dt):
     check(64, 64, 500, dt, scale=20.0)
 
