@@ -547,16 +547,29 @@ class _Call:
             _refuse(self.what, f"tensors on device {self.place}, and another one is the current device")
         return torch.cuda.current_stream(self.place).cuda_stream
 
+    def room(self, w):
+        """(address, bytes) of a caller's workspace: the GPU writes all of it, so it has to be the GPU's, and in one piece."""
+        if isinstance(w, DeviceArray):
+            if w.ptr is None:
+                _refuse(self.what, "the workspace has been freed")
+            return w.ptr.value, w.nbytes
+        if not getattr(w, "is_cuda", False):
+            _refuse(self.what, "the workspace is not on the GPU")
+        if self.own and lib.without_torch:
+            _refuse(self.what, "a tensor as workspace, but torch was imported after the library's first call")
+        if w.get_device() != (sys.modules["torch"].cuda.current_device() if self.own else self.place):
+            _refuse(self.what, f"the workspace is on {w.device}")
+        if not w.is_contiguous():
+            _refuse(self.what, "the workspace has to be dense")
+        return w.data_ptr(), w.numel() * w.element_size()
+
     def run(self, fn, args, bytes_needed, workspace, stream):
         """fn(stream, *args, workspace, bytes), with a workspace of the call's own where none is given."""
         st = self.stream(stream)
         if workspace is None and bytes_needed == 0:
             status = fn(st, *args, None, 0)
         elif workspace is not None:
-            if isinstance(workspace, DeviceArray):
-                status = fn(st, *args, workspace.ptr.value, workspace.nbytes)
-            else:
-                status = fn(st, *args, workspace.data_ptr(), workspace.numel() * workspace.element_size())
+            status = fn(st, *args, *self.room(workspace))
         elif stream is not None and not (self.own and stream == lib.dnpeff_stream()):
             _refuse(self.what, "a workspace has to be given with a stream")
         elif not self.own:

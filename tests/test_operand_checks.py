@@ -1,0 +1,76 @@
+"""What the op_* calls refuse before anything is queued: no GPU is needed to see it."""
+
+import numpy as np
+import pytest
+import torch
+
+import npeff_ref_amd as d
+from npeff_ref_amd import binding
+
+
+class OnGpu:
+    """What a tensor on a GPU tells about itself."""
+
+    is_cuda, shape, dtype = True, (64,), torch.float32
+
+    def __init__(self, device=0, dense=True):
+        self.at, self.dense, self.device = device, dense, f"cuda:{device}"
+
+    def get_device(self):
+        return self.at
+
+    def is_contiguous(self):
+        return self.dense
+
+    def data_ptr(self):
+        return 4096
+
+    def numel(self):
+        return 64
+
+    def element_size(self):
+        return 4
+
+
+def call_of(own):
+    c = object.__new__(binding._Call)
+    c.what, c.own, c.place, c.type, c.first = "op", own, -2 if own else 0, binding.F32, None
+    return c
+
+
+@pytest.fixture
+def device0(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+
+
+@pytest.mark.parametrize("own", [False, True])
+@pytest.mark.parametrize("bad", ["host", "host_bytes", "array", "number", "strided", "elsewhere", "freed"])
+def test_a_workspace_is_looked_at(own, bad, device0):
+    freed = object.__new__(d.DeviceArray)
+    freed.shape, freed.dtype, freed.nbytes, freed.ptr = (64,), np.dtype(np.float32), 256, None
+    w = {
+        "host": torch.empty(64),
+        "host_bytes": torch.empty(256, dtype=torch.uint8)[::2],
+        "array": np.empty(64),
+        "number": 4096,
+        "strided": OnGpu(dense=False),
+        "elsewhere": OnGpu(device=1),
+        "freed": freed,
+    }[bad]
+    called = []
+    with pytest.raises(d.DnpeffError, match="workspace"):
+        call_of(own).run(lambda *a: called.append(a), (), 128, w, 7)
+    assert not called
+
+
+@pytest.mark.parametrize("own", [False, True])
+def test_a_workspace_on_the_gpu_is_passed_on(own, device0):
+    called = []
+    call_of(own).run(lambda *a: called.append(a), (1, 2), 128, OnGpu(), 7)
+    assert called == [(7, 1, 2, 4096, 256)]
+
+
+def test_a_second_runtime_gets_no_workspace(device0, monkeypatch):
+    monkeypatch.setattr(binding.lib, "without_torch", True)
+    with pytest.raises(d.DnpeffError, match="torch was imported after"):
+        call_of(True).run(lambda *a: 0, (), 128, OnGpu(), 7)
