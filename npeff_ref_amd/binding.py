@@ -337,6 +337,10 @@ class DeviceArray:
         it.  Its own work has to be finished, or ordered before the library's stream."""
         if not t.is_cuda or not t.is_contiguous() or str(t.dtype) not in _VIEWED:
             raise DnpeffError(f"a view of {tuple(t.shape)} {t.dtype} on {t.device}: a dense tensor on the GPU is wanted")
+        if lib.without_torch:
+            raise DnpeffError("a view of a tensor, but torch was imported after the library's first call, with a HIP runtime of its own")
+        if t.get_device() != sys.modules["torch"].cuda.current_device():
+            raise DnpeffError(f"a view of a tensor on {t.device}, and another device is the current one")
         d = object.__new__(DeviceArray)
         d.shape, d.dtype, d._owner = tuple(t.shape), np.dtype(_VIEWED[str(t.dtype)]), t
         d.nbytes = t.numel() * t.element_size()

@@ -74,3 +74,12 @@ def test_a_second_runtime_gets_no_workspace(device0, monkeypatch):
     monkeypatch.setattr(binding.lib, "without_torch", True)
     with pytest.raises(d.DnpeffError, match="torch was imported after"):
         call_of(True).run(lambda *a: 0, (), 128, OnGpu(), 7)
+
+
+def test_views_of_memory_that_the_library_cannot_reach(device0, monkeypatch):
+    assert d.DeviceArray.view(OnGpu()).ptr.value == 4096
+    with pytest.raises(d.DnpeffError, match="current"):
+        d.DeviceArray.view(OnGpu(device=1))
+    monkeypatch.setattr(binding.lib, "without_torch", True)
+    with pytest.raises(d.DnpeffError, match="torch was imported after"):
+        d.DeviceArray.view(OnGpu())
