@@ -82,7 +82,7 @@ __global__ __launch_bounds__(256) void k_bias_sums(group_rows G, int64_t N, cons
   int before = 0;
   for (int b = 0; b < g; b += 64) {
     const int t = b + lane < g ? (int)((G.count(b + lane) + tall - 1) / tall) : 0;
-    before += __shfl(wave_scan(t, lane), 63, 64);
+    before = add_up(before, __shfl(wave_scan(t, lane), 63, 64));
   }
   int tiles = (int)((G.count(g) + tall - 1) / tall);
   if (tiles > tiles_most - before) tiles = tiles_most - before;  // (groups that overlap: no more than there were)
@@ -94,7 +94,7 @@ __global__ __launch_bounds__(256) void k_bias_sums(group_rows G, int64_t N, cons
   db[g * N + n] = (T)s;
 }
 
-int64_t slope_tiles(int64_t rows, int groups, int tall) { return rows / tall + (groups + 1 < rows ? groups + 1 : rows); }
+int64_t slope_tiles(int64_t rows, int groups, int tall) { return group_rows{nullptr, groups, rows}.most_tiles(tall); }
 
 struct layer {
   int64_t rows, n_in, n_out;

@@ -157,8 +157,9 @@ __device__ __forceinline__ void slopes_of(float* v, const float* z, int act) {
 
 // ---- rows in groups ----------------------------------------------------------------------------------------------
 // Group g holds rows ends[g] .. ends[g + 1] (the first from row 0, whatever ends[0] says); rows past the last
-// end belong to none and count as group `groups`.  Ends outside the rows, or falling, are taken as the nearest
-// that do not: no read or write goes by them unchecked.
+// end belong to none and count as group `groups`.  Ends outside the rows are taken as the nearest inside, a group whose end
+// falls is empty.  Groups may then overlap, and their tiles add up to more than there can be: counts of tiles stop at
+// 2^31 - 1, and launches at most_tiles, so no read or write goes by the ends unchecked.
 struct group_rows {
   const int64_t* ends;
   int groups;
@@ -182,13 +183,16 @@ struct group_rows {
     const int64_t n = last(g) - first(g);
     return n > 0 ? n : 0;
   }
+  // Tiles of `tall` rows that groups which do not overlap take at most.
+  __host__ __device__ __forceinline__ int64_t most_tiles(int tall) const { return rows / tall + (groups + 1 < rows ? groups + 1 : rows); }
 };
 
-__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive sum over the lanes
+__device__ __forceinline__ int add_up(int a, int b) { return __builtin_elementwise_add_sat(a, b); }
+__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive sum over the lanes, of counts; 2^31 - 1 at most
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
     const int u = __shfl_up(v, d, 64);
-    if (lane >= d) v += u;
+    if (lane >= d) v = add_up(v, u);
   }
   return v;
 }
@@ -198,22 +202,23 @@ __device__ __forceinline__ int group_tiles(const group_rows& G, int tall, int la
   for (int b = 0; b <= G.groups; b += 64) {
     const int g = b + lane;
     const int t = g <= G.groups ? (int)((G.count(g) + tall - 1) / tall) : 0;
-    sum += __shfl(wave_scan(t, lane), 63, 64);
+    sum = add_up(sum, __shfl(wave_scan(t, lane), 63, 64));
   }
-  return sum;
+  const int64_t most = G.most_tiles(tall);
+  return sum < most ? sum : (int)most;
 }
-// The group of tile `tile` of them, its number within that group, and (tiles_before) the tiles of the groups before it.
+// The group of tile `tile` of them, and its number within that group.
 __device__ __forceinline__ void group_of_tile(const group_rows& G, int tall, int lane, int tile, int* group, int* within) {
   int before = 0;
   for (int b = 0; b <= G.groups; b += 64) {
     const int g = b + lane;
     const int t = g <= G.groups ? (int)((G.count(g) + tall - 1) / tall) : 0;
-    const int upto = before + wave_scan(t, lane);
+    const int upto = add_up(before, wave_scan(t, lane));
     const unsigned long long hit = __ballot(tile < upto);
     if (hit) {
       const int l = __ffsll(hit) - 1;
       *group = __builtin_amdgcn_readfirstlane(b + l);
-      *within = __builtin_amdgcn_readfirstlane(tile - __shfl(upto - t, l, 64));
+      *within = __builtin_amdgcn_readfirstlane(tile - (l > 0 ? __shfl(upto, l - 1, 64) : before));  // (what is not past `tile` is exact)
       return;
     }
     before = __shfl(upto, 63, 64);
@@ -1226,7 +1231,7 @@ int launch_tiles(const args& p, hipStream_t st) {
   const int64_t nt = ceil_div(p.N, BN) - p.tn_first;
   int64_t mt = ceil_div(p.M, BM) - p.tm_first, sheets = 1;
   if (p.mode == BY_ROWS)
-    mt = p.G.rows / BM + (p.G.groups + 1 < p.G.rows ? p.G.groups + 1 : p.G.rows);
+    mt = p.G.most_tiles(BM);
   else
     sheets = p.mode == BY_REDUCTION ? p.G.groups : p.splits;
   const int64_t many = mt * nt * sheets;

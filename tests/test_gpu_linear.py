@@ -272,6 +272,23 @@ def test_falling_and_wild_ends_stay_inside():
         assert (guard[[0, 65]] == 3).all() and (dW[[0, 5]] == 3).all() and (db[[0, 5]] == 3).all()
 
 
+def test_overlapping_groups_of_more_tiles_than_32_bits_count():
+    """65534 groups whose ends go up to all rows and down again: 2.3e9 tiles of 128 rows by their counts.  As above, every access is
+    inside the arrays."""
+    rows, groups = 9_000_000, 65_534
+    ends = torch.zeros(groups + 1, dtype=torch.int64)
+    ends[1::2] = rows
+    ends = ends.cuda()
+    X = torch.ones(rows, 8, dtype=torch.bfloat16, device="cuda")
+    W = torch.ones(groups, 8, 8, dtype=torch.bfloat16, device="cuda")
+    Y, dX = [torch.full((rows + 2, 8), 3.0, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    db = torch.full((groups + 2, 8), 3.0, dtype=torch.bfloat16, device="cuda")
+    d.op_linear(X, W, Y[1:-1], groups=ends)
+    d.op_linear_backward(X, X, W, pre=X, act="relu", dX=dX[1:-1], dbias=db[1:-1], groups=ends)
+    torch.cuda.synchronize()
+    assert (Y[[0, -1]] == 3).all() and (dX[[0, -1]] == 3).all() and (db[[0, -1]] == 3).all()
+
+
 def test_same_bits_again_and_on_another_stream():
     X, W = rand((500, 1000), "bf16", 1), rand((300, 1000), "bf16", 2)
     Y = [torch.zeros(500, 300, dtype=torch.bfloat16, device="cuda") for _ in range(3)]
