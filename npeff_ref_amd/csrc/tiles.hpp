@@ -87,10 +87,10 @@ __device__ __forceinline__ float sigmoid(float z) {
   if (EXACT) return 1.f / (1.f + expf(-z));
   return __builtin_amdgcn_rcpf(1.f + __expf(-z));
 }
+// (1 + tanh(u)) / 2 = sigmoid(2u): by itself, so that what is left of it below zero is not rounded away next to 1
 template <bool EXACT>
-__device__ __forceinline__ float gelu_tanh_t(float z) {
-  // tanh(u) = 2 sigmoid(2u) - 1
-  return 2.f * sigmoid<EXACT>(1.5957691216057308f * (z + 0.044715f * z * z * z)) - 1.f;
+__device__ __forceinline__ float gelu_tanh_s(float z) {
+  return sigmoid<EXACT>(1.5957691216057308f * (z + 0.044715f * z * z * z));
 }
 // The normal distribution's Phi(z), and *e = exp(-z^2 / 2).  16-bit results: erfc(x) = exp(-x^2) t Q(t) for x >= 0 with
 // t = 1 / (1 + 0.45 x) and Q the polynomial of degree 7 whose largest relative error on [0, 12] is smallest (fitted for this:
@@ -124,7 +124,7 @@ __device__ __forceinline__ void act_of(float* z, int act) {
     }
   } else if (act == DNPEFF_ACT_GELU_TANH) {
 #pragma unroll
-    for (int t = 0; t < W; t++) z[t] *= 0.5f * (1.f + gelu_tanh_t<EXACT>(z[t]));
+    for (int t = 0; t < W; t++) z[t] *= gelu_tanh_s<EXACT>(z[t]);
   }
 }
 // v *= act'(z)
@@ -149,8 +149,8 @@ __device__ __forceinline__ void slopes_of(float* v, const float* z, int act) {
   } else if (act == DNPEFF_ACT_GELU_TANH) {
 #pragma unroll
     for (int t = 0; t < W; t++) {
-      const float u = gelu_tanh_t<EXACT>(z[t]);
-      v[t] *= 0.5f * (1.f + u) + 0.5f * z[t] * (1.f - u * u) * 0.79788456080286536f * (1.f + 0.134145f * z[t] * z[t]);
+      const float s = gelu_tanh_s<EXACT>(z[t]);
+      v[t] *= s + z[t] * (s * (1.f - s)) * 1.5957691216057308f * (1.f + 0.134145f * z[t] * z[t]);
     }
   }
 }

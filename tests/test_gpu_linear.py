@@ -153,6 +153,33 @@ def test_activations(act, dt):
 
 
 @pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+@pytest.mark.parametrize("rows", [16, 200])
+def test_left_tail_of_activations(rows, act, dt):
+    """z s(w) and its slope, s the logistic function and w = z or sqrt(8 / pi) (z + 0.044715 z^3), by their own size at z from -8 to -3: w is
+    off by 9 units of 2^-24 with the exponential's argument, s and what is made of it by a few more."""
+    z = torch.linspace(-8, -3, rows).to(DTYPES[dt])
+    one = torch.ones(24, 1, dtype=DTYPES[dt], device="cuda")
+    X = z[:, None].cuda()
+    Y = torch.zeros(rows, 24, dtype=DTYPES[dt], device="cuda")
+    d.op_linear(X, one, Y, act=act)
+    z64 = z.double().requires_grad_(True)
+    w = z64 if act == "silu" else (8 / np.pi) ** 0.5 * (z64 + 0.044715 * z64**3)
+    want = z64 * torch.sigmoid(w)  # (1 + tanh in 64 bits has nothing left at -8 either)
+    want.sum().backward()
+    w = w.detach()
+    near = (9 * w.abs() + 30) * EPS32
+    s = torch.sigmoid(w)
+    for got in Y.double().cpu().T:
+        assert ((got - want.detach()).abs() <= want.detach().abs() * (near + 1.01 * HALF[dt]) + TINY[dt]).all()
+    dX = torch.zeros_like(X)
+    d.op_linear_backward(torch.ones(rows, 1, dtype=DTYPES[dt], device="cuda"), X, one[:1], pre=X, act=act, dX=dX)
+    terms = s + (z64.grad - s).abs()  # (the slope is the difference of two such)
+    off = (dX[:, 0].double().cpu() - z64.grad).abs()
+    assert (off <= terms * near + z64.grad.abs() * 2.1 * HALF[dt] + 2 * TINY[dt]).all()
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
 @pytest.mark.parametrize("lay", [(8, 0), (8, 8), (1, 0), (3, 1), (4, 4)])
 def test_strides_and_alignments(lay, dt):
     check_forward(140, 144, 136, dt, act="relu", bias=True, residual=True, lay=lay)
