@@ -150,7 +150,8 @@ __device__ __forceinline__ void slopes_of(float* v, const float* z, int act) {
 #pragma unroll
     for (int t = 0; t < W; t++) {
       const float s = gelu_tanh_s<EXACT>(z[t]);
-      v[t] *= s + z[t] * (s * (1.f - s)) * 1.5957691216057308f * (1.f + 0.134145f * z[t] * z[t]);
+      // (z^2 is kept finite: where it would not be, s (1 - s) is zero)
+      v[t] *= s + z[t] * (s * (1.f - s)) * 1.5957691216057308f * (1.f + 0.134145f * fminf(z[t] * z[t], 1e30f));
     }
   }
 }

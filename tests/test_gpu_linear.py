@@ -179,6 +179,16 @@ def test_left_tail_of_activations(rows, act, dt):
     assert (off <= terms * near + z64.grad.abs() * 2.1 * HALF[dt] + 2 * TINY[dt]).all()
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_slopes_far_out(dt):
+    z = torch.tensor([-3e38, -1e25, -1e19, 1e13, 1e25, 3e38]).to(DTYPES[dt]).cuda()[:, None]
+    one = torch.ones(1, 1, dtype=DTYPES[dt], device="cuda")
+    for act in ("silu", "gelu", "gelu_tanh"):
+        dX = torch.zeros_like(z)
+        d.op_linear_backward(torch.ones_like(z), z, one, pre=z, act=act, dX=dX)
+        assert dX[:, 0].tolist() == [0, 0, 0, 1, 1, 1]
+
+
 @pytest.mark.parametrize("dt", list(DTYPES))
 @pytest.mark.parametrize("lay", [(8, 0), (8, 8), (1, 0), (3, 1), (4, 4)])
 def test_strides_and_alignments(lay, dt):
