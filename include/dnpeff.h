@@ -563,8 +563,8 @@ int dnpeff_op_init_uniform(int matrix_id, int64_t logical_rows, int64_t logical_
  * All arrays are device memory, row-major with the last index contiguous; ld* are elements from one row to the next
  * (>= the row's width).  `type` is that of every array not declared with one of its own; sums, softmax statistics
  * and losses are fp32, results are rounded once.  16-bit operands are multiplied as they are, fp32 ones as three
- * bf16 numbers that add up to them, in the six products that matter next to fp32 (an operand that is not finite
- * makes NaN of what it reaches).  Any size (widths up to 2^24) and any alignment of whole elements is taken; 16-bit
+ * bf16 numbers that add up to them, in the six products that matter next to fp32; infinities, NaN and the largest
+ * numbers go through either way as through fp32 products.  Any size (widths up to 2^24) and any alignment of whole elements is taken; 16-bit
  * operands of the products whose rows do not begin and end on 16 bytes (pointer, ld and width) are copied to such
  * rows in the workspace first, fp32 ones always.  Products of few rows, and both gradients of the loss of few
  * tokens, take all operands as they lie, fp32 through fp32 instructions.  Outputs must not overlap inputs, except Y

@@ -302,18 +302,22 @@ __device__ __forceinline__ void store_op(typename num<T>::op* p, int64_t plane, 
     store_row<T, W>(p, v);
   } else {
     float rest[W];
+    loose<__bf16, W> q[3];
 #pragma unroll
-    for (int t = 0; t < W; t++) rest[t] = v[t];
-#pragma unroll
-    for (int h = 0; h < 3; h++) {
-      loose<__bf16, W> q;
-#pragma unroll
-      for (int t = 0; t < W; t++) {
-        q[t] = (__bf16)rest[t];
-        rest[t] -= (float)q[t];
-      }
-      *(loose<__bf16, W>*)(p + h * plane) = q;
+    for (int t = 0; t < W; t++) {
+      // An infinity is (1, 0, infinity) of its sign: of the products of planes only the one with the other's high plane is
+      // infinite then, as the product itself is (infinity, 0, 0 would meet low planes of either sign).  Finite values that
+      // would round to infinity begin with the largest bf16.
+      constexpr float MOST = 0x1.fep127f;
+      const bool past = fabsf(v[t]) > MOST, inf = fabsf(v[t]) == INFINITY;
+      q[0][t] = (__bf16)(past ? copysignf(inf ? 1.f : MOST, v[t]) : v[t]);
+      rest[t] = v[t] - (float)q[0][t];
+      q[1][t] = (__bf16)(inf ? 0.f : rest[t]);
+      rest[t] -= (float)q[1][t];
+      q[2][t] = (__bf16)rest[t];
     }
+#pragma unroll
+    for (int h = 0; h < 3; h++) *(loose<__bf16, W>*)(p + h * plane) = q[h];
   }
 }
 

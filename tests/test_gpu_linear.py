@@ -296,6 +296,42 @@ def test_infinities_and_nan_stay_in_their_rows():
     assert torch.equal(Y[rest], clean[rest])
 
 
+def same_where_not_finite(got, want, bound):
+    got, want = got.double().cpu(), want.double()
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isposinf(), want.isposinf())
+    assert torch.equal(got.isneginf(), want.isneginf())
+    ok = torch.isfinite(want)
+    assert ((got - want).abs()[ok] <= bound[ok]).all()
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("rows, n_in, n_out", [(12, 40, 24), (50, 96, 200), (300, 64, 200), (100, 5000, 96)])
+def test_infinities_and_large_numbers(rows, n_in, n_out, dt):
+    """Infinities give infinities of the product's sign (NaN where they meet zeros or each other), and numbers up to the type's
+    largest what they are worth, however many rows there are."""
+    X, W = rand((rows, n_in), dt, 1), rand((n_out, n_in), dt, 2, 1e-3)
+    inf, most = float("inf"), torch.finfo(DTYPES[dt]).max
+    X[1, 3], X[2, 5], X[3, 7], X[3, 9], X[4, 11], X[5, 0], X[6, 1], X[7, 2] = inf, -inf, inf, inf, float("nan"), most, -most, most * 0.999
+    X[8, 4] = inf
+    W[5, 4], W[6, 6], W[7, 8] = 0.0, inf, -inf
+    X[9, 6] = -inf
+    x, w = X.double().cpu(), W.double().cpu()
+    bound = (n_in + 40) * EPS32 * 1.2 * (x.abs() @ w.abs().T) + HALF[dt] * 1.01 * (x @ w.T).abs()
+    Y = torch.zeros(rows, n_out, dtype=DTYPES[dt], device="cuda")
+    d.op_linear(X, W, Y)
+    same_where_not_finite(Y, x @ w.T, bound)
+    # dX of such W, dW of such X, for dY with the same
+    dY = rand((rows, n_out), dt, 3, 1e-3)
+    dY[0, 3], dY[1, 2], dY[9, 1] = inf, -inf, 0.0
+    g = dY.double().cpu()
+    dX, dW = torch.zeros_like(X), torch.zeros_like(W)
+    d.op_linear_backward(dY, X, W, dX=dX, dW=dW)
+    for got, a, b in ((dX, g, w), (dW, g.T, x)):
+        want = a @ b
+        k = a.shape[1]
+        same_where_not_finite(got, want, (k + 40) * EPS32 * 1.2 * (a.abs() @ b.abs()) + HALF[dt] * 1.01 * want.abs())
+
+
 def test_falling_and_wild_ends_stay_inside():
     """No promise of values, but every access is inside the arrays: guards around the outputs keep theirs."""
     X, W = rand((64, 64), "bf16", 1), rand((4, 128, 64), "bf16", 2)
