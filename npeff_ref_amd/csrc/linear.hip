@@ -35,7 +35,7 @@ __global__ __launch_bounds__(256) void k_slopes(group_rows G, int64_t N, const T
   if (group < 0) return;
   const int64_t m0 = G.first(group) + (int64_t)within * tall, m_end = G.last(group);
   const bool held = group < G.groups;
-  const int64_t n = ((int64_t)blockIdx.y * 64 + lane) * W;
+  const int64_t n = (((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * 64 + lane) * W;
   const int there = n < N ? (N - n < W ? (int)(N - n) : W) : 0;
   float sum[W];
 #pragma unroll
@@ -213,8 +213,9 @@ int backward(hipStream_t st, const layer& l, const void* dY, int64_t lddy, const
   constexpr int PIECE = 16 / sizeof(T);
   const int tall = slope_rows(l.rows, l.n_out, sizeof(T));
   if ((dz || dbias) && l.rows > 0) {
-    const dim3 grid((unsigned)slope_tiles(l.rows, G.groups, tall), (unsigned)ceil_div(l.n_out, 64 * PIECE));
-    DN_CHECK(grid.y <= 65535, "dnpeff_linear_backward: n_out = %lld is too wide for one launch", (long long)l.n_out);
+    constexpr int64_t STRIPS = 32768;  // of columns in a launch's second dimension, the rest in its third
+    const int64_t strips = ceil_div(l.n_out, 64 * PIECE);
+    const dim3 grid((unsigned)slope_tiles(l.rows, G.groups, tall), (unsigned)(strips < STRIPS ? strips : STRIPS), (unsigned)ceil_div(strips, STRIPS));
     k_slopes<T><<<grid, 256, 0, st>>>(G, l.n_out, (const T*)dY, lddy, (const T*)pre, ldp, act, dz, packed_ld(l.n_out), sums, tall);
     DN_LAUNCH_CHECK();
   }

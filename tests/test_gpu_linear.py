@@ -461,6 +461,24 @@ def test_offsets_past_32_bits():
     assert not out[1].any()
 
 
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+def test_the_widest_layer(dt):
+    """2^24 columns, forward and backward; the last ones against the formulas."""
+    rows, n_in, n_out = 3, 2, 1 << 24
+    X, W = rand((rows, n_in), dt, 1), rand((n_out, n_in), dt, 2)
+    dY, Y = rand((rows, n_out), dt, 3), torch.zeros(rows, n_out, dtype=DTYPES[dt], device="cuda")
+    d.op_linear(X, W, Y, act="relu")
+    dX, dW, db = torch.zeros_like(X), torch.zeros_like(W), torch.zeros(n_out, dtype=DTYPES[dt], device="cuda")
+    d.op_linear_backward(dY, X, W, pre=Y, act="relu", dX=dX, dW=dW, dbias=db)
+    dZ = dY.double() * (Y > 0)
+    for at in (slice(0, 600), slice(8_388_500, 8_388_800), slice(n_out - 600, n_out)):
+        w, g = W[at].double(), dZ[:, at]
+        close(Y[:, at], (X.double() @ w.T).clamp(min=0), X.double().abs() @ w.abs().T, n_in, dt)
+        close(dW[at], g.T @ X.double(), g.abs().T @ X.double().abs(), rows, dt)
+        close(db[at], g.sum(0), g.abs().sum(0), rows, dt)
+    close(dX, dZ @ W.double(), dZ.abs() @ W.double().abs(), n_out, dt)
+
+
 def test_refusals():
     X, W, Y = torch.zeros(8, 16, device="cuda"), torch.zeros(4, 16, device="cuda"), torch.zeros(8, 4, device="cuda")
 
