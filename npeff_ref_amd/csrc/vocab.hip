@@ -22,29 +22,30 @@ DN_STORE_PRODUCTS(extern, __bf16)
 
 namespace {
 
-// One wave per token.
+// One wave per token (four a workgroup, every gridDim.x * 4th: a launch has at most 2^32 lanes).
+constexpr int64_t JOIN_MOST = (int64_t)1 << 22;
 __global__ __launch_bounds__(256) void k_join_loss(int64_t rows, int parts_n, const float2* parts, const float* hit, const int32_t* labels,
                                                    int64_t words, float* loss, float* lse) {
-  const int64_t m = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
   const int lane = threadIdx.x & 63;
-  if (m >= rows) return;
-  float top = -INFINITY;
-  for (int i = lane; i < parts_n; i += 64) top = fmaxf(top, parts[m * parts_n + i].x);
+  for (int64_t m = (int64_t)blockIdx.x * 4 + threadIdx.x / 64; m < rows; m += (int64_t)gridDim.x * 4) {
+    float top = -INFINITY;
+    for (int i = lane; i < parts_n; i += 64) top = fmaxf(top, parts[m * parts_n + i].x);
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
-  const float from = top == -INFINITY ? 0.f : top;
-  float sum = 0.f;
-  for (int i = lane; i < parts_n; i += 64) {
-    const float2 s = parts[m * parts_n + i];
-    if (s.x != -INFINITY || s.y != 0.f) sum += s.y * expf(s.x - from);
-  }
+    for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
+    const float from = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    for (int i = lane; i < parts_n; i += 64) {
+      const float2 s = parts[m * parts_n + i];
+      if (s.x != -INFINITY || s.y != 0.f) sum += s.y * expf(s.x - from);
+    }
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d, 64);
-  if (lane == 0) {
-    const float l = logf(sum) + from;
-    const int32_t label = labels[m];
-    if (lse) lse[m] = l;
-    if (loss) loss[m] = label < 0 ? 0.f : label >= words ? __builtin_nanf("") : l - hit[m];
+    for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d, 64);
+    if (lane == 0) {
+      const float l = logf(sum) + from;
+      const int32_t label = labels[m];
+      if (lse) lse[m] = l;
+      if (loss) loss[m] = label < 0 ? 0.f : label >= words ? __builtin_nanf("") : l - hit[m];
+    }
   }
 }
 
@@ -273,7 +274,8 @@ int loss_forward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, cons
     DN_TRY((launch_few<T, E_LOSS>(p, st, &parts_n)));
   else
     DN_TRY((launch_product<T, true, true, E_LOSS>(p, nullptr, st, &parts_n)));
-  k_join_loss<<<(unsigned)ceil_div(rows, 4), 256, 0, st>>>(rows, parts_n, p.parts, p.hit, labels, words, loss, lse);
+  const int64_t blocks = ceil_div(rows, 4);
+  k_join_loss<<<(unsigned)(blocks < JOIN_MOST ? blocks : JOIN_MOST), 256, 0, st>>>(rows, parts_n, p.parts, p.hit, labels, words, loss, lse);
   DN_LAUNCH_CHECK();
   return 0;
 }

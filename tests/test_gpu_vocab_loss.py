@@ -202,6 +202,24 @@ def test_a_vocabulary_past_32_bits(rows):
     assert ((loss - (want - z.gather(1, y.long()[:, None])[:, 0])).abs() <= 4 * size + 600_064 * EPS32).all()
 
 
+def test_more_tokens_than_a_launch_has_waves():
+    rows = (1 << 26) + 70
+    g = torch.Generator(device="cuda").manual_seed(1)
+    X = torch.randn(rows, 8, generator=g, device="cuda", dtype=torch.bfloat16)
+    E = rand((16, 8), "bf16", 2)
+    y = (torch.arange(rows, dtype=torch.int32, device="cuda") % 17) - 1
+    loss, lse = torch.full((rows,), 9.0, device="cuda"), torch.full((rows,), 9.0, device="cuda")
+    d.op_vocab_loss(X, E, y, loss, lse)
+    for at in (slice(0, 500), slice(1 << 24, (1 << 24) + 500), slice(rows - 500, rows)):
+        z = X[at].double() @ E.double().T
+        want = torch.logsumexp(z, 1)
+        size = (16 * EPS32 * (X[at].double().abs() @ E.double().abs().T)).max(1).values + 80 * EPS32 + 2 * EPS32 * want.abs()
+        assert ((lse[at] - want).abs() <= 2 * size).all()
+        has = y[at] >= 0
+        hit = z.gather(1, y[at].long().clamp(min=0)[:, None])[:, 0]
+        assert ((loss[at] - torch.where(has, want - hit, 0.0)).abs() <= torch.where(has, 4 * size, 0.0)).all()
+
+
 def test_all_masked_and_labels_outside():
     X, E = rand((70, 64), "bf16", 1), rand((900, 64), "bf16", 2)
     y = torch.full((70,), -1, dtype=torch.int32, device="cuda")
