@@ -20,8 +20,11 @@ DN_STORE_PRODUCTS(, __bf16)
 namespace {
 
 // Rows of a group that one workgroup of k_slopes takes (a wave every fourth of them): 64, or 16 where those would leave
-// CUs without work (777 x 515 in fp32: 20 -> 8.5 us).
-int slope_rows(int64_t rows, int64_t n_out, int size) { return ceil_div(rows, 64) * ceil_div(n_out * size, 1024) >= 1024 ? 64 : 16; }
+// CUs without work (777 x 515 in fp32: 20 -> 8.5 us), or 256 where a launch would not hold so many workgroups.
+int slope_rows(int64_t rows, int64_t n_out, int size) {
+  if (rows >= (int64_t)1 << 29) return 256;
+  return ceil_div(rows, 64) * ceil_div(n_out * size, 1024) >= 1024 ? 64 : 16;
+}
 
 // dZ = dY act'(Z), and the column sums of each tile of rows.  A lane has 16 bytes of each row.
 template <class T>

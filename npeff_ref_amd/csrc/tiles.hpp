@@ -698,6 +698,12 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
   }
 }
 
+// A launch's dimension holds 2^32 lanes (more are cut off without an error): workgroups past 2^22 go on in its second.  (A
+// multiple of 8, for the XCDs.)
+constexpr int64_t GRID_X = (int64_t)1 << 22;
+inline dim3 grid_of(int64_t blocks) { return dim3((unsigned)(blocks < GRID_X ? blocks : GRID_X), (unsigned)ceil_div(blocks, GRID_X)); }
+__device__ __forceinline__ unsigned block_id() { return blockIdx.y * gridDim.x + blockIdx.x; }
+
 template <class T, int BM, int BN, int WM, int WN, bool A_ROWS, bool B_ROWS, int E>
 __global__ __launch_bounds__(WM* WN * 64, 2) void k_tiles(args p) {
   typedef typename num<T>::op O;
@@ -715,9 +721,10 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_tiles(args p) {
   const int plane = mt * nt, many = plane * (p.mode == BY_REDUCTION ? p.G.groups : p.splits);
   // Workgroups go to the XCDs round-robin: each XCD gets a run of tiles, in blocks of a few tiles of m by all of n, so
   // that what its workgroups read at one time is shared in its L2.
-  const int xcd = blockIdx.x % 8, share = many / 8, more = many % 8;
-  if ((int)blockIdx.x >= many) return;
-  const int tile = xcd * share + (xcd < more ? xcd : more) + blockIdx.x / 8;
+  const unsigned id = block_id();
+  const int xcd = id % 8, share = many / 8, more = many % 8;
+  if ((int)id >= many) return;
+  const int tile = xcd * share + (xcd < more ? xcd : more) + id / 8;
   place<T> w;
   w.A = (const O*)p.A, w.B = (const O*)p.B;
   w.sheet = tile / plane;
@@ -1191,10 +1198,11 @@ struct pack_args {
 template <class T>
 __global__ __launch_bounds__(256) void k_pack(pack_args p) {
   constexpr int CH = 8;
-  const int w = blockIdx.x < p.first[1] ? 0 : blockIdx.x < p.first[2] ? 1 : 2;
+  const int64_t id = block_id();
+  const int w = id < p.first[1] ? 0 : id < p.first[2] ? 1 : 2;
   const matrix m = p.m[w];
   const int64_t ld = (m.width + 63) / 64 * 64, per_row = ld / CH;
-  const int64_t at = ((int64_t)blockIdx.x - p.first[w]) * 256 + threadIdx.x, row = at / per_row;
+  const int64_t at = (id - p.first[w]) * 256 + threadIdx.x, row = at / per_row;
   if (row >= m.rows * m.sheets) return;
   const int c = (int)(at - row * per_row) * CH, there = m.keep && m.keep[row] < 0 ? 0 : (int)(m.width - c);
   const T* src = (const T*)m.p + (m.sheets > 1 ? row / m.rows * m.sheet + row % m.rows * m.ld : row * m.ld) + c;
@@ -1226,7 +1234,7 @@ inline int pack(matrix* m, int n, char* room, hipStream_t st) {
   if (blocks == 0) return 0;
   for (int i = k; i < 4; i++) p.first[i] = blocks;
   DN_CHECK(blocks < (int64_t)1 << 31, "operands of %lld MB that have to be copied", (long long)(blocks >> 8));
-  k_pack<T><<<(unsigned)blocks, 256, 0, st>>>(p);
+  k_pack<T><<<grid_of(blocks), 256, 0, st>>>(p);
   DN_LAUNCH_CHECK();
   return 0;
 }
@@ -1242,7 +1250,7 @@ int launch_tiles(const args& p, hipStream_t st) {
   const int64_t many = mt * nt * sheets;
   if (many == 0) return 0;
   DN_CHECK(many < (int64_t)1 << 31, "product of %lld x %lld: too many tiles for one launch", (long long)p.M, (long long)p.N);
-  k_tiles<T, BM, BN, WM, WN, A_ROWS, B_ROWS, E><<<(unsigned)many, WM * WN * 64, 0, st>>>(p);
+  k_tiles<T, BM, BN, WM, WN, A_ROWS, B_ROWS, E><<<grid_of(many), WM * WN * 64, 0, st>>>(p);
   DN_LAUNCH_CHECK();
   return 0;
 }
@@ -1334,6 +1342,7 @@ int launch_few(args p, hipStream_t st, int* parts_n = nullptr) {
   p.parts_n = (int)ceil_div(p.N, cols);
   if (parts_n) *parts_n = p.parts_n;
   const dim3 grid((unsigned)ceil_div(p.N, cols), (unsigned)slots);
+  DN_CHECK(grid.x < 1u << 23, "product of %lld columns: too many for one launch", (long long)p.N);
   // 16, 32 or 64 rows for each reading of B (fp32 products of 64000 x 2048, 16 at a time and so: 32 rows 266 and 164 us, 48 391 and
   // 233, the loss of 64 rows 449 and 253)
   const int64_t each = p.mode == BY_ROWS ? ceil_div(p.M, p.G.groups) : p.M;

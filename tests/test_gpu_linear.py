@@ -479,6 +479,26 @@ def test_the_widest_layer(dt):
     close(dX, dZ @ W.double(), dZ.abs() @ W.double().abs(), n_out, dt)
 
 
+def test_more_rows_to_copy_than_a_launch_dimension_holds():
+    rows = (1 << 29) + 300
+    X = torch.randn(rows, 1, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda", dtype=torch.float16)
+    W, Y = rand((1, 1), "f16", 2), torch.full((rows, 1), 7.0, dtype=torch.float16, device="cuda")
+    d.op_linear(X, W, Y)
+    for i in range(0, rows, 1 << 27):  # (one product, rounded once)
+        assert torch.equal(Y[i : i + (1 << 27)], (X[i : i + (1 << 27)].float() * W.float()).half())
+    torch.cuda.empty_cache()
+
+
+def test_column_sums_of_more_rows_than_a_launch_dimension_holds():
+    rows = (1 << 30) + (1 << 16)
+    dY = torch.ones(rows, 1, device="cuda")
+    db = torch.zeros(1, device="cuda")
+    room = torch.empty(1 << 27, dtype=torch.uint8, device="cuda")  # (all three gradients would take 768 GB)
+    d.op_linear_backward(dY, dY, dY[:1], dbias=db, workspace=room)
+    assert db.item() == rows
+    torch.cuda.empty_cache()
+
+
 def test_refusals():
     X, W, Y = torch.zeros(8, 16, device="cuda"), torch.zeros(4, 16, device="cuda"), torch.zeros(8, 4, device="cuda")
 

@@ -220,6 +220,23 @@ def test_more_tokens_than_a_launch_has_waves():
         assert ((loss[at] - torch.where(has, want - hit, 0.0)).abs() <= torch.where(has, 4 * size, 0.0)).all()
 
 
+def test_more_tiles_than_a_launch_dimension_holds():
+    """2 million tokens and 262,400 words: 8.4 million tiles of 256 x 256, of 512 lanes each."""
+    rows, words = 1 << 21, (1 << 18) + 256
+    X, E = rand((rows, 8), "bf16", 1), rand((words, 8), "bf16", 2)
+    y = torch.randint(0, words, (rows,), generator=torch.Generator().manual_seed(3), dtype=torch.int32).cuda()
+    loss, lse = torch.full((rows,), 9.0, device="cuda"), torch.full((rows,), 9.0, device="cuda")
+    d.op_vocab_loss(X, E, y, loss, lse)
+    for at in (slice(0, 150), slice(rows // 3, rows // 3 + 150), slice(rows - 150, rows)):
+        z = X[at].double() @ E.double().T
+        want = torch.logsumexp(z, 1)
+        size = (16 * EPS32 * (X[at].double().abs() @ E.double().abs().T)).max(1).values
+        off = 2 * size + (words + 64) * EPS32 + 2 * EPS32 * want.abs()
+        assert ((lse[at] - want).abs() <= off).all()
+        assert ((loss[at] - (want - z.gather(1, y[at].long()[:, None])[:, 0])).abs() <= 2 * off).all()
+    torch.cuda.empty_cache()
+
+
 def test_all_masked_and_labels_outside():
     X, E = rand((70, 64), "bf16", 1), rand((900, 64), "bf16", 2)
     y = torch.full((70,), -1, dtype=torch.int32, device="cuda")

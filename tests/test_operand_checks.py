@@ -1,5 +1,7 @@
 """What the op_* calls refuse before anything is queued: no GPU is needed to see it."""
 
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
@@ -83,3 +85,10 @@ def test_views_of_memory_that_the_library_cannot_reach(device0, monkeypatch):
     monkeypatch.setattr(binding.lib, "without_torch", True)
     with pytest.raises(d.DnpeffError, match="torch was imported after"):
         d.DeviceArray.view(OnGpu())
+
+
+def test_more_words_than_a_launch_dimension_holds():
+    """Refused before anything is read or queued: the addresses are nobody's."""
+    at, words = C.c_void_p(16), (1 << 31) - 100
+    assert d.lib.dnpeff_vocab_loss(None, binding.BF16, 1, 8, words, at, 8, at, 8, at, at, at, at, 1 << 40) != 0
+    assert b"too many for one launch" in d.lib.dnpeff_last_error()
