@@ -587,7 +587,7 @@ enum { DNPEFF_ACT_NONE = 0, DNPEFF_ACT_RELU = 1, DNPEFF_ACT_GELU = 2, DNPEFF_ACT
  * With n_groups > 0 (at most 65535; else 0 and ends NULL) the rows are in groups with a weight each, as a router
  * leaves the tokens of its experts: group g holds rows ends[g] .. ends[g + 1] - 1 (n_groups + 1 device words,
  * ends[0] = 0, not falling, the last at most `rows`), W is [n_groups, n_out, n_in] with w_group elements from a
- * group's to the next one's, bias [n_groups, n_out].  Groups may be empty.  Rows past the last end belong to none:
+ * group's to the next one's (a row of each side by side does as well as one after the other), bias [n_groups, n_out].  Groups may be empty.  Rows past the last end belong to none:
  * their product is zero, without bias and activation (Y = residual or 0, pre = 0).  The ends are only read on the
  * device; values that break these rules give undefined results but no access outside the arrays. */
 int dnpeff_linear_workspace(int type, int64_t rows, int64_t n_in, int64_t n_out, int n_groups, int aligned, int64_t* forward_bytes,

@@ -531,7 +531,7 @@ class _Call:
         if n == 2:
             return a.data_ptr(), ld, 0
         group = st[-3] if shape[-3] > 1 else shape[-2] * ld
-        if group < (shape[-2] - 1) * ld + width:
+        if group < (shape[-2] - 1) * ld + width and not (group >= width and (shape[-3] - 1) * group + width <= ld):
             _refuse(self.what, f"{name}: matrices overlap")
         return a.data_ptr(), ld, group
 

@@ -117,6 +117,15 @@ int check_layer(const char* what, int type, const layer& l) {
            what, l.groups, l.ends ? "given" : "not given");
   return 0;
 }
+// Matrices of groups `apart` elements from one to the next; those that are written must not share elements: each after the
+// one before, or a row of each side by side.
+int check_apart(const char* what, const char* name, const layer& l, const void* p, int64_t ld, int64_t apart, bool written) {
+  if (p == nullptr || l.groups < 2) return 0;
+  const bool after = apart >= (l.n_out - 1) * ld + l.n_in, beside = apart >= l.n_in && (l.groups - 1) * apart + l.n_in <= ld;
+  DN_CHECK(written ? after || beside : apart >= 0, "%s: matrices of %s are %lld elements apart, their rows %lld", what, name, (long long)apart,
+           (long long)ld);
+  return 0;
+}
 int check_act(const char* what, int act) {
   DN_CHECK(act >= DNPEFF_ACT_NONE && act <= DNPEFF_ACT_SILU, "%s: unknown activation %d", what, act);
   return 0;
@@ -307,6 +316,7 @@ DN_API int dnpeff_linear(void* stream, int type, int64_t rows, int64_t n_in, int
   if (rows == 0) return 0;
   DN_TRY(check_array(me, "X", X, ldx, n_in, type, false));
   DN_TRY(check_array(me, "W", W, ldw, n_in, type, false));
+  DN_TRY(check_apart(me, "W", l, W, ldw, w_group, false));
   DN_TRY(check_array(me, "Y", Y, ldy, n_out, type, false));
   DN_TRY(check_array(me, "bias", bias, n_out, n_out, type, true));
   DN_TRY(check_array(me, "residual", residual, ldr, n_out, type, true));
@@ -327,9 +337,11 @@ DN_API int dnpeff_linear_backward(void* stream, int type, int64_t rows, int64_t 
   DN_TRY(check_array(me, "dY", dY, lddy, n_out, type, rows == 0));
   DN_TRY(check_array(me, "X", X, ldx, n_in, type, rows == 0 || !dW));
   DN_TRY(check_array(me, "W", W, ldw, n_in, type, !dX));
+  DN_TRY(check_apart(me, "W", l, W, ldw, w_group, false));
   DN_TRY(check_array(me, "pre", pre, ldp, n_out, type, rows == 0 || act == DNPEFF_ACT_NONE));
   DN_TRY(check_array(me, "dX", dX, lddx, n_in, type, true));
   DN_TRY(check_array(me, "dW", dW, lddw, n_in, type, true));
+  DN_TRY(check_apart(me, "dW", l, dW, lddw, dw_group, true));
   DN_TRY(check_array(me, "dbias", dbias, n_out, n_out, type, true));
   return DN_BY_TYPE(type, backward<T>((hipStream_t)stream, l, dY, lddy, X, ldx, W, ldw, w_group, pre, ldp, act, dX, lddx, dW, lddw,
                                       dw_group, dbias, (char*)workspace, workspace_bytes));

@@ -223,6 +223,38 @@ def test_groups(sizes, padding, dt):
     check_backward(rows, 72, 136, dt, act="gelu", sizes=sizes)
 
 
+def check_strided_groups(rows_of, n_in, n_out, dt, lay, beside=False):
+    """Forward, backward and per-example gradients of groups whose arrays are wider than their rows, all of them."""
+    sizes, n = rows_of, len(rows_of)
+    rows = sum(sizes) + 4
+    X, W = rand((rows, n_in), dt, 1), rand((n, n_out, n_in), dt, 2, n_in**-0.5)
+    b, R, dY, pre = rand((n, n_out), dt, 3), rand((rows, n_out), dt, 4), rand((rows, n_out), dt, 5), rand((rows, n_out), dt, 6)
+    put = lambda t: wide(t, *lay)  # noqa: E731
+    weights = (lambda t: wide(t.transpose(0, 1), *lay).transpose(0, 1)) if beside else put
+    dense = {}
+    for name, f, w in (("dense", lambda t: t.clone(), lambda t: t.clone()), ("wide", put, weights)):
+        y, z, gx, gw = f(torch.zeros_like(R)), f(torch.zeros_like(R)), f(torch.zeros_like(X)), w(torch.zeros_like(W))
+        gb, out = torch.zeros_like(b), torch.zeros(n, n_out, n_in, device="cuda")
+        d.op_linear(f(X), w(W), y, bias=b, act="silu", residual=f(R), pre=z, groups=ends_of(sizes))
+        d.op_linear_backward(f(dY), f(X), w(W), pre=f(pre), act="gelu", dX=gx, dW=gw, dbias=gb, groups=ends_of(sizes))
+        d.op_example_grads(f(dY), f(X), ends_of(sizes), out, square=True)
+        dense[name] = (y, z, gx, gw, gb, out)
+        if name == "wide":  # what lies between the rows is as it was
+            for t in (y, z, gx, gw):
+                gap = t.as_strided(t.shape[:-1] + (lay[0],), t.stride(), t.storage_offset() + t.shape[-1])
+                assert (gap == 7).all()
+    for a, b in zip(dense["dense"], dense["wide"]):
+        assert torch.equal(a, b)  # the same sums in the same order
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("beside", [False, True])
+@pytest.mark.parametrize("lay", [(8, 0), (8, 8), (1, 0), (3, 1)])
+def test_groups_of_strided_arrays(lay, beside, dt):
+    check_strided_groups([5, 0, 130, 1, 64], 72, 136, dt, lay, beside)
+    check_strided_groups([3, 0, 5], 33, 65, dt, lay, beside)
+
+
 @pytest.mark.parametrize("dt", ["f16", "bf16"])
 def test_groups_on_large_tiles(dt):
     sizes = [700, 0, 256, 1300, 3, 1741]

@@ -92,3 +92,15 @@ def test_more_words_than_a_launch_dimension_holds():
     at, words = C.c_void_p(16), (1 << 31) - 100
     assert d.lib.dnpeff_vocab_loss(None, binding.BF16, 1, 8, words, at, 8, at, 8, at, at, at, at, 1 << 40) != 0
     assert b"too many for one launch" in d.lib.dnpeff_last_error()
+
+
+def test_matrices_of_groups_that_share_elements():
+    """As above: weights of groups that lie backwards, and gradients of theirs that overlap, are refused."""
+    at, none, room = C.c_void_p(16), C.c_void_p(0), 1 << 40
+    forward = d.lib.dnpeff_linear
+    assert forward(None, binding.F32, 40, 8, 4, at, 8, at, 8, -32, none, 0, none, 0, at, 4, none, 0, 3, at, at, room) != 0
+    assert b"matrices of W" in d.lib.dnpeff_last_error()
+    backward = d.lib.dnpeff_linear_backward
+    for lddw, dw_group in ((8, 31), (8, 0), (8, -64), (10, 32)):
+        bad = backward(None, binding.F32, 40, 8, 4, at, 4, at, 8, at, 8, 32, none, 0, 0, at, 8, at, lddw, dw_group, none, 3, at, at, room)
+        assert bad != 0 and b"matrices of dW" in d.lib.dnpeff_last_error()
