@@ -316,6 +316,34 @@ def test_no_rows():
     assert not out.any()
 
 
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("lay", [(8, 8), (3, 1)])
+def test_strided_arrays_on_large_tiles_and_split_reductions(lay, dt):
+    check_forward(3601, 200, 3848, dt, act="silu", bias=True, residual=True, lay=lay)
+    check_backward(3601, 3848, 200, dt, act="silu", lay=lay)
+    check_forward(100, 5000, 96, dt, act="gelu", bias=True, residual=True, lay=lay)
+    check_backward(2500, 90, 100, dt, act="relu", lay=lay)
+
+
+def test_fp32_groups_on_large_tiles():
+    sizes = [700, 0, 256, 1300, 3, 1741]
+    check_forward(sum(sizes) + 9, 136, 3000, "f32", act="gelu_tanh", sizes=sizes)
+    check_backward(sum(sizes) + 9, 3000, 136, "f32", sizes=sizes, bias=False)
+    check_backward(sum(sizes) + 9, 1000, 2000, "f32", sizes=sizes, act="silu")
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("rows, n_in, n_out, sizes", [(12, 40, 77, None), (12, 40, 77, [5, 0, 4]), (300, 64, 133, None), (300, 64, 133, [100, 0, 190]),
+                                                      (100, 5000, 99, None), (3601, 200, 3843, None)])
+def test_the_residual_may_be_the_result(rows, n_in, n_out, sizes, dt):
+    X, W = rand((rows, n_in), dt, 1), rand((() if sizes is None else (len(sizes),)) + (n_out, n_in), dt, 2, n_in**-0.5)
+    R, groups = rand((rows, n_out), dt, 3), None if sizes is None else ends_of(sizes)
+    Y = torch.zeros_like(R)
+    d.op_linear(X, W, Y, act="silu", residual=R, groups=groups)
+    d.op_linear(X, W, R, act="silu", residual=R, groups=groups)
+    assert torch.equal(Y, R)
+
+
 def test_infinities_and_nan_stay_in_their_rows():
     X, W = rand((300, 64), "bf16", 1), rand((200, 64), "bf16", 2)
     Y, clean = torch.zeros(300, 200, dtype=torch.bfloat16, device="cuda"), torch.zeros(300, 200, dtype=torch.bfloat16, device="cuda")
@@ -375,6 +403,17 @@ def test_falling_and_wild_ends_stay_inside():
         d.op_linear(X, W, guard[1:65], groups=e)
         d.op_linear_backward(guard[1:65], X, W, dW=dW[1:5], dbias=db[1:5], groups=e)
         assert (guard[[0, 65]] == 3).all() and (dW[[0, 5]] == 3).all() and (db[[0, 5]] == 3).all()
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("rows", [5, 16])
+def test_falling_and_wild_ends_of_few_rows_stay_inside(rows, dt):
+    X, W = rand((rows, 64), dt, 1), rand((4, 40, 64), dt, 2)
+    for ends in ([0, 5, 2, 16, 1], [0, 1 << 40, -5, 3, 64], [7, 7, 7, 7, 7], [0, 3, 3, 3, 4]):
+        e = torch.tensor(ends, dtype=torch.int64, device="cuda")
+        Y, pre = [torch.full((rows + 2, 40), 3.0, dtype=DTYPES[dt], device="cuda") for _ in range(2)]
+        d.op_linear(X, W, Y[1:-1], pre=pre[1:-1], groups=e)
+        assert (Y[[0, -1]] == 3).all() and (pre[[0, -1]] == 3).all()
 
 
 def test_overlapping_groups_of_more_tiles_than_32_bits_count():

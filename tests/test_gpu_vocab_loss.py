@@ -122,6 +122,12 @@ def test_large_tiles(dt):
     check(1500, 72, 9001, dt)
 
 
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("extra", [1, 8])
+def test_strided_arrays_on_large_tiles(extra, dt):
+    check(1500, 72, 9001, dt, extra=extra)
+
+
 @pytest.mark.parametrize("rows, n_in, words", [(4200, 200, 4203), (1000, 264, 17_001), (300, 1024, 17_000)])
 @pytest.mark.parametrize("dt", list(DTYPES))
 def test_whole_rounds_of_large_tiles_and_a_rest(rows, n_in, words, dt):
@@ -182,6 +188,82 @@ def test_pieces_of_the_vocabulary_give_the_whole():
         assert (got.double() - exact).norm() <= 2 * HALF["bf16"] * exact.norm()
         err = (got.double() - exact).abs()
         assert (err.norm(dim=1) <= 3 * HALF["bf16"] * exact.norm(dim=1) + 1e-6).all()
+
+
+def gradient_bounds(z, has, dl, dt, n_in, words, size):
+    """(p, the rows' weights, p's relative error) from 64-bit logits, as in check(); size: of the products in a row's largest logit."""
+    logit = (n_in + 8) * EPS32 * size + 4 * EPS32 * z.abs().max(1).values
+    lse = torch.logsumexp(z, 1)
+    off = 2 * logit + (words + 64) * EPS32 + 2 * EPS32 * lse.abs()
+    p = torch.softmax(z, 1)
+    weight = torch.where(has, dl.double(), 0.0)[:, None]
+    relative = (2 * off + 32 * EPS32 + 4 * z.abs().max(1).values * EPS32)[:, None]
+    return p, weight, relative
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+@pytest.mark.parametrize("n_in, extra", [(65, 0), (200, 8), (72, 1)])
+def test_pieces_of_the_vocabulary_in_other_types_and_widths(n_in, extra, dt):
+    """As above, every entry by its own bound: two pieces in fp16, four in fp32."""
+    rows, words = 4096, 70_000
+    X, E, y = rand((rows, n_in), dt, 1), rand((words, n_in), dt, 2, 2 * n_in**-0.5), labels_of(rows, words, 3)
+    dl = torch.randn(rows, generator=torch.Generator().manual_seed(4)).cuda()
+    x, e = padded(X, extra), padded(E, extra)
+    loss, lse = torch.zeros(rows, device="cuda"), torch.zeros(rows, device="cuda")
+    d.op_vocab_loss(x, e, y, loss, lse)
+    gx, ge = padded(torch.zeros_like(X), extra), padded(torch.zeros_like(E), extra)
+    d.op_vocab_loss_backward(x, e, y, lse, dl, dX=gx, dE=ge)
+    X64, E64, has = X.double(), E.double(), y >= 0
+    size = (X64.abs() @ E64.abs().T).max(1).values
+    p, weight, relative = gradient_bounds(X64 @ E64.T, has, dl, dt, n_in, words, size)
+    G = p.clone()
+    G.scatter_add_(1, y.long().clamp(min=0)[:, None], torch.full((rows, 1), -1.0, dtype=torch.float64, device="cuda"))
+    err = (p * relative + G.abs() * HALF[dt] * 1.01 + 2 * EPS32) * weight.abs()
+    del p
+    if dt == "f16":
+        err += 2.0**-25 * 2 * weight.abs().max() * has[:, None]
+    G *= weight
+    for got, exact, all_of, e_sum, k in (
+        (gx, G @ E64, G.abs() @ E64.abs(), err @ E64.abs(), words),
+        (ge, G.T @ X64, G.abs().T @ X64.abs(), err.T @ X64.abs(), rows),
+    ):
+        bound = e_sum + (k + 16) * EPS32 * all_of + HALF[dt] * 1.01 * exact.abs() + (2.0**-25 if dt == "f16" else 0)
+        assert torch.isfinite(got).all() and ((got.double() - exact).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("rows", [3, 40])
+def test_gradients_of_a_vocabulary_past_32_bits(rows):
+    """600,000 words of 4096 and the gradients of all: rows of dE from both ends, and dX, which takes all of E."""
+    words, n_in = 600_000, 4096
+    g = torch.Generator(device="cuda").manual_seed(1)
+    E = torch.empty(words, n_in, dtype=torch.bfloat16, device="cuda")
+    for i in range(0, words, 100_000):
+        E[i : i + 100_000] = torch.randn(100_000, n_in, generator=g, device="cuda") * 0.03
+    X, dl = rand((rows, n_in), "bf16", 2), torch.ones(rows, device="cuda")
+    y = torch.randint(0, words, (rows,), generator=torch.Generator().manual_seed(3), dtype=torch.int32).cuda()
+    y[0], y[1] = words - 1, 5
+    loss, lse = torch.zeros(rows, device="cuda"), torch.zeros(rows, device="cuda")
+    d.op_vocab_loss(X, E, y, loss, lse)
+    dX, dE = torch.zeros_like(X), torch.full_like(E, 9.0)
+    d.op_vocab_loss_backward(X, E, y, lse, dl, dX=dX, dE=dE)
+    X64, parts = X.double(), [slice(i, i + 100_000) for i in range(0, words, 100_000)]
+    z = torch.cat([X64 @ E[at].double().T for at in parts], 1)
+    size = X64.abs().sum(1) * E.abs().max().double()
+    p, _, relative = gradient_bounds(z, y >= 0, dl, "bf16", n_in, words, size)
+    G = p.clone()
+    G.scatter_add_(1, y.long()[:, None], torch.full((rows, 1), -1.0, dtype=torch.float64, device="cuda"))
+    err = p * relative + G.abs() * HALF["bf16"] * 1.01 + 2 * EPS32
+    for at in (slice(0, 2000), slice(524_200, 524_400), slice(words - 2000, words)):  # (524,288 x 4096 is 2^31)
+        exact, all_of = G[:, at].T @ X64, G[:, at].abs().T @ X64.abs()
+        bound = err[:, at].T @ X64.abs() + (rows + 16) * EPS32 * all_of + HALF["bf16"] * 1.01 * exact.abs()
+        assert ((dE[at].double() - exact).abs() <= bound).all()
+    exact, bound = torch.zeros_like(X64), torch.zeros_like(X64)
+    for at in parts:
+        e64 = E[at].double()
+        exact += G[:, at] @ e64
+        bound += err[:, at] @ e64.abs() + (words + 16) * EPS32 * (G[:, at].abs() @ e64.abs())
+    assert ((dX.double() - exact).abs() <= bound + HALF["bf16"] * 1.01 * exact.abs()).all()
+    torch.cuda.empty_cache()
 
 
 @pytest.mark.parametrize("rows", [3, 40])
