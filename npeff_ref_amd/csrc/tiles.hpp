@@ -391,10 +391,9 @@ __device__ __forceinline__ void residual_of(const P& p, int64_t m, int64_t n, fl
   if (p.residual) load_row<T, W>((const T*)p.residual + m * p.ldr + n, r);
 }
 
-// A buffer load of 16 bytes per lane to LDS: lane l's go to lds + 16 l.  (The compiler does not see what the load needs: five
-// wait states after a lane's write of an address or of the buffer's words, one after m0's.)
+// A buffer load of 16 bytes per lane to LDS: lane l's go to lds + 16 l.
 __device__ __forceinline__ void to_lds(v4i buffer, unsigned lds, int offset) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer) : "memory");
 }
 __device__ __forceinline__ int64_t uniform(int64_t v) {
   const unsigned lo = __builtin_amdgcn_readfirstlane((int)(unsigned)v), hi = __builtin_amdgcn_readfirstlane((int)((uint64_t)v >> 32));
@@ -813,6 +812,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_tiles(args p) {
     }
     auto whole_stage = [&](unsigned stage) {
       begin();
+      asm volatile("s_nop 4");  // (between a lane's write of an address and the loads)
 #pragma unroll
       for (int e = 0; e < LA + LB; e++) load(stage, e);
       end_stage();
