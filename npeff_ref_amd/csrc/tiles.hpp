@@ -391,7 +391,10 @@ __device__ __forceinline__ void residual_of(const P& p, int64_t m, int64_t n, fl
   if (p.residual) load_row<T, W>((const T*)p.residual + m * p.ldr + n, r);
 }
 
-// A buffer load of 16 bytes per lane to LDS: lane l's go to lds + 16 l.
+// A buffer load of 16 bytes per lane to LDS: lane l's go to lds + 16 l.  The compiler does not see what the load needs: a wait
+// state after m0's write, given here, and five after a lane's write of the buffer's words.  These are given before the first
+// stages, where the words come from lanes; later ones are scalar work, and a test looks for such writes in the built code
+// (given with each load, they cost small fp32 products 2 % and large ones 0.6; once a stage, large ones 0.8).
 __device__ __forceinline__ void to_lds(v4i buffer, unsigned lds, int offset) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer) : "memory");
 }
