@@ -564,7 +564,7 @@ int dnpeff_op_init_uniform(int matrix_id, int64_t logical_rows, int64_t logical_
  * (>= the row's width).  `type` is that of every array not declared with one of its own; sums, softmax statistics
  * and losses are fp32, results are rounded once.  16-bit operands are multiplied as they are, fp32 ones as three
  * bf16 numbers that add up to them, in the six products that matter next to fp32; infinities, NaN and the largest
- * numbers go through either way as through fp32 products.  Any size (widths up to 2^24) and any alignment of whole elements is taken; 16-bit
+ * numbers go through either way as through fp32 products, numbers below 2^-110 keep an error of 2^-134.  Any size (widths up to 2^24) and any alignment of whole elements is taken; 16-bit
  * operands of the products whose rows do not begin and end on 16 bytes (pointer, ld and width) are copied to such
  * rows in the workspace first, fp32 ones always.  Products of few rows, and both gradients of the loss of few
  * tokens, take all operands as they lie, fp32 through fp32 instructions.  Outputs must not overlap inputs, except Y
@@ -573,7 +573,7 @@ int dnpeff_op_init_uniform(int matrix_id, int64_t logical_rows, int64_t logical_
  * Calls are queued on `stream`, a hipStream_t of the caller's (NULL: HIP's null stream) or dnpeff_stream(), and
  * allocate nothing and wait for nothing, so they can be captured in a HIP graph.  The workspace belongs to the
  * caller, aligned to 16 bytes and at least as large as the *_workspace call says for the same sizes (aligned: 1
- * where the inputs' pointers and ld are multiples of 16 bytes and ld below 2^25; 0 serves any), and is free for
+ * where the inputs' pointers, ld and distances of groups are multiples of 16 bytes and ld below 2^25; 0 serves any), and is free for
  * other use once the stream has passed the call; with 0 bytes asked for it may be NULL.  Every sum is taken in an
  * order that the sizes alone decide. */
 enum { DNPEFF_F32 = 0, DNPEFF_F16 = 1, DNPEFF_BF16 = 2 };

@@ -469,7 +469,7 @@ def op_threshold_compact(x: "DeviceArray", divisor: float, threshold: float):
 # ---- operators of a language model whose Fishers are wanted ----------------------------------------------------
 # Operands are DeviceArrays (float32, float16, or uint16 holding the bits of bfloat16) or torch's tensors on the current
 # device, all of one kind in a call.  Calls are queued on `stream` (a stream's handle): by default the library's for
-# DeviceArrays, torch's current one for tensors.
+# DeviceArrays, torch's current one for tensors.  They write into what they are given, unseen by autograd.
 
 F32, F16, BF16 = 0, 1, 2
 ACTS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}

@@ -68,8 +68,6 @@ struct num<__bf16> {
 // The planes of the t-th term, the smallest first: low high, high low, middle middle, middle high, high middle, high high.
 __device__ __forceinline__ int plane_a(int t) { return (0x0052 >> (2 * t)) & 3; }
 __device__ __forceinline__ int plane_b(int t) { return (0x0118 >> (2 * t)) & 3; }
-// W consecutive values as an operand holds them: as they are, or in planes so far apart.
-
 
 __device__ __forceinline__ v4f mma(v8b a, v8b b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ v4f mma(v8h a, v8h b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
@@ -94,7 +92,7 @@ __device__ __forceinline__ float gelu_tanh_s(float z) {
 }
 // The normal distribution's Phi(z), and *e = exp(-z^2 / 2).  16-bit results: erfc(x) = exp(-x^2) t Q(t) for x >= 0 with
 // t = 1 / (1 + 0.45 x) and Q the polynomial of degree 7 whose largest relative error on [0, 12] is smallest (fitted for this:
-// 3.4e-7, in fp32 6.5e-7), far below half a unit of those types; fp32 takes the library's erfc.
+// 3.8e-7 with these coefficients, in fp32 6.5e-7), far below half a unit of those types; fp32 takes the library's erfc.
 template <bool EXACT>
 __device__ __forceinline__ float normal(float z, float* e) {
   if (EXACT) {
