@@ -564,11 +564,11 @@ int dnpeff_op_init_uniform(int matrix_id, int64_t logical_rows, int64_t logical_
  * (>= the row's width).  `type` is that of every array not declared with one of its own; sums, softmax statistics
  * and losses are fp32, results are rounded once.  16-bit operands are multiplied as they are, fp32 ones as three
  * bf16 numbers that add up to them, in the six products that matter next to fp32; infinities, NaN and the largest
- * numbers go through either way as through fp32 products, numbers below 2^-110 keep an error of 2^-134.  Any size (widths up to 2^24) and any alignment of whole elements is taken; 16-bit
- * operands of the products whose rows do not begin and end on 16 bytes (pointer, ld and width) are copied to such
- * rows in the workspace first, fp32 ones always.  Products of few rows, and both gradients of the loss of few
- * tokens, take all operands as they lie, fp32 through fp32 instructions.  Outputs must not overlap inputs, except Y
- * and residual, which may be one array.
+ * numbers go through either way as through fp32 products, numbers below 2^-110 keep an error of 2^-134.  Any size
+ * (widths up to 2^24) and any alignment of whole elements is taken; 16-bit operands of the products whose rows do not
+ * begin and end on 16 bytes (pointer, ld and width) are copied to such rows in the workspace first, fp32 ones always.
+ * Products of few rows, and both gradients of the loss of few tokens, take all operands as they lie, fp32 through
+ * fp32 instructions.  Outputs must not overlap inputs, except Y and residual, which may be one array.
  *
  * Calls are queued on `stream`, a hipStream_t of the caller's (NULL: HIP's null stream) or dnpeff_stream(), and
  * allocate nothing and wait for nothing, so they can be captured in a HIP graph.  The workspace belongs to the
@@ -626,8 +626,9 @@ int dnpeff_vocab_loss(void* stream, int type, int64_t rows, int64_t n_in, int64_
 /* Its gradients for dloss [rows], the gradients of the tokens' losses, from the lse of the forward call: dX [rows,
  * n_in] and dE [n_words, n_in], either may be NULL.  The vocabulary goes by in pieces whose logits are formed again;
  * (softmax - label) dloss is rounded to `type` once for the products (16-bit types: after dividing by the largest
- * |dloss|, which fp32 puts back; of few tokens it stays fp32 and whole). Tokens without a label contribute nothing, whatever
- * their rows of X hold (for dE, X is copied without them); a label of n_words and more makes dX's row and dE NaN. */
+ * |dloss|, which fp32 puts back; of few tokens it stays fp32 and whole).  Tokens without a label contribute nothing,
+ * whatever their rows of X hold (for dE, X is copied without them); a label of n_words and more makes dX's row and dE
+ * NaN. */
 int dnpeff_vocab_loss_backward(void* stream, int type, int64_t rows, int64_t n_in, int64_t n_words, const void* X, int64_t ldx,
                                const void* E, int64_t lde, const int32_t* labels, const float* lse, const float* dloss, void* dX,
                                int64_t lddx, void* dE, int64_t ldde, void* workspace, int64_t workspace_bytes);
