@@ -633,6 +633,46 @@ int dnpeff_vocab_loss_backward(void* stream, int type, int64_t rows, int64_t n_i
                                const void* E, int64_t lde, const int32_t* labels, const float* lse, const float* dloss, void* dX,
                                int64_t lddx, void* dE, int64_t ldde, void* workspace, int64_t workspace_bytes);
 
+/* What a model answers, at a temperature T > 0 (z = X E^T / T): lse[t] = log sum exp z[t, v]; logp[t, j] = z[t, w] - lse[t]
+ * of each row's given words w = words[t, j] (n_given at most 4096; both arrays [rows, n_given], dense); entropy[t] =
+ * - sum p log p, in nats; and the n_top likeliest words (at most 128 and n_words) with their log p, the likeliest first:
+ * top_words, top_logp [rows, n_top], dense.  Which word is the likelier is decided by the products in 64 bits among the
+ * n_top + 8 that lead in fp32; of equal ones the lower comes first.  A negative given word has logp 0, one of n_words and more
+ * NaN.  A row whose lse is not finite (infinities or NaN among its logits) has entropy NaN and alternatives -1 with NaN.
+ * With n_given = 0 words and logp may be NULL, with n_top = 0 the alternatives; lse and entropy may be NULL.
+ * The workspace call serves dnpeff_vocab_distill and its gradients as well (n_given: the listed words, n_top = 0). */
+int dnpeff_vocab_probs_workspace(int type, int64_t rows, int64_t n_in, int64_t n_words, int n_given, int n_top, int aligned,
+                                 int64_t* forward_bytes, int64_t* backward_bytes);
+int dnpeff_vocab_probs(void* stream, int type, int64_t rows, int64_t n_in, int64_t n_words, const void* X, int64_t ldx,
+                       const void* E, int64_t lde, float temperature, int n_given, const int32_t* words, float* logp, float* lse,
+                       float* entropy, int n_top, int32_t* top_words, float* top_logp, void* workspace, int64_t workspace_bytes);
+/* The gradients dX and dE of logp and entropy for dlogp [rows, n_given] and dentropy [rows] (either may be NULL: zero), from the
+ * logp, lse and entropy of the forward call at the same temperature (entropy may be NULL without dentropy):
+ *   dz_v = (sum_j dlogp_j [v = w_j] - p_v (sum_j dlogp_j + dentropy (log p_v + entropy))) / T,
+ * rounded to `type` once for the products as in dnpeff_vocab_loss_backward.  Rows without a gradient (every dlogp of a word and
+ * dentropy 0) contribute nothing, whatever their rows of X hold; a given word of n_words and more makes dX's row and dE
+ * NaN.  A word may be given twice. */
+int dnpeff_vocab_probs_backward(void* stream, int type, int64_t rows, int64_t n_in, int64_t n_words, const void* X, int64_t ldx,
+                                const void* E, int64_t lde, float temperature, int n_given, const int32_t* words, const float* logp,
+                                const float* lse, const float* entropy, const float* dlogp, const float* dentropy, void* dX,
+                                int64_t lddx, void* dE, int64_t ldde, void* workspace, int64_t workspace_bytes);
+
+/* Distillation: the divergence of a student's probabilities from those of a teacher, of which the likeliest words are known with
+ * their logits (or log p), words and logits [rows, n_listed] (1 to 4096), dense: with q = softmax(logits / T) over a row's listed words
+ *   loss[t] = sum_j q_j (log q_j - logp[t, j]),  logp and lse as above, at the same T.
+ * Entries of a negative word or a logit of -infinity are not listed; a row without any has loss 0.  NaN or +infinity among a
+ * row's listed logits, or a listed word of n_words and more, make its loss NaN.  loss, logp and lse may be NULL. */
+int dnpeff_vocab_distill(void* stream, int type, int64_t rows, int64_t n_in, int64_t n_words, const void* X, int64_t ldx,
+                         const void* E, int64_t lde, float temperature, int n_listed, const int32_t* words, const float* logits,
+                         float* loss, float* logp, float* lse, void* workspace, int64_t workspace_bytes);
+/* Its gradients for dloss [rows], from the logp and lse of the forward call: dz_v = (p_v - sum_j q_j [v = w_j]) dloss / T (the
+ * factor T^2 that keeps gradients of different temperatures alike is the caller's, in dloss).  Rows without listed words
+ * contribute nothing, whatever their rows of X hold; where the loss is NaN for the lists' sake dX's row and dE are. */
+int dnpeff_vocab_distill_backward(void* stream, int type, int64_t rows, int64_t n_in, int64_t n_words, const void* X, int64_t ldx,
+                                  const void* E, int64_t lde, float temperature, int n_listed, const int32_t* words,
+                                  const float* logits, const float* logp, const float* lse, const float* dloss, void* dX,
+                                  int64_t lddx, void* dE, int64_t ldde, void* workspace, int64_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

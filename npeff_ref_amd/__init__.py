@@ -53,6 +53,11 @@ from .binding import (  # noqa: F401
     op_example_grads,
     op_vocab_loss,
     op_vocab_loss_backward,
+    op_vocab_probs,
+    op_vocab_probs_backward,
+    op_vocab_distill,
+    op_vocab_distill_backward,
     linear_workspace,
     vocab_loss_workspace,
+    vocab_probs_workspace,
 )

@@ -180,6 +180,28 @@ SIGNATURES = {
         C.c_int,
         [_p, C.c_int, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _p, _p, _p, _i64, _p, _i64, _p, _i64],
     ),
+    "dnpeff_vocab_probs_workspace": (
+        C.c_int,
+        [C.c_int, _i64, _i64, _i64, C.c_int, C.c_int, C.c_int, C.POINTER(_i64), C.POINTER(_i64)],
+    ),
+    "dnpeff_vocab_probs": (
+        C.c_int,
+        [_p, C.c_int, _i64, _i64, _i64, _p, _i64, _p, _i64, _f32, C.c_int, _p, _p, _p, _p, C.c_int, _p, _p, _p, _i64],
+    ),
+    "dnpeff_vocab_probs_backward": (
+        C.c_int,
+        [_p, C.c_int, _i64, _i64, _i64, _p, _i64, _p, _i64, _f32, C.c_int, _p, _p, _p, _p, _p, _p, _p, _i64, _p, _i64, _p,
+         _i64],
+    ),
+    "dnpeff_vocab_distill": (
+        C.c_int,
+        [_p, C.c_int, _i64, _i64, _i64, _p, _i64, _p, _i64, _f32, C.c_int, _p, _p, _p, _p, _p, _p, _i64],
+    ),
+    "dnpeff_vocab_distill_backward": (
+        C.c_int,
+        [_p, C.c_int, _i64, _i64, _i64, _p, _i64, _p, _i64, _f32, C.c_int, _p, _p, _p, _p, _p, _p, _i64, _p, _i64, _p,
+         _i64],
+    ),
 }
 
 KERNEL_CLASSES = ["spmm_n", "spmm_n_reduce", "gram_H", "xg_mu_W", "spmm_t", "gram_W", "xg_mu_H"]
@@ -537,7 +559,7 @@ class _Call:
 
     def dense(self, name, a, shape, kind=None):
         p, ld, group = self.array(name, a, shape, kind)
-        if len(shape) > 1 and p is not None and (ld != shape[-1] or (len(shape) > 2 and group != shape[-2] * shape[-1])):
+        if len(shape) > 1 and p is not None and 0 not in shape and (ld != shape[-1] or (len(shape) > 2 and group != shape[-2] * shape[-1])):
             _refuse(self.what, f"{name} has to be dense")
         return p
 
@@ -621,6 +643,12 @@ def linear_workspace(rows, n_in, n_out, dtype="float32", n_groups=0, aligned=Fal
 def vocab_loss_workspace(rows, n_in, n_words, dtype="float32", aligned=False):
     """The same of op_vocab_loss and op_vocab_loss_backward."""
     return _bytes("dnpeff_vocab_loss_workspace", _KINDS[str(dtype)], rows, n_in, n_words, int(aligned))
+
+
+def vocab_probs_workspace(rows, n_in, n_words, n_given=0, n_top=0, dtype="float32", aligned=False):
+    """The same of op_vocab_probs and op_vocab_probs_backward, and of op_vocab_distill and its gradients (n_given: the listed
+    words)."""
+    return _bytes("dnpeff_vocab_probs_workspace", _KINDS[str(dtype)], rows, n_in, n_words, n_given, n_top, int(aligned))
 
 
 def _layer(c, X_rows, W, groups):
@@ -734,6 +762,99 @@ def op_vocab_loss_backward(X, E, labels, lse, dloss, dX=None, dE=None, workspace
     c.run(lib.dnpeff_vocab_loss_backward,
           (c.type, rows, n_in, words, x, ldx, e, lde, c.dense("labels", labels, (rows,), "i4"),
            c.dense("lse", lse, (rows,), F32), c.dense("dloss", dloss, (rows,), F32), gx, lddx, ge, ldde),
+          need, workspace, stream)
+
+
+def _head(c, X, E):
+    """rows, n_in, words, the leading arguments of a call, and whether its arrays begin their rows on 16 bytes."""
+    if len(X.shape) != 2 or len(E.shape) != 2:
+        _refuse(c.what, f"X is {tuple(X.shape)}, E {tuple(E.shape)}")
+    (rows, n_in), words = X.shape, E.shape[0]
+    x, ldx, _ = c.array("X", X, (rows, n_in))
+    e, lde, _ = c.array("E", E, (words, n_in))
+    return rows, n_in, words, (c.type, rows, n_in, words, x, ldx, e, lde), _on16(c, (x, ldx, 0), (e, lde, 0))
+
+
+def _list(c, name, a, rows):
+    """How many words of a row an array [rows, many] (or None) holds."""
+    if a is None:
+        return 0
+    if len(a.shape) != 2:
+        _refuse(c.what, f"{name} is {tuple(a.shape)}, not ({rows}, any)")
+    return a.shape[1]
+
+
+def op_vocab_probs(X, E, words=None, logp=None, lse=None, entropy=None, top_words=None, top_logp=None, temperature=1.0,
+                   workspace=None, stream=None):
+    """The log probabilities of given words, the entropy and the likeliest words, of logits X E^T / temperature
+    (dnpeff_vocab_probs)."""
+    c = _Call("op_vocab_probs", X)
+    rows, n_in, n_words, head, on16 = _head(c, X, E)
+    n, k = _list(c, "words", words, rows), _list(c, "top_words", top_words, rows)
+    if (words is None) != (logp is None) or (top_words is None) != (top_logp is None):
+        _refuse(c.what, "words come with logp, and top_words with top_logp")
+    need = 0
+    if workspace is None:
+        need = _bytes("dnpeff_vocab_probs_workspace", c.type, rows, n_in, n_words, n, k, on16)[0]
+    c.run(lib.dnpeff_vocab_probs,
+          head + (temperature, n, c.dense("words", words, (rows, n), "i4"), c.dense("logp", logp, (rows, n), F32),
+                  c.dense("lse", lse, (rows,), F32), c.dense("entropy", entropy, (rows,), F32), k,
+                  c.dense("top_words", top_words, (rows, k), "i4"), c.dense("top_logp", top_logp, (rows, k), F32)),
+          need, workspace, stream)
+
+
+def op_vocab_probs_backward(X, E, words, logp, lse, entropy=None, dlogp=None, dentropy=None, dX=None, dE=None,
+                            temperature=1.0, workspace=None, stream=None):
+    """The gradients of op_vocab_probs for dlogp and dentropy, into those of dX and dE that are given
+    (dnpeff_vocab_probs_backward)."""
+    c = _Call("op_vocab_probs_backward", X)
+    rows, n_in, n_words, head, on16 = _head(c, X, E)
+    n = _list(c, "words", words, rows)
+    if dlogp is not None and words is None:
+        _refuse(c.what, "dlogp without words")
+    gx, lddx, _ = c.array("dX", dX, (rows, n_in))
+    ge, ldde, _ = c.array("dE", dE, (n_words, n_in))
+    need = 0
+    if workspace is None:
+        need = _bytes("dnpeff_vocab_probs_workspace", c.type, rows, n_in, n_words, n, 0, on16)[1]
+    c.run(lib.dnpeff_vocab_probs_backward,
+          head + (temperature, n, c.dense("words", words, (rows, n), "i4"), c.dense("logp", logp, (rows, n), F32),
+                  c.dense("lse", lse, (rows,), F32), c.dense("entropy", entropy, (rows,), F32),
+                  c.dense("dlogp", dlogp, (rows, n), F32), c.dense("dentropy", dentropy, (rows,), F32), gx, lddx, ge, ldde),
+          need, workspace, stream)
+
+
+def op_vocab_distill(X, E, words, logits, loss=None, logp=None, lse=None, temperature=1.0, workspace=None, stream=None):
+    """The divergence of the probabilities of X E^T / temperature from those of a teacher's listed words and logits
+    (dnpeff_vocab_distill)."""
+    c = _Call("op_vocab_distill", X)
+    rows, n_in, n_words, head, on16 = _head(c, X, E)
+    n = _list(c, "words", words, rows)
+    need = 0
+    if workspace is None:
+        need = _bytes("dnpeff_vocab_probs_workspace", c.type, rows, n_in, n_words, n, 0, on16)[0]
+    c.run(lib.dnpeff_vocab_distill,
+          head + (temperature, n, c.dense("words", words, (rows, n), "i4"), c.dense("logits", logits, (rows, n), F32),
+                  c.dense("loss", loss, (rows,), F32), c.dense("logp", logp, (rows, n), F32),
+                  c.dense("lse", lse, (rows,), F32)),
+          need, workspace, stream)
+
+
+def op_vocab_distill_backward(X, E, words, logits, logp, lse, dloss, dX=None, dE=None, temperature=1.0, workspace=None,
+                              stream=None):
+    """The gradients of op_vocab_distill for dloss, into those of dX and dE that are given (dnpeff_vocab_distill_backward)."""
+    c = _Call("op_vocab_distill_backward", X)
+    rows, n_in, n_words, head, on16 = _head(c, X, E)
+    n = _list(c, "words", words, rows)
+    gx, lddx, _ = c.array("dX", dX, (rows, n_in))
+    ge, ldde, _ = c.array("dE", dE, (n_words, n_in))
+    need = 0
+    if workspace is None:
+        need = _bytes("dnpeff_vocab_probs_workspace", c.type, rows, n_in, n_words, n, 0, on16)[1]
+    c.run(lib.dnpeff_vocab_distill_backward,
+          head + (temperature, n, c.dense("words", words, (rows, n), "i4"), c.dense("logits", logits, (rows, n), F32),
+                  c.dense("logp", logp, (rows, n), F32), c.dense("lse", lse, (rows,), F32),
+                  c.dense("dloss", dloss, (rows,), F32), gx, lddx, ge, ldde),
           need, workspace, stream)
 
 

@@ -228,7 +228,14 @@ __device__ __forceinline__ void group_of_tile(const group_rows& G, int tall, int
 
 // ---- a product ---------------------------------------------------------------------------------------------------
 enum { ONE = 0, BY_ROWS = 1, BY_REDUCTION = 2 };                      // groups: none, of rows of A and C, of the reduction
-enum { E_LINEAR = 0, E_STORE = 1, E_LOSS = 2, E_LOSS_GRAD = 3 };     // what becomes of a tile
+enum { E_LINEAR = 0, E_STORE = 1, E_LOSS = 2, E_LOSS_GRAD = 3, E_PROBS = 4, E_PROBS_GRAD = 5 };  // what becomes of a tile
+constexpr bool is_stats(int e) { return e == E_LOSS || e == E_PROBS; }
+constexpr bool is_grad(int e) { return e == E_LOSS_GRAD || e == E_PROBS_GRAD; }
+// A row of the logits' gradient but for its listed words: dz = p (a + b log p), and 0 where the row is not alive.
+struct slope_row {
+  float lse, a, b;
+  int alive;
+};
 
 struct args {
   const void *A, *B;        // (of num<T>::op)
@@ -262,6 +269,13 @@ struct args {
   int parts_n, part0;
   float* hit;               // [M] the label's logit
   int64_t word0, words;
+  // E_PROBS, E_PROBS_GRAD
+  float inv_heat;           // logits are multiplied by it
+  float* weighted;          // [M][parts_n]: of each tile's words, sum of exp(z - max) (z - max)
+  float *tops, *logits;     // (or NULL) [M][chunks]: the largest logit of each chunk of words; [M][ldl]: the logits of the
+  int64_t chunks, ldl;      // chunks whose largest is not below the row's floor (NULL: of all); ldl is a multiple of 64
+  const float* floor;
+  const slope_row* slopes;  // [M]
 };
 
 // A kernel's arguments where they lie: read where they are needed, not kept in registers throughout.
@@ -372,6 +386,21 @@ __device__ __forceinline__ void finish_grad(const P& p, int64_t m, int64_t n, fl
   for (int t = 0; t < W; t++) {
     const float g = (__expf(v[t] - lse) - (t == mine ? 1.f : 0.f)) * w;
     v[t] = t < there ? g : 0.f;
+  }
+  store_op<T, W>((typename num<T>::op*)p.out + m * p.ldc + n, p.M * p.ldc, v);
+}
+// p (a + b log p): the same of probabilities and entropies
+__device__ __forceinline__ float slope_of(float z, const slope_row& t) {
+  const float l = z - t.lse, lp = l < -150.f ? -150.f : l;  // (p is 0 there; NaN stays)
+  return __expf(lp) * fmaf(t.b, lp, t.a);
+}
+template <class T, int W, class P>
+__device__ __forceinline__ void finish_slope(const P& p, int64_t m, int64_t n, float* v, const slope_row& t, float shrink) {
+  const int there = t.alive == 0 || n >= p.N ? 0 : p.N - n < W ? (int)(p.N - n) : W;
+#pragma unroll
+  for (int e = 0; e < W; e++) {
+    const float g = slope_of(v[e] * p.inv_heat, t) * shrink;
+    v[e] = e < there ? g : 0.f;
   }
   store_op<T, W>((typename num<T>::op*)p.out + m * p.ldc + n, p.M * p.ldc, v);
 }
@@ -511,16 +540,16 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
   const int lane = tid & 63;
   const int wm = wave / WN, wn = wave % WN, q = lane >> 4;
   const int64_t m_wave = w.m0 + wm * (BM / WM), n_wave = w.n0 + wn * (BN / WN), m_end = w.m_end;
-  if constexpr (E != E_LOSS) {
+  if constexpr (!is_stats(E)) {
     // Each wave by itself, 64 of its rows at a time: through LDS, so that its lanes take consecutive values of a row, and
     // whole lines go out.  Piece c of row r at c ^ (r & 15).  (The rows go by in a loop: unrolled over all of them the code
     // would not fit the instruction cache.)
     constexpr int COLS = BN / WN, BLOCKS = 4;
     static_assert(COLS == 64 && FM % BLOCKS == 0, "a row of a wave's part is 16 pieces of 16 bytes");
     const unsigned mine = room + wave * (BLOCKS * 4096);
-    const int64_t n_end = E == E_LOSS_GRAD ? p.ldc : p.N;
+    const int64_t n_end = is_grad(E) ? p.ldc : p.N;
     if (n_wave >= n_end) return;
-    const float shrink = E == E_LOSS_GRAD && p.shrink ? *p.shrink : 1.f;
+    const float shrink = is_grad(E) && p.shrink ? *p.shrink : 1.f;
     // Rows m_top .. of 64: W values a lane, `lanes` side by side.  Where the columns end within a wave's part (tail) the last
     // lane begins as much earlier as makes its values whole: both lanes have the same for what they share.
     const int cols = n_end - n_wave < COLS ? (int)(n_end - n_wave) : COLS;
@@ -535,7 +564,8 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
       typedef loose<T, W> piece;
       float bias[W];
       piece more[AT_ONCE], next[AT_ONCE];  // the residual of a turn's rows, and of the next turn's
-      token these[AT_ONCE], those[AT_ONCE];  // what the loss needs of them
+      typedef typename std::conditional<E == E_PROBS_GRAD, slope_row, token>::type of_row;
+      of_row these[AT_ONCE], those[AT_ONCE];  // what the loss needs of them
       auto fetch = [&](int r0) {
 #pragma unroll
         for (int u = 0; u < AT_ONCE; u++) {
@@ -543,6 +573,8 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
           const int64_t m = m_top + (r < last ? r : last);
           if constexpr (E == E_LOSS_GRAD)
             those[u] = token{p.labels[m], p.lse[m], p.dloss[m]};
+          else if constexpr (E == E_PROBS_GRAD)
+            those[u] = p.slopes[m];
           else
             next[u] = *(const piece*)((const T*)p.residual + m * p.ldr + n);
         }
@@ -551,7 +583,7 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
         bias_of<T, W>(p, n, w.group, w.held, bias);
         if (p.residual) fetch(0);
       }
-      if constexpr (E == E_LOSS_GRAD) fetch(0);
+      if constexpr (is_grad(E)) fetch(0);
 #pragma unroll 1
       for (int r0 = 0; r0 < 16 * BLOCKS && r0 <= last; r0 += STEP * AT_ONCE) {
         if (E == E_LINEAR && p.residual) {
@@ -559,7 +591,7 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
           for (int u = 0; u < AT_ONCE; u++) more[u] = next[u];
           fetch(r0 + STEP * AT_ONCE);
         }
-        if constexpr (E == E_LOSS_GRAD) {
+        if constexpr (is_grad(E)) {
 #pragma unroll
           for (int u = 0; u < AT_ONCE; u++) these[u] = those[u];
           fetch(r0 + STEP * AT_ONCE);
@@ -589,6 +621,8 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
               finish_linear<T, W>(p, m, n, v, bias, res, w.held);
             } else if constexpr (E == E_LOSS_GRAD) {
               finish_grad<T, W>(p, m, n, v, these[u], shrink);
+            } else if constexpr (E == E_PROBS_GRAD) {
+              finish_slope<T, W>(p, m, n, v, these[u], shrink);
             } else {
               finish_store<T, W>(p, w.sheet, m, n, v);
             }
@@ -617,7 +651,7 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
           rows_out(four(), std::integral_constant<int, 16>(), std::false_type(), m_top);
         else
           rows_out(full(), std::integral_constant<int, 64 / W>(), std::false_type(), m_top);
-      } else if (E != E_LOSS_GRAD) {  // (a row of g is whole waves' parts)
+      } else if (!is_grad(E)) {  // (a row of g is whole waves' parts)
         if (cols >= W)
           rows_out(full(), std::integral_constant<int, 64 / W>(), std::true_type(), m_top);
         else if (cols >= 4)
@@ -633,21 +667,37 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
     // lane groups, the waves side by side (through LDS).
     __syncthreads();
     DN_LDS float2* side = lds_at<float2>(room);  // [WN][BM]
+    DN_LDS float* side_w = lds_at<float>(room + WN * BM * 8);
     const int m_there = (int)(m_end - w.m0 < BM ? m_end - w.m0 : BM);
     const bool whole = n_wave + FN * 16 <= p.N;
     const int there = whole ? FN * 16 : (int)(p.N - n_wave < 0 ? 0 : p.N - n_wave) - q * 4;
     int labels[FM];  // (asked for together)
+    float floors[FM];
+    if constexpr (E == E_LOSS) {
 #pragma unroll
-    for (int i = 0; i < FM; i++) {
-      const int64_t m = m_wave + i * 16 + (lane & 15);
-      labels[i] = p.labels[m < m_end ? m : m_end - 1];
+      for (int i = 0; i < FM; i++) {
+        const int64_t m = m_wave + i * 16 + (lane & 15);
+        labels[i] = p.labels[m < m_end ? m : m_end - 1];
+      }
+    } else {
+      const bool some = p.tops != nullptr && p.floor != nullptr;
+#pragma unroll
+      for (int i = 0; i < FM; i++) {
+        const int64_t m = m_wave + i * 16 + (lane & 15);
+        floors[i] = some ? p.floor[m < m_end ? m : m_end - 1] : -INFINITY;
+      }
+      const float inv_heat = p.inv_heat;
+#pragma unroll
+      for (int i = 0; i < FM; i++)
+#pragma unroll
+        for (int j = 0; j < FN; j++) acc[i][j] *= inv_heat;
     }
 #pragma unroll
     for (int i = 0; i < FM; i++) {
       const int64_t m = m_wave + i * 16 + (lane & 15);
       // (the label's column among the lane's, or none)
-      const int64_t place = m < m_end ? labels[i] - (n_wave + q * 4) : -1;
-      const int mine = place >= 0 && place < 64 && labels[i] < p.N ? (int)place : -1;
+      const int64_t place = E == E_LOSS && m < m_end ? labels[i] - (n_wave + q * 4) : -1;
+      const int mine = E == E_LOSS && place >= 0 && place < 64 && labels[i] < p.N ? (int)place : -1;
       float top = -INFINITY, hit = 0.f;
       if (whole) {
 #pragma unroll
@@ -663,19 +713,42 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
             top = fmaxf(top, acc[i][j][e]);
           }
       }
+      if constexpr (E == E_LOSS) {
 #pragma unroll
-      for (int j = 0; j < FN; j++)
+        for (int j = 0; j < FN; j++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) hit = j * 16 + e == mine ? acc[i][j][e] : hit;
-      if (mine >= 0 && (mine & 15) < 4) p.hit[m] = hit;
+          for (int e = 0; e < 4; e++) hit = j * 16 + e == mine ? acc[i][j][e] : hit;
+        if (mine >= 0 && (mine & 15) < 4) p.hit[m] = hit;
+      }
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
       const float from = top == -INFINITY ? 0.f : top;
-      float sum = 0.f;
+      float sum = 0.f, weighted = 0.f;
+      if constexpr (E == E_LOSS) {
 #pragma unroll
-      for (int j = 0; j < FN; j++)
+        for (int j = 0; j < FN; j++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) sum += __expf(acc[i][j][e] - from);
+          for (int e = 0; e < 4; e++) sum += __expf(acc[i][j][e] - from);
+      } else {
+        if (p.tops && m < m_end && n_wave < p.N) {
+          if (q == 0) p.tops[m * p.chunks + (n_wave >> 6)] = top;
+          if (!(top < floors[i])) {
+#pragma unroll
+            for (int j = 0; j < FN; j++) *(v4f*)(p.logits + m * p.ldl + n_wave + j * 16 + q * 4) = acc[i][j];
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < FN; j++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const float z = acc[i][j][e] - from, x = __expf(z);
+            sum += x;
+            weighted = fmaf(x, fmaxf(z, -150.f), weighted);  // (x is 0 there)
+          }
+        weighted += __shfl_xor(weighted, 16, 64);
+        weighted += __shfl_xor(weighted, 32, 64);
+        if (q == 0) side_w[wn * BM + wm * (BM / WM) + i * 16 + lane] = weighted;
+      }
       sum += __shfl_xor(sum, 16, 64);
       sum += __shfl_xor(sum, 32, 64);
       if (q == 0) {
@@ -694,7 +767,17 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
         const float x = side[v * BM + m].x, y = side[v * BM + m].y;
         if (x != -INFINITY || y != 0.f) sum += y * __expf(x - from);
       }
-      p.parts[(w.m0 + m) * p.parts_n + p.part0 + w.tn] = float2{top, sum};
+      const int64_t to = (w.m0 + m) * p.parts_n + p.part0 + w.tn;
+      p.parts[to] = float2{top, sum};
+      if constexpr (E == E_PROBS) {
+        float weighted = 0.f;
+#pragma unroll
+        for (int v = 0; v < WN; v++) {
+          const float x = side[v * BM + m].x, y = side[v * BM + m].y;
+          if (x != -INFINITY || y != 0.f) weighted += __expf(x - from) * fmaf(fmaxf(x - from, -150.f), y, side_w[v * BM + m]);
+        }
+        p.weighted[to] = weighted;
+      }
     }
   }
 }
@@ -884,6 +967,7 @@ __global__ __launch_bounds__(512, 2) void k_few(args p, int parts) {
   constexpr int CH = 16 / sizeof(T), STEP = 4 * CH, AHEAD = 8 / COLS;
   __shared__ v4f sums[COLS][8][64];
   __shared__ float2 stats[8][16];
+  __shared__ float stats_w[8][16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int q = lane >> 4, part = wave % parts;
   const int64_t n0 = ((int64_t)blockIdx.x * (8 / parts) + wave / parts) * (16 * COLS);
@@ -1021,26 +1105,61 @@ __global__ __launch_bounds__(512, 2) void k_few(args p, int parts) {
               if (n < p.N) ((float*)p.out)[n * 16 + (lane & 15)] = g;
             }
         }
+      } else if constexpr (E == E_PROBS_GRAD) {
+        if (part == 0) {
+          const slope_row t = m < m_end ? p.slopes[m] : slope_row{0.f, 0.f, 0.f, 0};
+#pragma unroll
+          for (int h = 0; h < COLS; h++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const int64_t n = n0 + h * 16 + q * 4 + e;
+              const float g = t.alive ? slope_of(acc[h][e] * p.inv_heat, t) : 0.f;
+              if (n < p.N) ((float*)p.out)[n * 16 + (lane & 15)] = g;
+            }
+        }
       } else {
         if (part == 0) {
-          const int64_t label = m < m_end ? (int64_t)p.labels[m] : -1;
-          float top = -INFINITY, sum = 0.f;
+          const int64_t label = E == E_LOSS && m < m_end ? (int64_t)p.labels[m] : -1;
+          float top = -INFINITY, sum = 0.f, weighted = 0.f;
+          if constexpr (E == E_PROBS) {
+#pragma unroll
+            for (int h = 0; h < COLS; h++) acc[h] *= p.inv_heat;
+          }
 #pragma unroll
           for (int h = 0; h < COLS; h++)
 #pragma unroll
             for (int t = 0; t < 4; t++) {
               const int64_t n = n0 + h * 16 + q * 4 + t;
               if (n < p.N) top = fmaxf(top, acc[h][t]);
-              if (n == label && n < p.N) p.hit[m] = acc[h][t];
+              if (E == E_LOSS && n == label && n < p.N) p.hit[m] = acc[h][t];
             }
           top = fmaxf(top, __shfl_xor(top, 16, 64));
           top = fmaxf(top, __shfl_xor(top, 32, 64));
           const float from = top == -INFINITY ? 0.f : top;
+          if constexpr (E == E_PROBS) {
+            if (p.tops && m < m_end && n0 < p.N) {  // (a chunk is a wave's columns)
+              if (q == 0) p.tops[m * p.chunks + n0 / (16 * COLS)] = top;
+#pragma unroll
+              for (int h = 0; h < COLS; h++) {
+                const int64_t n = n0 + h * 16 + q * 4;
+                if (n < p.ldl) *(v4f*)(p.logits + m * p.ldl + n) = acc[h];
+              }
+            }
+          }
 #pragma unroll
           for (int h = 0; h < COLS; h++)
 #pragma unroll
             for (int t = 0; t < 4; t++)
-              if (n0 + h * 16 + q * 4 + t < p.N) sum += __expf(acc[h][t] - from);
+              if (n0 + h * 16 + q * 4 + t < p.N) {
+                const float z = acc[h][t] - from, x = __expf(z);
+                sum += x;
+                if (E == E_PROBS) weighted = fmaf(x, fmaxf(z, -150.f), weighted);
+              }
+          if constexpr (E == E_PROBS) {
+            weighted += __shfl_xor(weighted, 16, 64);
+            weighted += __shfl_xor(weighted, 32, 64);
+            if (q == 0) stats_w[wave][lane] = weighted;
+          }
           sum += __shfl_xor(sum, 16, 64);
           sum += __shfl_xor(sum, 32, 64);
           if (q == 0) stats[wave][lane] = float2{top, sum};
@@ -1055,6 +1174,14 @@ __global__ __launch_bounds__(512, 2) void k_few(args p, int parts) {
             if (s.x != -INFINITY || s.y != 0.f) sum += s.y * __expf(s.x - from);
           }
           p.parts[(m_top + threadIdx.x) * p.parts_n + blockIdx.x] = float2{top, sum};
+          if constexpr (E == E_PROBS) {
+            float weighted = 0.f;
+            for (int w = 0; w < 8; w += parts) {
+              const float2 s = stats[w][threadIdx.x];
+              if (s.x != -INFINITY || s.y != 0.f) weighted += __expf(s.x - from) * fmaf(fmaxf(s.x - from, -150.f), s.y, stats_w[w][threadIdx.x]);
+            }
+            p.weighted[(m_top + threadIdx.x) * p.parts_n + blockIdx.x] = weighted;
+          }
         }
         __syncthreads();
       }
@@ -1333,7 +1460,7 @@ inline int few_parts(int64_t blocks) {
   return parts;
 }
 template <class T, int E>
-int launch_few(args p, hipStream_t st, int* parts_n = nullptr) {
+int launch_few(args p, hipStream_t st, int* parts_n = nullptr, int* chunk = nullptr) {
   const int64_t slots = p.mode == BY_ROWS ? (p.G.groups + 1 < p.M ? p.G.groups + 1 : p.M) : 1;
   DN_CHECK(slots <= 65535, "product of %lld rows in %d groups: too many for one launch", (long long)p.M, p.G.groups);
   // 32 columns a wave where they are enough for three on every CU (one token of 32000 words of 4096: 43.5 us at 16, 41.1 at 32;
@@ -1342,12 +1469,14 @@ int launch_few(args p, hipStream_t st, int* parts_n = nullptr) {
   const int parts = few_parts(ceil_div(p.N, wide) * slots), cols = wide * 8 / parts;
   p.parts_n = (int)ceil_div(p.N, cols);
   if (parts_n) *parts_n = p.parts_n;
+  p.chunks = ceil_div(p.N, wide);
+  if (chunk) *chunk = wide;
   const dim3 grid((unsigned)ceil_div(p.N, cols), (unsigned)slots);
   DN_CHECK(grid.x < 1u << 23, "product of %lld columns: too many for one launch", (long long)p.N);
   // 16, 32 or 64 rows for each reading of B (fp32 products of 64000 x 2048, 16 at a time and so: 32 rows 266 and 164 us, 48 391 and
   // 233, the loss of 64 rows 449 and 253)
   const int64_t each = p.mode == BY_ROWS ? ceil_div(p.M, p.G.groups) : p.M;
-  const int rows = E == E_LOSS_GRAD || each <= 16 ? 1 : each <= 32 ? 2 : 4;
+  const int rows = is_grad(E) || each <= 16 ? 1 : each <= 32 ? 2 : 4;
   auto launch = [&](auto cols_of, auto rows_of) { k_few<T, decltype(cols_of)::value, decltype(rows_of)::value, E><<<grid, 512, 0, st>>>(p, parts); };
   auto launch_cols = [&](auto rows_of) {
     if (wide == 32)
@@ -1355,7 +1484,7 @@ int launch_few(args p, hipStream_t st, int* parts_n = nullptr) {
     else
       launch(std::integral_constant<int, 1>(), rows_of);
   };
-  if constexpr (E != E_LOSS_GRAD) {
+  if constexpr (!is_grad(E)) {
     if (rows == 4) launch_cols(std::integral_constant<int, 4>());
     if (rows == 2) launch_cols(std::integral_constant<int, 2>());
   }

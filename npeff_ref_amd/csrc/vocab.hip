@@ -7,6 +7,9 @@
 // tile; a second kernel joins them.  Backward: the vocabulary goes by in pieces; the logits of a piece are formed again,
 // turned into g where they are summed, and multiplied on both sides.  g is rounded to the operands' type, once: its
 // products run on the matrix cores of that type, and the rounding (2^-9 of a value in bf16) is that of the results.
+//
+// The same of what a model answers, at a temperature T (z = X E^T / T): log p of given words, the entropy, the likeliest
+// words; and of a student that learns from a teacher's likeliest words (answers, further down).
 #include "tiles.hpp"
 
 using namespace dn;
@@ -280,12 +283,44 @@ int loss_forward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, cons
   return 0;
 }
 
+// Places of the logits' gradient that have values of their own (E_PROBS_GRAD): those of a row's listed words.
+struct spots {
+  int64_t rows;
+  int many;            // of a row
+  const int32_t* word; // [rows][many], negative: none
+  const float* g;
+};
+// They take the place of what the tiles (or FEW: k_few, [words][16]) left there.
+template <class T, bool FEW>
+__global__ __launch_bounds__(256) void k_spots(spots s, int64_t word0, int64_t words, const float* shrink, void* out, int64_t ldc, int64_t plane) {
+  const int64_t all = s.rows * s.many;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const int64_t n = (int64_t)s.word[i] - word0;
+    if (s.word[i] < 0 || n < 0 || n >= words) continue;
+    const int64_t m = i / s.many;
+    const float g = s.g[i] * (shrink ? *shrink : 1.f);
+    if constexpr (FEW)
+      ((float*)out)[n * 16 + m] = g;
+    else
+      store_op<T, 1>((typename num<T>::op*)out + m * ldc + n, plane, &g);
+  }
+}
+template <class T, bool FEW>
+int put_spots(const spots& s, int64_t word0, int64_t words, const float* shrink, void* out, int64_t ldc, int64_t plane, hipStream_t st) {
+  const int64_t blocks = ceil_div(s.rows * s.many, 256);
+  if (blocks == 0) return 0;
+  k_spots<T, FEW><<<(unsigned)(blocks < JOIN_MOST ? blocks : JOIN_MOST), 256, 0, st>>>(s, word0, words, shrink, out, ldc, plane);
+  DN_LAUNCH_CHECK();
+  return 0;
+}
+
 // (back_is_few)
-template <class T>
-int few_backward(hipStream_t st, const args& logits, char* g, float* parts, void* dX, int64_t lddx, void* dE, int64_t ldde) {
+template <class T, int E>
+int few_backward(hipStream_t st, const args& logits, const spots& own, char* g, float* parts, void* dX, int64_t lddx, void* dE, int64_t ldde) {
   args p = logits;
   p.out = g;
-  DN_TRY((launch_few<T, E_LOSS_GRAD>(p, st)));
+  DN_TRY((launch_few<T, E>(p, st)));
+  if constexpr (E == E_PROBS_GRAD) DN_TRY((put_spots<T, true>(own, 0, p.N, nullptr, g, 0, 0, st)));
   const int64_t splits = back_splits(p.K, p.N);
   back_args b{};
   b.rows = (int)p.M, b.n_in = p.K, b.words = p.N, b.run = ceil_div(p.N, splits * 8);
@@ -305,20 +340,24 @@ int few_backward(hipStream_t st, const args& logits, char* g, float* parts, void
   DN_LAUNCH_CHECK();
   return 0;
 }
-template <class T>
+// of: what the epilogue of the logits (EPILOGUE) takes of the rows; labels: rows of a negative one have no gradient; dloss: the
+// rows' weights, which k_shrink brings to the range of the type.
+template <class T, int EPILOGUE>
 int loss_backward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, const void* X, int64_t ldx, const void* E, int64_t lde,
-                  const int32_t* labels, const float* lse, const float* dloss, void* dX, int64_t lddx, void* dE, int64_t ldde, char* ws,
-                  int64_t ws_bytes) {
+                  const args& of, const spots& own, void* dX, int64_t lddx, void* dE, int64_t ldde, char* ws, int64_t ws_bytes,
+                  const char* me) {
+  const int32_t* labels = of.labels;
+  const float* dloss = of.dloss;
   grad_room<T> r(rows, n_in, words, X, ldx, E, lde, dE ? labels : nullptr);
-  DN_TRY(check_room("dnpeff_vocab_loss_backward", r.all, ws, ws_bytes));
+  DN_TRY(check_room(me, r.all, ws, ws_bytes));
   if (back_is_few<T>(rows, n_in)) {
     if (!dX && !dE) return 0;
-    args p{};
+    args p = of;
     p.A = X, p.lda = ldx, p.B = E, p.ldb = lde;
     p.M = rows, p.N = words, p.K = n_in;
     p.mode = ONE;
-    p.labels = labels, p.lse = lse, p.dloss = dloss, p.words = words;
-    return few_backward<T>(st, p, ws + 256, (float*)(ws + 256 + r.g), dX, lddx, dE, ldde);
+    p.words = words;
+    return few_backward<T, EPILOGUE>(st, p, own, ws + 256, (float*)(ws + 256 + r.g), dX, lddx, dE, ldde);
   }
   float* both = (float*)ws;
   ws += 256;
@@ -336,14 +375,15 @@ int loss_backward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, con
     const int64_t n = words - w0 < r.piece ? words - w0 : r.piece;
     const void* Ep = (const typename num<T>::op*)r.m[1].p + w0 * r.m[1].ld;
     const bool first = w0 == 0, last = w0 + n == words;
-    args p{};
+    args p = of;
     p.A = r.m[0].p, p.lda = r.m[0].ld, p.B = Ep, p.ldb = r.m[1].ld;
     p.a_plane = r.m[0].plane, p.b_plane = r.m[1].plane;
     p.M = rows, p.N = n, p.K = n_in;
     p.mode = ONE;
-    p.labels = labels, p.lse = lse, p.dloss = dloss, p.shrink = shrink, p.word0 = w0, p.words = words;
+    p.shrink = shrink, p.word0 = w0, p.words = words;
     p.out = g, p.ldc = padded(n);
-    DN_TRY((launch_product<T, true, true, E_LOSS_GRAD>(p, nullptr, st)));
+    DN_TRY((launch_product<T, true, true, EPILOGUE>(p, nullptr, st)));
+    if constexpr (EPILOGUE == E_PROBS_GRAD) DN_TRY((put_spots<T, false>(own, w0, n, shrink, g, p.ldc, p.M * p.ldc, st)));
     if (dX) {
       args q{};
       q.A = g, q.lda = padded(n), q.B = Ep, q.ldb = r.m[1].ld;
@@ -369,6 +409,603 @@ int loss_backward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, con
   return 0;
 }
 
+// ---- answers -----------------------------------------------------------------------------------------------------
+//   logp[t, j] = z[t, w_tj] - lse_t,  H_t = lse_t - sum_v p z = log s - W / s  with s = sum exp(z - max), W = sum exp(z - max) (z - max)
+//   loss_t = sum_j q_j (log q_j - logp[t, j]),  q = softmax over the listed words of l / T
+//
+// Alternatives.  The tiles leave the largest logit of every chunk of words (64; of few rows 16 or 32) and the logits
+// themselves.  The KEEP = n + 8 largest lie in the KEEP chunks of the largest maxima (in any other chunk every word is behind the KEEP
+// that lead those), so what has to be read of the logits are these chunks.  The vocabulary goes by in pieces: from the first
+// piece on a row has KEEP words, and a chunk that does not reach the least of them is not even stored.  The last n + 8 are then
+// put in order by their products in 64 bits: the order is that of the exact logits, not of a summation's, and equal ones
+// (the same embedding twice) keep the order of the words.
+constexpr int MOST_TOP = 128, SPARE = 8, MOST_KEEP = MOST_TOP + SPARE;
+constexpr int MOST_LISTED = 4096;
+constexpr int64_t BLOCK_ROWS = 65536;                 // rows at a time, for the workspace's sake
+constexpr int64_t LOGIT_BYTES = (int64_t)512 << 20;  // of a piece's logits
+
+// Floats in the order of their values (equal zeros equal); 1: NaN, 0 is below all.
+__device__ __forceinline__ unsigned key_of(float v) {
+  if (v != v) return 1;
+  const unsigned u = __float_as_uint(v + 0.f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(unsigned key) {
+  return key <= 1 ? -INFINITY : __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+
+struct running {  // a row's statistics so far
+  float top, sum, weighted;
+  int kept;
+};
+struct answer_args {
+  int64_t rows, n_in, words;   // words: of the whole vocabulary
+  int64_t word0, piece;        // this piece's
+  int first, last;
+  const float2* parts;         // [rows][parts_n]
+  const float* weighted;
+  int parts_n;
+  // alternatives (n_top > 0)
+  const float *tops, *logits;  // [rows][chunks], [rows][ldl]
+  int64_t chunks, ldl;
+  int chunk, n_top, keep;
+  running* state;              // [rows]
+  unsigned* kept_key;          // [rows][keep], in the order of the words
+  int32_t* kept_word;
+  float* floor;                // [rows]
+  int32_t* top_words;
+  float* top_logp;
+  // given or listed words
+  const void *X, *E;
+  int64_t ldx, lde;
+  float inv_heat;
+  int n_given;
+  const int32_t* given;        // [rows][n_given]
+  float *logp, *lse, *entropy;
+  const float* teacher;        // (or NULL) [rows][n_given]
+  float* loss;
+};
+
+// The product of two rows in 64 bits, in every lane.
+template <class T>
+__device__ __forceinline__ double dot_rows(const T* a, const T* b, int64_t n, int lane) {
+  constexpr int W = 16 / sizeof(T);
+  double s = 0.0;
+  int64_t k = (int64_t)lane * W;
+#pragma unroll 4
+  for (; k + W <= n; k += 64 * W) {
+    const loose<T, W> x = *(const loose<T, W>*)(a + k), y = *(const loose<T, W>*)(b + k);
+#pragma unroll
+    for (int t = 0; t < W; t++) s = fma((double)(float)x[t], (double)(float)y[t], s);
+  }
+  for (int t = 0; t < W && k + t < n; t++) s = fma((double)(float)a[k + t], (double)(float)b[k + t], s);
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) s += __shfl_xor(s, d, 64);
+  return s;
+}
+
+template <int THREADS>
+struct pick_room {
+  static constexpr int WAVES = THREADS / 64;
+  int hist[256];
+  int count[2][WAVES];
+  unsigned prefix, mask;
+  int left, whole;
+};
+// How many of n items have a key that is not 0.
+template <int THREADS, class Key>
+__device__ __forceinline__ int count_keys(pick_room<THREADS>& r, int64_t n, Key key) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int mine = 0;
+  for (int64_t i = threadIdx.x; i < n; i += THREADS) mine += key(i) != 0;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) mine += __shfl_xor(mine, d, 64);
+  __syncthreads();
+  if (lane == 0) r.count[0][wave] = mine;
+  __syncthreads();
+  int all = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; w++) all += r.count[0][w];
+  return all;
+}
+// The `need` items of the largest keys, of equal ones the first, handed to take(place, item, key) in the order of the items; needs as
+// many items with keys.  Digit by digit: how many have each value of the next 8 bits, the value among them at which `need` is reached.
+template <int THREADS, class Key, class Take>
+__device__ __forceinline__ void pick(pick_room<THREADS>& r, int64_t n, int need, bool all, Key key, Take take) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __syncthreads();
+  if (tid == 0) r.prefix = all ? 1u : 0u, r.mask = all ? 0xffffffffu : 0u, r.left = need, r.whole = all;
+  unsigned prefix = all ? 1u : 0u, mask = all ? 0xffffffffu : 0u;
+  int left = need;
+  for (int shift = 24; shift >= 0 && !all; shift -= 8) {
+    for (int i = tid; i < 256; i += THREADS) r.hist[i] = 0;
+    __syncthreads();
+    for (int64_t i = tid; i < n; i += THREADS) {
+      const unsigned k = key(i);
+      if (k != 0 && (k & mask) == prefix) atomicAdd(&r.hist[(k >> shift) & 255], 1);
+    }
+    __syncthreads();
+    if (wave == 0) {
+      // lane l: the four values from 252 - 4 l down
+      int own[4], sum = 0;
+#pragma unroll
+      for (int e = 0; e < 4; e++) own[e] = r.hist[255 - 4 * lane - e], sum += own[e];
+      int before = sum;
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) {
+        const int u = __shfl_up(before, d, 64);
+        if (lane >= d) before += u;
+      }
+      before -= sum;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        if (before < left && before + own[e] >= left) {
+          r.prefix = prefix | (unsigned)(255 - 4 * lane - e) << shift;
+          r.left = left - before;
+          r.whole = own[e] == left - before;
+        }
+        before += own[e];
+      }
+    }
+    __syncthreads();
+    prefix = r.prefix, left = r.left;
+    mask |= 255u << shift;
+    if (r.whole) break;
+  }
+  // those above the prefix, and the first `left` of those that have it
+  int taken = 0, equal = 0;
+  for (int64_t base = 0; base < n && taken < need; base += THREADS) {
+    const int64_t i = base + tid;
+    const unsigned k = i < n ? key(i) : 0u;
+    const bool above = k != 0 && (all || (k & mask) > prefix), same = k != 0 && !all && (k & mask) == prefix;
+    const unsigned long long a = __ballot(above), b = __ballot(same), below = (1ull << lane) - 1;
+    __syncthreads();
+    if (lane == 0) r.count[0][wave] = __popcll(a), r.count[1][wave] = __popcll(b);
+    __syncthreads();
+    int a_before = 0, b_before = 0, a_all = 0, b_all = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; w++) {
+      const int x = r.count[0][w], y = r.count[1][w];
+      if (w < wave) a_before += x, b_before += y;
+      a_all += x, b_all += y;
+    }
+    a_before += __popcll(a & below), b_before += __popcll(b & below);
+    const int free = left - equal;  // of those that have the prefix
+    const int b_taken = b_before < free ? b_before : free;
+    if (above || (same && b_before < free)) take(taken + a_before + b_taken, i, k);
+    taken += a_all + (b_all < free ? b_all : free);
+    equal += b_all < free ? b_all : free;
+  }
+  __syncthreads();
+}
+
+// A workgroup has a row: joins its statistics; finds the words that lead it so far; after the last piece puts them in order and
+// takes the given words' products.
+template <class T, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_answers(answer_args p) {
+  constexpr int WAVES = THREADS / 64;
+  __shared__ pick_room<THREADS> room;
+  __shared__ unsigned key_[2][MOST_KEEP];
+  __shared__ int32_t word_[2][MOST_KEEP];
+  __shared__ int32_t lead[MOST_KEEP];  // chunks
+  __shared__ double exact_[MOST_KEEP];
+  __shared__ float red[3][WAVES];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  for (int64_t m = blockIdx.x; m < p.rows; m += gridDim.x) {
+    // -- statistics --
+    running so_far = running{-INFINITY, 0.f, 0.f, 0};
+    if (!p.first) so_far = p.state[m];
+    float top = so_far.top;
+    for (int i = tid; i < p.parts_n; i += THREADS) top = fmaxf(top, p.parts[m * p.parts_n + i].x);
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
+    __syncthreads();
+    if (lane == 0) red[0][wave] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) top = fmaxf(top, red[0][w]);
+    const float from = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, weighted = 0.f;
+    auto add = [&](float x, float s, float w) {
+      if (x != -INFINITY || s != 0.f) {
+        const float f = expf(x - from);
+        sum += s * f;
+        weighted += f * fmaf(fmaxf(x - from, -150.f), s, w);
+      }
+    };
+    for (int i = tid; i < p.parts_n; i += THREADS) {
+      const float2 s = p.parts[m * p.parts_n + i];
+      add(s.x, s.y, p.weighted[m * p.parts_n + i]);
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d, 64), weighted += __shfl_xor(weighted, d, 64);
+    if (lane == 0) red[1][wave] = sum, red[2][wave] = weighted;
+    __syncthreads();
+    sum = weighted = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) sum += red[1][w], weighted += red[2][w];
+    add(so_far.top, so_far.sum, so_far.weighted);
+    const float lse = logf(sum) + from;
+    const bool sound = fabsf(lse) < INFINITY;
+
+    // -- alternatives --
+    int kept = so_far.kept, at = 0;
+    if (p.n_top > 0) {
+      for (int i = tid; i < kept; i += THREADS) key_[0][i] = p.kept_key[m * p.keep + i], word_[0][i] = p.kept_word[m * p.keep + i];
+      const float* tops = p.tops + m * p.chunks;
+      // (a chunk that only reaches what a full list ends with comes after it)
+      unsigned least = kept == p.keep ? key_of(p.floor[m]) : 0u;
+      auto chunk_key = [&](int64_t c) {
+        const unsigned k = key_of(tops[c]);
+        return k > least ? k : 0u;
+      };
+      int many = count_keys<THREADS>(room, p.chunks, chunk_key);
+      const bool all = many <= p.keep;
+      if (!all) many = p.keep;
+      unsigned reach = 0xffffffffu;  // the least of the chosen chunks' maxima
+      if (many > 0) {
+        pick<THREADS>(room, p.chunks, many, all, chunk_key, [&](int to, int64_t c, unsigned) { lead[to] = (int32_t)c; });
+        if (!all) {
+          for (int i = tid; i < many; i += THREADS) {
+            const unsigned k = chunk_key(lead[i]);
+            reach = k < reach ? k : reach;
+          }
+#pragma unroll
+          for (int d = 1; d < 64; d *= 2) {
+            const unsigned o = (unsigned)__shfl_xor((int)reach, d, 64);
+            reach = o < reach ? o : reach;
+          }
+          if (lane == 0) room.hist[wave] = (int)reach;
+          __syncthreads();
+#pragma unroll
+          for (int w = 0; w < WAVES; w++) reach = (unsigned)room.hist[w] < reach ? (unsigned)room.hist[w] : reach;
+          least = reach - 1;
+        }
+        // the list, then the chunks' words: in the order of the words
+        const float* z = p.logits + m * p.ldl;
+        const int n = kept + many * p.chunk;
+        auto place = [&](int64_t i) { return (int64_t)lead[(i - kept) / p.chunk] * p.chunk + (i - kept) % p.chunk; };
+        auto item_key = [&](int64_t i) {
+          if (i < kept) return key_[0][i];
+          const int64_t w = place(i);
+          const unsigned k = w < p.piece ? key_of(z[w]) : 0u;
+          return k > least ? k : 0u;
+        };
+        int found = count_keys<THREADS>(room, n, item_key);
+        const bool every = found <= p.keep;
+        if (!every) found = p.keep;
+        pick<THREADS>(room, n, found, every, item_key, [&](int to, int64_t i, unsigned k) {
+          key_[1][to] = k;
+          word_[1][to] = i < kept ? word_[0][i] : (int32_t)(p.word0 + place(i));
+        });
+        kept = found, at = 1;
+      }
+      __syncthreads();
+    }
+    if (!p.last) {
+      for (int i = tid; i < kept; i += THREADS) p.kept_key[m * p.keep + i] = key_[at][i], p.kept_word[m * p.keep + i] = word_[at][i];
+      if (wave == 0) {
+        unsigned f = 0xffffffffu;
+        for (int i = lane; i < kept; i += 64) f = key_[at][i] < f ? key_[at][i] : f;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+          const unsigned o = (unsigned)__shfl_xor((int)f, d, 64);
+          f = o < f ? o : f;
+        }
+        if (lane == 0) {
+          p.state[m] = running{top, sum, weighted, kept};
+          p.floor[m] = kept == p.keep ? value_of(f) : -INFINITY;
+        }
+      }
+      __syncthreads();
+      continue;
+    }
+    if (tid == 0) {
+      if (p.lse) p.lse[m] = lse;
+      if (p.entropy) p.entropy[m] = sound ? logf(sum) - weighted / sum : __builtin_nanf("");
+    }
+    const T* x = (const T*)p.X + m * p.ldx;
+    if (p.n_top > 0) {
+      for (int i = wave; i < kept; i += WAVES) {
+        const double s = dot_rows<T>(x, (const T*)p.E + word_[at][i] * p.lde, p.n_in, lane);
+        if (lane == 0) exact_[i] = s == s ? s : -(double)INFINITY;
+      }
+      __syncthreads();
+      for (int i = tid; i < p.n_top; i += THREADS)
+        if (!sound || i >= kept) p.top_words[m * p.n_top + i] = -1, p.top_logp[m * p.n_top + i] = __builtin_nanf("");
+      for (int i = tid; i < kept && sound; i += THREADS) {
+        const double s = exact_[i];
+        int rank = 0;
+        for (int j = 0; j < kept; j++) rank += exact_[j] > s || (exact_[j] == s && j < i);
+        if (rank < p.n_top) {
+          p.top_words[m * p.n_top + rank] = word_[at][i];
+          p.top_logp[m * p.n_top + rank] = (float)(s * (double)p.inv_heat - (double)lse);
+        }
+      }
+    }
+    // -- given words --
+    for (int j = wave; j < p.n_given; j += WAVES) {
+      const int32_t w = p.given[m * p.n_given + j];
+      float l = 0.f;
+      if (w >= p.words)
+        l = __builtin_nanf("");
+      else if (w >= 0)
+        l = (float)(dot_rows<T>(x, (const T*)p.E + w * p.lde, p.n_in, lane) * (double)p.inv_heat - (double)lse);
+      if (lane == 0) p.logp[m * p.n_given + j] = l;
+    }
+    if (p.teacher) {
+      __syncthreads();  // (a workgroup's writes are there for all of it)
+      if (wave == 0) {
+        const float* l = p.teacher + m * p.n_given;
+        const int32_t* w = p.given + m * p.n_given;
+        const float *logp = p.logp + m * p.n_given;
+        float most = -INFINITY, all = 0.f, loss = 0.f;
+        bool odd = false;  // NaN or +infinity among them
+        for (int j = lane; j < p.n_given; j += 64)
+          if (w[j] >= 0 && l[j] != -INFINITY) most = fmaxf(most, l[j]), odd |= !(l[j] < INFINITY) || w[j] >= p.words;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) most = fmaxf(most, __shfl_xor(most, d, 64));
+        for (int j = lane; j < p.n_given; j += 64)
+          if (w[j] >= 0 && l[j] > -INFINITY) all += expf((l[j] - most) * p.inv_heat);
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d, 64);
+        const float log_all = logf(all);
+        for (int j = lane; j < p.n_given; j += 64)
+          if (w[j] >= 0 && l[j] > -INFINITY) {
+            const float log_q = (l[j] - most) * p.inv_heat - log_all, q = expf(log_q);
+            if (q != 0.f) loss += q * (log_q - logp[j]);
+          }
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) loss += __shfl_xor(loss, d, 64);
+        const bool bad = __any(odd);
+        if (lane == 0) p.loss[m] = bad ? __builtin_nanf("") : most == -INFINITY ? 0.f : loss;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// What the backward pass takes of every row: the slopes of all words, the listed words' own values (a word that is listed twice has
+// one place, its first), the size of its gradients.  A wave has a row.
+//   probabilities and entropies  dz_v = (sum_j dlogp_j [v = w_j] - p_v (sum_j dlogp_j + dH (log p_v + H))) / T
+//   a teacher's words            dz_v = (p_v - sum_j q_j [v = w_j]) dloss / T
+struct slope_args {
+  int64_t rows, words;
+  int many;
+  const int32_t* given;
+  const float *logp, *lse, *entropy;
+  const float *dlogp, *dentropy;  // (either may be NULL)
+  const float *teacher, *dloss;   // (teacher NULL: probabilities)
+  float inv_heat;
+  slope_row* slopes;
+  int32_t* alive;  // -1: no gradient
+  float* size;
+  int32_t* word;
+  float* g;
+};
+__global__ __launch_bounds__(256) void k_slope_rows(slope_args p) {
+  const int lane = threadIdx.x & 63;
+  const float nan = __builtin_nanf("");
+  for (int64_t m = (int64_t)blockIdx.x * 4 + threadIdx.x / 64; m < p.rows; m += (int64_t)gridDim.x * 4) {
+    const int32_t* given = p.given + m * p.many;
+    float a, b = 0.f, size, dloss = 0.f, most = -INFINITY, all = 0.f;
+    bool alive = false, bad = false;
+    if (p.teacher) {
+      const float* l = p.teacher + m * p.many;
+      bool odd = false;
+      for (int j = lane; j < p.many; j += 64) {
+        const int32_t w = given[j];
+        if (w < 0 || l[j] == -INFINITY) continue;
+        most = fmaxf(most, l[j]);
+        odd |= !(l[j] < INFINITY) || w >= p.words;
+        alive = true;
+      }
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) most = fmaxf(most, __shfl_xor(most, d, 64));
+      for (int j = lane; j < p.many; j += 64)
+        if (given[j] >= 0 && l[j] > -INFINITY) all += expf((l[j] - most) * p.inv_heat);
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d, 64);
+      bad = __any(odd), alive = __any(alive);
+      dloss = p.dloss[m] * p.inv_heat;
+      a = dloss, size = fabsf(dloss);
+    } else {
+      float sum = 0.f, sizes = 0.f;
+      for (int j = lane; j < p.many; j += 64) {
+        const int32_t w = given[j];
+        if (w < 0) continue;
+        const float d = p.dlogp ? p.dlogp[m * p.many + j] : 0.f;
+        sum += d, sizes += fabsf(d);
+        alive |= d != 0.f || w >= p.words, bad |= w >= p.words;
+      }
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d, 64), sizes += __shfl_xor(sizes, d, 64);
+      const float dh = p.dentropy ? p.dentropy[m] : 0.f;
+      bad = __any(bad), alive = __any(alive) || dh != 0.f;
+      a = -sum;
+      if (dh != 0.f) a = -fmaf(dh, p.entropy[m], sum), b = -dh * p.inv_heat;
+      a *= p.inv_heat;
+      // (p |log p + H| is at most 8 with 2^31 words: p (1 - p) log of those, and 1 / e)
+      size = (sizes + 8.f * fabsf(dh)) * p.inv_heat;
+    }
+    if (bad) a = nan;
+    if (lane == 0) {
+      p.slopes[m] = slope_row{p.lse[m], a, b, alive ? 1 : 0};
+      p.alive[m] = alive ? 0 : -1;
+      p.size[m] = size;
+    }
+    // the listed words: 64 of them against 64 at a time
+    auto weight = [&](int j) {
+      if (j >= p.many || given[j] < 0) return 0.f;
+      if (!p.teacher) return p.dlogp ? p.dlogp[m * p.many + j] * p.inv_heat : 0.f;
+      const float l = p.teacher[m * p.many + j];
+      return l == -INFINITY ? 0.f : -expf((l - most) * p.inv_heat) / all * dloss;
+    };
+    for (int j0 = 0; j0 < p.many; j0 += 64) {
+      const int j = j0 + lane;
+      const int32_t w = j < p.many ? given[j] : -1;
+      float sum = 0.f;
+      bool first = true;
+      for (int i0 = 0; i0 < p.many; i0 += 64) {
+        const int i = i0 + lane;
+        const int32_t wi = i < p.many ? given[i] : -1;
+        const float gi = weight(i);
+        const int there = p.many - i0 < 64 ? p.many - i0 : 64;
+        for (int t = 0; t < there; t++) {
+          const int32_t o = __builtin_amdgcn_readlane(wi, t);
+          const float g = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(gi), t));
+          if (o == w) sum += g, first &= i0 + t >= j;
+        }
+      }
+      if (j < p.many) {
+        const float l = p.logp[m * p.many + j];
+        const slope_row t{0.f, a, b, 1};
+        p.word[m * p.many + j] = w >= 0 && w < p.words && first && alive ? w : -1;
+        p.g[m * p.many + j] = slope_of(l, t) + sum;
+      }
+    }
+  }
+}
+
+// Rows, and of them at a time, of the forward pass; its workspace.
+struct answer_room {
+  int64_t blocks, each;
+  bool few;
+  int64_t packs[2] = {0, 0};  // of a block's X, of E
+  int64_t piece, parts, weighted, state, tops, logits, kept, floor, logp, all;
+  int keep;
+};
+template <class T>
+answer_room answer_room_of(int64_t rows, int64_t n_in, int64_t words, int n_given, int n_top, const matrix& X, const matrix& E) {
+  answer_room r;
+  r.blocks = rows > BLOCK_ROWS ? ceil_div(rows, BLOCK_ROWS) : 1;
+  r.each = ceil_div(rows, r.blocks);
+  r.few = is_few<T>(r.each, 0, words, n_in, true);
+  if (!r.few) {
+    matrix x = X;
+    x.rows = r.each;
+    r.packs[0] = packed_bytes<T>(x), r.packs[1] = packed_bytes<T>(E);
+  }
+  r.keep = n_top > 0 ? (n_top + SPARE < words ? n_top + SPARE : (int)words) : 0;
+  r.piece = words;
+  if (n_top > 0) {
+    int64_t most = LOGIT_BYTES / (4 * r.each) / 256 * 256;
+    if (most < 1024) most = 1024;
+    if (most < words) r.piece = ceil_div(ceil_div(words, ceil_div(words, most)), 256) * 256;
+  }
+  r.parts = round256(r.each * ceil_div(r.piece, r.few ? 16 : 128) * 8);
+  r.weighted = round256(r.each * ceil_div(r.piece, r.few ? 16 : 128) * 4);
+  r.state = n_top > 0 ? round256(r.each * (int64_t)sizeof(running)) : 0;
+  r.tops = n_top > 0 ? round256(r.each * ceil_div(r.piece, r.few ? 16 : 64) * 4) : 0;
+  r.logits = n_top > 0 ? round256(r.each * padded(r.piece) * 4) : 0;
+  r.kept = round256(r.each * r.keep * 4);
+  r.floor = n_top > 0 ? round256(r.each * 4) : 0;
+  r.logp = round256(r.each * (int64_t)n_given * 4);
+  r.all = r.packs[0] + r.packs[1] + r.parts + r.weighted + r.state + r.tops + r.logits + 2 * r.kept + r.floor + r.logp;
+  return r;
+}
+
+// to: what is wanted, of all rows.
+template <class T>
+int answers_forward(hipStream_t st, const char* me, const answer_args& to, char* ws, int64_t ws_bytes) {
+  const int64_t words = to.words;
+  matrix all_x{to.X, to.ldx, to.rows, to.n_in, 1, 0, 0, nullptr}, e{to.E, to.lde, words, to.n_in, 1, 0, 0, nullptr};
+  const answer_room r = answer_room_of<T>(to.rows, to.n_in, words, to.n_given, to.n_top, all_x, e);
+  DN_TRY(check_room(me, r.all, ws, ws_bytes));
+  if (!r.few) DN_TRY(pack<T>(&e, 1, ws, st));
+  ws += r.packs[1];
+  char* x_room = ws;
+  auto take = [&](int64_t bytes) {
+    char* at = ws;
+    ws += bytes;
+    return at;
+  };
+  take(r.packs[0]);
+  answer_args a = to;
+  float2* parts = (float2*)take(r.parts);
+  float* weighted = (float*)take(r.weighted);
+  a.state = (running*)take(r.state);
+  float *tops = (float*)take(r.tops), *logits = (float*)take(r.logits);
+  a.kept_key = (unsigned*)take(r.kept);
+  a.kept_word = (int32_t*)take(r.kept);
+  a.floor = (float*)take(r.floor);
+  float* logp_room = (float*)take(r.logp);
+  a.parts = parts, a.weighted = weighted, a.tops = tops, a.logits = logits, a.keep = r.keep;
+  for (int64_t b = 0; b < r.blocks; b++) {
+    const int64_t m0 = b * r.each, rows = to.rows - m0 < r.each ? to.rows - m0 : r.each;
+    matrix x = all_x;
+    x.p = (const T*)to.X + m0 * to.ldx, x.rows = rows;
+    a.X = x.p, a.rows = rows;
+    a.given = to.given ? to.given + m0 * to.n_given : nullptr;
+    a.logp = to.logp ? to.logp + m0 * to.n_given : logp_room;
+    a.teacher = to.teacher ? to.teacher + m0 * to.n_given : nullptr;
+    a.lse = to.lse ? to.lse + m0 : nullptr, a.entropy = to.entropy ? to.entropy + m0 : nullptr, a.loss = to.loss ? to.loss + m0 : nullptr;
+    a.top_words = to.top_words ? to.top_words + m0 * to.n_top : nullptr, a.top_logp = to.top_logp ? to.top_logp + m0 * to.n_top : nullptr;
+    if (!r.few) DN_TRY(pack<T>(&x, 1, x_room, st));
+    for (int64_t w0 = 0; w0 < words; w0 += r.piece) {
+      const int64_t n = words - w0 < r.piece ? words - w0 : r.piece;
+      args p{};
+      p.A = x.p, p.lda = x.ld, p.a_plane = x.plane, p.b_plane = e.plane, p.ldb = e.ld;
+      p.M = rows, p.N = n, p.K = to.n_in;
+      p.mode = ONE;
+      p.inv_heat = to.inv_heat;
+      p.parts = parts, p.weighted = weighted;
+      a.chunk = 64, a.chunks = ceil_div(n, 64);
+      if (to.n_top > 0) p.tops = tops, p.logits = logits, p.ldl = padded(n), p.chunks = a.chunks, p.floor = w0 > 0 ? a.floor : nullptr;
+      if (r.few) {
+        p.B = (const T*)e.p + w0 * e.ld;
+        DN_TRY((launch_few<T, E_PROBS>(p, st, &a.parts_n, &a.chunk)));
+        a.chunks = ceil_div(n, a.chunk);
+      } else {
+        p.B = (const typename num<T>::op*)e.p + w0 * e.ld;
+        DN_TRY((launch_product<T, true, true, E_PROBS>(p, nullptr, st, &a.parts_n)));
+      }
+      a.first = w0 == 0, a.last = w0 + n == words, a.word0 = w0, a.piece = n, a.ldl = padded(n);
+      if (rows <= 512)
+        k_answers<T, 1024><<<(unsigned)rows, 1024, 0, st>>>(a);
+      else
+        k_answers<T, 256><<<(unsigned)rows, 256, 0, st>>>(a);
+      DN_LAUNCH_CHECK();
+    }
+  }
+  return 0;
+}
+
+struct slope_room {
+  int64_t slopes, alive, size, word, g, all;
+  slope_room(int64_t rows, int many)
+      : slopes(round256(rows * (int64_t)sizeof(slope_row))), alive(round256(rows * 4)), size(round256(rows * 4)),
+        word(round256(rows * many * 4)), g(round256(rows * many * 4)), all(slopes + alive + size + word + g) {}
+};
+template <class T>
+int answers_backward(hipStream_t st, const char* me, slope_args s, int64_t n_in, const void* X, int64_t ldx, const void* E, int64_t lde,
+                     void* dX, int64_t lddx, void* dE, int64_t ldde, char* ws, int64_t ws_bytes) {
+  const slope_room own(s.rows, s.many);
+  const grad_room<T> r(s.rows, n_in, s.words, X, ldx, E, lde, (const int32_t*)ws);
+  DN_TRY(check_room(me, own.all + r.all, ws, ws_bytes));
+  s.slopes = (slope_row*)ws;
+  s.alive = (int32_t*)(ws + own.slopes);
+  s.size = (float*)(ws + own.slopes + own.alive);
+  s.word = (int32_t*)(ws + own.slopes + own.alive + own.size);
+  s.g = (float*)(ws + own.slopes + own.alive + own.size + own.word);
+  if (s.rows > 0) {
+    const int64_t blocks = ceil_div(s.rows, 4);
+    k_slope_rows<<<(unsigned)(blocks < JOIN_MOST ? blocks : JOIN_MOST), 256, 0, st>>>(s);
+    DN_LAUNCH_CHECK();
+  }
+  args of{};
+  of.labels = s.alive, of.dloss = s.size, of.slopes = s.slopes, of.inv_heat = s.inv_heat;
+  return loss_backward<T, E_PROBS_GRAD>(st, s.rows, n_in, s.words, X, ldx, E, lde, of, spots{s.rows, s.many, s.word, s.g}, dX, lddx, dE,
+                                        ldde, ws + own.all, ws_bytes - own.all, me);
+}
+int check_answers(const char* me, int64_t n_words, float temperature, int n_given, int n_top) {
+  const float inv = 1.f / temperature;
+  DN_CHECK(temperature > 0.f && inv > 0.f && inv < INFINITY, "%s: temperature = %g", me, (double)temperature);
+  DN_CHECK(n_given >= 0 && n_given <= MOST_LISTED, "%s: %d words of a row: 0 to %d", me, n_given, MOST_LISTED);
+  DN_CHECK(n_top >= 0 && n_top <= MOST_TOP && n_top <= n_words, "%s: %d alternatives of %lld words: 0 to %d of them", me, n_top,
+           (long long)n_words, MOST_TOP);
+  return 0;
+}
 int check_head(const char* me, int type, int64_t rows, int64_t n_in, int64_t words) {
   DN_CHECK(type == DNPEFF_F32 || type == DNPEFF_F16 || type == DNPEFF_BF16, "%s: unknown type %d", me, type);
   DN_CHECK(rows >= 0 && n_in >= 1 && words >= 1 && rows < ((int64_t)1 << 31) && n_in <= ((int64_t)1 << 24) && words < ((int64_t)1 << 31),
@@ -416,6 +1053,119 @@ DN_API int dnpeff_vocab_loss_backward(void* stream, int type, int64_t rows, int6
   DN_TRY(check_array(me, "dloss", dloss, 1, 1, DNPEFF_F32, rows == 0));
   DN_TRY(check_array(me, "dX", dX, lddx, n_in, type, true));
   DN_TRY(check_array(me, "dE", dE, ldde, n_in, type, true));
-  return DN_BY_TYPE(type, loss_backward<T>((hipStream_t)stream, rows, n_in, n_words, X, ldx, E, lde, labels, lse, dloss, dX, lddx, dE,
-                                           ldde, (char*)workspace, workspace_bytes));
+  args of{};
+  of.labels = labels, of.lse = lse, of.dloss = dloss;
+  return DN_BY_TYPE(type, (loss_backward<T, E_LOSS_GRAD>((hipStream_t)stream, rows, n_in, n_words, X, ldx, E, lde, of, spots{}, dX, lddx, dE,
+                                                         ldde, (char*)workspace, workspace_bytes, me)));
+}
+DN_API int dnpeff_vocab_probs_workspace(int type, int64_t rows, int64_t n_in, int64_t n_words, int n_given, int n_top, int aligned,
+                                        int64_t* forward_bytes, int64_t* backward_bytes) {
+  clear_error();
+  const char* me = "dnpeff_vocab_probs_workspace";
+  DN_TRY(check_head(me, type, rows, n_in, n_words));
+  DN_TRY(check_answers(me, n_words, 1.f, n_given, n_top));
+  const void* p = (const void*)(uintptr_t)(aligned ? 16 : 1);
+  const matrix x{p, n_in, rows, n_in, 1, 0, 0, nullptr}, e{p, n_in, n_words, n_in, 1, 0, 0, nullptr};
+  if (forward_bytes) *forward_bytes = rows == 0 ? 0 : DN_BY_TYPE(type, (answer_room_of<T>(rows, n_in, n_words, n_given, n_top, x, e).all));
+  if (backward_bytes)
+    *backward_bytes = slope_room(rows, n_given).all + DN_BY_TYPE(type, (grad_room<T>(rows, n_in, n_words, p, n_in, p, n_in, (const int32_t*)p).all));
+  return 0;
+}
+
+DN_API int dnpeff_vocab_probs(void* stream, int type, int64_t rows, int64_t n_in, int64_t n_words, const void* X, int64_t ldx, const void* E,
+                              int64_t lde, float temperature, int n_given, const int32_t* words, float* logp, float* lse, float* entropy,
+                              int n_top, int32_t* top_words, float* top_logp, void* workspace, int64_t workspace_bytes) {
+  clear_error();
+  const char* me = "dnpeff_vocab_probs";
+  DN_TRY(check_head(me, type, rows, n_in, n_words));
+  DN_TRY(check_answers(me, n_words, temperature, n_given, n_top));
+  if (rows == 0) return 0;
+  DN_TRY(check_array(me, "X", X, ldx, n_in, type, false));
+  DN_TRY(check_array(me, "E", E, lde, n_in, type, false));
+  DN_TRY(check_array(me, "words", words, 1, 1, DNPEFF_F32, n_given == 0));
+  DN_TRY(check_array(me, "logp", logp, 1, 1, DNPEFF_F32, n_given == 0));
+  DN_TRY(check_array(me, "lse", lse, 1, 1, DNPEFF_F32, true));
+  DN_TRY(check_array(me, "entropy", entropy, 1, 1, DNPEFF_F32, true));
+  DN_TRY(check_array(me, "top_words", top_words, 1, 1, DNPEFF_F32, n_top == 0));
+  DN_TRY(check_array(me, "top_logp", top_logp, 1, 1, DNPEFF_F32, n_top == 0));
+  answer_args a{};
+  a.rows = rows, a.n_in = n_in, a.words = n_words, a.X = X, a.ldx = ldx, a.E = E, a.lde = lde, a.inv_heat = 1.f / temperature;
+  a.n_given = n_given, a.given = words, a.logp = logp, a.lse = lse, a.entropy = entropy;
+  a.n_top = n_top, a.top_words = top_words, a.top_logp = top_logp;
+  return DN_BY_TYPE(type, answers_forward<T>((hipStream_t)stream, me, a, (char*)workspace, workspace_bytes));
+}
+
+DN_API int dnpeff_vocab_probs_backward(void* stream, int type, int64_t rows, int64_t n_in, int64_t n_words, const void* X, int64_t ldx,
+                                       const void* E, int64_t lde, float temperature, int n_given, const int32_t* words, const float* logp,
+                                       const float* lse, const float* entropy, const float* dlogp, const float* dentropy, void* dX,
+                                       int64_t lddx, void* dE, int64_t ldde, void* workspace, int64_t workspace_bytes) {
+  clear_error();
+  const char* me = "dnpeff_vocab_probs_backward";
+  const bool none = rows == 0;
+  DN_TRY(check_head(me, type, rows, n_in, n_words));
+  DN_TRY(check_answers(me, n_words, temperature, n_given, 0));
+  DN_TRY(check_array(me, "X", X, ldx, n_in, type, none));
+  DN_TRY(check_array(me, "E", E, lde, n_in, type, none));
+  DN_TRY(check_array(me, "words", words, 1, 1, DNPEFF_F32, none || n_given == 0));
+  DN_TRY(check_array(me, "logp", logp, 1, 1, DNPEFF_F32, none || n_given == 0));
+  DN_TRY(check_array(me, "lse", lse, 1, 1, DNPEFF_F32, none));
+  DN_TRY(check_array(me, "entropy", entropy, 1, 1, DNPEFF_F32, none || dentropy == nullptr));
+  DN_TRY(check_array(me, "dlogp", dlogp, 1, 1, DNPEFF_F32, true));
+  DN_TRY(check_array(me, "dentropy", dentropy, 1, 1, DNPEFF_F32, true));
+  DN_TRY(check_array(me, "dX", dX, lddx, n_in, type, true));
+  DN_TRY(check_array(me, "dE", dE, ldde, n_in, type, true));
+  slope_args s{};
+  s.rows = rows, s.words = n_words, s.many = n_given, s.given = words, s.logp = logp, s.lse = lse, s.entropy = entropy;
+  s.dlogp = dlogp, s.dentropy = dentropy, s.inv_heat = 1.f / temperature;
+  return DN_BY_TYPE(type, answers_backward<T>((hipStream_t)stream, me, s, n_in, X, ldx, E, lde, dX, lddx, dE, ldde, (char*)workspace,
+                                              workspace_bytes));
+}
+
+DN_API int dnpeff_vocab_distill(void* stream, int type, int64_t rows, int64_t n_in, int64_t n_words, const void* X, int64_t ldx,
+                                const void* E, int64_t lde, float temperature, int n_listed, const int32_t* words, const float* logits,
+                                float* loss, float* logp, float* lse, void* workspace, int64_t workspace_bytes) {
+  clear_error();
+  const char* me = "dnpeff_vocab_distill";
+  DN_TRY(check_head(me, type, rows, n_in, n_words));
+  DN_TRY(check_answers(me, n_words, temperature, n_listed, 0));
+  DN_CHECK(n_listed >= 1, "%s: no words are listed", me);
+  if (rows == 0) return 0;
+  DN_TRY(check_array(me, "X", X, ldx, n_in, type, false));
+  DN_TRY(check_array(me, "E", E, lde, n_in, type, false));
+  DN_TRY(check_array(me, "words", words, 1, 1, DNPEFF_F32, false));
+  DN_TRY(check_array(me, "logits", logits, 1, 1, DNPEFF_F32, false));
+  DN_TRY(check_array(me, "loss", loss, 1, 1, DNPEFF_F32, true));
+  DN_TRY(check_array(me, "logp", logp, 1, 1, DNPEFF_F32, true));
+  DN_TRY(check_array(me, "lse", lse, 1, 1, DNPEFF_F32, true));
+  answer_args a{};
+  a.rows = rows, a.n_in = n_in, a.words = n_words, a.X = X, a.ldx = ldx, a.E = E, a.lde = lde, a.inv_heat = 1.f / temperature;
+  a.n_given = n_listed, a.given = words, a.logp = logp, a.lse = lse;
+  if (loss) a.teacher = logits, a.loss = loss;
+  return DN_BY_TYPE(type, answers_forward<T>((hipStream_t)stream, me, a, (char*)workspace, workspace_bytes));
+}
+
+DN_API int dnpeff_vocab_distill_backward(void* stream, int type, int64_t rows, int64_t n_in, int64_t n_words, const void* X, int64_t ldx,
+                                         const void* E, int64_t lde, float temperature, int n_listed, const int32_t* words,
+                                         const float* logits, const float* logp, const float* lse, const float* dloss, void* dX,
+                                         int64_t lddx, void* dE, int64_t ldde, void* workspace, int64_t workspace_bytes) {
+  clear_error();
+  const char* me = "dnpeff_vocab_distill_backward";
+  const bool none = rows == 0;
+  DN_TRY(check_head(me, type, rows, n_in, n_words));
+  DN_TRY(check_answers(me, n_words, temperature, n_listed, 0));
+  DN_CHECK(n_listed >= 1, "%s: no words are listed", me);
+  DN_TRY(check_array(me, "X", X, ldx, n_in, type, none));
+  DN_TRY(check_array(me, "E", E, lde, n_in, type, none));
+  DN_TRY(check_array(me, "words", words, 1, 1, DNPEFF_F32, none));
+  DN_TRY(check_array(me, "logits", logits, 1, 1, DNPEFF_F32, none));
+  DN_TRY(check_array(me, "logp", logp, 1, 1, DNPEFF_F32, none));
+  DN_TRY(check_array(me, "lse", lse, 1, 1, DNPEFF_F32, none));
+  DN_TRY(check_array(me, "dloss", dloss, 1, 1, DNPEFF_F32, none));
+  DN_TRY(check_array(me, "dX", dX, lddx, n_in, type, true));
+  DN_TRY(check_array(me, "dE", dE, ldde, n_in, type, true));
+  slope_args s{};
+  s.rows = rows, s.words = n_words, s.many = n_listed, s.given = words, s.logp = logp, s.lse = lse;
+  s.teacher = logits, s.dloss = dloss, s.inv_heat = 1.f / temperature;
+  return DN_BY_TYPE(type, answers_backward<T>((hipStream_t)stream, me, s, n_in, X, ldx, E, lde, dX, lddx, dE, ldde, (char*)workspace,
+                                              workspace_bytes));
 }
