@@ -272,9 +272,12 @@ struct args {
   // E_PROBS, E_PROBS_GRAD
   float inv_heat;           // logits are multiplied by it
   float* weighted;          // [M][parts_n]: of each tile's words, sum of exp(z - max) (z - max)
-  float *tops, *logits;     // (or NULL) [M][chunks]: the largest logit of each chunk of words; [M][ldl]: the logits of the
-  int64_t chunks, ldl;      // chunks whose largest is not below the row's floor (NULL: of all); ldl is a multiple of 64
+  float* tops;              // (or NULL) [M][chunks]: the largest logit of each chunk of words
+  float* logits;            // [M][ldl], ldl a multiple of 64: logits of the chunks that are stored: with tops those whose
+  int64_t chunks, ldl;      // largest is not below the row's floor (NULL: all), and those that are wanted
   const float* floor;
+  const unsigned* wanted;   // (or NULL) [M][ld_wanted]: a bit for each chunk, chunk0 the first of this piece
+  int64_t chunk0, ld_wanted;
   const slope_row* slopes;  // [M]
 };
 
@@ -673,6 +676,7 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
     const int there = whole ? FN * 16 : (int)(p.N - n_wave < 0 ? 0 : p.N - n_wave) - q * 4;
     int labels[FM];  // (asked for together)
     float floors[FM];
+    unsigned wanted[FM];
     if constexpr (E == E_LOSS) {
 #pragma unroll
       for (int i = 0; i < FM; i++) {
@@ -680,11 +684,14 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
         labels[i] = p.labels[m < m_end ? m : m_end - 1];
       }
     } else {
-      const bool some = p.tops != nullptr && p.floor != nullptr;
+      const bool all = p.tops != nullptr && p.floor == nullptr, some = p.tops != nullptr && p.floor != nullptr;
+      const bool here = n_wave < p.N, bits = p.wanted != nullptr && here;
+      const int64_t chunk = p.chunk0 + (n_wave >> 6);
 #pragma unroll
       for (int i = 0; i < FM; i++) {
-        const int64_t m = m_wave + i * 16 + (lane & 15);
-        floors[i] = some ? p.floor[m < m_end ? m : m_end - 1] : -INFINITY;
+        const int64_t m_i = m_wave + i * 16 + (lane & 15), m = m_i < m_end ? m_i : m_end - 1;
+        floors[i] = some ? p.floor[m] : INFINITY;
+        wanted[i] = all && here ? 1u : bits ? p.wanted[m * p.ld_wanted + (chunk >> 5)] >> (chunk & 31) & 1u : 0u;
       }
       const float inv_heat = p.inv_heat;
 #pragma unroll
@@ -730,9 +737,9 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
 #pragma unroll
           for (int e = 0; e < 4; e++) sum += __expf(acc[i][j][e] - from);
       } else {
-        if (p.tops && m < m_end && n_wave < p.N) {
-          if (q == 0) p.tops[m * p.chunks + (n_wave >> 6)] = top;
-          if (!(top < floors[i])) {
+        if (m < m_end) {
+          if (p.tops && q == 0 && n_wave < p.N) p.tops[m * p.chunks + (n_wave >> 6)] = top;
+          if (wanted[i] || (top >= floors[i] && n_wave < p.N)) {
 #pragma unroll
             for (int j = 0; j < FN; j++) *(v4f*)(p.logits + m * p.ldl + n_wave + j * 16 + q * 4) = acc[i][j];
           }

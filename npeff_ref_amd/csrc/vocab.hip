@@ -422,7 +422,10 @@ int loss_backward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, con
 constexpr int MOST_TOP = 128, SPARE = 8, MOST_KEEP = MOST_TOP + SPARE;
 constexpr int MOST_LISTED = 4096;
 constexpr int64_t BLOCK_ROWS = 65536;                 // rows at a time, for the workspace's sake
-constexpr int64_t LOGIT_BYTES = (int64_t)512 << 20;  // of a piece's logits
+constexpr int64_t LOGIT_BYTES = (int64_t)2 << 30;  // of a piece's logits
+// Given words' logits: rows of E read again and multiplied in 64 bits, or, where that would be so many bytes, taken from the tiles (us
+// there and here: 20 words of 2000 rows of 1024, 82 MB, 904 and 924 with the gradients; 100 of 1999 of 1030, 412 MB, 420 and 340).
+constexpr int64_t STORED_FROM = (int64_t)128 << 20;
 
 // Floats in the order of their values (equal zeros equal); 1: NaN, 0 is below all.
 __device__ __forceinline__ unsigned key_of(float v) {
@@ -461,130 +464,225 @@ struct answer_args {
   float inv_heat;
   int n_given;
   const int32_t* given;        // [rows][n_given]
+  int stored;                  // their logits are among those of the pieces
   float *logp, *lse, *entropy;
   const float* teacher;        // (or NULL) [rows][n_given]
   float* loss;
 };
 
-// The product of two rows in 64 bits, in every lane.
-template <class T>
-__device__ __forceinline__ double dot_rows(const T* a, const T* b, int64_t n, int lane) {
+// The products of a row with C others in 64 bits, in every lane.
+template <class T, int C>
+__device__ __forceinline__ void dot_rows(const T* a, const T* const* b, int64_t n, int lane, double* sum) {
   constexpr int W = 16 / sizeof(T);
-  double s = 0.0;
+  typedef loose<T, W> piece;
+#pragma unroll
+  for (int c = 0; c < C; c++) sum[c] = 0.0;
   int64_t k = (int64_t)lane * W;
-#pragma unroll 4
+#pragma unroll 2
   for (; k + W <= n; k += 64 * W) {
-    const loose<T, W> x = *(const loose<T, W>*)(a + k), y = *(const loose<T, W>*)(b + k);
+    const piece x = *(const piece*)(a + k);
+    piece y[C];
 #pragma unroll
-    for (int t = 0; t < W; t++) s = fma((double)(float)x[t], (double)(float)y[t], s);
+    for (int c = 0; c < C; c++) y[c] = *(const piece*)(b[c] + k);
+    double d[W];
+#pragma unroll
+    for (int t = 0; t < W; t++) d[t] = (double)(float)x[t];
+#pragma unroll
+    for (int c = 0; c < C; c++)
+#pragma unroll
+      for (int t = 0; t < W; t++) sum[c] = fma(d[t], (double)(float)y[c][t], sum[c]);
   }
-  for (int t = 0; t < W && k + t < n; t++) s = fma((double)(float)a[k + t], (double)(float)b[k + t], s);
+  for (int t = 0; t < W && k + t < n; t++)
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) s += __shfl_xor(s, d, 64);
-  return s;
+    for (int c = 0; c < C; c++) sum[c] = fma((double)(float)a[k + t], (double)(float)b[c][k + t], sum[c]);
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2)
+#pragma unroll
+    for (int c = 0; c < C; c++) sum[c] += __shfl_xor(sum[c], d, 64);
 }
 
+// Selection by a workgroup among n items with keys (0: not an item), which a thread keeps where n is at most THREADS HELD.
+constexpr int MOST_HELD = 8;
 template <int THREADS>
 struct pick_room {
-  static constexpr int WAVES = THREADS / 64;
   int hist[256];
-  int count[2][WAVES];
-  unsigned prefix, mask;
-  int left, whole;
+  unsigned part[3][MOST_HELD * THREADS / 64];  // per round and wave
+  unsigned low, high;
+  int left, done;
 };
-// How many of n items have a key that is not 0.
-template <int THREADS, class Key>
-__device__ __forceinline__ int count_keys(pick_room<THREADS>& r, int64_t n, Key key) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int mine = 0;
-  for (int64_t i = threadIdx.x; i < n; i += THREADS) mine += key(i) != 0;
+template <int THREADS, int HELD>
+struct picker {
+  static constexpr int WAVES = THREADS / 64;
+  pick_room<THREADS>& r;
+  const int tid = threadIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int64_t n;
+  unsigned key[HELD];
+  int count;          // of the items
+  unsigned low, high; // the least and the largest key
+  __device__ __forceinline__ picker(pick_room<THREADS>& room) : r(room) {}
+
+  template <class Key, class F>
+  __device__ __forceinline__ void each(Key key_at, F f) {
+    if (n <= THREADS * HELD) {
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) mine += __shfl_xor(mine, d, 64);
-  __syncthreads();
-  if (lane == 0) r.count[0][wave] = mine;
-  __syncthreads();
-  int all = 0;
-#pragma unroll
-  for (int w = 0; w < THREADS / 64; w++) all += r.count[0][w];
-  return all;
-}
-// The `need` items of the largest keys, of equal ones the first, handed to take(place, item, key) in the order of the items; needs as
-// many items with keys.  Digit by digit: how many have each value of the next 8 bits, the value among them at which `need` is reached.
-template <int THREADS, class Key, class Take>
-__device__ __forceinline__ void pick(pick_room<THREADS>& r, int64_t n, int need, bool all, Key key, Take take) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  __syncthreads();
-  if (tid == 0) r.prefix = all ? 1u : 0u, r.mask = all ? 0xffffffffu : 0u, r.left = need, r.whole = all;
-  unsigned prefix = all ? 1u : 0u, mask = all ? 0xffffffffu : 0u;
-  int left = need;
-  for (int shift = 24; shift >= 0 && !all; shift -= 8) {
-    for (int i = tid; i < 256; i += THREADS) r.hist[i] = 0;
-    __syncthreads();
-    for (int64_t i = tid; i < n; i += THREADS) {
-      const unsigned k = key(i);
-      if (k != 0 && (k & mask) == prefix) atomicAdd(&r.hist[(k >> shift) & 255], 1);
+      for (int h = 0; h < HELD; h++) f(key[h]);
+    } else {
+      for (int64_t i = tid; i < n; i += THREADS) f(key_at(i));
     }
-    __syncthreads();
-    if (wave == 0) {
-      // lane l: the four values from 252 - 4 l down
-      int own[4], sum = 0;
+  }
+  template <class Key>
+  __device__ __forceinline__ void look(int64_t n_items, Key key_at) {
+    n = n_items;
+    if (n <= THREADS * HELD) {
 #pragma unroll
-      for (int e = 0; e < 4; e++) own[e] = r.hist[255 - 4 * lane - e], sum += own[e];
-      int before = sum;
+      for (int h = 0; h < HELD; h++) key[h] = h * THREADS + tid < n ? key_at(h * THREADS + tid) : 0u;
+    }
+    unsigned c = 0, lo = 0xffffffffu, hi = 0;
+    each(key_at, [&](unsigned k) {
+      c += k != 0;
+      lo = k != 0 && k < lo ? k : lo;
+      hi = k > hi ? k : hi;
+    });
 #pragma unroll
-      for (int d = 1; d < 64; d *= 2) {
-        const int u = __shfl_up(before, d, 64);
-        if (lane >= d) before += u;
+    for (int d = 1; d < 64; d *= 2) {
+      c += (unsigned)__shfl_xor((int)c, d, 64);
+      const unsigned l = (unsigned)__shfl_xor((int)lo, d, 64), h = (unsigned)__shfl_xor((int)hi, d, 64);
+      lo = l < lo ? l : lo, hi = h > hi ? h : hi;
+    }
+    if (WAVES > 1) {
+      __syncthreads();
+      if (lane == 0) r.part[0][wave] = c, r.part[1][wave] = lo, r.part[2][wave] = hi;
+      __syncthreads();
+      c = 0;
+#pragma unroll
+      for (int w = 0; w < WAVES; w++) {
+        c += r.part[0][w];
+        lo = r.part[1][w] < lo ? r.part[1][w] : lo, hi = r.part[2][w] > hi ? r.part[2][w] : hi;
       }
-      before -= sum;
+    }
+    count = (int)c, low = lo, high = hi;
+  }
+  // The `need` items (of `count` or fewer) of the largest keys, of equal ones the first, to take(place, item, key) in the order of the items: the
+  // range of the keys in 256 parts, how many are in each, the part in which the last of them lies, and so on within it.
+  template <class Key, class Take>
+  __device__ __forceinline__ void pick(int need, Key key_at, Take take) {
+    unsigned lo = low, hi = high;
+    int left = need;
+    bool done = need >= count;
+    if (done) hi = 0xffffffffu, left = count;  // (all are in the range)
+    __syncthreads();
+    while (!done) {
+      const unsigned span = hi - lo;
+      const int shift = span < 256 ? 0 : 24 - __builtin_clz(span);
+      for (int i = tid; i < 256; i += THREADS) r.hist[i] = 0;
+      __syncthreads();
+      each(key_at, [&](unsigned k) {
+        if (k >= lo && k <= hi) atomicAdd(&r.hist[(k - lo) >> shift], 1);
+      });
+      __syncthreads();
+      if (wave == 0) {
+        // lane l: the four parts from 255 - 4 l down
+        int own[4], sum = 0;
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        if (before < left && before + own[e] >= left) {
-          r.prefix = prefix | (unsigned)(255 - 4 * lane - e) << shift;
-          r.left = left - before;
-          r.whole = own[e] == left - before;
+        for (int e = 0; e < 4; e++) own[e] = r.hist[255 - 4 * lane - e], sum += own[e];
+        int before = sum;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+          const int u = __shfl_up(before, d, 64);
+          if (lane >= d) before += u;
         }
-        before += own[e];
+        before -= sum;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          if (before < left && before + own[e] >= left) {
+            const unsigned l = lo + ((unsigned)(255 - 4 * lane - e) << shift), h = l + ((1u << shift) - 1);
+            r.low = l, r.high = h < hi ? h : hi, r.left = left - before;
+            r.done = shift == 0 || own[e] == left - before;
+          }
+          before += own[e];
+        }
+      }
+      __syncthreads();
+      lo = r.low, hi = r.high, left = r.left, done = r.done != 0;
+    }
+    // those above the range, and the first `left` of those in it
+    const unsigned long long below = (1ull << lane) - 1;
+    if (n <= THREADS * HELD) {
+      unsigned long long above[HELD], in[HELD];
+#pragma unroll
+      for (int h = 0; h < HELD; h++) {
+        above[h] = __ballot(key[h] > hi), in[h] = __ballot(key[h] != 0 && key[h] >= lo && key[h] <= hi);
+        if (WAVES > 1 && lane == 0) r.part[0][h * WAVES + wave] = __popcll(above[h]), r.part[1][h * WAVES + wave] = __popcll(in[h]);
+      }
+      if (WAVES > 1) {
+        __syncthreads();
+        if (wave == 0) {  // sums of what comes before
+          int a_all = 0, b_all = 0;
+          for (int i0 = 0; i0 < HELD * WAVES; i0 += 64) {
+            const int i = i0 + lane;
+            const int a = i < HELD * WAVES ? (int)r.part[0][i] : 0, b = i < HELD * WAVES ? (int)r.part[1][i] : 0;
+            int x = a, y = b;
+#pragma unroll
+            for (int d = 1; d < 64; d *= 2) {
+              const int u = __shfl_up(x, d, 64), v = __shfl_up(y, d, 64);
+              if (lane >= d) x += u, y += v;
+            }
+            if (i < HELD * WAVES) r.part[0][i] = a_all + x - a, r.part[1][i] = b_all + y - b;
+            a_all += __shfl(x, 63, 64), b_all += __shfl(y, 63, 64);
+          }
+        }
+        __syncthreads();
+      }
+      int a_before = 0, b_before = 0;
+#pragma unroll
+      for (int h = 0; h < HELD; h++) {
+        if (WAVES > 1) a_before = (int)r.part[0][h * WAVES + wave], b_before = (int)r.part[1][h * WAVES + wave];
+        const int a = a_before + __popcll(above[h] & below), b = b_before + __popcll(in[h] & below);
+        const bool up = key[h] > hi, same = (in[h] >> lane) & 1;
+        if (up || (same && b < left)) take(a + (b < left ? b : left), (int64_t)h * THREADS + tid, key[h]);
+        if (WAVES == 1) a_before += __popcll(above[h]), b_before += __popcll(in[h]);
+      }
+    } else {
+      int a_before = 0, b_before = 0;
+      for (int64_t base = 0; base < n; base += THREADS) {
+        const int64_t i = base + tid;
+        const unsigned k = i < n ? key_at(i) : 0u;
+        const bool up = k > hi, same = k != 0 && k >= lo && k <= hi;
+        const unsigned long long above = __ballot(up), in = __ballot(same);
+        int a = a_before, b = b_before, a_all = __popcll(above), b_all = __popcll(in);
+        if (WAVES > 1) {
+          __syncthreads();
+          if (lane == 0) r.part[0][wave] = a_all, r.part[1][wave] = b_all;
+          __syncthreads();
+          a_all = b_all = 0;
+#pragma unroll
+          for (int w = 0; w < WAVES; w++) {
+            if (w < wave) a += (int)r.part[0][w], b += (int)r.part[1][w];
+            a_all += (int)r.part[0][w], b_all += (int)r.part[1][w];
+          }
+        }
+        a += __popcll(above & below), b += __popcll(in & below);
+        if (up || (same && b < left)) take(a + (b < left ? b : left), i, k);
+        a_before += a_all, b_before += b_all;
       }
     }
     __syncthreads();
-    prefix = r.prefix, left = r.left;
-    mask |= 255u << shift;
-    if (r.whole) break;
   }
-  // those above the prefix, and the first `left` of those that have it
-  int taken = 0, equal = 0;
-  for (int64_t base = 0; base < n && taken < need; base += THREADS) {
-    const int64_t i = base + tid;
-    const unsigned k = i < n ? key(i) : 0u;
-    const bool above = k != 0 && (all || (k & mask) > prefix), same = k != 0 && !all && (k & mask) == prefix;
-    const unsigned long long a = __ballot(above), b = __ballot(same), below = (1ull << lane) - 1;
-    __syncthreads();
-    if (lane == 0) r.count[0][wave] = __popcll(a), r.count[1][wave] = __popcll(b);
-    __syncthreads();
-    int a_before = 0, b_before = 0, a_all = 0, b_all = 0;
-#pragma unroll
-    for (int w = 0; w < THREADS / 64; w++) {
-      const int x = r.count[0][w], y = r.count[1][w];
-      if (w < wave) a_before += x, b_before += y;
-      a_all += x, b_all += y;
-    }
-    a_before += __popcll(a & below), b_before += __popcll(b & below);
-    const int free = left - equal;  // of those that have the prefix
-    const int b_taken = b_before < free ? b_before : free;
-    if (above || (same && b_before < free)) take(taken + a_before + b_taken, i, k);
-    taken += a_all + (b_all < free ? b_all : free);
-    equal += b_all < free ? b_all : free;
-  }
-  __syncthreads();
-}
+};
 
 // A workgroup has a row: joins its statistics; finds the words that lead it so far; after the last piece puts them in order and
 // takes the given words' products.
-template <class T, int THREADS>
+// PART: both, or after the last piece too the leading words are left in memory and another launch takes them on.
+enum { ALL_OF_IT = 0, SELECT = 1, FINISH = 2, NO_TOPS = 3 };
+template <class T, int THREADS, int PART>
 __global__ __launch_bounds__(THREADS) void k_answers(answer_args p) {
   constexpr int WAVES = THREADS / 64;
+  constexpr int HELD = MOST_HELD, AT_ONCE = 4;  // items of a thread; rows of E that a wave multiplies at a time
+  constexpr int LIST = 512;
   __shared__ pick_room<THREADS> room;
+  __shared__ unsigned list_key[LIST];
+  __shared__ int32_t list_word[LIST];
+  __shared__ int group_first[MOST_KEEP + 1];  // of 64 of the chunks' words
   __shared__ unsigned key_[2][MOST_KEEP];
   __shared__ int32_t word_[2][MOST_KEEP];
   __shared__ int32_t lead[MOST_KEEP];  // chunks
@@ -594,7 +692,8 @@ __global__ __launch_bounds__(THREADS) void k_answers(answer_args p) {
   for (int64_t m = blockIdx.x; m < p.rows; m += gridDim.x) {
     // -- statistics --
     running so_far = running{-INFINITY, 0.f, 0.f, 0};
-    if (!p.first) so_far = p.state[m];
+    if (!p.first || PART == FINISH) so_far = p.state[m];
+    if (PART == FINISH) p.parts_n = 0;
     float top = so_far.top;
     for (int i = tid; i < p.parts_n; i += THREADS) top = fmaxf(top, p.parts[m * p.parts_n + i].x);
 #pragma unroll
@@ -630,7 +729,11 @@ __global__ __launch_bounds__(THREADS) void k_answers(answer_args p) {
 
     // -- alternatives --
     int kept = so_far.kept, at = 0;
-    if (p.n_top > 0) {
+    if (PART == FINISH && p.n_top > 0) {
+      for (int i = tid; i < kept; i += THREADS) word_[0][i] = p.kept_word[m * p.keep + i];
+      __syncthreads();
+    }
+    if ((PART == ALL_OF_IT || PART == SELECT) && p.n_top > 0) {
       for (int i = tid; i < kept; i += THREADS) key_[0][i] = p.kept_key[m * p.keep + i], word_[0][i] = p.kept_word[m * p.keep + i];
       const float* tops = p.tops + m * p.chunks;
       // (a chunk that only reaches what a full list ends with comes after it)
@@ -639,50 +742,97 @@ __global__ __launch_bounds__(THREADS) void k_answers(answer_args p) {
         const unsigned k = key_of(tops[c]);
         return k > least ? k : 0u;
       };
-      int many = count_keys<THREADS>(room, p.chunks, chunk_key);
-      const bool all = many <= p.keep;
-      if (!all) many = p.keep;
-      unsigned reach = 0xffffffffu;  // the least of the chosen chunks' maxima
-      if (many > 0) {
-        pick<THREADS>(room, p.chunks, many, all, chunk_key, [&](int to, int64_t c, unsigned) { lead[to] = (int32_t)c; });
-        if (!all) {
-          for (int i = tid; i < many; i += THREADS) {
-            const unsigned k = chunk_key(lead[i]);
-            reach = k < reach ? k : reach;
-          }
+      picker<THREADS, HELD> chunks(room);
+      chunks.look(p.chunks, chunk_key);
+      if (chunks.count > 0) {
+        const int many = chunks.count < p.keep ? chunks.count : p.keep;
+        unsigned reach = 0xffffffffu;  // the least of the chosen chunks' maxima
+        chunks.pick(many, chunk_key, [&](int to, int64_t c, unsigned k) {
+          lead[to] = (int32_t)c;
+          reach = k < reach ? k : reach;
+        });
+        if (many < chunks.count) {
 #pragma unroll
           for (int d = 1; d < 64; d *= 2) {
             const unsigned o = (unsigned)__shfl_xor((int)reach, d, 64);
             reach = o < reach ? o : reach;
           }
-          if (lane == 0) room.hist[wave] = (int)reach;
-          __syncthreads();
+          if (WAVES > 1) {
+            if (lane == 0) room.part[0][wave] = reach;
+            __syncthreads();
 #pragma unroll
-          for (int w = 0; w < WAVES; w++) reach = (unsigned)room.hist[w] < reach ? (unsigned)room.hist[w] : reach;
+            for (int w = 0; w < WAVES; w++) reach = room.part[0][w] < reach ? room.part[0][w] : reach;
+          }
           least = reach - 1;
         }
-        // the list, then the chunks' words: in the order of the words
+        // The row's list, then the chunks' words that may join it: in the order of the words.  Of a chunk few do, so they are first
+        // put together in LDS (where there is room; if not, all the chunks' words are items).
         const float* z = p.logits + m * p.ldl;
-        const int n = kept + many * p.chunk;
-        auto place = [&](int64_t i) { return (int64_t)lead[(i - kept) / p.chunk] * p.chunk + (i - kept) % p.chunk; };
-        auto item_key = [&](int64_t i) {
-          if (i < kept) return key_[0][i];
-          const int64_t w = place(i);
+        const int bits = p.chunk == 64 ? 6 : p.chunk == 32 ? 5 : 4, in_chunks = many << bits, groups = (in_chunks + 63) >> 6;
+        auto place = [&](int i) { return ((int64_t)lead[i >> bits] << bits) + (i & (p.chunk - 1)); };
+        auto word_key = [&](int i) {
+          const int64_t w = i < in_chunks ? place(i) : p.piece;
           const unsigned k = w < p.piece ? key_of(z[w]) : 0u;
           return k > least ? k : 0u;
         };
-        int found = count_keys<THREADS>(room, n, item_key);
-        const bool every = found <= p.keep;
-        if (!every) found = p.keep;
-        pick<THREADS>(room, n, found, every, item_key, [&](int to, int64_t i, unsigned k) {
-          key_[1][to] = k;
-          word_[1][to] = i < kept ? word_[0][i] : (int32_t)(p.word0 + place(i));
-        });
+        for (int g = wave; g < groups; g += WAVES) {
+          const int c = __popcll(__ballot(word_key(g * 64 + lane) != 0));
+          if (lane == 0) group_first[g] = c;
+        }
+        __syncthreads();
+        if (wave == 0) {
+          int all = 0;
+          for (int g0 = 0; g0 < groups; g0 += 64) {
+            const int c = g0 + lane < groups ? group_first[g0 + lane] : 0;
+            int x = c;
+#pragma unroll
+            for (int d = 1; d < 64; d *= 2) {
+              const int u = __shfl_up(x, d, 64);
+              if (lane >= d) x += u;
+            }
+            if (g0 + lane < groups) group_first[g0 + lane] = kept + all + x - c;
+            all += __shfl(x, 63, 64);
+          }
+          if (lane == 0) group_first[groups] = kept + all;
+        }
+        __syncthreads();
+        const int listed = group_first[groups];
+        int found;
+        if (listed <= LIST) {
+          for (int i = tid; i < kept; i += THREADS) list_key[i] = key_[0][i], list_word[i] = word_[0][i];
+          for (int g = wave; g < groups; g += WAVES) {
+            const unsigned k = word_key(g * 64 + lane);
+            const unsigned long long in = __ballot(k != 0);
+            const int to = group_first[g] + __popcll(in & ((1ull << lane) - 1));
+            if (k != 0) list_key[to] = k, list_word[to] = (int32_t)(p.word0 + place(g * 64 + lane));
+          }
+          __syncthreads();
+          picker<THREADS, LIST / THREADS> items(room);
+          auto item_key = [&](int64_t i) { return list_key[i]; };
+          items.look(listed, item_key);
+          found = items.count < p.keep ? items.count : p.keep;
+          items.pick(found, item_key, [&](int to, int64_t i, unsigned k) { key_[1][to] = k, word_[1][to] = list_word[i]; });
+        } else {
+          picker<THREADS, HELD> items(room);
+          auto item_key = [&](int64_t i) { return i < kept ? key_[0][i] : word_key((int)i - kept); };
+          items.look(kept + in_chunks, item_key);
+          found = items.count < p.keep ? items.count : p.keep;
+          items.pick(found, item_key, [&](int to, int64_t i, unsigned k) {
+            key_[1][to] = k;
+            word_[1][to] = i < kept ? word_[0][i] : (int32_t)(p.word0 + place((int)i - kept));
+          });
+        }
         kept = found, at = 1;
       }
       __syncthreads();
     }
-    if (!p.last) {
+    if (p.stored && PART != FINISH) {
+      for (int j = tid; j < p.n_given; j += THREADS) {
+        const int64_t w = (int64_t)p.given[m * p.n_given + j] - p.word0;
+        if (w >= 0 && w < p.piece) p.logp[m * p.n_given + j] = p.logits[m * p.ldl + w];
+      }
+    }
+    if (PART == SELECT || (PART != FINISH && !p.last)) {
       for (int i = tid; i < kept; i += THREADS) p.kept_key[m * p.keep + i] = key_[at][i], p.kept_word[m * p.keep + i] = word_[at][i];
       if (wave == 0) {
         unsigned f = 0xffffffffu;
@@ -694,7 +844,7 @@ __global__ __launch_bounds__(THREADS) void k_answers(answer_args p) {
         }
         if (lane == 0) {
           p.state[m] = running{top, sum, weighted, kept};
-          p.floor[m] = kept == p.keep ? value_of(f) : -INFINITY;
+          if (p.n_top > 0) p.floor[m] = kept == p.keep ? value_of(f) : -INFINITY;
         }
       }
       __syncthreads();
@@ -705,11 +855,38 @@ __global__ __launch_bounds__(THREADS) void k_answers(answer_args p) {
       if (p.entropy) p.entropy[m] = sound ? logf(sum) - weighted / sum : __builtin_nanf("");
     }
     const T* x = (const T*)p.X + m * p.ldx;
-    if (p.n_top > 0) {
-      for (int i = wave; i < kept; i += WAVES) {
-        const double s = dot_rows<T>(x, (const T*)p.E + word_[at][i] * p.lde, p.n_in, lane);
-        if (lane == 0) exact_[i] = s == s ? s : -(double)INFINITY;
+    // the leading words' products, and the given words'
+    const int jobs = kept + (p.stored ? 0 : p.n_given);
+    for (int i = wave * AT_ONCE; i < jobs; i += WAVES * AT_ONCE) {
+      const T* e[AT_ONCE];
+      double s[AT_ONCE];
+      int32_t w[AT_ONCE];
+      bool any = false;
+#pragma unroll
+      for (int c = 0; c < AT_ONCE; c++) {
+        w[c] = i + c >= jobs ? -1 : i + c < kept ? word_[at][i + c] : p.given[m * p.n_given + i + c - kept];
+        any |= w[c] >= 0;
+        e[c] = (const T*)p.E + (w[c] >= 0 && w[c] < p.words ? w[c] : 0) * p.lde;
       }
+      if (any) dot_rows<T, AT_ONCE>(x, e, p.n_in, lane, s);
+#pragma unroll
+      for (int c = 0; c < AT_ONCE; c++) {
+        if (lane != c || i + c >= jobs) continue;
+        if (i + c < kept)
+          exact_[i + c] = s[c] == s[c] ? s[c] : -(double)INFINITY;
+        else
+          p.logp[m * p.n_given + i + c - kept] =
+              w[c] < 0 ? 0.f : w[c] >= p.words ? __builtin_nanf("") : (float)(s[c] * (double)p.inv_heat - (double)lse);
+      }
+    }
+    if (p.stored) {
+      for (int j = tid; j < p.n_given; j += THREADS) {  // (what this thread or an earlier launch has written)
+        const int32_t w = p.given[m * p.n_given + j];
+        float* to = p.logp + m * p.n_given + j;
+        *to = w < 0 ? 0.f : w >= p.words ? __builtin_nanf("") : *to - lse;
+      }
+    }
+    if (PART != NO_TOPS && p.n_top > 0) {
       __syncthreads();
       for (int i = tid; i < p.n_top; i += THREADS)
         if (!sound || i >= kept) p.top_words[m * p.n_top + i] = -1, p.top_logp[m * p.n_top + i] = __builtin_nanf("");
@@ -722,16 +899,6 @@ __global__ __launch_bounds__(THREADS) void k_answers(answer_args p) {
           p.top_logp[m * p.n_top + rank] = (float)(s * (double)p.inv_heat - (double)lse);
         }
       }
-    }
-    // -- given words --
-    for (int j = wave; j < p.n_given; j += WAVES) {
-      const int32_t w = p.given[m * p.n_given + j];
-      float l = 0.f;
-      if (w >= p.words)
-        l = __builtin_nanf("");
-      else if (w >= 0)
-        l = (float)(dot_rows<T>(x, (const T*)p.E + w * p.lde, p.n_in, lane) * (double)p.inv_heat - (double)lse);
-      if (lane == 0) p.logp[m * p.n_given + j] = l;
     }
     if (p.teacher) {
       __syncthreads();  // (a workgroup's writes are there for all of it)
@@ -867,10 +1034,33 @@ __global__ __launch_bounds__(256) void k_slope_rows(slope_args p) {
   }
 }
 
+// A bit for every chunk of 64 words that holds one of a row's given words; a wave has a row, and BITS words of it at a time.
+__global__ __launch_bounds__(256) void k_wanted(int64_t rows, int many, const int32_t* given, int64_t words, unsigned* wanted, int64_t ld) {
+  constexpr int BITS = 512;
+  __shared__ unsigned bits[4][BITS];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int64_t m = (int64_t)blockIdx.x * 4 + wave; m < rows; m += (int64_t)gridDim.x * 4) {
+    for (int64_t from = 0; from < ld; from += BITS) {
+      const int there = ld - from < BITS ? (int)(ld - from) : BITS;
+      for (int i = lane; i < there; i += 64) bits[wave][i] = 0;
+      asm volatile("" ::: "memory");  // (a wave's LDS accesses happen in their order)
+      for (int j = lane; j < many; j += 64) {
+        const int32_t w = given[m * many + j];
+        const int64_t at = (w >> 11) - from;
+        if (w >= 0 && w < words && at >= 0 && at < there) atomicOr(&bits[wave][at], 1u << (w >> 6 & 31));
+      }
+      asm volatile("" ::: "memory");
+      for (int i = lane; i < there; i += 64) wanted[m * ld + from + i] = bits[wave][i];
+      asm volatile("" ::: "memory");
+    }
+  }
+}
+
 // Rows, and of them at a time, of the forward pass; its workspace.
 struct answer_room {
   int64_t blocks, each;
-  bool few;
+  bool few, stored;
+  int64_t wanted, ld_wanted;
   int64_t packs[2] = {0, 0};  // of a block's X, of E
   int64_t piece, parts, weighted, state, tops, logits, kept, floor, logp, all;
   int keep;
@@ -887,21 +1077,25 @@ answer_room answer_room_of(int64_t rows, int64_t n_in, int64_t words, int n_give
     r.packs[0] = packed_bytes<T>(x), r.packs[1] = packed_bytes<T>(E);
   }
   r.keep = n_top > 0 ? (n_top + SPARE < words ? n_top + SPARE : (int)words) : 0;
+  r.stored = !r.few && r.each * n_given * n_in * (int64_t)sizeof(T) >= STORED_FROM;
+  const bool logits = n_top > 0 || r.stored;
   r.piece = words;
-  if (n_top > 0) {
+  if (logits) {
     int64_t most = LOGIT_BYTES / (4 * r.each) / 256 * 256;
     if (most < 1024) most = 1024;
     if (most < words) r.piece = ceil_div(ceil_div(words, ceil_div(words, most)), 256) * 256;
   }
+  r.ld_wanted = r.stored ? ceil_div(words, 2048) : 0;
+  r.wanted = round256(r.each * r.ld_wanted * 4);
   r.parts = round256(r.each * ceil_div(r.piece, r.few ? 16 : 128) * 8);
   r.weighted = round256(r.each * ceil_div(r.piece, r.few ? 16 : 128) * 4);
-  r.state = n_top > 0 ? round256(r.each * (int64_t)sizeof(running)) : 0;
+  r.state = logits ? round256(r.each * (int64_t)sizeof(running)) : 0;
   r.tops = n_top > 0 ? round256(r.each * ceil_div(r.piece, r.few ? 16 : 64) * 4) : 0;
-  r.logits = n_top > 0 ? round256(r.each * padded(r.piece) * 4) : 0;
+  r.logits = logits ? round256(r.each * padded(r.piece) * 4) : 0;
   r.kept = round256(r.each * r.keep * 4);
   r.floor = n_top > 0 ? round256(r.each * 4) : 0;
   r.logp = round256(r.each * (int64_t)n_given * 4);
-  r.all = r.packs[0] + r.packs[1] + r.parts + r.weighted + r.state + r.tops + r.logits + 2 * r.kept + r.floor + r.logp;
+  r.all = r.packs[0] + r.packs[1] + r.parts + r.weighted + r.state + r.tops + r.logits + 2 * r.kept + r.floor + r.logp + r.wanted;
   return r;
 }
 
@@ -930,6 +1124,8 @@ int answers_forward(hipStream_t st, const char* me, const answer_args& to, char*
   a.kept_word = (int32_t*)take(r.kept);
   a.floor = (float*)take(r.floor);
   float* logp_room = (float*)take(r.logp);
+  unsigned* wanted = (unsigned*)take(r.wanted);
+  a.stored = r.stored;
   a.parts = parts, a.weighted = weighted, a.tops = tops, a.logits = logits, a.keep = r.keep;
   for (int64_t b = 0; b < r.blocks; b++) {
     const int64_t m0 = b * r.each, rows = to.rows - m0 < r.each ? to.rows - m0 : r.each;
@@ -942,6 +1138,11 @@ int answers_forward(hipStream_t st, const char* me, const answer_args& to, char*
     a.lse = to.lse ? to.lse + m0 : nullptr, a.entropy = to.entropy ? to.entropy + m0 : nullptr, a.loss = to.loss ? to.loss + m0 : nullptr;
     a.top_words = to.top_words ? to.top_words + m0 * to.n_top : nullptr, a.top_logp = to.top_logp ? to.top_logp + m0 * to.n_top : nullptr;
     if (!r.few) DN_TRY(pack<T>(&x, 1, x_room, st));
+    if (r.stored) {
+      const int64_t blocks = ceil_div(rows, 4);
+      k_wanted<<<(unsigned)blocks, 256, 0, st>>>(rows, to.n_given, a.given, words, wanted, r.ld_wanted);
+      DN_LAUNCH_CHECK();
+    }
     for (int64_t w0 = 0; w0 < words; w0 += r.piece) {
       const int64_t n = words - w0 < r.piece ? words - w0 : r.piece;
       args p{};
@@ -951,7 +1152,9 @@ int answers_forward(hipStream_t st, const char* me, const answer_args& to, char*
       p.inv_heat = to.inv_heat;
       p.parts = parts, p.weighted = weighted;
       a.chunk = 64, a.chunks = ceil_div(n, 64);
-      if (to.n_top > 0) p.tops = tops, p.logits = logits, p.ldl = padded(n), p.chunks = a.chunks, p.floor = w0 > 0 ? a.floor : nullptr;
+      p.logits = logits, p.ldl = padded(n);
+      if (to.n_top > 0) p.tops = tops, p.chunks = a.chunks, p.floor = w0 > 0 ? a.floor : nullptr;
+      if (r.stored) p.wanted = wanted, p.ld_wanted = r.ld_wanted, p.chunk0 = w0 / 64;
       if (r.few) {
         p.B = (const T*)e.p + w0 * e.ld;
         DN_TRY((launch_few<T, E_PROBS>(p, st, &a.parts_n, &a.chunk)));
@@ -961,11 +1164,19 @@ int answers_forward(hipStream_t st, const char* me, const answer_args& to, char*
         DN_TRY((launch_product<T, true, true, E_PROBS>(p, nullptr, st, &a.parts_n)));
       }
       a.first = w0 == 0, a.last = w0 + n == words, a.word0 = w0, a.piece = n, a.ldl = padded(n);
+      // (a row's workgroup: us of 512, 256 and 128 threads, 1 row of 32000 words with 8 alternatives 16, 22 and 39; with 20 of 50001,
+      // 2000 rows, 150, 90 and 65)
       if (rows <= 512)
-        k_answers<T, 1024><<<(unsigned)rows, 1024, 0, st>>>(a);
+        k_answers<T, 512, ALL_OF_IT><<<(unsigned)rows, 512, 0, st>>>(a);
+      else if (a.n_top == 0)
+        k_answers<T, 128, NO_TOPS><<<(unsigned)rows, 128, 0, st>>>(a);
       else
-        k_answers<T, 256><<<(unsigned)rows, 256, 0, st>>>(a);
+        k_answers<T, 128, SELECT><<<(unsigned)rows, 128, 0, st>>>(a);
       DN_LAUNCH_CHECK();
+      if (rows > 512 && a.n_top > 0 && a.last) {
+        k_answers<T, 256, FINISH><<<(unsigned)rows, 256, 0, st>>>(a);
+        DN_LAUNCH_CHECK();
+      }
     }
   }
   return 0;
