@@ -437,6 +437,14 @@ __device__ __forceinline__ float value_of(unsigned key) {
   return key <= 1 ? -INFINITY : __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
+// A kernel's only argument where it lies: read where it is needed.
+template <class A>
+__device__ __forceinline__ const __attribute__((address_space(4))) A& arguments() {
+  typedef const __attribute__((address_space(4))) A kept;
+  kept* p = (kept*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *p;
+}
 struct running {  // a row's statistics so far
   float top, sum, weighted;
   int kept;
@@ -470,51 +478,111 @@ struct answer_args {
   float* loss;
 };
 
-// The products of a row with C others in 64 bits, in every lane.
-template <class T, int C>
-__device__ __forceinline__ void dot_rows(const T* a, const T* const* b, int64_t n, int lane, double* sum) {
+// Over the lanes of a wave, by the row shifts of its own registers: (LDS is not asked) lane l ends with the result of lanes 0 .. l; in their order.
+template <int CONTROL, int ROWS, class V>
+__device__ __forceinline__ V from_lane(V none, V v) {
+  union {
+    V v;
+    int i[sizeof(V) / 4];
+  } a, b;
+  a.v = none, b.v = v;
+#pragma unroll
+  for (unsigned t = 0; t < sizeof(V) / 4; t++) a.i[t] = __builtin_amdgcn_update_dpp(a.i[t], b.i[t], CONTROL, ROWS, 0xf, false);
+  return a.v;
+}
+template <class V, class Op>
+__device__ __forceinline__ V scan_lanes(V v, V none, Op op) {
+  v = op(from_lane<0x111, 0xf>(none, v), v);  // (the lane before, in rows of 16)
+  v = op(from_lane<0x112, 0xf>(none, v), v);
+  v = op(from_lane<0x114, 0xf>(none, v), v);
+  v = op(from_lane<0x118, 0xf>(none, v), v);
+  v = op(from_lane<0x142, 0xa>(none, v), v);  // (the last of the row before, to the second and fourth)
+  v = op(from_lane<0x143, 0xc>(none, v), v);  // (lane 31, to the upper half)
+  return v;
+}
+template <class V, class Op>
+__device__ __forceinline__ V over_lanes(V v, V none, Op op) {
+  union {
+    V v;
+    int i;
+  } a;
+  a.v = scan_lanes(v, none, op);
+  a.i = __builtin_amdgcn_readlane(a.i, 63);
+  return a.v;
+}
+struct plus_of {
+  template <class V>
+  __device__ V operator()(V a, V b) const { return a + b; }
+};
+struct max_of {
+  __device__ float operator()(float a, float b) const { return fmaxf(a, b); }
+  __device__ unsigned operator()(unsigned a, unsigned b) const { return a > b ? a : b; }
+};
+struct min_of {
+  __device__ unsigned operator()(unsigned a, unsigned b) const { return a < b ? a : b; }
+};
+
+// The products of a row with C others in S: a lane's part of them, the lanes in this one's order `lane` of `lanes`.
+template <class T, int C, class S>
+__device__ __forceinline__ void dot_rows(const T* a, const T* const* b, int64_t n, int lane, int lanes, S* sum) {
   constexpr int W = 16 / sizeof(T);
   typedef loose<T, W> piece;
 #pragma unroll
-  for (int c = 0; c < C; c++) sum[c] = 0.0;
-  int64_t k = (int64_t)lane * W;
-#pragma unroll 2
-  for (; k + W <= n; k += 64 * W) {
-    const piece x = *(const piece*)(a + k);
-    piece y[C];
+  for (int c = 0; c < C; c++) sum[c] = 0;
+  auto add = [&](const piece& x, const piece* y, int from) {
+    S d[W];
 #pragma unroll
-    for (int c = 0; c < C; c++) y[c] = *(const piece*)(b[c] + k);
-    double d[W];
-#pragma unroll
-    for (int t = 0; t < W; t++) d[t] = (double)(float)x[t];
+    for (int t = 0; t < W; t++) d[t] = (S)(float)x[t];
 #pragma unroll
     for (int c = 0; c < C; c++)
 #pragma unroll
-      for (int t = 0; t < W; t++) sum[c] = fma(d[t], (double)(float)y[c][t], sum[c]);
+      for (int t = 0; t < W; t++) sum[c] = t >= from ? fma(d[t], (S)(float)y[c][t], sum[c]) : sum[c];
+  };
+  int64_t k = (int64_t)lane * W;
+  piece x, y[C];
+#pragma unroll 1
+  for (; k + W <= n; k += lanes * W) {
+    x = *(const piece*)(a + k);
+#pragma unroll
+    for (int c = 0; c < C; c++) y[c] = *(const piece*)(b[c] + k);
+    add(x, y, 0);
   }
-  for (int t = 0; t < W && k + t < n; t++)
+  if (k < n) {
+    if (n >= W) {  // the row's last values, of which the first are another lane's
+      x = *(const piece*)(a + n - W);
 #pragma unroll
-    for (int c = 0; c < C; c++) sum[c] = fma((double)(float)a[k + t], (double)(float)b[c][k + t], sum[c]);
+      for (int c = 0; c < C; c++) y[c] = *(const piece*)(b[c] + n - W);
+      add(x, y, (int)(k + W - n));
+    } else {
+      for (int t = 0; t < n; t++)
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2)
-#pragma unroll
-    for (int c = 0; c < C; c++) sum[c] += __shfl_xor(sum[c], d, 64);
+        for (int c = 0; c < C; c++) sum[c] = fma((S)(float)a[t], (S)(float)b[c][t], sum[c]);
+    }
+  }
 }
 
-// Selection by a workgroup among n items with keys (0: not an item), which a thread keeps where n is at most THREADS HELD.
+// Selection among n items with keys (0: not an item), which a thread keeps where n is at most THREADS HELD: by a workgroup, or
+// (THREADS = 64) by one wave of it, which waits for nobody.
 constexpr int MOST_HELD = 8;
 template <int THREADS>
 struct pick_room {
   int hist[256];
-  unsigned part[3][MOST_HELD * THREADS / 64];  // per round and wave
+  unsigned part[3][MOST_HELD * (THREADS / 64)];  // per round and wave
   unsigned low, high;
   int left, done;
 };
 template <int THREADS, int HELD>
 struct picker {
-  static constexpr int WAVES = THREADS / 64;
+  static constexpr int WAVES = THREADS / 64, waves = WAVES;
   pick_room<THREADS>& r;
-  const int tid = threadIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, tid = THREADS == 64 ? lane : threadIdx.x, wave = THREADS == 64 ? 0 : threadIdx.x >> 6;
+  // (a wave's LDS accesses happen in their order)
+  __device__ static __forceinline__ void sync() {
+    if (THREADS == 64)
+      asm volatile("" ::: "memory");
+    else
+      __syncthreads();
+  }
   int64_t n;
   unsigned key[HELD];
   int count;          // of the items
@@ -527,15 +595,17 @@ struct picker {
 #pragma unroll
       for (int h = 0; h < HELD; h++) f(key[h]);
     } else {
+#pragma unroll 1
       for (int64_t i = tid; i < n; i += THREADS) f(key_at(i));
     }
   }
-  template <class Key>
-  __device__ __forceinline__ void look(int64_t n_items, Key key_at) {
+  // key_at(i) of an item; held(h): the same of the item h THREADS + tid
+  template <class Key, class Held>
+  __device__ __forceinline__ void look(int64_t n_items, Key key_at, Held held) {
     n = n_items;
     if (n <= THREADS * HELD) {
 #pragma unroll
-      for (int h = 0; h < HELD; h++) key[h] = h * THREADS + tid < n ? key_at(h * THREADS + tid) : 0u;
+      for (int h = 0; h < HELD; h++) key[h] = h * THREADS + tid < n ? held(h) : 0u;
     }
     unsigned c = 0, lo = 0xffffffffu, hi = 0;
     each(key_at, [&](unsigned k) {
@@ -543,16 +613,13 @@ struct picker {
       lo = k != 0 && k < lo ? k : lo;
       hi = k > hi ? k : hi;
     });
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      c += (unsigned)__shfl_xor((int)c, d, 64);
-      const unsigned l = (unsigned)__shfl_xor((int)lo, d, 64), h = (unsigned)__shfl_xor((int)hi, d, 64);
-      lo = l < lo ? l : lo, hi = h > hi ? h : hi;
-    }
+    c = over_lanes(c, 0u, plus_of());
+    lo = over_lanes(lo, 0xffffffffu, min_of());
+    hi = over_lanes(hi, 0u, max_of());
     if (WAVES > 1) {
-      __syncthreads();
+      sync();
       if (lane == 0) r.part[0][wave] = c, r.part[1][wave] = lo, r.part[2][wave] = hi;
-      __syncthreads();
+      sync();
       c = 0;
 #pragma unroll
       for (int w = 0; w < WAVES; w++) {
@@ -570,28 +637,22 @@ struct picker {
     int left = need;
     bool done = need >= count;
     if (done) hi = 0xffffffffu, left = count;  // (all are in the range)
-    __syncthreads();
+    sync();
     while (!done) {
       const unsigned span = hi - lo;
       const int shift = span < 256 ? 0 : 24 - __builtin_clz(span);
       for (int i = tid; i < 256; i += THREADS) r.hist[i] = 0;
-      __syncthreads();
+      sync();
       each(key_at, [&](unsigned k) {
         if (k >= lo && k <= hi) atomicAdd(&r.hist[(k - lo) >> shift], 1);
       });
-      __syncthreads();
+      sync();
       if (wave == 0) {
         // lane l: the four parts from 255 - 4 l down
         int own[4], sum = 0;
 #pragma unroll
         for (int e = 0; e < 4; e++) own[e] = r.hist[255 - 4 * lane - e], sum += own[e];
-        int before = sum;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-          const int u = __shfl_up(before, d, 64);
-          if (lane >= d) before += u;
-        }
-        before -= sum;
+        int before = scan_lanes(sum, 0, plus_of()) - sum;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           if (before < left && before + own[e] >= left) {
@@ -602,48 +663,50 @@ struct picker {
           before += own[e];
         }
       }
-      __syncthreads();
+      sync();
       lo = r.low, hi = r.high, left = r.left, done = r.done != 0;
     }
     // those above the range, and the first `left` of those in it
     const unsigned long long below = (1ull << lane) - 1;
-    if (n <= THREADS * HELD) {
+    if (WAVES == 1 && n <= THREADS * HELD) {
+      int a_before = 0, b_before = 0;
+#pragma unroll
+      for (int h = 0; h < HELD; h++) {
+        const bool up = key[h] > hi, same = key[h] != 0 && key[h] >= lo && key[h] <= hi;
+        const unsigned long long above = __ballot(up), in = __ballot(same);
+        const int a = a_before + __popcll(above & below), b = b_before + __popcll(in & below);
+        if (up || (same && b < left)) take(a + (b < left ? b : left), (int64_t)h * THREADS + tid, key[h]);
+        a_before += __popcll(above), b_before += __popcll(in);
+      }
+    } else if (n <= THREADS * HELD) {
       unsigned long long above[HELD], in[HELD];
 #pragma unroll
       for (int h = 0; h < HELD; h++) {
         above[h] = __ballot(key[h] > hi), in[h] = __ballot(key[h] != 0 && key[h] >= lo && key[h] <= hi);
-        if (WAVES > 1 && lane == 0) r.part[0][h * WAVES + wave] = __popcll(above[h]), r.part[1][h * WAVES + wave] = __popcll(in[h]);
+        if (lane == 0) r.part[0][h * WAVES + wave] = __popcll(above[h]), r.part[1][h * WAVES + wave] = __popcll(in[h]);
       }
-      if (WAVES > 1) {
-        __syncthreads();
-        if (wave == 0) {  // sums of what comes before
-          int a_all = 0, b_all = 0;
-          for (int i0 = 0; i0 < HELD * WAVES; i0 += 64) {
-            const int i = i0 + lane;
-            const int a = i < HELD * WAVES ? (int)r.part[0][i] : 0, b = i < HELD * WAVES ? (int)r.part[1][i] : 0;
-            int x = a, y = b;
-#pragma unroll
-            for (int d = 1; d < 64; d *= 2) {
-              const int u = __shfl_up(x, d, 64), v = __shfl_up(y, d, 64);
-              if (lane >= d) x += u, y += v;
-            }
-            if (i < HELD * WAVES) r.part[0][i] = a_all + x - a, r.part[1][i] = b_all + y - b;
-            a_all += __shfl(x, 63, 64), b_all += __shfl(y, 63, 64);
-          }
+      sync();
+      if (wave == 0) {  // sums of what comes before
+        int a_all = 0, b_all = 0;
+        for (int i0 = 0; i0 < HELD * WAVES; i0 += 64) {
+          const int i = i0 + lane;
+          const int a = i < HELD * WAVES ? (int)r.part[0][i] : 0, b = i < HELD * WAVES ? (int)r.part[1][i] : 0;
+          const int x = scan_lanes(a, 0, plus_of()), y = scan_lanes(b, 0, plus_of());
+          if (i < HELD * WAVES) r.part[0][i] = a_all + x - a, r.part[1][i] = b_all + y - b;
+          a_all += __builtin_amdgcn_readlane(x, 63), b_all += __builtin_amdgcn_readlane(y, 63);
         }
-        __syncthreads();
       }
-      int a_before = 0, b_before = 0;
+      sync();
 #pragma unroll
       for (int h = 0; h < HELD; h++) {
-        if (WAVES > 1) a_before = (int)r.part[0][h * WAVES + wave], b_before = (int)r.part[1][h * WAVES + wave];
+        const int a_before = (int)r.part[0][h * WAVES + wave], b_before = (int)r.part[1][h * WAVES + wave];
         const int a = a_before + __popcll(above[h] & below), b = b_before + __popcll(in[h] & below);
         const bool up = key[h] > hi, same = (in[h] >> lane) & 1;
         if (up || (same && b < left)) take(a + (b < left ? b : left), (int64_t)h * THREADS + tid, key[h]);
-        if (WAVES == 1) a_before += __popcll(above[h]), b_before += __popcll(in[h]);
       }
     } else {
       int a_before = 0, b_before = 0;
+#pragma unroll 1
       for (int64_t base = 0; base < n; base += THREADS) {
         const int64_t i = base + tid;
         const unsigned k = i < n ? key_at(i) : 0u;
@@ -651,9 +714,9 @@ struct picker {
         const unsigned long long above = __ballot(up), in = __ballot(same);
         int a = a_before, b = b_before, a_all = __popcll(above), b_all = __popcll(in);
         if (WAVES > 1) {
-          __syncthreads();
+          sync();
           if (lane == 0) r.part[0][wave] = a_all, r.part[1][wave] = b_all;
-          __syncthreads();
+          sync();
           a_all = b_all = 0;
 #pragma unroll
           for (int w = 0; w < WAVES; w++) {
@@ -666,7 +729,7 @@ struct picker {
         a_before += a_all, b_before += b_all;
       }
     }
-    __syncthreads();
+    sync();
   }
 };
 
@@ -675,11 +738,14 @@ struct picker {
 // PART: both, or after the last piece too the leading words are left in memory and another launch takes them on.
 enum { ALL_OF_IT = 0, SELECT = 1, FINISH = 2, NO_TOPS = 3 };
 template <class T, int THREADS, int PART>
-__global__ __launch_bounds__(THREADS) void k_answers(answer_args p) {
+__global__ __launch_bounds__(THREADS) void k_answers(answer_args) {
   constexpr int WAVES = THREADS / 64;
-  constexpr int HELD = MOST_HELD, AT_ONCE = 4;  // items of a thread; rows of E that a wave multiplies at a time
-  constexpr int LIST = 512;
+  constexpr bool TOPS = PART == ALL_OF_IT || PART == SELECT, FEW = THREADS >= 512;
+  constexpr int HELD = THREADS == 64 ? 2 * MOST_HELD : MOST_HELD, AT_ONCE = FEW ? 6 : 4;  // items of a thread; rows of E that a wave multiplies at a time
+  constexpr int LIST = 256, PARTS = 4;
   __shared__ pick_room<THREADS> room;
+  pick_room<64>& wave_room = *(pick_room<64>*)&room;
+  __shared__ int chosen;
   __shared__ unsigned list_key[LIST];
   __shared__ int32_t list_word[LIST];
   __shared__ int group_first[MOST_KEEP + 1];  // of 64 of the chunks' words
@@ -688,21 +754,62 @@ __global__ __launch_bounds__(THREADS) void k_answers(answer_args p) {
   __shared__ int32_t lead[MOST_KEEP];  // chunks
   __shared__ double exact_[MOST_KEEP];
   __shared__ float red[3][WAVES];
+  __shared__ double part_of[FEW ? WAVES : 1][FEW ? MOST_KEEP : 1];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  for (int64_t m = blockIdx.x; m < p.rows; m += gridDim.x) {
+  // Rows of E that are multiplied later, read ahead to the caches, and the row of X: a lane has a line.  (Each read of them from memory,
+  // one after the other, would be 2 us.)
+  auto touch = [&](int64_t m, int many, auto word) {
+    auto& p = arguments<answer_args>();
+    unsigned sum = 0;
+    const int64_t bytes = p.n_in * (int64_t)sizeof(T);
+    const int lines = (int)((bytes + 127) / 128);
+    if ((int64_t)(many + 1) * lines > 8 * THREADS) return sum;
+#pragma unroll 4
+    for (int i = tid; i < (many + 1) * lines; i += THREADS) {
+      const int32_t w = i < lines ? 0 : word(i / lines - 1);
+      const char* row = i < lines ? (const char*)((const T*)p.X + m * p.ldx) : (const char*)((const T*)p.E + (w >= 0 && w < p.words ? w : 0) * p.lde);
+      sum += *(const unsigned char*)(row + i % lines * 128);
+    }
+    return sum;
+  };
+  for (int64_t m = blockIdx.x; m < arguments<answer_args>().rows; m += gridDim.x) {
     // -- statistics --
+    auto& p0 = arguments<answer_args>();
     running so_far = running{-INFINITY, 0.f, 0.f, 0};
-    if (!p.first || PART == FINISH) so_far = p.state[m];
-    if (PART == FINISH) p.parts_n = 0;
+    if (!p0.first || PART == FINISH) so_far = p0.state[m];
+    const int parts_n = PART == FINISH ? 0 : p0.parts_n;
+    // (what is read first is asked for together: a read takes 1 to 2 us)
+    float tops_here[TOPS ? HELD : 1];
+    if (TOPS && p0.n_top > 0 && p0.chunks <= THREADS * HELD) {
+#pragma unroll
+      for (int h = 0; h < HELD; h++) tops_here[h] = h * THREADS + tid < p0.chunks ? p0.tops[m * p0.chunks + h * THREADS + tid] : 0.f;
+    }
+    float2 own[PARTS];
+    float own_w[PARTS];
+    const bool held = parts_n <= PARTS * THREADS;
+#pragma unroll
+    for (int i = 0; i < PARTS; i++) {
+      const bool here = held && i * THREADS + tid < parts_n;
+      const int64_t at = m * parts_n + i * THREADS + tid;
+      own[i] = here ? p0.parts[at] : float2{-INFINITY, 0.f};
+      own_w[i] = here ? p0.weighted[at] : 0.f;
+    }
+    unsigned touched = 0;
+    if (FEW && p0.last && !p0.stored) touched = touch(m, p0.n_given, [&](int i) { return p0.given[m * p0.n_given + i]; });
     float top = so_far.top;
-    for (int i = tid; i < p.parts_n; i += THREADS) top = fmaxf(top, p.parts[m * p.parts_n + i].x);
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
-    __syncthreads();
-    if (lane == 0) red[0][wave] = top;
-    __syncthreads();
+    for (int i = 0; i < PARTS; i++) top = fmaxf(top, own[i].x);
+    if (!held) {
+      for (int i = tid; i < parts_n; i += THREADS) top = fmaxf(top, p0.parts[m * parts_n + i].x);
+    }
+    top = over_lanes(top, -INFINITY, max_of());
+    if (WAVES > 1) {
+      __syncthreads();
+      if (lane == 0) red[0][wave] = top;
+      __syncthreads();
 #pragma unroll
-    for (int w = 0; w < WAVES; w++) top = fmaxf(top, red[0][w]);
+      for (int w = 0; w < WAVES; w++) top = fmaxf(top, red[0][w]);
+    }
     const float from = top == -INFINITY ? 0.f : top;
     float sum = 0.f, weighted = 0.f;
     auto add = [&](float x, float s, float w) {
@@ -712,28 +819,36 @@ __global__ __launch_bounds__(THREADS) void k_answers(answer_args p) {
         weighted += f * fmaf(fmaxf(x - from, -150.f), s, w);
       }
     };
-    for (int i = tid; i < p.parts_n; i += THREADS) {
-      const float2 s = p.parts[m * p.parts_n + i];
-      add(s.x, s.y, p.weighted[m * p.parts_n + i]);
+#pragma unroll
+    for (int i = 0; i < PARTS; i++) add(own[i].x, own[i].y, own_w[i]);
+    if (!held) {
+#pragma unroll 1
+      for (int i = tid; i < parts_n; i += THREADS) {
+        const float2 s = p0.parts[m * parts_n + i];
+        add(s.x, s.y, p0.weighted[m * parts_n + i]);
+      }
     }
+    sum = over_lanes(sum, 0.f, plus_of()), weighted = over_lanes(weighted, 0.f, plus_of());
+    if (WAVES > 1) {
+      if (lane == 0) red[1][wave] = sum, red[2][wave] = weighted;
+      __syncthreads();
+      sum = weighted = 0.f;
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d, 64), weighted += __shfl_xor(weighted, d, 64);
-    if (lane == 0) red[1][wave] = sum, red[2][wave] = weighted;
-    __syncthreads();
-    sum = weighted = 0.f;
-#pragma unroll
-    for (int w = 0; w < WAVES; w++) sum += red[1][w], weighted += red[2][w];
+      for (int w = 0; w < WAVES; w++) sum += red[1][w], weighted += red[2][w];
+    }
+    asm volatile("" ::"v"(touched));
     add(so_far.top, so_far.sum, so_far.weighted);
     const float lse = logf(sum) + from;
     const bool sound = fabsf(lse) < INFINITY;
 
     // -- alternatives --
+    auto& p = arguments<answer_args>();
     int kept = so_far.kept, at = 0;
     if (PART == FINISH && p.n_top > 0) {
       for (int i = tid; i < kept; i += THREADS) word_[0][i] = p.kept_word[m * p.keep + i];
       __syncthreads();
     }
-    if ((PART == ALL_OF_IT || PART == SELECT) && p.n_top > 0) {
+    if (TOPS && p.n_top > 0) {
       for (int i = tid; i < kept; i += THREADS) key_[0][i] = p.kept_key[m * p.keep + i], word_[0][i] = p.kept_word[m * p.keep + i];
       const float* tops = p.tops + m * p.chunks;
       // (a chunk that only reaches what a full list ends with comes after it)
@@ -743,20 +858,19 @@ __global__ __launch_bounds__(THREADS) void k_answers(answer_args p) {
         return k > least ? k : 0u;
       };
       picker<THREADS, HELD> chunks(room);
-      chunks.look(p.chunks, chunk_key);
-      if (chunks.count > 0) {
-        const int many = chunks.count < p.keep ? chunks.count : p.keep;
+      chunks.look(p.chunks, chunk_key, [&](int h) {
+        const unsigned k = key_of(tops_here[h]);
+        return k > least ? k : 0u;
+      });
+      const int many = chunks.count < p.keep ? chunks.count : p.keep;
+      if (many > 0) {
         unsigned reach = 0xffffffffu;  // the least of the chosen chunks' maxima
         chunks.pick(many, chunk_key, [&](int to, int64_t c, unsigned k) {
           lead[to] = (int32_t)c;
           reach = k < reach ? k : reach;
         });
         if (many < chunks.count) {
-#pragma unroll
-          for (int d = 1; d < 64; d *= 2) {
-            const unsigned o = (unsigned)__shfl_xor((int)reach, d, 64);
-            reach = o < reach ? o : reach;
-          }
+          reach = over_lanes(reach, 0xffffffffu, min_of());
           if (WAVES > 1) {
             if (lane == 0) room.part[0][wave] = reach;
             __syncthreads();
@@ -775,6 +889,7 @@ __global__ __launch_bounds__(THREADS) void k_answers(answer_args p) {
           const unsigned k = w < p.piece ? key_of(z[w]) : 0u;
           return k > least ? k : 0u;
         };
+#pragma unroll 2
         for (int g = wave; g < groups; g += WAVES) {
           const int c = __popcll(__ballot(word_key(g * 64 + lane) != 0));
           if (lane == 0) group_first[g] = c;
@@ -784,14 +899,9 @@ __global__ __launch_bounds__(THREADS) void k_answers(answer_args p) {
           int all = 0;
           for (int g0 = 0; g0 < groups; g0 += 64) {
             const int c = g0 + lane < groups ? group_first[g0 + lane] : 0;
-            int x = c;
-#pragma unroll
-            for (int d = 1; d < 64; d *= 2) {
-              const int u = __shfl_up(x, d, 64);
-              if (lane >= d) x += u;
-            }
+            const int x = scan_lanes(c, 0, plus_of());
             if (g0 + lane < groups) group_first[g0 + lane] = kept + all + x - c;
-            all += __shfl(x, 63, 64);
+            all += __builtin_amdgcn_readlane(x, 63);
           }
           if (lane == 0) group_first[groups] = kept + all;
         }
@@ -800,6 +910,7 @@ __global__ __launch_bounds__(THREADS) void k_answers(answer_args p) {
         int found;
         if (listed <= LIST) {
           for (int i = tid; i < kept; i += THREADS) list_key[i] = key_[0][i], list_word[i] = word_[0][i];
+#pragma unroll 2
           for (int g = wave; g < groups; g += WAVES) {
             const unsigned k = word_key(g * 64 + lane);
             const unsigned long long in = __ballot(k != 0);
@@ -807,15 +918,20 @@ __global__ __launch_bounds__(THREADS) void k_answers(answer_args p) {
             if (k != 0) list_key[to] = k, list_word[to] = (int32_t)(p.word0 + place(g * 64 + lane));
           }
           __syncthreads();
-          picker<THREADS, LIST / THREADS> items(room);
-          auto item_key = [&](int64_t i) { return list_key[i]; };
-          items.look(listed, item_key);
-          found = items.count < p.keep ? items.count : p.keep;
-          items.pick(found, item_key, [&](int to, int64_t i, unsigned k) { key_[1][to] = k, word_[1][to] = list_word[i]; });
+          if (wave == 0) {
+            picker<64, LIST / 64> items(wave_room);
+            auto item_key = [&](int64_t i) { return list_key[i]; };
+            items.look(listed, item_key, [&](int h) { return list_key[h * 64 + lane]; });
+            found = items.count < p.keep ? items.count : p.keep;
+            items.pick(found, item_key, [&](int to, int64_t i, unsigned k) { key_[1][to] = k, word_[1][to] = list_word[i]; });
+            if (lane == 0) chosen = found;
+          }
+          __syncthreads();
+          found = chosen;
         } else {
           picker<THREADS, HELD> items(room);
           auto item_key = [&](int64_t i) { return i < kept ? key_[0][i] : word_key((int)i - kept); };
-          items.look(kept + in_chunks, item_key);
+          items.look(kept + in_chunks, item_key, [&](int h) { return item_key(h * THREADS + tid); });
           found = items.count < p.keep ? items.count : p.keep;
           items.pick(found, item_key, [&](int to, int64_t i, unsigned k) {
             key_[1][to] = k;
@@ -826,106 +942,141 @@ __global__ __launch_bounds__(THREADS) void k_answers(answer_args p) {
       }
       __syncthreads();
     }
-    if (p.stored && PART != FINISH) {
-      for (int j = tid; j < p.n_given; j += THREADS) {
-        const int64_t w = (int64_t)p.given[m * p.n_given + j] - p.word0;
-        if (w >= 0 && w < p.piece) p.logp[m * p.n_given + j] = p.logits[m * p.ldl + w];
+    auto& p1 = p;
+    if (p1.stored && PART != FINISH) {
+      for (int j = tid; j < p1.n_given; j += THREADS) {
+        const int64_t w = (int64_t)p1.given[m * p1.n_given + j] - p1.word0;
+        if (w >= 0 && w < p1.piece) p1.logp[m * p1.n_given + j] = p1.logits[m * p1.ldl + w];
       }
     }
-    if (PART == SELECT || (PART != FINISH && !p.last)) {
-      for (int i = tid; i < kept; i += THREADS) p.kept_key[m * p.keep + i] = key_[at][i], p.kept_word[m * p.keep + i] = word_[at][i];
+    if (PART == SELECT || (PART != FINISH && !p1.last)) {
+      for (int i = tid; i < kept; i += THREADS) p1.kept_key[m * p1.keep + i] = key_[at][i], p1.kept_word[m * p1.keep + i] = word_[at][i];
       if (wave == 0) {
         unsigned f = 0xffffffffu;
         for (int i = lane; i < kept; i += 64) f = key_[at][i] < f ? key_[at][i] : f;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-          const unsigned o = (unsigned)__shfl_xor((int)f, d, 64);
-          f = o < f ? o : f;
-        }
+        f = over_lanes(f, 0xffffffffu, min_of());
         if (lane == 0) {
-          p.state[m] = running{top, sum, weighted, kept};
-          if (p.n_top > 0) p.floor[m] = kept == p.keep ? value_of(f) : -INFINITY;
+          p1.state[m] = running{top, sum, weighted, kept};
+          if (p1.n_top > 0) p1.floor[m] = kept == p1.keep ? value_of(f) : -INFINITY;
         }
       }
       __syncthreads();
       continue;
     }
     if (tid == 0) {
-      if (p.lse) p.lse[m] = lse;
-      if (p.entropy) p.entropy[m] = sound ? logf(sum) - weighted / sum : __builtin_nanf("");
+      if (p1.lse) p1.lse[m] = lse;
+      if (p1.entropy) p1.entropy[m] = sound ? logf(sum) - weighted / sum : __builtin_nanf("");
     }
-    const T* x = (const T*)p.X + m * p.ldx;
-    // the leading words' products, and the given words'
-    const int jobs = kept + (p.stored ? 0 : p.n_given);
-    for (int i = wave * AT_ONCE; i < jobs; i += WAVES * AT_ONCE) {
-      const T* e[AT_ONCE];
-      double s[AT_ONCE];
-      int32_t w[AT_ONCE];
-      bool any = false;
+    const T* x = (const T*)p1.X + m * p1.ldx;
+    auto& p2 = arguments<answer_args>();
+    // The products of `many` words' rows, each given to put(i, product) in one lane.  Few rows: `share` waves have a part each of a
+    // product; else a wave has all of it.
+    constexpr int W = 16 / sizeof(T);
+    int share = 1;
+    while (FEW && share < WAVES && share * 64 * W < p2.n_in) share *= 2;
+    auto products = [&](auto zero, int many, auto word, auto put) {
+      typedef decltype(zero) S;
+      for (int i0 = 0; i0 < many; i0 += MOST_KEEP) {
+        const int there = many - i0 < MOST_KEEP ? many - i0 : MOST_KEEP;
+#pragma unroll 1
+        for (int i = wave / share * AT_ONCE; i < there; i += WAVES / share * AT_ONCE) {
+          const T* e[AT_ONCE];
+          S s[AT_ONCE];
+          bool any = false;
 #pragma unroll
-      for (int c = 0; c < AT_ONCE; c++) {
-        w[c] = i + c >= jobs ? -1 : i + c < kept ? word_[at][i + c] : p.given[m * p.n_given + i + c - kept];
-        any |= w[c] >= 0;
-        e[c] = (const T*)p.E + (w[c] >= 0 && w[c] < p.words ? w[c] : 0) * p.lde;
-      }
-      if (any) dot_rows<T, AT_ONCE>(x, e, p.n_in, lane, s);
+          for (int c = 0; c < AT_ONCE; c++) {
+            const int32_t w = word(i0 + (i + c < there ? i + c : there - 1));
+            any |= w >= 0;
+            e[c] = (const T*)p2.E + (w >= 0 && w < p2.words ? w : 0) * p2.lde;
+            s[c] = 0;
+          }
+          if (any) {
+            dot_rows<T, AT_ONCE, S>(x, e, p2.n_in, FEW ? tid & (share * 64 - 1) : lane, share * 64, s);
 #pragma unroll
-      for (int c = 0; c < AT_ONCE; c++) {
-        if (lane != c || i + c >= jobs) continue;
-        if (i + c < kept)
-          exact_[i + c] = s[c] == s[c] ? s[c] : -(double)INFINITY;
-        else
-          p.logp[m * p.n_given + i + c - kept] =
-              w[c] < 0 ? 0.f : w[c] >= p.words ? __builtin_nanf("") : (float)(s[c] * (double)p.inv_heat - (double)lse);
+            for (int c = 0; c < AT_ONCE; c++) s[c] = scan_lanes(s[c], zero, plus_of());
+          }
+          if (lane == 63) {
+#pragma unroll
+            for (int c = 0; c < AT_ONCE; c++)
+              if (i + c < there) {
+                if (FEW)
+                  part_of[wave % share][i + c] = s[c];
+                else
+                  put(i0 + i + c, s[c]);
+              }
+          }
+        }
+        if (FEW) {
+          __syncthreads();
+          for (int i = tid; i < there; i += THREADS) {
+            S s = 0;
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) s += w < share ? (S)part_of[w][i] : zero;
+            put(i0 + i, s);
+          }
+          __syncthreads();
+        }
+      }
+    };
+    if (TOPS || PART == FINISH) {
+      auto word = [&](int i) { return word_[at][i]; };
+      const unsigned touched = FEW && kept > 0 ? touch(m, kept, word) : 0u;
+      asm volatile("" ::"v"(touched));
+      products(0.0, kept, word, [&](int i, double s) { exact_[i] = s == s ? s : -(double)INFINITY; });
+    }
+    if (!p2.stored)
+      products(0.f, p2.n_given, [&](int j) { return p2.given[m * p2.n_given + j]; }, [&](int j, float s) {
+        const int32_t w = p2.given[m * p2.n_given + j];
+        p2.logp[m * p2.n_given + j] = w < 0 ? 0.f : w >= p2.words ? __builtin_nanf("") : s * p2.inv_heat - lse;
+      });
+    if (p2.stored) {
+      for (int j = tid; j < p2.n_given; j += THREADS) {  // (what this thread or an earlier launch has written)
+        const int32_t w = p2.given[m * p2.n_given + j];
+        float* to = p2.logp + m * p2.n_given + j;
+        *to = w < 0 ? 0.f : w >= p2.words ? __builtin_nanf("") : *to - lse;
       }
     }
-    if (p.stored) {
-      for (int j = tid; j < p.n_given; j += THREADS) {  // (what this thread or an earlier launch has written)
-        const int32_t w = p.given[m * p.n_given + j];
-        float* to = p.logp + m * p.n_given + j;
-        *to = w < 0 ? 0.f : w >= p.words ? __builtin_nanf("") : *to - lse;
-      }
-    }
-    if (PART != NO_TOPS && p.n_top > 0) {
+    if (PART != NO_TOPS && p2.n_top > 0) {
       __syncthreads();
-      for (int i = tid; i < p.n_top; i += THREADS)
-        if (!sound || i >= kept) p.top_words[m * p.n_top + i] = -1, p.top_logp[m * p.n_top + i] = __builtin_nanf("");
+      for (int i = tid; i < p2.n_top; i += THREADS)
+        if (!sound || i >= kept) p2.top_words[m * p2.n_top + i] = -1, p2.top_logp[m * p2.n_top + i] = __builtin_nanf("");
       for (int i = tid; i < kept && sound; i += THREADS) {
         const double s = exact_[i];
         int rank = 0;
+#pragma unroll 4
         for (int j = 0; j < kept; j++) rank += exact_[j] > s || (exact_[j] == s && j < i);
-        if (rank < p.n_top) {
-          p.top_words[m * p.n_top + rank] = word_[at][i];
-          p.top_logp[m * p.n_top + rank] = (float)(s * (double)p.inv_heat - (double)lse);
+        if (rank < p2.n_top) {
+          p2.top_words[m * p2.n_top + rank] = word_[at][i];
+          p2.top_logp[m * p2.n_top + rank] = (float)(s * (double)p2.inv_heat - (double)lse);
         }
       }
     }
-    if (p.teacher) {
+    if (p2.teacher) {
       __syncthreads();  // (a workgroup's writes are there for all of it)
       if (wave == 0) {
-        const float* l = p.teacher + m * p.n_given;
-        const int32_t* w = p.given + m * p.n_given;
-        const float *logp = p.logp + m * p.n_given;
+        const float* l = p2.teacher + m * p2.n_given;
+        const int32_t* w = p2.given + m * p2.n_given;
+        const float *logp = p2.logp + m * p2.n_given;
         float most = -INFINITY, all = 0.f, loss = 0.f;
         bool odd = false;  // NaN or +infinity among them
-        for (int j = lane; j < p.n_given; j += 64)
-          if (w[j] >= 0 && l[j] != -INFINITY) most = fmaxf(most, l[j]), odd |= !(l[j] < INFINITY) || w[j] >= p.words;
+        for (int j = lane; j < p2.n_given; j += 64)
+          if (w[j] >= 0 && l[j] != -INFINITY) most = fmaxf(most, l[j]), odd |= !(l[j] < INFINITY) || w[j] >= p2.words;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) most = fmaxf(most, __shfl_xor(most, d, 64));
-        for (int j = lane; j < p.n_given; j += 64)
-          if (w[j] >= 0 && l[j] > -INFINITY) all += expf((l[j] - most) * p.inv_heat);
+        for (int j = lane; j < p2.n_given; j += 64)
+          if (w[j] >= 0 && l[j] > -INFINITY) all += expf((l[j] - most) * p2.inv_heat);
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d, 64);
         const float log_all = logf(all);
-        for (int j = lane; j < p.n_given; j += 64)
+        for (int j = lane; j < p2.n_given; j += 64)
           if (w[j] >= 0 && l[j] > -INFINITY) {
-            const float log_q = (l[j] - most) * p.inv_heat - log_all, q = expf(log_q);
+            const float log_q = (l[j] - most) * p2.inv_heat - log_all, q = expf(log_q);
             if (q != 0.f) loss += q * (log_q - logp[j]);
           }
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) loss += __shfl_xor(loss, d, 64);
         const bool bad = __any(odd);
-        if (lane == 0) p.loss[m] = bad ? __builtin_nanf("") : most == -INFINITY ? 0.f : loss;
+        if (lane == 0) p2.loss[m] = bad ? __builtin_nanf("") : most == -INFINITY ? 0.f : loss;
       }
     }
     __syncthreads();
@@ -1164,19 +1315,20 @@ int answers_forward(hipStream_t st, const char* me, const answer_args& to, char*
         DN_TRY((launch_product<T, true, true, E_PROBS>(p, nullptr, st, &a.parts_n)));
       }
       a.first = w0 == 0, a.last = w0 + n == words, a.word0 = w0, a.piece = n, a.ldl = padded(n);
-      // (a row's workgroup: us of 512, 256 and 128 threads, 1 row of 32000 words with 8 alternatives 16, 22 and 39; with 20 of 50001,
-      // 2000 rows, 150, 90 and 65)
-      if (rows <= 512)
+      // us of a row in 512 threads and in fewer: 64 rows of 32000 words with 20 alternatives 38 and 54 (two launches), 512 rows 75 and 77
+      if (a.n_top == 0) {
+        if (rows <= 256)
+          k_answers<T, 512, NO_TOPS><<<(unsigned)rows, 512, 0, st>>>(a);
+        else
+          k_answers<T, 128, NO_TOPS><<<(unsigned)rows, 128, 0, st>>>(a);
+      } else if (rows <= 512) {
         k_answers<T, 512, ALL_OF_IT><<<(unsigned)rows, 512, 0, st>>>(a);
-      else if (a.n_top == 0)
-        k_answers<T, 128, NO_TOPS><<<(unsigned)rows, 128, 0, st>>>(a);
-      else
-        k_answers<T, 128, SELECT><<<(unsigned)rows, 128, 0, st>>>(a);
-      DN_LAUNCH_CHECK();
-      if (rows > 512 && a.n_top > 0 && a.last) {
-        k_answers<T, 256, FINISH><<<(unsigned)rows, 256, 0, st>>>(a);
+      } else {
+        k_answers<T, 64, SELECT><<<(unsigned)rows, 64, 0, st>>>(a);
         DN_LAUNCH_CHECK();
+        if (a.last) k_answers<T, 256, FINISH><<<(unsigned)rows, 256, 0, st>>>(a);
       }
+      DN_LAUNCH_CHECK();
     }
   }
   return 0;
