@@ -738,7 +738,7 @@ struct picker {
 // PART: both, or after the last piece too the leading words are left in memory and another launch takes them on.
 enum { ALL_OF_IT = 0, SELECT = 1, FINISH = 2, NO_TOPS = 3 };
 template <class T, int THREADS, int PART>
-__global__ __launch_bounds__(THREADS) void k_answers(answer_args) {
+__global__ __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 4) void k_answers(answer_args) {
   constexpr int WAVES = THREADS / 64;
   constexpr bool TOPS = PART == ALL_OF_IT || PART == SELECT, FEW = THREADS >= 512;
   constexpr int HELD = THREADS == 64 ? 2 * MOST_HELD : MOST_HELD, AT_ONCE = FEW ? 6 : 4;  // items of a thread; rows of E that a wave multiplies at a time
@@ -814,9 +814,9 @@ __global__ __launch_bounds__(THREADS) void k_answers(answer_args) {
     float sum = 0.f, weighted = 0.f;
     auto add = [&](float x, float s, float w) {
       if (x != -INFINITY || s != 0.f) {
-        const float f = expf(x - from);
+        const float f = __builtin_amdgcn_exp2f(x - from);
         sum += s * f;
-        weighted += f * fmaf(fmaxf(x - from, -150.f), s, w);
+        weighted += f * fmaf(fmaxf(x - from, -200.f), s, w);
       }
     };
 #pragma unroll
@@ -838,7 +838,8 @@ __global__ __launch_bounds__(THREADS) void k_answers(answer_args) {
     }
     asm volatile("" ::"v"(touched));
     add(so_far.top, so_far.sum, so_far.weighted);
-    const float lse = logf(sum) + from;
+    constexpr float LOG_2 = 0.69314718055994531f;
+    const float lse = (log2f(sum) + from) * LOG_2;
     const bool sound = fabsf(lse) < INFINITY;
 
     // -- alternatives --
@@ -889,34 +890,56 @@ __global__ __launch_bounds__(THREADS) void k_answers(answer_args) {
           const unsigned k = w < p.piece ? key_of(z[w]) : 0u;
           return k > least ? k : 0u;
         };
-#pragma unroll 2
-        for (int g = wave; g < groups; g += WAVES) {
-          const int c = __popcll(__ballot(word_key(g * 64 + lane) != 0));
-          if (lane == 0) group_first[g] = c;
-        }
-        __syncthreads();
-        if (wave == 0) {
-          int all = 0;
-          for (int g0 = 0; g0 < groups; g0 += 64) {
-            const int c = g0 + lane < groups ? group_first[g0 + lane] : 0;
-            const int x = scan_lanes(c, 0, plus_of());
-            if (g0 + lane < groups) group_first[g0 + lane] = kept + all + x - c;
-            all += __builtin_amdgcn_readlane(x, 63);
+        int listed = kept;
+        for (int i = tid; i < kept; i += THREADS) list_key[i] = key_[0][i], list_word[i] = word_[0][i];
+        auto put = [&](int g, unsigned k, unsigned long long in, int from) {
+          const int to = from + __popcll(in & ((1ull << lane) - 1));
+          if (k != 0 && to < LIST) list_key[to] = k, list_word[to] = (int32_t)(p.word0 + place(g * 64 + lane));
+        };
+        if constexpr (WAVES == 1) {
+          // (eight reads on their way at a time: two 260 us for 8192 rows, 72 chunks each)
+          constexpr int READS = 8;
+#pragma unroll 1
+          for (int g0 = 0; g0 < groups; g0 += READS) {
+            unsigned k[READS];
+#pragma unroll
+            for (int t = 0; t < READS; t++) k[t] = word_key((g0 + t) * 64 + lane);
+#pragma unroll
+            for (int t = 0; t < READS; t++) {
+              const unsigned long long in = __ballot(k[t] != 0);
+              put(g0 + t, k[t], in, listed);
+              listed += __popcll(in);
+            }
           }
-          if (lane == 0) group_first[groups] = kept + all;
-        }
-        __syncthreads();
-        const int listed = group_first[groups];
-        int found;
-        if (listed <= LIST) {
-          for (int i = tid; i < kept; i += THREADS) list_key[i] = key_[0][i], list_word[i] = word_[0][i];
+        } else {
 #pragma unroll 2
           for (int g = wave; g < groups; g += WAVES) {
-            const unsigned k = word_key(g * 64 + lane);
-            const unsigned long long in = __ballot(k != 0);
-            const int to = group_first[g] + __popcll(in & ((1ull << lane) - 1));
-            if (k != 0) list_key[to] = k, list_word[to] = (int32_t)(p.word0 + place(g * 64 + lane));
+            const int c = __popcll(__ballot(word_key(g * 64 + lane) != 0));
+            if (lane == 0) group_first[g] = c;
           }
+          __syncthreads();
+          if (wave == 0) {
+            int all = 0;
+            for (int g0 = 0; g0 < groups; g0 += 64) {
+              const int c = g0 + lane < groups ? group_first[g0 + lane] : 0;
+              const int x = scan_lanes(c, 0, plus_of());
+              if (g0 + lane < groups) group_first[g0 + lane] = kept + all + x - c;
+              all += __builtin_amdgcn_readlane(x, 63);
+            }
+            if (lane == 0) group_first[groups] = kept + all;
+          }
+          __syncthreads();
+          listed = group_first[groups];
+          if (listed <= LIST) {
+#pragma unroll 2
+            for (int g = wave; g < groups; g += WAVES) {
+              const unsigned k = word_key(g * 64 + lane);
+              put(g, k, __ballot(k != 0), group_first[g]);
+            }
+          }
+        }
+        int found;
+        if (listed <= LIST) {
           __syncthreads();
           if (wave == 0) {
             picker<64, LIST / 64> items(wave_room);
@@ -965,7 +988,7 @@ __global__ __launch_bounds__(THREADS) void k_answers(answer_args) {
     }
     if (tid == 0) {
       if (p1.lse) p1.lse[m] = lse;
-      if (p1.entropy) p1.entropy[m] = sound ? logf(sum) - weighted / sum : __builtin_nanf("");
+      if (p1.entropy) p1.entropy[m] = sound ? (log2f(sum) - weighted / sum) * LOG_2 : __builtin_nanf("");
     }
     const T* x = (const T*)p1.X + m * p1.ldx;
     auto& p2 = arguments<answer_args>();
@@ -1254,12 +1277,11 @@ answer_room answer_room_of(int64_t rows, int64_t n_in, int64_t words, int n_give
 template <class T>
 int answers_forward(hipStream_t st, const char* me, const answer_args& to, char* ws, int64_t ws_bytes) {
   const int64_t words = to.words;
-  matrix all_x{to.X, to.ldx, to.rows, to.n_in, 1, 0, 0, nullptr}, e{to.E, to.lde, words, to.n_in, 1, 0, 0, nullptr};
+  matrix all_x{to.X, to.ldx, to.rows, to.n_in, 1, 0, 0, nullptr}, e{to.E, to.lde, words, to.n_in, 1, 0, 0, nullptr}, both[2];
   const answer_room r = answer_room_of<T>(to.rows, to.n_in, words, to.n_given, to.n_top, all_x, e);
   DN_TRY(check_room(me, r.all, ws, ws_bytes));
-  if (!r.few) DN_TRY(pack<T>(&e, 1, ws, st));
+  char* x_room = ws;  // (E behind it)
   ws += r.packs[1];
-  char* x_room = ws;
   auto take = [&](int64_t bytes) {
     char* at = ws;
     ws += bytes;
@@ -1288,7 +1310,12 @@ int answers_forward(hipStream_t st, const char* me, const answer_args& to, char*
     a.teacher = to.teacher ? to.teacher + m0 * to.n_given : nullptr;
     a.lse = to.lse ? to.lse + m0 : nullptr, a.entropy = to.entropy ? to.entropy + m0 : nullptr, a.loss = to.loss ? to.loss + m0 : nullptr;
     a.top_words = to.top_words ? to.top_words + m0 * to.n_top : nullptr, a.top_logp = to.top_logp ? to.top_logp + m0 * to.n_top : nullptr;
-    if (!r.few) DN_TRY(pack<T>(&x, 1, x_room, st));
+    if (!r.few) {
+      both[0] = x, both[1] = e;
+      DN_TRY(pack<T>(both, b == 0 ? 2 : 1, x_room, st));
+      x = both[0];
+      if (b == 0) e = both[1];
+    }
     if (r.stored) {
       const int64_t blocks = ceil_div(rows, 4);
       k_wanted<<<(unsigned)blocks, 256, 0, st>>>(rows, to.n_given, a.given, words, wanted, r.ld_wanted);
