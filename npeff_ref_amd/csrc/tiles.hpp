@@ -691,7 +691,7 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
 #pragma unroll
       for (int i = 0; i < FM; i++) {
         const int64_t m_i = m_wave + i * 16 + (lane & 15), m = m_i < m_end ? m_i : m_end - 1;
-        floors[i] = some ? p.floor[m] : INFINITY;
+        floors[i] = some ? p.floor[m] : __builtin_nanf("");  // (nothing reaches that, infinity included)
         wanted[i] = all_of && here ? 1u : flags ? p.wanted[m * p.ld_wanted + (chunk >> 5)] >> (chunk & 31) & 1u : 0u;
       }
     }

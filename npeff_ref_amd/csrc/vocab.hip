@@ -1330,7 +1330,7 @@ int answers_forward(hipStream_t st, const char* me, const answer_args& to, char*
       p.inv_heat = to.inv_heat;
       p.parts = parts, p.weighted = weighted;
       a.chunk = 64, a.chunks = ceil_div(n, 64);
-      p.logits = logits, p.ldl = padded(n);
+      if (r.logits > 0) p.logits = logits, p.ldl = padded(n);
       if (to.n_top > 0) p.tops = tops, p.chunks = a.chunks, p.floor = w0 > 0 ? a.floor : nullptr;
       if (r.stored) p.wanted = wanted, p.ld_wanted = r.ld_wanted, p.chunk0 = w0 / 64;
       if (r.few) {

@@ -3,7 +3,7 @@ words, with their gradients, against the formulas in 64 bits.
 
 A logit is a sum of n_in products in fp32: off by (n_in + 8) 2^-24 times the sum of their sizes, and by its own rounding; lse by twice the
 worst of a row's logits and the rounding of the exponentials and their sum (n_words + 64 operations).  A given word's logit is summed
-in 64 bits, so its logp is off as lse is, and rounded.  The entropy log s + sum p (max - z): logits off by d move it by at most
+in fp32 too: of the two logit errors in lse's bound one is its own, and logp is rounded.  The entropy log s + sum p (max - z): logits off by d move it by at most
 2 H d, exponentials off relatively by r by at most r (1 + log s + sum p (max - z)).  The order of the alternatives is that of 64 bits.
 dz = p (a + b log p) + listed: p is off relatively as exp(z - lse) is, a as the entropy; dz is rounded to the type, the products
 sum these errors over words or tokens, and are rounded once more."""
@@ -246,6 +246,35 @@ def test_large_tiles(rows, n_in, words, dt):
     check_distill(rows, n_in, words, dt, listed=20)
 
 
+@pytest.mark.parametrize("rows, n_in, words, listed, dt", [(1500, 256, 9001, 200, "bf16"), (1500, 255, 9001, 200, "f16"), (700, 515, 3000, 100, "f32")])
+def test_long_lists_come_from_the_tiles(rows, n_in, words, listed, dt):
+    """Lists whose rows of E are more than 128 MB: their logits are the tiles' own."""
+    check_distill(rows, n_in, words, dt, listed=listed)
+    check_probs(rows, n_in, words, dt, given=listed, top=20, heat=1.3)
+
+
+def test_long_lists_and_pieces_of_the_vocabulary():
+    """Both, where the logits of all words would be more than 2 GB: three pieces."""
+    rows, n_in, words, listed = 60_000, 128, 20_001, 10
+    X, E = rand((rows, n_in), "bf16", 1), rand((words, n_in), "bf16", 2, 0.2)
+    w, logits = teacher_of(rows, listed, words, 3)
+    loss, logp, lse, top_words, top_logp = empty(rows), empty(rows, listed), empty(rows), empty(rows, 9, dtype=torch.int32), empty(rows, 9)
+    d.op_vocab_distill(X, E, w, logits, loss=loss, logp=logp, lse=lse, temperature=1.2)
+    again, entropy = empty(rows, listed), empty(rows)
+    d.op_vocab_probs(X, E, w, logp=again, entropy=entropy, top_words=top_words, top_logp=top_logp, temperature=1.2)
+    assert torch.equal(again, logp)
+    q = torch.softmax(torch.where((w >= 0) & (logits > -float("inf")), logits.double(), -1e30) / 1.2, 1) * ((w >= 0) & (logits > -float("inf")))
+    want = (torch.special.xlogy(q, q) - q * logp.double()).sum(1)
+    assert ((loss - want).abs() <= 128 * EPS32 * (1 + (q * logp.abs()).sum(1))).all()
+    for i in range(0, rows, 6000):
+        at = slice(i, i + 6000)
+        x = Exact(X[at], E, 1.2)
+        near(lse[at], x.lse, x.off, "lse")
+        near(logp[at], x.logp(w[at]), x.logp_off(w[at]), "logp")
+        near(entropy[at], x.entropy, x.off_entropy, "entropy")
+        check_tops(x, top_words[at], top_logp[at], 9)
+
+
 def test_the_list_is_at_most_4096_long():
     check_distill(3, 16, 5000, "f32", listed=4096)
 
@@ -268,6 +297,20 @@ def test_ties_go_to_the_lower_word(rows):
     E[:] = -0.0
     d.op_vocab_probs(X, E, top_words=top_words, top_logp=top_logp)
     assert (top_words.cpu() == torch.arange(30, dtype=torch.int32)).all()
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+def test_ties_in_large_tiles_and_the_rest(dt):
+    """Words that are alike on both sides of the border between tiles of both sizes, and more of them than there are places."""
+    rows, words = 1000, 17_001
+    X, E = rand((rows, 264), dt, 1), rand((words, 264), dt, 2, 0.05)
+    E[torch.arange(100, words, 450, device="cuda")] = rand((1, 264), dt, 3, 0.3)
+    top_words, top_logp = empty(rows, 20, dtype=torch.int32), empty(rows, 20)
+    d.op_vocab_probs(X, E, top_words=top_words, top_logp=top_logp)
+    z = X.double() @ E.double().T
+    z = torch.where(torch.arange(words, device="cuda") % 450 == 100, z[:, 100:101], z)  # (equal, also where a library's sums are not)
+    v, at = z.sort(dim=1, descending=True, stable=True)
+    assert torch.equal(top_words, at[:, :20].to(torch.int32))
 
 
 @pytest.mark.parametrize("dt", list(DTYPES))
@@ -434,6 +477,29 @@ def test_rows_that_are_not_numbers(rows, dt):
         outs.append({k: torch.cat([v[:1], v[2:]]) for k, v in o.items()})
     for other in outs[1:]:
         assert all(torch.equal(other[k], v) for k, v in outs[0].items())
+
+
+@pytest.mark.parametrize("rows, given", [(4, 2), (70, 2), (1500, 2), (600, 1500)])
+@pytest.mark.parametrize("top", [0, 5])
+def test_logits_of_infinity_write_nothing_past_the_workspace(rows, given, top):
+    """A row whose logits are all infinite, with and without alternatives, lists short and long: the other rows and what lies around
+    the workspace stay as they are."""
+    X, E, w = rand((rows, 80), "bf16", 1), rand((3000, 80), "bf16", 2, 0.3), words_of(rows, given, 3000, 3, masked=0.0)
+    E[:, 7] = E[:, 7].abs() + 0.1
+    size = d.vocab_probs_workspace(rows, 80, 3000, given, top, torch.bfloat16, True)[0]
+    outs = []
+    for big in (0.5, float("inf")):
+        X[1, 7] = big
+        buf = torch.full((size + (64 << 20),), 123, dtype=torch.uint8, device="cuda")
+        o = dict(logp=empty(rows, given), lse=empty(rows), entropy=empty(rows))
+        if top:
+            o.update(top_words=empty(rows, top, dtype=torch.int32), top_logp=empty(rows, top))
+        d.op_vocab_probs(X, E, w, workspace=buf[:size], **o)
+        assert (buf[size:] == 123).all()
+        if big > 1:
+            assert not torch.isfinite(o["lse"][1])
+        outs.append({k: torch.cat([v[:1], v[2:]]) for k, v in o.items()})
+    assert all(torch.equal(v, outs[1][k]) for k, v in outs[0].items())
 
 
 @pytest.mark.parametrize("rows", [4, 70])
