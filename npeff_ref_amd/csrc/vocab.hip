@@ -423,6 +423,7 @@ constexpr int MOST_TOP = 128, SPARE = 8, MOST_KEEP = MOST_TOP + SPARE;
 constexpr int MOST_LISTED = 4096;
 constexpr int64_t BLOCK_ROWS = 65536;                 // rows at a time, for the workspace's sake
 constexpr int64_t LOGIT_BYTES = (int64_t)2 << 30;  // of a piece's logits
+constexpr int64_t WHOLE_BYTES = (int64_t)128 << 20;
 // Given words' logits: rows of E read again and multiplied in 64 bits, or, where that would be so many bytes, taken from the tiles (us
 // there and here: 20 words of 2000 rows of 1024, 82 MB, 904 and 924 with the gradients; 100 of 1999 of 1030, 412 MB, 420 and 340).
 constexpr int64_t STORED_FROM = (int64_t)128 << 20;
@@ -742,7 +743,7 @@ __global__ __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 4) void k_answers(ans
   constexpr int WAVES = THREADS / 64;
   constexpr bool TOPS = PART == ALL_OF_IT || PART == SELECT, FEW = THREADS >= 512;
   constexpr int HELD = THREADS == 64 ? 2 * MOST_HELD : MOST_HELD, AT_ONCE = FEW ? 6 : 4;  // items of a thread; rows of E that a wave multiplies at a time
-  constexpr int LIST = 256, PARTS = 4;
+  constexpr int LIST = 512, PARTS = 4;
   __shared__ pick_room<THREADS> room;
   pick_room<64>& wave_room = *(pick_room<64>*)&room;
   __shared__ int chosen;
@@ -896,6 +897,26 @@ __global__ __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 4) void k_answers(ans
           const int to = from + __popcll(in & ((1ull << lane) - 1));
           if (k != 0 && to < LIST) list_key[to] = k, list_word[to] = (int32_t)(p.word0 + place(g * 64 + lane));
         };
+        if (WAVES == 1 && many == chunks.count && kept + in_chunks > LIST) {
+          // No chunk could be left out: the words in 256 parts, of whose maxima the KEEP largest are KEEP words.
+          unsigned most[4] = {0, 0, 0, 0};
+          for (int i = lane; i < kept; i += 64) most[0] = key_[0][i] > most[0] ? key_[0][i] : most[0];
+#pragma unroll 2
+          for (int g = 0; g < groups; g += 4)
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+              const unsigned k = word_key((g + t) * 64 + lane);
+              most[t] = k > most[t] ? k : most[t];
+            }
+          picker<64, 4> parts(wave_room);
+          parts.look(256, [&](int64_t) { return 0u; }, [&](int h) { return h == 0 ? most[0] : h == 1 ? most[1] : h == 2 ? most[2] : most[3]; });
+          if (parts.count >= p.keep) {
+            unsigned reach = 0xffffffffu;
+            parts.pick(p.keep, [&](int64_t) { return 0u; }, [&](int, int64_t, unsigned k) { reach = k < reach ? k : reach; });
+            reach = over_lanes(reach, 0xffffffffu, min_of());
+            least = reach - 1 > least ? reach - 1 : least;
+          }
+        }
         if constexpr (WAVES == 1) {
           // (eight reads on their way at a time: two 260 us for 8192 rows, 72 chunks each)
           constexpr int READS = 8;
@@ -1234,7 +1255,7 @@ __global__ __launch_bounds__(256) void k_wanted(int64_t rows, int many, const in
 struct answer_room {
   int64_t blocks, each;
   bool few, stored;
-  int64_t wanted, ld_wanted;
+  int64_t first, wanted, ld_wanted;  // first: words of the first piece (0: as of the others)
   int64_t packs[2] = {0, 0};  // of a block's X, of E
   int64_t piece, parts, weighted, state, tops, logits, kept, floor, logp, all;
   int keep;
@@ -1253,19 +1274,25 @@ answer_room answer_room_of(int64_t rows, int64_t n_in, int64_t words, int n_give
   r.keep = n_top > 0 ? (n_top + SPARE < words ? n_top + SPARE : (int)words) : 0;
   r.stored = !r.few && r.each * n_given * n_in * (int64_t)sizeof(T) >= STORED_FROM;
   const bool logits = n_top > 0 || r.stored;
-  r.piece = words;
+  r.piece = words, r.first = 0;
   if (logits) {
     int64_t most = LOGIT_BYTES / (4 * r.each) / 256 * 256;
     if (most < 1024) most = 1024;
-    if (most < words) r.piece = ceil_div(ceil_div(words, ceil_div(words, most)), 256) * 256;
+    // A first piece small enough that storing all of it costs little, and large enough to know a floor for the others from (us with and without: 2000
+    // rows of 50001 words with 20 alternatives 302 and 319, 8192 of 131072 with 64 7531 and 7695, 600 of 128000 with 5 270 and 299).
+    const int64_t few_words = ceil_div((int64_t)r.keep * 96, 2048) * 2048;
+    if (n_top > 0 && !r.few && 4 * r.each * words > WHOLE_BYTES && 6 * few_words <= words) r.first = few_words < most ? few_words : most;
+    const int64_t rest = words - r.first;
+    if (most < rest) r.piece = ceil_div(ceil_div(rest, ceil_div(rest, most)), 256) * 256;
+    else if (rest > 0) r.piece = rest;
   }
   r.ld_wanted = r.stored ? ceil_div(words, 2048) : 0;
   r.wanted = round256(r.each * r.ld_wanted * 4);
-  r.parts = round256(r.each * ceil_div(r.piece, r.few ? 16 : 128) * 8);
-  r.weighted = round256(r.each * ceil_div(r.piece, r.few ? 16 : 128) * 4);
+  r.parts = round256(r.each * ceil_div(r.piece > r.first ? r.piece : r.first, r.few ? 16 : 128) * 8);
+  r.weighted = round256(r.each * ceil_div(r.piece > r.first ? r.piece : r.first, r.few ? 16 : 128) * 4);
   r.state = logits ? round256(r.each * (int64_t)sizeof(running)) : 0;
-  r.tops = n_top > 0 ? round256(r.each * ceil_div(r.piece, r.few ? 16 : 64) * 4) : 0;
-  r.logits = logits ? round256(r.each * padded(r.piece) * 4) : 0;
+  r.tops = n_top > 0 ? round256(r.each * ceil_div(r.piece > r.first ? r.piece : r.first, r.few ? 16 : 64) * 4) : 0;
+  r.logits = logits ? round256(r.each * padded(r.piece > r.first ? r.piece : r.first) * 4) : 0;
   r.kept = round256(r.each * r.keep * 4);
   r.floor = n_top > 0 ? round256(r.each * 4) : 0;
   r.logp = round256(r.each * (int64_t)n_given * 4);
@@ -1321,8 +1348,9 @@ int answers_forward(hipStream_t st, const char* me, const answer_args& to, char*
       k_wanted<<<(unsigned)blocks, 256, 0, st>>>(rows, to.n_given, a.given, words, wanted, r.ld_wanted);
       DN_LAUNCH_CHECK();
     }
-    for (int64_t w0 = 0; w0 < words; w0 += r.piece) {
-      const int64_t n = words - w0 < r.piece ? words - w0 : r.piece;
+    for (int64_t w0 = 0, n; w0 < words; w0 += n) {
+      n = w0 == 0 && r.first > 0 ? r.first : r.piece;
+      if (n > words - w0) n = words - w0;
       args p{};
       p.A = x.p, p.lda = x.ld, p.a_plane = x.plane, p.b_plane = e.plane, p.ldb = e.ld;
       p.M = rows, p.N = n, p.K = to.n_in;

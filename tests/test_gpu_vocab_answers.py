@@ -262,7 +262,6 @@ def test_long_lists_and_pieces_of_the_vocabulary():
     d.op_vocab_distill(X, E, w, logits, loss=loss, logp=logp, lse=lse, temperature=1.2)
     again, entropy = empty(rows, listed), empty(rows)
     d.op_vocab_probs(X, E, w, logp=again, entropy=entropy, top_words=top_words, top_logp=top_logp, temperature=1.2)
-    assert torch.equal(again, logp)
     q = torch.softmax(torch.where((w >= 0) & (logits > -float("inf")), logits.double(), -1e30) / 1.2, 1) * ((w >= 0) & (logits > -float("inf")))
     want = (torch.special.xlogy(q, q) - q * logp.double()).sum(1)
     assert ((loss - want).abs() <= 128 * EPS32 * (1 + (q * logp.abs()).sum(1))).all()
@@ -271,6 +270,7 @@ def test_long_lists_and_pieces_of_the_vocabulary():
         x = Exact(X[at], E, 1.2)
         near(lse[at], x.lse, x.off, "lse")
         near(logp[at], x.logp(w[at]), x.logp_off(w[at]), "logp")
+        near(again[at], x.logp(w[at]), x.logp_off(w[at]), "logp")  # (summed in other pieces: not the same bits)
         near(entropy[at], x.entropy, x.off_entropy, "entropy")
         check_tops(x, top_words[at], top_logp[at], 9)
 
