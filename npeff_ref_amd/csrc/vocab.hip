@@ -500,12 +500,13 @@ __device__ __forceinline__ V from_lane(V none, V v) {
   for (unsigned t = 0; t < sizeof(V) / 4; t++) a.i[t] = __builtin_amdgcn_update_dpp(a.i[t], b.i[t], CONTROL, ROWS, 0xf, false);
   return a.v;
 }
-template <class V, class Op>
+template <bool WAVE = true, class V, class Op>  // (else within rows of 16 lanes)
 __device__ __forceinline__ V scan_lanes(V v, V none, Op op) {
   v = op(from_lane<0x111, 0xf>(none, v), v);  // (the lane before, in rows of 16)
   v = op(from_lane<0x112, 0xf>(none, v), v);
   v = op(from_lane<0x114, 0xf>(none, v), v);
   v = op(from_lane<0x118, 0xf>(none, v), v);
+  if (!WAVE) return v;
   v = op(from_lane<0x142, 0xa>(none, v), v);  // (the last of the row before, to the second and fourth)
   v = op(from_lane<0x143, 0xc>(none, v), v);  // (lane 31, to the upper half)
   return v;
@@ -765,7 +766,7 @@ __global__ __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 4) void k_answers(ans
   __shared__ int32_t lead[MOST_KEEP];  // chunks
   __shared__ double exact_[MOST_KEEP];
   __shared__ float red[3][WAVES];
-  __shared__ double part_of[FEW ? WAVES : 1][FEW ? MOST_KEEP : 1];
+  __shared__ double part_of[FEW ? WAVES * 4 : 1][FEW ? MOST_KEEP : 1];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // Rows of E that are multiplied later, read ahead to the caches, and the row of X: a lane has a line.  (Each read of them from memory,
   // one after the other, would be 2 us.)
@@ -972,7 +973,25 @@ __global__ __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 4) void k_answers(ans
         int found;
         if (listed <= LIST) {
           __syncthreads();
-          if (wave == 0) {
+          if (FEW && listed <= THREADS) {
+            // each word's rank among them, and its place among those that stay (0.5 us where a wave's selection takes 2)
+            const unsigned k = tid < listed ? list_key[tid] : 0u;
+            int rank = 0, to = 0;
+#pragma unroll 4
+            for (int j = 0; j < listed; j++) rank += list_key[j] > k || (list_key[j] == k && j < tid);
+            const bool stays = tid < listed && rank < p.keep;
+            const unsigned long long in = __ballot(stays);
+            if (lane == 0) room.part[0][wave] = __popcll(in);
+            __syncthreads();
+            found = 0;
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) {
+              if (w < wave) to += (int)room.part[0][w];
+              found += (int)room.part[0][w];
+            }
+            to += __popcll(in & ((1ull << lane) - 1));
+            if (stays) key_[1][to] = k, word_[1][to] = list_word[tid];
+          } else if (wave == 0) {
             picker<64, LIST / 64> items(wave_room);
             auto item_key = [&](int64_t i) { return list_key[i]; };
             items.look(listed, item_key, [&](int h) { return list_key[h * 64 + lane]; });
@@ -980,8 +999,10 @@ __global__ __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 4) void k_answers(ans
             items.pick(found, item_key, [&](int to, int64_t i, unsigned k) { key_[1][to] = k, word_[1][to] = list_word[i]; });
             if (lane == 0) chosen = found;
           }
-          __syncthreads();
-          found = chosen;
+          if (!(FEW && listed <= THREADS)) {
+            __syncthreads();
+            found = chosen;
+          }
         } else {
           picker<THREADS, HELD> items(room);
           auto item_key = [&](int64_t i) { return i < kept ? key_[0][i] : word_key((int)i - kept); };
@@ -1047,14 +1068,14 @@ __global__ __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 4) void k_answers(ans
           if (any) {
             dot_rows<T, AT_ONCE, S>(x, e, p2.n_in, FEW ? tid & (share * 64 - 1) : lane, share * 64, s);
 #pragma unroll
-            for (int c = 0; c < AT_ONCE; c++) s[c] = scan_lanes(s[c], zero, plus_of());
+            for (int c = 0; c < AT_ONCE; c++) s[c] = scan_lanes<!FEW>(s[c], zero, plus_of());
           }
-          if (lane == 63) {
+          if (FEW ? lane % 16 == 15 : lane == 63) {
 #pragma unroll
             for (int c = 0; c < AT_ONCE; c++)
               if (i + c < there) {
                 if (FEW)
-                  part_of[wave % share][i + c] = s[c];
+                  part_of[wave % share * 4 + lane / 16][i + c] = s[c];
                 else
                   put(i0 + i + c, s[c]);
               }
@@ -1065,24 +1086,32 @@ __global__ __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 4) void k_answers(ans
           for (int i = tid; i < there; i += THREADS) {
             S s = 0;
 #pragma unroll
-            for (int w = 0; w < WAVES; w++) s += w < share ? (S)part_of[w][i] : zero;
+            for (int w = 0; w < WAVES * 4; w++) s += w < share * 4 ? (S)part_of[w][i] : zero;
             put(i0 + i, s);
           }
           __syncthreads();
         }
       }
     };
+    auto given_word = [&](int j) { return p2.given[m * p2.n_given + j]; };
+    auto put_given = [&](int j, double s) {
+      const int32_t w = given_word(j);
+      p2.logp[m * p2.n_given + j] = w < 0 ? 0.f : w >= p2.words ? __builtin_nanf("") : (float)(s * (double)p2.inv_heat - (double)lse);
+    };
+    // (a few given words go with the leading ones: a turn of them takes 2 us)
+    const bool together = FEW && kept > 0 && p2.n_given <= AT_ONCE;
     if (TOPS || PART == FINISH) {
-      auto word = [&](int i) { return word_[at][i]; };
+      auto word = [&](int i) { return i < kept ? word_[at][i] : given_word(i - kept); };
       const unsigned touched = FEW && kept > 0 ? touch(m, kept, word) : 0u;
       asm volatile("" ::"v"(touched));
-      products(0.0, kept, word, [&](int i, double s) { exact_[i] = s == s ? s : -(double)INFINITY; });
-    }
-    if (!p2.stored)
-      products(0.f, p2.n_given, [&](int j) { return p2.given[m * p2.n_given + j]; }, [&](int j, float s) {
-        const int32_t w = p2.given[m * p2.n_given + j];
-        p2.logp[m * p2.n_given + j] = w < 0 ? 0.f : w >= p2.words ? __builtin_nanf("") : s * p2.inv_heat - lse;
+      products(0.0, kept + (together && !p2.stored ? p2.n_given : 0), word, [&](int i, double s) {
+        if (i < kept)
+          exact_[i] = s == s ? s : -(double)INFINITY;
+        else
+          put_given(i - kept, s);
       });
+    }
+    if (!p2.stored && !together) products(0.f, p2.n_given, given_word, [&](int j, float s) { put_given(j, s); });
     if (p2.stored) {
       for (int j = tid; j < p2.n_given; j += THREADS) {  // (what this thread or an earlier launch has written)
         const int32_t w = p2.given[m * p2.n_given + j];
@@ -1115,20 +1144,17 @@ __global__ __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 4) void k_answers(ans
         bool odd = false;  // NaN or +infinity among them
         for (int j = lane; j < p2.n_given; j += 64)
           if (w[j] >= 0 && l[j] != -INFINITY) most = fmaxf(most, l[j]), odd |= !(l[j] < INFINITY) || w[j] >= p2.words;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) most = fmaxf(most, __shfl_xor(most, d, 64));
+        most = over_lanes(most, -INFINITY, max_of());
         for (int j = lane; j < p2.n_given; j += 64)
           if (w[j] >= 0 && l[j] > -INFINITY) all += expf((l[j] - most) * p2.inv_heat);
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d, 64);
+        all = over_lanes(all, 0.f, plus_of());
         const float log_all = logf(all);
         for (int j = lane; j < p2.n_given; j += 64)
           if (w[j] >= 0 && l[j] > -INFINITY) {
             const float log_q = (l[j] - most) * p2.inv_heat - log_all, q = expf(log_q);
             if (q != 0.f) loss += q * (log_q - logp[j]);
           }
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) loss += __shfl_xor(loss, d, 64);
+        loss = over_lanes(loss, 0.f, plus_of());
         const bool bad = __any(odd);
         if (lane == 0) p2.loss[m] = bad ? __builtin_nanf("") : most == -INFINITY ? 0.f : loss;
       }
