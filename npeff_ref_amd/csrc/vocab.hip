@@ -10,7 +10,7 @@
 //
 // The same of what a model answers, at a temperature T (z = X E^T / T): log p of given words, the entropy, the likeliest
 // words; and of a student that learns from a teacher's likeliest words (answers, further down).
-#include "tiles.hpp"
+#include "planes.hpp"
 
 using namespace dn;
 using namespace dn::tl;
@@ -223,7 +223,16 @@ struct loss_room {  // of the forward pass
     all = packs + parts + round256(rows * 4);
   }
 };
+// The answers' fp32 products of few tiles go through planes.hpp.  (Those of the loss keep the order of their sums.)
 template <class T>
+constexpr bool may_be_planes(int epilogue) {
+  return sizeof(T) == 4 && (epilogue == E_PROBS || epilogue == E_PROBS_GRAD);
+}
+template <class T, int EPILOGUE>
+int64_t floats_of(int64_t M, int64_t N, int64_t K) {
+  return may_be_planes<T>(EPILOGUE) && better_in_planes(M, N, true) ? plane_split_floats(M, N, K) : split_floats<T>(M, N, K);
+}
+template <class T, int EPILOGUE>
 struct grad_room {
   int64_t packs = 0, piece, g, sums, parts, all;
   matrix m[2];
@@ -246,7 +255,7 @@ struct grad_room {
     const int64_t last = words - (ceil_div(words, piece) - 1) * piece;
     parts = 0;
     for (int64_t n : {piece, last})
-      for (int64_t f : {split_floats<T>(rows, n_in, n), split_floats<T>(n, n_in, rows)})
+      for (int64_t f : {floats_of<T, EPILOGUE>(rows, n_in, n), floats_of<T, EPILOGUE>(n, n_in, rows)})
         if (round256(4 * f) > parts) parts = round256(4 * f);
     all = 256 + packs + g + sums + parts;
   }
@@ -340,6 +349,14 @@ int few_backward(hipStream_t st, const args& logits, const spots& own, char* g, 
   DN_LAUNCH_CHECK();
   return 0;
 }
+// A product of a pass whose logits end in EPILOGUE.
+template <class T, bool A_ROWS, bool B_ROWS, int E, int EPILOGUE>
+int launch_either(const args& p, float* parts, hipStream_t st, int* parts_n = nullptr) {
+  if constexpr (may_be_planes<T>(EPILOGUE)) {
+    if (better_in_planes(p.M, p.N, E == E_STORE)) return launch_planes<A_ROWS, B_ROWS, E>(p, parts, st, parts_n);
+  }
+  return launch_product<T, A_ROWS, B_ROWS, E>(p, parts, st, parts_n);
+}
 // of: what the epilogue of the logits (EPILOGUE) takes of the rows; labels: rows of a negative one have no gradient; dloss: the
 // rows' weights, which k_shrink brings to the range of the type.
 template <class T, int EPILOGUE>
@@ -348,7 +365,7 @@ int loss_backward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, con
                   const char* me) {
   const int32_t* labels = of.labels;
   const float* dloss = of.dloss;
-  grad_room<T> r(rows, n_in, words, X, ldx, E, lde, dE ? labels : nullptr);
+  grad_room<T, EPILOGUE> r(rows, n_in, words, X, ldx, E, lde, dE ? labels : nullptr);
   DN_TRY(check_room(me, r.all, ws, ws_bytes));
   if (back_is_few<T>(rows, n_in)) {
     if (!dX && !dE) return 0;
@@ -382,7 +399,7 @@ int loss_backward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, con
     p.mode = ONE;
     p.shrink = shrink, p.word0 = w0, p.words = words;
     p.out = g, p.ldc = padded(n);
-    DN_TRY((launch_product<T, true, true, EPILOGUE>(p, nullptr, st)));
+    DN_TRY((launch_either<T, true, true, EPILOGUE, EPILOGUE>(p, nullptr, st)));
     if constexpr (EPILOGUE == E_PROBS_GRAD) DN_TRY((put_spots<T, false>(own, w0, n, shrink, g, p.ldc, p.M * p.ldc, st)));
     if (dX) {
       args q{};
@@ -393,7 +410,7 @@ int loss_backward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, con
       q.sums = first && last ? nullptr : sums, q.add_sums = !first;
       q.ldc = ceil_div(n_in, 4) * 4;
       if (last) q.out = dX, q.ldo = lddx, q.scale = grow;
-      DN_TRY((launch_product<T, true, false, E_STORE>(q, parts, st)));
+      DN_TRY((launch_either<T, true, false, E_STORE, EPILOGUE>(q, parts, st)));
     }
     if (dE) {
       args q{};
@@ -403,7 +420,7 @@ int loss_backward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, con
       q.mode = ONE;
       T* to = (T*)dE + w0 * ldde;
       q.out = to, q.ldo = ldde, q.scale = grow;
-      DN_TRY((launch_product<T, false, false, E_STORE>(q, parts, st)));
+      DN_TRY((launch_either<T, false, false, E_STORE, EPILOGUE>(q, parts, st)));
     }
   }
   return 0;
@@ -1403,7 +1420,7 @@ int answers_forward(hipStream_t st, const char* me, const answer_args& to, char*
         a.chunks = ceil_div(n, a.chunk);
       } else {
         p.B = (const typename num<T>::op*)e.p + w0 * e.ld;
-        DN_TRY((launch_product<T, true, true, E_PROBS>(p, nullptr, st, &a.parts_n)));
+        DN_TRY((launch_either<T, true, true, E_PROBS, E_PROBS>(p, nullptr, st, &a.parts_n)));
       }
       a.first = w0 == 0, a.last = w0 + n == words, a.word0 = w0, a.piece = n, a.ldl = padded(n);
       // us of a row in 512 threads and in fewer: 64 rows of 32000 words with 20 alternatives 38 and 54 (two launches), 512 rows 75 and 77
@@ -1435,7 +1452,7 @@ template <class T>
 int answers_backward(hipStream_t st, const char* me, slope_args s, int64_t n_in, const void* X, int64_t ldx, const void* E, int64_t lde,
                      void* dX, int64_t lddx, void* dE, int64_t ldde, char* ws, int64_t ws_bytes) {
   const slope_room own(s.rows, s.many);
-  const grad_room<T> r(s.rows, n_in, s.words, X, ldx, E, lde, (const int32_t*)ws);
+  const grad_room<T, E_PROBS_GRAD> r(s.rows, n_in, s.words, X, ldx, E, lde, (const int32_t*)ws);
   DN_TRY(check_room(me, own.all + r.all, ws, ws_bytes));
   s.slopes = (slope_row*)ws;
   s.alive = (int32_t*)(ws + own.slopes);
@@ -1475,7 +1492,7 @@ DN_API int dnpeff_vocab_loss_workspace(int type, int64_t rows, int64_t n_in, int
   DN_TRY(check_head("dnpeff_vocab_loss_workspace", type, rows, n_in, n_words));
   const void* p = (const void*)(uintptr_t)(aligned ? 16 : 1);
   if (forward_bytes) *forward_bytes = DN_BY_TYPE(type, (loss_room<T>(rows, n_in, n_words, p, n_in, p, n_in).all));
-  if (backward_bytes) *backward_bytes = DN_BY_TYPE(type, (grad_room<T>(rows, n_in, n_words, p, n_in, p, n_in, (const int32_t*)p).all));
+  if (backward_bytes) *backward_bytes = DN_BY_TYPE(type, (grad_room<T, E_LOSS_GRAD>(rows, n_in, n_words, p, n_in, p, n_in, (const int32_t*)p).all));
   return 0;
 }
 
@@ -1522,7 +1539,7 @@ DN_API int dnpeff_vocab_probs_workspace(int type, int64_t rows, int64_t n_in, in
   const matrix x{p, n_in, rows, n_in, 1, 0, 0, nullptr}, e{p, n_in, n_words, n_in, 1, 0, 0, nullptr};
   if (forward_bytes) *forward_bytes = rows == 0 ? 0 : DN_BY_TYPE(type, (answer_room_of<T>(rows, n_in, n_words, n_given, n_top, x, e).all));
   if (backward_bytes)
-    *backward_bytes = slope_room(rows, n_given).all + DN_BY_TYPE(type, (grad_room<T>(rows, n_in, n_words, p, n_in, p, n_in, (const int32_t*)p).all));
+    *backward_bytes = slope_room(rows, n_given).all + DN_BY_TYPE(type, (grad_room<T, E_PROBS_GRAD>(rows, n_in, n_words, p, n_in, p, n_in, (const int32_t*)p).all));
   return 0;
 }
 

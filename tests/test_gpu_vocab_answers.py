@@ -246,6 +246,14 @@ def test_large_tiles(rows, n_in, words, dt):
     check_distill(rows, n_in, words, dt, listed=20)
 
 
+# Tiles of 128 x 128: reductions of one stage of 32 up to seven, split and whole, of the logits and of both gradients; full rounds of 256 and more.
+@pytest.mark.parametrize("rows, n_in, words", [(60, 1, 700), (60, 32, 129), (60, 33, 127), (129, 65, 300), (127, 97, 500), (200, 150, 64), (200, 224, 33), (250, 515, 9000),
+                                               (1000, 515, 4000), (1025, 130, 4000), (1500, 72, 9001)])
+def test_products_of_fp32(rows, n_in, words):
+    check_probs(rows, n_in, words, "f32")
+    check_distill(rows, n_in, words, "f32")
+
+
 @pytest.mark.parametrize("rows, n_in, words, listed, dt", [(1500, 256, 9001, 200, "bf16"), (1500, 255, 9001, 200, "f16"), (700, 515, 3000, 100, "f32")])
 def test_long_lists_come_from_the_tiles(rows, n_in, words, listed, dt):
     """Lists whose rows of E are more than 128 MB: their logits are the tiles' own."""
