@@ -684,8 +684,8 @@ struct picker {
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           if (before < left && before + own[e] >= left) {
-            const unsigned l = lo + ((unsigned)(255 - 4 * lane - e) << shift), h = l + ((1u << shift) - 1);
-            r.low = l, r.high = h < hi ? h : hi, r.left = left - before;
+            const unsigned l = lo + ((unsigned)(255 - 4 * lane - e) << shift), span = (1u << shift) - 1;
+            r.low = l, r.high = span < hi - l ? l + span : hi, r.left = left - before;  // (l + span may pass 32 bits)
             r.done = shift == 0 || own[e] == left - before;
           }
           before += own[e];

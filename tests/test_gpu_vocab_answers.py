@@ -510,6 +510,26 @@ def test_logits_of_infinity_write_nothing_past_the_workspace(rows, given, top):
     assert all(torch.equal(v, outs[1][k]) for k, v in outs[0].items())
 
 
+@pytest.mark.parametrize("rows", [3, 70, 600])
+@pytest.mark.parametrize("words, top", [(700, 128), (8000, 128), (8000, 5), (120, 3)])
+@pytest.mark.parametrize("dt", list(DTYPES))
+def test_infinities_of_both_signs(rows, words, top, dt):
+    """A row of which half the logits are infinity and half minus infinity, and one of minus infinity and NaN: where more of the former are
+    there than are wanted, the range of what is looked at ends with the last number that there is."""
+    X, E = rand((rows, 64), dt, 1), rand((words, 64), dt, 2, 0.3)
+    w = words_of(rows, 2, words, 3, masked=0.0)
+    outs = []
+    for bad in (0.5, float("inf")):
+        X[1:3] = 0
+        X[1, 3], X[2, 5], X[2, 6] = bad, bad, bad if dt == "f32" else -bad
+        o = dict(logp=empty(rows, 2), lse=empty(rows), entropy=empty(rows), top_words=empty(rows, top, dtype=torch.int32), top_logp=empty(rows, top))
+        d.op_vocab_probs(X, E, w, **o)
+        if bad > 1:
+            assert (o["top_words"][1:3] == -1).all() and o["top_logp"][1:3].isnan().all() and o["entropy"][1:3].isnan().all()
+        outs.append({k: torch.cat([v[:1], v[3:]]) for k, v in o.items()})
+    assert all(torch.equal(v, outs[1][k]) for k, v in outs[0].items())
+
+
 @pytest.mark.parametrize("rows", [4, 70])
 def test_a_word_that_is_minus_infinity(rows):
     """A word with probability 0: it counts nowhere."""
