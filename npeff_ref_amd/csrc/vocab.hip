@@ -444,7 +444,7 @@ int loss_backward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, con
 //
 // What bounds them: E of few rows (one token of 32000 words of 4096 in bf16: 43 us at 6.2 TB/s, and 20 for the one workgroup that
 // selects and orders, which waits for memory); the matrix cores of many.  8192 tokens of 131072 words of 4096 in bf16 with 64
-// alternatives: products 6.8 ms (1300 TFLOP/s), selection 0.25, 4.8 GB of E's rows read again for their order 0.74 (6.5 TB/s).
+// alternatives: products 6.8 ms (1300 TFLOP/s), selection 0.43, 4.8 GB of E's rows read again for their order 0.74 (6.5 TB/s).
 constexpr int MOST_TOP = 128, SPARE = 8, MOST_KEEP = MOST_TOP + SPARE;
 constexpr int MOST_LISTED = 4096;
 constexpr int64_t BLOCK_ROWS = 65536;                 // rows at a time, for the workspace's sake
