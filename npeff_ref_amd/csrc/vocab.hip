@@ -914,11 +914,13 @@ __global__ __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 4) void k_answers(ans
         const float* z = p.logits + m * p.ldl;
         const int bits = p.chunk == 64 ? 6 : p.chunk == 32 ? 5 : 4, in_chunks = many << bits, groups = (in_chunks + 63) >> 6;
         auto place = [&](int i) { return ((int64_t)lead[i >> bits] << bits) + (i & (p.chunk - 1)); };
-        auto word_key = [&](int i) {
-          const int64_t w = i < in_chunks ? place(i) : p.piece;
-          const unsigned k = w < p.piece ? key_of(z[w]) : 0u;
+        // (read whether it is a word or not, so that several reads are on their way: of each behind a branch the wave would wait)
+        auto value = [&](int i) { return z[place(i < in_chunks ? i : 0)]; };
+        auto key_here = [&](int i, float v) {
+          const unsigned k = i < in_chunks && place(i) < p.piece ? key_of(v) : 0u;
           return k > least ? k : 0u;
         };
+        auto word_key = [&](int i) { return key_here(i, value(i)); };
         int listed = kept;
         for (int i = tid; i < kept; i += THREADS) list_key[i] = key_[0][i], list_word[i] = word_[0][i];
         auto put = [&](int g, unsigned k, unsigned long long in, int from) {
@@ -950,13 +952,14 @@ __global__ __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 4) void k_answers(ans
           constexpr int READS = 8;
 #pragma unroll 1
           for (int g0 = 0; g0 < groups; g0 += READS) {
-            unsigned k[READS];
+            float v[READS];
 #pragma unroll
-            for (int t = 0; t < READS; t++) k[t] = word_key((g0 + t) * 64 + lane);
+            for (int t = 0; t < READS; t++) v[t] = value((g0 + t) * 64 + lane);
 #pragma unroll
             for (int t = 0; t < READS; t++) {
-              const unsigned long long in = __ballot(k[t] != 0);
-              put(g0 + t, k[t], in, listed);
+              const unsigned k = key_here((g0 + t) * 64 + lane, v[t]);
+              const unsigned long long in = __ballot(k != 0);
+              put(g0 + t, k, in, listed);
               listed += __popcll(in);
             }
           }
