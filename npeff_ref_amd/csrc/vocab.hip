@@ -927,41 +927,51 @@ __global__ __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 4) void k_answers(ans
           const int to = from + __popcll(in & ((1ull << lane) - 1));
           if (k != 0 && to < LIST) list_key[to] = k, list_word[to] = (int32_t)(p.word0 + place(g * 64 + lane));
         };
-        if (WAVES == 1 && many == chunks.count && kept + in_chunks > LIST) {
-          // No chunk could be left out: the words in 256 parts, of whose maxima the KEEP largest are KEEP words.
-          unsigned most[4] = {0, 0, 0, 0};
-          for (int i = lane; i < kept; i += 64) most[0] = key_[0][i] > most[0] ? key_[0][i] : most[0];
-#pragma unroll 2
-          for (int g = 0; g < groups; g += 4)
-#pragma unroll
-            for (int t = 0; t < 4; t++) {
-              const unsigned k = word_key((g + t) * 64 + lane);
-              most[t] = k > most[t] ? k : most[t];
-            }
-          picker<64, 4> parts(wave_room);
-          parts.look(256, [&](int64_t) { return 0u; }, [&](int h) { return h == 0 ? most[0] : h == 1 ? most[1] : h == 2 ? most[2] : most[3]; });
-          if (parts.count >= p.keep) {
-            unsigned reach = 0xffffffffu;
-            parts.pick(p.keep, [&](int64_t) { return 0u; }, [&](int, int64_t, unsigned k) { reach = k < reach ? k : reach; });
-            reach = over_lanes(reach, 0xffffffffu, min_of());
-            least = reach - 1 > least ? reach - 1 : least;
-          }
-        }
         if constexpr (WAVES == 1) {
-          // (eight reads on their way at a time: two 260 us for 8192 rows, 72 chunks each)
-          constexpr int READS = 8;
+          // Where no chunk could be left out nothing but the row's list bounds the words: they are looked at in 256 parts, of whose maxima the KEEP
+          // largest are KEEP words, if there is no full list, or those above its end are too many.
+          const bool all_of_them = many == chunks.count && kept + in_chunks > LIST;
+          for (bool in_parts = all_of_them && kept < p.keep;; in_parts = true) {
+            if (in_parts) {
+              unsigned most[4] = {0, 0, 0, 0};
+              for (int i = lane; i < kept; i += 64) most[0] = key_[0][i] > most[0] ? key_[0][i] : most[0];
 #pragma unroll 1
-          for (int g0 = 0; g0 < groups; g0 += READS) {
-            float v[READS];
+              for (int g = 0; g < groups; g += 4) {
+                float v[4];
 #pragma unroll
-            for (int t = 0; t < READS; t++) v[t] = value((g0 + t) * 64 + lane);
+                for (int t = 0; t < 4; t++) v[t] = value((g + t) * 64 + lane);
 #pragma unroll
-            for (int t = 0; t < READS; t++) {
-              const unsigned k = key_here((g0 + t) * 64 + lane, v[t]);
-              const unsigned long long in = __ballot(k != 0);
-              put(g0 + t, k, in, listed);
-              listed += __popcll(in);
+                for (int t = 0; t < 4; t++) {
+                  const unsigned k = key_here((g + t) * 64 + lane, v[t]);
+                  most[t] = k > most[t] ? k : most[t];
+                }
+              }
+              picker<64, 4> parts(wave_room);
+              parts.look(256, [&](int64_t) { return 0u; }, [&](int h) { return h == 0 ? most[0] : h == 1 ? most[1] : h == 2 ? most[2] : most[3]; });
+              if (parts.count >= p.keep) {
+                unsigned reach = 0xffffffffu;
+                parts.pick(p.keep, [&](int64_t) { return 0u; }, [&](int, int64_t, unsigned k) { reach = k < reach ? k : reach; });
+                reach = over_lanes(reach, 0xffffffffu, min_of());
+                least = reach - 1 > least ? reach - 1 : least;
+              }
             }
+            // (eight reads on their way at a time: 72 chunks of each of 8192 rows 20 us; sixteen no less)
+            constexpr int READS = 8;
+            listed = kept;
+#pragma unroll 1
+            for (int g0 = 0; g0 < groups; g0 += READS) {
+              float v[READS];
+#pragma unroll
+              for (int t = 0; t < READS; t++) v[t] = value((g0 + t) * 64 + lane);
+#pragma unroll
+              for (int t = 0; t < READS; t++) {
+                const unsigned k = key_here((g0 + t) * 64 + lane, v[t]);
+                const unsigned long long in = __ballot(k != 0);
+                put(g0 + t, k, in, listed);
+                listed += __popcll(in);
+              }
+            }
+            if (in_parts || !all_of_them || listed <= LIST) break;
           }
         } else {
 #pragma unroll 2
