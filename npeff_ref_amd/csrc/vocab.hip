@@ -1170,20 +1170,32 @@ __global__ __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 4) void k_answers(ans
         const float* l = p2.teacher + m * p2.n_given;
         const int32_t* w = p2.given + m * p2.n_given;
         const float *logp = p2.logp + m * p2.n_given;
+        // (the first 64 are kept: asked for together, and once)
+        const bool here = lane < p2.n_given;
+        const int first = here ? lane : 0;
+        const int32_t w_first = w[first], w0 = here ? w_first : -1;
+        const float l0 = l[first], logp0 = logp[first];
+        auto each = [&](auto f) {
+          f(w0, l0, logp0);
+          for (int j = lane + 64; j < p2.n_given; j += 64) f(w[j], l[j], logp[j]);
+        };
         float most = -INFINITY, all = 0.f, loss = 0.f;
         bool odd = false;  // NaN or +infinity among them
-        for (int j = lane; j < p2.n_given; j += 64)
-          if (w[j] >= 0 && l[j] != -INFINITY) most = fmaxf(most, l[j]), odd |= !(l[j] < INFINITY) || w[j] >= p2.words;
+        each([&](int32_t w, float l, float) {
+          if (w >= 0 && l != -INFINITY) most = fmaxf(most, l), odd |= !(l < INFINITY) || w >= p2.words;
+        });
         most = over_lanes(most, -INFINITY, max_of());
-        for (int j = lane; j < p2.n_given; j += 64)
-          if (w[j] >= 0 && l[j] > -INFINITY) all += expf((l[j] - most) * p2.inv_heat);
+        each([&](int32_t w, float l, float) {
+          if (w >= 0 && l > -INFINITY) all += expf((l - most) * p2.inv_heat);
+        });
         all = over_lanes(all, 0.f, plus_of());
         const float log_all = logf(all);
-        for (int j = lane; j < p2.n_given; j += 64)
-          if (w[j] >= 0 && l[j] > -INFINITY) {
-            const float log_q = (l[j] - most) * p2.inv_heat - log_all, q = expf(log_q);
-            if (q != 0.f) loss += q * (log_q - logp[j]);
+        each([&](int32_t w, float l, float logp) {
+          if (w >= 0 && l > -INFINITY) {
+            const float log_q = (l - most) * p2.inv_heat - log_all, q = expf(log_q);
+            if (q != 0.f) loss += q * (log_q - logp);
           }
+        });
         loss = over_lanes(loss, 0.f, plus_of());
         const bool bad = __any(odd);
         if (lane == 0) p2.loss[m] = bad ? __builtin_nanf("") : most == -INFINITY ? 0.f : loss;
