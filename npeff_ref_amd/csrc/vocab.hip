@@ -52,13 +52,25 @@ __global__ __launch_bounds__(256) void k_join_loss(int64_t rows, int parts_n, co
   }
 }
 
+// Places of the logits' gradient that have values of their own (E_PROBS_GRAD): those of a row's listed words.
+struct spots {
+  int64_t rows;
+  int many;            // of a row
+  const int32_t* word; // [rows][many], negative: none
+  const float* g;
+};
 // 16-bit types: both[0] brings the largest |dloss| of a labelled token to 1 (fp16: to 2^14, so that g stays below the
 // type's largest value and probabilities down to 4e-9 above its subnormal ones), both[1] takes the results back.  With
 // equal weights, as of a mean, a label's g is then -1 but for p, and its rounding not the same for every token: left as
 // they come, weights of 1 / 2000 put gradients off by up to 2^-11 (fp16) or 2^-8 as a whole.
+// Where the largest g are known before (`own`) the scale is less by the one of eight factors down to 2^(-7/8) with which those, or 2048 of
+// them, round with the least error: a value a little above a power of two may be off by twice as much of itself as one a little below, and
+// values of about one size can make up a batch (52 tokens with 44 listed words each in fp16: gradients off by 3.1e-4 of their norm
+// at the largest scale and 2.8e-4 at the best, where rounding them alone is 2.1e-4).
 template <class T>
-__global__ __launch_bounds__(1024) void k_shrink(int64_t rows, const int32_t* labels, const float* dloss, float* both) {
-  __shared__ float side[16];
+__global__ __launch_bounds__(1024) void k_shrink(int64_t rows, const int32_t* labels, const float* dloss, spots own, float* both) {
+  constexpr int SCALES = 8;
+  __shared__ float side[16], off_of[SCALES][16];
   float most = 0.f;
   for (int64_t i = threadIdx.x; i < rows; i += 1024) {
     const float a = fabsf(dloss[i]);
@@ -68,10 +80,43 @@ __global__ __launch_bounds__(1024) void k_shrink(int64_t rows, const int32_t* la
   for (int d = 1; d < 64; d *= 2) most = fmaxf(most, __shfl_xor(most, d, 64));
   if (threadIdx.x % 64 == 0) side[threadIdx.x / 64] = most;
   __syncthreads();
+  for (int i = 0; i < 16; i++) most = fmaxf(most, side[i]);
+  float top = std::is_same<T, _Float16>::value ? 16384.f : 1.f;
+  most = most > 0.f ? fmaxf(most, top * 1e-36f) : 1.f;  // (top / most stays finite)
+  const int64_t all = own.rows * own.many, step = all <= 2048 ? 1 : all / 2048 | 1;
+  if (all > 0) {
+    float off[SCALES];  // sums of squares
+#pragma unroll
+    for (int k = 0; k < SCALES; k++) off[k] = 0.f;
+    for (int64_t i = threadIdx.x * step; i < all; i += 1024 * step) {
+      const float g = own.g[i], a = fabsf(g) * (top / most);
+      const int32_t w = own.word[i];  // (asked for together)
+      if (w < 0 || !(a < INFINITY)) continue;
+#pragma unroll
+      for (int k = 0; k < SCALES; k++) {
+        const float v = a * exp2f(-0.125f * k), d = (v - (float)(T)v) * exp2f(0.125f * k);
+        off[k] = fmaf(d, d, off[k]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < SCALES; k++) {
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) off[k] += __shfl_xor(off[k], d, 64);
+      if (threadIdx.x % 64 == 0) off_of[k][threadIdx.x / 64] = off[k];
+    }
+    __syncthreads();
+  }
   if (threadIdx.x == 0) {
-    for (int i = 1; i < 16; i++) most = fmaxf(most, side[i]);
-    const float top = std::is_same<T, _Float16>::value ? 16384.f : 1.f;
-    most = most > 0.f ? fmaxf(most, top * 1e-36f) : 1.f;  // (top / most stays finite)
+    if (all > 0) {
+      float least = INFINITY;
+      int best = 0;
+      for (int k = 0; k < SCALES; k++) {
+        float sum = 0.f;
+        for (int i = 0; i < 16; i++) sum += off_of[k][i];
+        if (sum < least) least = sum, best = k;
+      }
+      top *= exp2f(-0.125f * best);
+    }
     both[0] = top / most;
     both[1] = most / top;
   }
@@ -292,13 +337,6 @@ int loss_forward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, cons
   return 0;
 }
 
-// Places of the logits' gradient that have values of their own (E_PROBS_GRAD): those of a row's listed words.
-struct spots {
-  int64_t rows;
-  int many;            // of a row
-  const int32_t* word; // [rows][many], negative: none
-  const float* g;
-};
 // They take the place of what the tiles (or FEW: k_few, [words][16]) left there.
 template <class T, bool FEW>
 __global__ __launch_bounds__(256) void k_spots(spots s, int64_t word0, int64_t words, const float* shrink, void* out, int64_t ldc, int64_t plane) {
@@ -384,7 +422,7 @@ int loss_backward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, con
   float* parts = r.parts ? (float*)(g + r.g + r.sums) : nullptr;
   const float *shrink = nullptr, *grow = nullptr;
   if constexpr (sizeof(T) == 2) {
-    k_shrink<T><<<1, 1024, 0, st>>>(rows, labels, dloss, both);
+    k_shrink<T><<<1, 1024, 0, st>>>(rows, labels, dloss, own, both);
     DN_LAUNCH_CHECK();
     shrink = both, grow = both + 1;
   }
@@ -444,7 +482,7 @@ int loss_backward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, con
 //
 // What bounds them: E of few rows (one token of 32000 words of 4096 in bf16: 43 us at 6.2 TB/s, and 20 for the one workgroup that
 // selects and orders, which waits for memory); the matrix cores of many.  8192 tokens of 131072 words of 4096 in bf16 with 64
-// alternatives: products 6.8 ms (1300 TFLOP/s), selection 0.43, 4.8 GB of E's rows read again for their order 0.74 (6.5 TB/s).
+// alternatives: products 6.8 ms (1300 TFLOP/s), selection 0.24, 4.8 GB of E's rows read again for their order 0.74 (6.5 TB/s).
 constexpr int MOST_TOP = 128, SPARE = 8, MOST_KEEP = MOST_TOP + SPARE;
 constexpr int MOST_LISTED = 4096;
 constexpr int64_t BLOCK_ROWS = 65536;                 // rows at a time, for the workspace's sake
@@ -1357,7 +1395,7 @@ answer_room answer_room_of(int64_t rows, int64_t n_in, int64_t words, int n_give
     int64_t most = LOGIT_BYTES / (4 * r.each) / 256 * 256;
     if (most < 1024) most = 1024;
     // A first piece small enough that storing all of it costs little, and large enough to know a floor for the others from (us with and without: 2000
-    // rows of 50001 words with 20 alternatives 302 and 319, 8192 of 131072 with 64 7531 and 7695, 600 of 128000 with 5 270 and 299).
+    // rows of 50001 words with 20 alternatives 299 and 315, 8192 of 131072 with 64 7620 and 7770, 600 of 128000 with 5 276 and 299).
     const int64_t few_words = ceil_div((int64_t)r.keep * 96, 2048) * 2048;
     if (n_top > 0 && !r.few && 4 * r.each * words > WHOLE_BYTES && 6 * few_words <= words) r.first = few_words < most ? few_words : most;
     const int64_t rest = words - r.first;
