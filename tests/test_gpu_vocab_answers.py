@@ -654,16 +654,16 @@ def test_gradients_against_differences(rows):
                     assert abs(got[side][i, j].item() - slope) <= 1e-4 * max(1.0, abs(slope))
 
 
-@pytest.mark.parametrize("rows", [5, 300])
-def test_captured_and_replayed(rows):
+@pytest.mark.parametrize("rows, dt", [(5, "bf16"), (300, "bf16"), (700, "f16"), (300, "f32")])
+def test_captured_and_replayed(rows, dt):
     """A teacher's alternatives, a student's loss and its gradients in one graph; every replay against eager calls."""
-    X, S = rand((rows, 128), "bf16", 1), rand((rows, 128), "bf16", 2)
-    E = rand((9000, 128), "bf16", 3, 0.3)
+    X, S = rand((rows, 128), dt, 1), rand((rows, 128), dt, 2)
+    E = rand((9000, 128), dt, 3, 0.3)
     top = dict(top_words=empty(rows, 20, dtype=torch.int32), top_logp=empty(rows, 20))
     loss, logp, lse, one = empty(rows), empty(rows, 20), empty(rows), torch.ones(rows, device="cuda")
     dX, dE = torch.zeros_like(S), torch.zeros_like(E)
-    forward, _ = d.vocab_probs_workspace(rows, 128, 9000, 0, 20, torch.bfloat16)
-    both = max(forward, *d.vocab_probs_workspace(rows, 128, 9000, 20, 0, torch.bfloat16))
+    forward, _ = d.vocab_probs_workspace(rows, 128, 9000, 0, 20, DTYPES[dt])
+    both = max(forward, *d.vocab_probs_workspace(rows, 128, 9000, 20, 0, DTYPES[dt]))
     ws = torch.empty(both, dtype=torch.uint8, device="cuda")
 
     def step():
@@ -678,8 +678,8 @@ def test_captured_and_replayed(rows):
     with torch.cuda.graph(graph):
         out = step()
     for i in range(4):
-        X.copy_(rand((rows, 128), "bf16", 10 + i))
-        S.copy_(rand((rows, 128), "bf16", 20 + i))
+        X.copy_(rand((rows, 128), dt, 10 + i))
+        S.copy_(rand((rows, 128), dt, 20 + i))
         graph.replay()
         torch.cuda.synchronize()
         got = [t.clone() for t in out]
@@ -710,7 +710,8 @@ def test_another_stream_and_arrays_of_the_library():
 
 
 def test_a_workspace_as_large_as_asked_for_is_enough_and_all_that_is_written():
-    for rows, n_in, words, dt, n, k in ((3, 65, 900, "f32", 2, 7), (70, 72, 4001, "bf16", 3, 20), (40, 65, 3000, "f16", 1, 5), (1500, 72, 9001, "bf16", 2, 128)):
+    for rows, n_in, words, dt, n, k in ((3, 65, 900, "f32", 2, 7), (70, 72, 4001, "bf16", 3, 20), (40, 65, 3000, "f16", 1, 5), (1500, 72, 9001, "bf16", 2, 128),
+                                           (200, 515, 9000, "f32", 2, 5), (1025, 130, 4000, "f32", 2, 5)):
         X, E, w = rand((rows, n_in), dt, 1), rand((words, n_in), dt, 2, 0.3), words_of(rows, n, words, 3)
         logp, lse, entropy = empty(rows, n), empty(rows), empty(rows)
         for aligned in (False, True) if n_in % 8 == 0 else (False,):
