@@ -271,10 +271,10 @@ struct args {
   float* hit;               // [M] the label's logit
   int64_t word0, words;
   // E_PROBS, E_PROBS_GRAD
-  float inv_heat;           // logits are multiplied by it
-  float* weighted;          // [M][parts_n]: of each tile's words, sum of exp(z - max) (z - max); here and in parts z in units of log 2
-  float* tops;              // (or NULL) [M][chunks]: the largest logit of each chunk of words
-  float* logits;            // [M][ldl], ldl a multiple of 64: logits of the chunks that are stored: with tops those whose
+  float inv_heat;           // 1 / T: logits z are products times it.  What is stored of them and parts' maxima are the products
+  float* weighted;          // [M][parts_n]: of each tile's words, sum of exp(z - max) (z - max), the last z in units of log 2
+  float* tops;              // (or NULL) [M][chunks]: the largest of each chunk of words
+  float* logits;            // [M][ldl], ldl a multiple of 64: of the chunks that are stored: with tops those whose
   int64_t chunks, ldl;      // largest is not below the row's floor (NULL: all), and those that are wanted
   const float* floor;
   const unsigned* wanted;   // (or NULL) [M][ld_wanted]: a bit for each chunk, chunk0 the first of this piece
@@ -695,7 +695,9 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
         wanted[i] = all_of && here ? 1u : flags ? p.wanted[m * p.ld_wanted + (chunk >> 5)] >> (chunk & 31) & 1u : 0u;
       }
     }
-    const float inv_heat = E == E_PROBS ? p.inv_heat : 1.f, bits = inv_heat * LOG2_E;
+    // (The difference first: of products times `bits` a maximum would be rounded, by 128 and more from 2^31 on, and its exponential be
+    // 0 or infinite.  bits is finite.)
+    const float bits = (E == E_PROBS ? p.inv_heat : 1.f) * LOG2_E;
 #pragma unroll
     for (int i = 0; i < FM; i++) {
       const int64_t m = m_wave + i * 16 + (lane & 15);
@@ -726,8 +728,6 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
       }
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const float most = top;
-      if (E == E_PROBS) top *= bits;
       const float from = top == -INFINITY ? 0.f : top;
       float sum = 0.f, weighted = 0.f;
       if constexpr (E == E_LOSS) {
@@ -737,17 +737,17 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
           for (int e = 0; e < 4; e++) sum += __expf(acc[i][j][e] - from);
       } else {
         if (m < m_end) {
-          if (p.tops && q == 0 && n_wave < p.N) p.tops[m * p.chunks + (n_wave >> 6)] = most * inv_heat;
-          if (wanted[i] || (most * inv_heat >= floors[i] && n_wave < p.N)) {
+          if (p.tops && q == 0 && n_wave < p.N) p.tops[m * p.chunks + (n_wave >> 6)] = top;
+          if (wanted[i] || (top >= floors[i] && n_wave < p.N)) {
 #pragma unroll
-            for (int j = 0; j < FN; j++) __builtin_nontemporal_store(acc[i][j] * inv_heat, (v4f*)(p.logits + m * p.ldl + n_wave + j * 16 + q * 4));
+            for (int j = 0; j < FN; j++) __builtin_nontemporal_store(acc[i][j], (v4f*)(p.logits + m * p.ldl + n_wave + j * 16 + q * 4));
           }
         }
 #pragma unroll
         for (int j = 0; j < FN; j++)
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            const float z = fmaf(acc[i][j][e], bits, -from), x = __builtin_amdgcn_exp2f(z);
+            const float z = (acc[i][j][e] - from) * bits, x = __builtin_amdgcn_exp2f(z);
             sum += x;
             weighted = fmaf(x, fmaxf(z, -200.f), weighted);  // (x is 0 there)
           }
@@ -771,7 +771,7 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
 #pragma unroll
       for (int v = 0; v < WN; v++) {
         const float x = side[v * BM + m].x, y = side[v * BM + m].y;
-        if (x != -INFINITY || y != 0.f) sum += y * (E == E_PROBS ? __builtin_amdgcn_exp2f(x - from) : __expf(x - from));
+        if (x != -INFINITY || y != 0.f) sum += y * (E == E_PROBS ? __builtin_amdgcn_exp2f((x - from) * bits) : __expf(x - from));
       }
       const int64_t to = (w.m0 + m) * p.parts_n + p.part0 + w.tn;
       p.parts[to] = float2{top, sum};
@@ -780,7 +780,8 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
 #pragma unroll
         for (int v = 0; v < WN; v++) {
           const float x = side[v * BM + m].x, y = side[v * BM + m].y;
-          if (x != -INFINITY || y != 0.f) weighted += __builtin_amdgcn_exp2f(x - from) * fmaf(fmaxf(x - from, -200.f), y, side_w[v * BM + m]);
+          const float z = (x - from) * bits;
+          if (x != -INFINITY || y != 0.f) weighted += __builtin_amdgcn_exp2f(z) * fmaf(fmaxf(z, -200.f), y, side_w[v * BM + m]);
         }
         p.weighted[to] = weighted;
       }
@@ -1124,6 +1125,7 @@ __global__ __launch_bounds__(512, 2) void k_few(args p, int parts) {
             }
         }
       } else {
+        const float bits = (E == E_PROBS ? p.inv_heat : 1.f) * LOG2_E;  // (as in finish_tile)
         if (part == 0) {
           const int64_t label = E == E_LOSS && m < m_end ? (int64_t)p.labels[m] : -1;
           float top = -INFINITY, sum = 0.f, weighted = 0.f;
@@ -1137,16 +1139,14 @@ __global__ __launch_bounds__(512, 2) void k_few(args p, int parts) {
             }
           top = fmaxf(top, __shfl_xor(top, 16, 64));
           top = fmaxf(top, __shfl_xor(top, 32, 64));
-          const float inv_heat = E == E_PROBS ? p.inv_heat : 1.f, bits = inv_heat * LOG2_E, most = top;
-          if (E == E_PROBS) top *= bits;
           const float from = top == -INFINITY ? 0.f : top;
           if constexpr (E == E_PROBS) {
             if (p.tops && m < m_end && n0 < p.N) {  // (a chunk is a wave's columns)
-              if (q == 0) p.tops[m * p.chunks + n0 / (16 * COLS)] = most * inv_heat;
+              if (q == 0) p.tops[m * p.chunks + n0 / (16 * COLS)] = top;
 #pragma unroll
               for (int h = 0; h < COLS; h++) {
                 const int64_t n = n0 + h * 16 + q * 4;
-                if (n < p.ldl) *(v4f*)(p.logits + m * p.ldl + n) = acc[h] * inv_heat;
+                if (n < p.ldl) *(v4f*)(p.logits + m * p.ldl + n) = acc[h];
               }
             }
           }
@@ -1155,7 +1155,7 @@ __global__ __launch_bounds__(512, 2) void k_few(args p, int parts) {
 #pragma unroll
             for (int t = 0; t < 4; t++)
               if (n0 + h * 16 + q * 4 + t < p.N) {
-                const float z = E == E_PROBS ? fmaf(acc[h][t], bits, -from) : acc[h][t] - from;
+                const float z = E == E_PROBS ? (acc[h][t] - from) * bits : acc[h][t] - from;
                 const float x = E == E_PROBS ? __builtin_amdgcn_exp2f(z) : __expf(z);
                 sum += x;
                 if (E == E_PROBS) weighted = fmaf(x, fmaxf(z, -200.f), weighted);
@@ -1176,14 +1176,15 @@ __global__ __launch_bounds__(512, 2) void k_few(args p, int parts) {
           const float from = top == -INFINITY ? 0.f : top;
           for (int w = 0; w < 8; w += parts) {
             const float2 s = stats[w][threadIdx.x];
-            if (s.x != -INFINITY || s.y != 0.f) sum += s.y * (E == E_PROBS ? __builtin_amdgcn_exp2f(s.x - from) : __expf(s.x - from));
+            if (s.x != -INFINITY || s.y != 0.f) sum += s.y * (E == E_PROBS ? __builtin_amdgcn_exp2f((s.x - from) * bits) : __expf(s.x - from));
           }
           p.parts[(m_top + threadIdx.x) * p.parts_n + blockIdx.x] = float2{top, sum};
           if constexpr (E == E_PROBS) {
             float weighted = 0.f;
             for (int w = 0; w < 8; w += parts) {
               const float2 s = stats[w][threadIdx.x];
-              if (s.x != -INFINITY || s.y != 0.f) weighted += __builtin_amdgcn_exp2f(s.x - from) * fmaf(fmaxf(s.x - from, -200.f), s.y, stats_w[w][threadIdx.x]);
+              const float z = (s.x - from) * bits;
+              if (s.x != -INFINITY || s.y != 0.f) weighted += __builtin_amdgcn_exp2f(z) * fmaf(fmaxf(z, -200.f), s.y, stats_w[w][threadIdx.x]);
             }
             p.weighted[(m_top + threadIdx.x) * p.parts_n + blockIdx.x] = weighted;
           }

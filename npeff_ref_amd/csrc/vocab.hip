@@ -468,7 +468,8 @@ int loss_backward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, con
 //   logp[t, j] = z[t, w_tj] - lse_t,  H_t = lse_t - sum_v p z = log s - W / s  with s = sum exp(z - max), W = sum exp(z - max) (z - max)
 //   loss_t = sum_j q_j (log q_j - logp[t, j]),  q = softmax over the listed words of l / T
 //
-// In the tiles' epilogues and the sums z is in units of log 2, so that a word costs a product, a hardware exponential and two additions.
+// Maxima are those of the products, and a word costs its difference from one, a product (by log2(e) / T), a hardware exponential and two
+// additions: rounding errors are then of the differences' size, whatever |z| / T.
 //
 // Alternatives.  The tiles leave the largest logit of every chunk of words (64; of few rows 16 or 32) and the logits
 // themselves.  The KEEP = n + 8 largest lie in the KEEP chunks of the largest maxima (in any other chunk every word is behind the KEEP
@@ -510,7 +511,7 @@ __device__ __forceinline__ const __attribute__((address_space(4))) A& arguments(
   asm volatile("" : "+s"(p));
   return *p;
 }
-struct running {  // a row's statistics so far
+struct running {  // a row's statistics so far (top: of the products)
   float top, sum, weighted;
   int kept;
 };
@@ -878,12 +879,13 @@ __global__ __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 4) void k_answers(ans
       for (int w = 0; w < WAVES; w++) top = fmaxf(top, red[0][w]);
     }
     const float from = top == -INFINITY ? 0.f : top;
+    const float bits = p0.inv_heat * LOG2_E;
     float sum = 0.f, weighted = 0.f;
     auto add = [&](float x, float s, float w) {
       if (x != -INFINITY || s != 0.f) {
-        const float f = __builtin_amdgcn_exp2f(x - from);
+        const float z = (x - from) * bits, f = __builtin_amdgcn_exp2f(z);
         sum += s * f;
-        weighted += f * fmaf(fmaxf(x - from, -200.f), s, w);
+        weighted += f * fmaf(fmaxf(z, -200.f), s, w);
       }
     };
 #pragma unroll
@@ -906,7 +908,7 @@ __global__ __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 4) void k_answers(ans
     asm volatile("" ::"v"(touched));
     add(so_far.top, so_far.sum, so_far.weighted);
     constexpr float LOG_2 = 0.69314718055994531f;
-    const float lse = (log2f(sum) + from) * LOG_2;
+    const float lse = fmaf(from, p0.inv_heat, log2f(sum) * LOG_2);
     const bool sound = fabsf(lse) < INFINITY;
 
     // -- alternatives --
@@ -1089,7 +1091,7 @@ __global__ __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 4) void k_answers(ans
     if (p1.stored && PART != FINISH) {
       for (int j = tid; j < p1.n_given; j += THREADS) {
         const int64_t w = (int64_t)p1.given[m * p1.n_given + j] - p1.word0;
-        if (w >= 0 && w < p1.piece) p1.logp[m * p1.n_given + j] = p1.logits[m * p1.ldl + w];
+        if (w >= 0 && w < p1.piece) p1.logp[m * p1.n_given + j] = p1.logits[m * p1.ldl + w] * p1.inv_heat;
       }
     }
     if (PART == SELECT || (PART != FINISH && !p1.last)) {
@@ -1534,7 +1536,7 @@ int answers_backward(hipStream_t st, const char* me, slope_args s, int64_t n_in,
 }
 int check_answers(const char* me, int64_t n_words, float temperature, int n_given, int n_top) {
   const float inv = 1.f / temperature;
-  DN_CHECK(temperature > 0.f && inv > 0.f && inv < INFINITY, "%s: temperature = %g", me, (double)temperature);
+  DN_CHECK(temperature > 0.f && inv > 0.f && inv * LOG2_E < INFINITY, "%s: temperature = %g", me, (double)temperature);
   DN_CHECK(n_given >= 0 && n_given <= MOST_LISTED, "%s: %d words of a row: 0 to %d", me, n_given, MOST_LISTED);
   DN_CHECK(n_top >= 0 && n_top <= MOST_TOP && n_top <= n_words, "%s: %d alternatives of %lld words: 0 to %d of them", me, n_top,
            (long long)n_words, MOST_TOP);

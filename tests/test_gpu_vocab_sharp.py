@@ -1,0 +1,80 @@
+"""What a model answers, distillation and their gradients where logits lie far apart: at temperatures so low that |z| / T goes
+up to 1e38, and of logits that are large themselves.
+
+Small whole numbers make the products exact in every type, and powers of two the temperatures, so that what is left are the roundings of
+the results: the bounds below hold none that grow with |z| / T but those of a result's own size.  A row's largest logits lead by 2^30 and
+more, its probabilities are 1 / (how many are largest) and 0: an exponential, the sum, its logarithm and the result are rounded, 8 half
+units in all.  Of arbitrary numbers a word that leads by more than the products' rounding has log p 0 all the same, since the given
+words' logits are the same sums as the row's largest."""
+
+import pytest
+import torch
+
+import npeff_ref_amd as d
+from test_gpu_vocab_answers import DTYPES, EPS32, Exact, check_grads, empty, near, rand, words_of
+
+pytestmark = pytest.mark.gpu
+
+TEMPERATURES = [2.0**-30, 2.0**-63, 2.0**-119]
+SHAPES = [(1, 4000), (3, 3000), (12, 3000), (40, 3000), (70, 2500), (200, 9001), (700, 3000), (1500, 9001)]
+
+
+def whole(shape, dt, seed):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randint(-2, 3, shape, generator=g).to(DTYPES[dt]).cuda()
+
+
+class Sharp:
+    """Of exact logits whose differences are 2^30 and more: the largest share the probability."""
+
+    def __init__(self, X, E, heat):
+        self.X, self.E = X.double(), E.double()
+        self.raw = self.X @ self.E.T
+        self.top = self.raw.max(1, keepdim=True).values
+        self.p = (self.raw == self.top).double()
+        self.many = self.p.sum(1)
+        self.p /= self.many[:, None]
+        self.entropy = self.many.log()
+        self.log_p = (self.raw - self.top) / heat - self.entropy[:, None]
+        self.lse = self.top[:, 0] / heat + self.entropy
+
+
+def answers(X, E, w, top, heat):
+    rows, given = w.shape
+    o = dict(logp=empty(rows, given), lse=empty(rows), entropy=empty(rows), top_words=empty(rows, top, dtype=torch.int32), top_logp=empty(rows, top))
+    d.op_vocab_probs(X, E, w, temperature=heat, **o)
+    return o
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("heat", TEMPERATURES)
+@pytest.mark.parametrize("rows, words", SHAPES)
+def test_answers_at_low_temperatures(rows, words, heat, dt):
+    X, E, w = whole((rows, 40), dt, 1), whole((words, 40), dt, 2), words_of(rows, 3, words, 3)
+    x = Sharp(X, E, heat)
+    w[0, 0] = int(x.raw[0].argmax())
+    o = answers(X, E, w, 9, heat)
+    near(o["lse"], x.lse, 8 * EPS32 * (1 + x.lse.abs()), "lse")
+    near(o["entropy"], x.entropy, 8 * EPS32 * (1 + x.entropy), "entropy")
+    assert torch.equal(o["top_words"], x.raw.sort(dim=1, descending=True, stable=True).indices[:, :9].to(torch.int32))
+
+
+def leading(rows, dt, n_in=264, words=9000):
+    X, E = rand((rows, n_in), dt, 1), rand((words, n_in), "f32", 2, 0.1)
+    first = torch.arange(rows, device="cuda") * 5 + 2
+    x = X.float()
+    E[first] += 4 * x / x.norm(dim=1, keepdim=True)
+    E = E.to(DTYPES[dt])
+    z = X.double() @ E.double().T
+    lead = z.gather(1, first[:, None])[:, 0]
+    z.scatter_(1, first[:, None], -1e9)
+    assert (lead - z.max(1).values > 20).all()
+    return X, E, first.to(torch.int32)
+
+
+def test_temperatures_too_low_for_32_bits_are_refused():
+    X, E = rand((3, 64), "bf16", 1), rand((90, 64), "bf16", 2)
+    for heat in (1e-39, 3e-39, 4.2e-39):  # (1 / T, or 1 / T in units of log 2, is infinite)
+        with pytest.raises(d.DnpeffError, match="temperature"):
+            d.op_vocab_probs(X, E, lse=empty(3), temperature=heat)
+    d.op_vocab_probs(X * 0, E, lse=empty(3), temperature=4.3e-39)
