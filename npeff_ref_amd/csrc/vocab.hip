@@ -908,7 +908,7 @@ __global__ __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 4) void k_answers(ans
     asm volatile("" ::"v"(touched));
     add(so_far.top, so_far.sum, so_far.weighted);
     constexpr float LOG_2 = 0.69314718055994531f;
-    const float lse = fmaf(from, p0.inv_heat, log2f(sum) * LOG_2);
+    const float log_sum = log2f(sum) * LOG_2, lse = fmaf(from, p0.inv_heat, log_sum);
     const bool sound = fabsf(lse) < INFINITY;
 
     // -- alternatives --
@@ -1091,7 +1091,7 @@ __global__ __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 4) void k_answers(ans
     if (p1.stored && PART != FINISH) {
       for (int j = tid; j < p1.n_given; j += THREADS) {
         const int64_t w = (int64_t)p1.given[m * p1.n_given + j] - p1.word0;
-        if (w >= 0 && w < p1.piece) p1.logp[m * p1.n_given + j] = p1.logits[m * p1.ldl + w] * p1.inv_heat;
+        if (w >= 0 && w < p1.piece) p1.logp[m * p1.n_given + j] = p1.logits[m * p1.ldl + w];
       }
     }
     if (PART == SELECT || (PART != FINISH && !p1.last)) {
@@ -1110,7 +1110,7 @@ __global__ __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 4) void k_answers(ans
     }
     if (tid == 0) {
       if (p1.lse) p1.lse[m] = lse;
-      if (p1.entropy) p1.entropy[m] = sound ? (log2f(sum) - weighted / sum) * LOG_2 : __builtin_nanf("");
+      if (p1.entropy) p1.entropy[m] = sound ? log_sum - weighted / sum * LOG_2 : __builtin_nanf("");
     }
     const T* x = (const T*)p1.X + m * p1.ldx;
     auto& p2 = arguments<answer_args>();
@@ -1164,9 +1164,15 @@ __global__ __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 4) void k_answers(ans
       }
     };
     auto given_word = [&](int j) { return p2.given[m * p2.n_given + j]; };
+    // log p of a word's product, from the difference to the largest (lse as it is stored is rounded, by 2^-24 |z| / T).  A given word's product
+    // may be a rounding above the largest.
+    auto log_p = [&](double s, double largest) {
+      const float l = (float)((s - largest) * (double)p2.inv_heat - (double)log_sum);
+      return l > 0.f ? 0.f : l;
+    };
     auto put_given = [&](int j, double s) {
       const int32_t w = given_word(j);
-      p2.logp[m * p2.n_given + j] = w < 0 ? 0.f : w >= p2.words ? __builtin_nanf("") : (float)(s * (double)p2.inv_heat - (double)lse);
+      p2.logp[m * p2.n_given + j] = w < 0 ? 0.f : w >= p2.words ? __builtin_nanf("") : log_p(s, from);
     };
     // (a few given words go with the leading ones: a turn of them takes 2 us)
     const bool together = FEW && kept > 0 && p2.n_given <= AT_ONCE;
@@ -1186,7 +1192,7 @@ __global__ __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 4) void k_answers(ans
       for (int j = tid; j < p2.n_given; j += THREADS) {  // (what this thread or an earlier launch has written)
         const int32_t w = p2.given[m * p2.n_given + j];
         float* to = p2.logp + m * p2.n_given + j;
-        *to = w < 0 ? 0.f : w >= p2.words ? __builtin_nanf("") : *to - lse;
+        *to = w < 0 ? 0.f : w >= p2.words ? __builtin_nanf("") : log_p(*to, from);
       }
     }
     if (PART != NO_TOPS && p2.n_top > 0) {
@@ -1195,12 +1201,13 @@ __global__ __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 4) void k_answers(ans
         if (!sound || i >= kept) p2.top_words[m * p2.n_top + i] = -1, p2.top_logp[m * p2.n_top + i] = __builtin_nanf("");
       for (int i = tid; i < kept && sound; i += THREADS) {
         const double s = exact_[i];
+        double largest = s;  // (products in 64 bits against one of them: what fp32 sums are off by would be the larger part of a small log p)
         int rank = 0;
 #pragma unroll 4
-        for (int j = 0; j < kept; j++) rank += exact_[j] > s || (exact_[j] == s && j < i);
+        for (int j = 0; j < kept; j++) rank += exact_[j] > s || (exact_[j] == s && j < i), largest = exact_[j] > largest ? exact_[j] : largest;
         if (rank < p2.n_top) {
           p2.top_words[m * p2.n_top + rank] = word_[at][i];
-          p2.top_logp[m * p2.n_top + rank] = (float)(s * (double)p2.inv_heat - (double)lse);
+          p2.top_logp[m * p2.n_top + rank] = log_p(s, largest);
         }
       }
     }

@@ -59,6 +59,39 @@ def test_answers_at_low_temperatures(rows, words, heat, dt):
     assert torch.equal(o["top_words"], x.raw.sort(dim=1, descending=True, stable=True).indices[:, :9].to(torch.int32))
 
 
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("heat", TEMPERATURES)
+@pytest.mark.parametrize("rows, words", SHAPES)
+def test_log_p_at_low_temperatures(rows, words, heat, dt):
+    X, E, w = whole((rows, 40), dt, 1), whole((words, 40), dt, 2), words_of(rows, 3, words, 3)
+    x = Sharp(X, E, heat)
+    w[0, 0] = int(x.raw[0].argmax())
+    o = answers(X, E, w, 9, heat)
+    want = torch.where(w >= 0, x.log_p.gather(1, w.long().clamp(min=0)), 0.0)
+    near(o["logp"], want, 8 * EPS32 * (1 + want.abs()), "logp")
+    v = x.log_p.gather(1, o["top_words"].long())
+    near(o["top_logp"], v, 8 * EPS32 * (1 + v.abs()), "top_logp")
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("heat", TEMPERATURES)
+@pytest.mark.parametrize("rows, words", SHAPES)
+def test_distillation_at_low_temperatures(rows, words, heat, dt):
+    X, E, w = whole((rows, 40), dt, 1), whole((words, 40), dt, 2), words_of(rows, 4, words, 3)
+    logits = whole((rows, 4), "f32", 4)
+    loss, logp, lse = empty(rows), empty(rows, 4), empty(rows)
+    d.op_vocab_distill(X, E, w, logits, loss=loss, logp=logp, lse=lse, temperature=heat)
+    x = Sharp(X, E, heat)
+    there = w >= 0
+    l = torch.where(there, logits.double(), -9.0)
+    q = ((l == l.max(1, keepdim=True).values) & there).double()
+    q /= q.sum(1, keepdim=True).clamp(min=1)
+    want = torch.where(there, x.log_p.gather(1, w.long().clamp(min=0)), 0.0)
+    near(logp, want, 8 * EPS32 * (1 + want.abs()), "logp")
+    exact, size = (torch.special.xlogy(q, q) - q * want).sum(1), (q * want.abs()).sum(1)
+    near(loss, exact, 16 * EPS32 * (1 + size), "loss")
+
+
 def leading(rows, dt, n_in=264, words=9000):
     X, E = rand((rows, n_in), dt, 1), rand((words, n_in), "f32", 2, 0.1)
     first = torch.arange(rows, device="cuda") * 5 + 2
@@ -70,6 +103,23 @@ def leading(rows, dt, n_in=264, words=9000):
     z.scatter_(1, first[:, None], -1e9)
     assert (lead - z.max(1).values > 20).all()
     return X, E, first.to(torch.int32)
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("rows", [1, 12, 40, 200, 700, 1500])
+def test_large_logits(rows, dt):
+    """At a temperature of 1 and logits of 4e4 and more: alternatives' log p come from products in 64 bits, so the leading one's is 0; given words' are
+    off by the rounding of fp32 products, and never above 0."""
+    X, E, first = leading(rows, dt)
+    E *= 1024
+    o = answers(X, E, first[:, None].contiguous(), 3, 1.0)
+    x = Exact(X, E, 1.0)
+    assert torch.equal(o["top_words"][:, 0], first)
+    near(o["top_logp"][:, 0], torch.zeros_like(x.lse), torch.full_like(x.lse, 4 * EPS32), "top_logp")
+    near(o["entropy"], torch.zeros_like(x.lse), torch.full_like(x.lse, 4 * EPS32), "entropy")
+    near(o["lse"], x.lse, x.off, "lse")
+    near(o["logp"][:, 0], torch.zeros_like(x.lse), 2 * x.logit, "logp")
+    assert (o["logp"] <= 0).all()
 
 
 def test_temperatures_too_low_for_32_bits_are_refused():
