@@ -639,9 +639,11 @@ int dnpeff_vocab_loss_backward(void* stream, int type, int64_t rows, int64_t n_i
  * top_words, top_logp [rows, n_top], dense.  Which word is the likelier is decided by the products in 64 bits among the
  * n_top + 8 that lead in fp32; of equal ones the lower comes first.  A negative given word has logp 0, one of n_words and more
  * NaN.  A row whose lse is not finite (infinity, NaN or a number past 3.4e38 among its logits, or nothing but -infinity) has entropy
- * NaN and alternatives -1 with NaN.  T is at least 4.3e-39: 1 / T in units of log 2 is then a number of 32 bits.  log p come from differences of
- * products, not from lse as it is rounded, and are never above 0.  The workspace of alternatives holds logits, up to 2 GB of them at a
- * time.
+ * NaN and alternatives -1 with NaN.  T is at least 4.3e-39: 1 / T in units of log 2 is then a number of 32 bits.
+ * log p come from differences of products, not from lse as it is rounded, and are never above 0.  They are off by what those differences
+ * are, times 1 / T: alternatives' are of 64 bits; a given word's product is summed in fp32 by itself, below T = 1/16 it is one of the very
+ * sums that lse is made of, so that of a word ahead of all others by more than fp32 sums are off log p is 0 at any T.
+ * The workspace of alternatives holds logits, up to 2 GB of them at a time.
  * With n_given = 0 words and logp may be NULL, with n_top = 0 the alternatives; lse and entropy may be NULL.
  * The workspace call serves dnpeff_vocab_distill and its gradients as well (n_given: the listed words, n_top = 0). */
 int dnpeff_vocab_probs_workspace(int type, int64_t rows, int64_t n_in, int64_t n_words, int n_given, int n_top, int aligned,

@@ -228,8 +228,9 @@ __device__ __forceinline__ void group_of_tile(const group_rows& G, int tall, int
 
 // ---- a product ---------------------------------------------------------------------------------------------------
 enum { ONE = 0, BY_ROWS = 1, BY_REDUCTION = 2 };                      // groups: none, of rows of A and C, of the reduction
-enum { E_LINEAR = 0, E_STORE = 1, E_LOSS = 2, E_LOSS_GRAD = 3, E_PROBS = 4, E_PROBS_GRAD = 5 };  // what becomes of a tile
-constexpr bool is_stats(int e) { return e == E_LOSS || e == E_PROBS; }
+enum { E_LINEAR = 0, E_STORE = 1, E_LOSS = 2, E_LOSS_GRAD = 3, E_PROBS = 4, E_PROBS_GRAD = 5, E_PROBS_LISTED = 6 };  // what becomes of a tile
+constexpr bool is_probs(int e) { return e == E_PROBS || e == E_PROBS_LISTED; }
+constexpr bool is_stats(int e) { return e == E_LOSS || is_probs(e); }
 constexpr bool is_grad(int e) { return e == E_LOSS_GRAD || e == E_PROBS_GRAD; }
 // A row of the logits' gradient but for its listed words: dz = p (a + b log p), and 0 where the row is not alive.
 constexpr float LOG2_E = 1.4426950408889634f;
@@ -279,6 +280,11 @@ struct args {
   const float* floor;
   const unsigned* wanted;   // (or NULL) [M][ld_wanted]: a bit for each chunk, chunk0 the first of this piece
   int64_t chunk0, ld_wanted;
+  // E_PROBS_LISTED: the same, and the products of words that are given, negative ones and those of other pieces left out.  (In the same
+  // kernel this would cost the others registers: 2000 x 50001 of 1024 208 us with it, 205 without.)
+  const int32_t* listed;    // [M][n_listed]
+  int n_listed;
+  float* listed_z;
   const slope_row* slopes;  // [M]
 };
 
@@ -407,6 +413,39 @@ __device__ __forceinline__ void finish_slope(const P& p, int64_t m, int64_t n, f
     v[e] = e < there ? g : 0.f;
   }
   store_op<T, W>((typename num<T>::op*)p.out + m * p.ldc + n, p.M * p.ldc, v);
+}
+// The products of row m's listed words among `there` from `first` on: a wave has 16 rows, four consecutive words of each 16 a lane (so the
+// four lanes of a row look through its list together).  here: the row is one.
+template <int BLOCKS, class P>
+__device__ __forceinline__ void listed_of(const P& p, bool here, int64_t m, int first, int there, int lane, const v4f (&acc)[BLOCKS]) {
+  constexpr int AHEAD = 4;
+  const int32_t* list = p.listed + (here ? m * p.n_listed : 0);
+  const int q = lane >> 4, many = here ? p.n_listed : 0;
+#pragma unroll 1
+  for (int g0 = 0; g0 < p.n_listed; g0 += 4 * AHEAD) {
+    int at[AHEAD];
+    bool any = false;
+#pragma unroll
+    for (int t = 0; t < AHEAD; t++) {
+      const int g = g0 + t * 4 + q, word = g < many ? list[g] : -1;
+      at[t] = word >= first && word - first < there ? word - first : -1;
+      any |= at[t] >= 0;
+    }
+    if (!__any(any)) continue;
+#pragma unroll
+    for (int t = 0; t < AHEAD; t++)
+#pragma unroll 1
+      for (int r = 0; r < 4; r++) {
+        const int place = __shfl(at[t], r * 16 + (lane & 15), 64) - q * 4;
+        if (place < 0 || (place & 15) >= 4) continue;
+        float z = 0.f;
+#pragma unroll
+        for (int j = 0; j < BLOCKS; j++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) z = j * 16 + e == place ? acc[j][e] : z;
+        p.listed_z[m * p.n_listed + g0 + t * 4 + r] = z;
+      }
+  }
 }
 template <class T, int W, class P>
 __device__ __forceinline__ void bias_of(const P& p, int64_t n, int group, bool held, float* b) {
@@ -697,7 +736,7 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
     }
     // (The difference first: of products times `bits` a maximum would be rounded, by 128 and more from 2^31 on, and its exponential be
     // 0 or infinite.  bits is finite.)
-    const float bits = (E == E_PROBS ? p.inv_heat : 1.f) * LOG2_E;
+    const float bits = (is_probs(E) ? p.inv_heat : 1.f) * LOG2_E;
 #pragma unroll
     for (int i = 0; i < FM; i++) {
       const int64_t m = m_wave + i * 16 + (lane & 15);
@@ -736,6 +775,10 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
 #pragma unroll
           for (int e = 0; e < 4; e++) sum += __expf(acc[i][j][e] - from);
       } else {
+        if constexpr (E == E_PROBS_LISTED) {
+          if (n_wave < p.N)
+            listed_of<FN>(p, m < m_end, m, (int)(p.word0 + n_wave), (int)(p.N - n_wave < FN * 16 ? p.N - n_wave : FN * 16), lane, acc[i]);
+        }
         if (m < m_end) {
           if (p.tops && q == 0 && n_wave < p.N) p.tops[m * p.chunks + (n_wave >> 6)] = top;
           if (wanted[i] || (top >= floors[i] && n_wave < p.N)) {
@@ -771,11 +814,11 @@ __device__ __forceinline__ void finish_tile(kargs& p, const place<T>& w, v4f (&a
 #pragma unroll
       for (int v = 0; v < WN; v++) {
         const float x = side[v * BM + m].x, y = side[v * BM + m].y;
-        if (x != -INFINITY || y != 0.f) sum += y * (E == E_PROBS ? __builtin_amdgcn_exp2f((x - from) * bits) : __expf(x - from));
+        if (x != -INFINITY || y != 0.f) sum += y * (is_probs(E) ? __builtin_amdgcn_exp2f((x - from) * bits) : __expf(x - from));
       }
       const int64_t to = (w.m0 + m) * p.parts_n + p.part0 + w.tn;
       p.parts[to] = float2{top, sum};
-      if constexpr (E == E_PROBS) {
+      if constexpr (is_probs(E)) {
         float weighted = 0.f;
 #pragma unroll
         for (int v = 0; v < WN; v++) {
@@ -1125,7 +1168,7 @@ __global__ __launch_bounds__(512, 2) void k_few(args p, int parts) {
             }
         }
       } else {
-        const float bits = (E == E_PROBS ? p.inv_heat : 1.f) * LOG2_E;  // (as in finish_tile)
+        const float bits = (is_probs(E) ? p.inv_heat : 1.f) * LOG2_E;  // (as in finish_tile)
         if (part == 0) {
           const int64_t label = E == E_LOSS && m < m_end ? (int64_t)p.labels[m] : -1;
           float top = -INFINITY, sum = 0.f, weighted = 0.f;
@@ -1140,7 +1183,11 @@ __global__ __launch_bounds__(512, 2) void k_few(args p, int parts) {
           top = fmaxf(top, __shfl_xor(top, 16, 64));
           top = fmaxf(top, __shfl_xor(top, 32, 64));
           const float from = top == -INFINITY ? 0.f : top;
-          if constexpr (E == E_PROBS) {
+          if constexpr (is_probs(E)) {
+            if constexpr (E == E_PROBS_LISTED) {
+              if (n0 < p.N)
+                listed_of<COLS>(p, m < m_end, m, (int)(p.word0 + n0), (int)(p.N - n0 < COLS * 16 ? p.N - n0 : COLS * 16), lane, acc);
+            }
             if (p.tops && m < m_end && n0 < p.N) {  // (a chunk is a wave's columns)
               if (q == 0) p.tops[m * p.chunks + n0 / (16 * COLS)] = top;
 #pragma unroll
@@ -1155,12 +1202,12 @@ __global__ __launch_bounds__(512, 2) void k_few(args p, int parts) {
 #pragma unroll
             for (int t = 0; t < 4; t++)
               if (n0 + h * 16 + q * 4 + t < p.N) {
-                const float z = E == E_PROBS ? (acc[h][t] - from) * bits : acc[h][t] - from;
-                const float x = E == E_PROBS ? __builtin_amdgcn_exp2f(z) : __expf(z);
+                const float z = is_probs(E) ? (acc[h][t] - from) * bits : acc[h][t] - from;
+                const float x = is_probs(E) ? __builtin_amdgcn_exp2f(z) : __expf(z);
                 sum += x;
-                if (E == E_PROBS) weighted = fmaf(x, fmaxf(z, -200.f), weighted);
+                if (is_probs(E)) weighted = fmaf(x, fmaxf(z, -200.f), weighted);
               }
-          if constexpr (E == E_PROBS) {
+          if constexpr (is_probs(E)) {
             weighted += __shfl_xor(weighted, 16, 64);
             weighted += __shfl_xor(weighted, 32, 64);
             if (q == 0) stats_w[wave][lane] = weighted;
@@ -1176,10 +1223,10 @@ __global__ __launch_bounds__(512, 2) void k_few(args p, int parts) {
           const float from = top == -INFINITY ? 0.f : top;
           for (int w = 0; w < 8; w += parts) {
             const float2 s = stats[w][threadIdx.x];
-            if (s.x != -INFINITY || s.y != 0.f) sum += s.y * (E == E_PROBS ? __builtin_amdgcn_exp2f((s.x - from) * bits) : __expf(s.x - from));
+            if (s.x != -INFINITY || s.y != 0.f) sum += s.y * (is_probs(E) ? __builtin_amdgcn_exp2f((s.x - from) * bits) : __expf(s.x - from));
           }
           p.parts[(m_top + threadIdx.x) * p.parts_n + blockIdx.x] = float2{top, sum};
-          if constexpr (E == E_PROBS) {
+          if constexpr (is_probs(E)) {
             float weighted = 0.f;
             for (int w = 0; w < 8; w += parts) {
               const float2 s = stats[w][threadIdx.x];

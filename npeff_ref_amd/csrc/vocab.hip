@@ -271,7 +271,7 @@ struct loss_room {  // of the forward pass
 // The answers' fp32 products of few tiles go through planes.hpp.  (Those of the loss keep the order of their sums.)
 template <class T>
 constexpr bool may_be_planes(int epilogue) {
-  return sizeof(T) == 4 && (epilogue == E_PROBS || epilogue == E_PROBS_GRAD);
+  return sizeof(T) == 4 && (is_probs(epilogue) || epilogue == E_PROBS_GRAD);
 }
 template <class T, int EPILOGUE>
 int64_t floats_of(int64_t M, int64_t N, int64_t K) {
@@ -492,6 +492,13 @@ constexpr int64_t WHOLE_BYTES = (int64_t)128 << 20; // of all logits that are st
 // Given words' logits: rows of E read again and multiplied in fp32, or, where that would be so many bytes, taken from the tiles (us
 // there and here: 20 words of 2000 rows of 1024, 82 MB, 904 and 924 with the gradients; 100 of 1999 of 1030, 412 MB, 420 and 340).
 constexpr int64_t STORED_FROM = (int64_t)128 << 20;
+// Below a temperature of 1/16 given words' products are always the tiles' own: another order of the same sum is off by some 2^-24 |z| / T, which
+// at T = 1e-6 leaves nothing of a log p that should be 0, and of one sum the difference to itself is 0.  (Each tile then looks
+// through the rows' lists.  us from rows of E and here: 2000 rows of 50001 words of 1024 with one given word 202 and 237, with 20 209 and 293, one
+// row of 32000 words of 4096 48 and 46.)
+constexpr float SHARP = 16.f;  // 1 / T
+// answer_args::stored: given words' products are among the logits of the pieces; are in logp already
+enum { NOT_STORED = 0, IN_LOGITS = 1, IN_PLACE = 2 };
 
 // Floats in the order of their values (equal zeros equal); 1: NaN, 0 is below all.
 __device__ __forceinline__ unsigned key_of(float v) {
@@ -538,7 +545,7 @@ struct answer_args {
   float inv_heat;
   int n_given;
   const int32_t* given;        // [rows][n_given]
-  int stored;                  // their logits are among those of the pieces
+  int stored;
   float *logp, *lse, *entropy;
   const float* teacher;        // (or NULL) [rows][n_given]
   float* loss;
@@ -1088,7 +1095,7 @@ __global__ __launch_bounds__(THREADS, THREADS >= 512 ? 2 : 4) void k_answers(ans
       __syncthreads();
     }
     auto& p1 = p;
-    if (p1.stored && PART != FINISH) {
+    if (p1.stored == IN_LOGITS && PART != FINISH) {
       for (int j = tid; j < p1.n_given; j += THREADS) {
         const int64_t w = (int64_t)p1.given[m * p1.n_given + j] - p1.word0;
         if (w >= 0 && w < p1.piece) p1.logp[m * p1.n_given + j] = p1.logits[m * p1.ldl + w];
@@ -1450,7 +1457,7 @@ int answers_forward(hipStream_t st, const char* me, const answer_args& to, char*
   a.floor = (float*)take(r.floor);
   float* logp_room = (float*)take(r.logp);
   unsigned* wanted = (unsigned*)take(r.wanted);
-  a.stored = r.stored;
+  a.stored = r.stored ? IN_LOGITS : to.n_given > 0 && to.inv_heat > SHARP ? IN_PLACE : NOT_STORED;
   a.parts = parts, a.weighted = weighted, a.tops = tops, a.logits = logits, a.keep = r.keep;
   for (int64_t b = 0; b < r.blocks; b++) {
     const int64_t m0 = b * r.each, rows = to.rows - m0 < r.each ? to.rows - m0 : r.each;
@@ -1480,19 +1487,26 @@ int answers_forward(hipStream_t st, const char* me, const answer_args& to, char*
       p.A = x.p, p.lda = x.ld, p.a_plane = x.plane, p.b_plane = e.plane, p.ldb = e.ld;
       p.M = rows, p.N = n, p.K = to.n_in;
       p.mode = ONE;
-      p.inv_heat = to.inv_heat;
+      p.inv_heat = to.inv_heat, p.word0 = w0;
       p.parts = parts, p.weighted = weighted;
       a.chunk = 64, a.chunks = ceil_div(n, 64);
       if (r.logits > 0) p.logits = logits, p.ldl = padded(n);
       if (to.n_top > 0) p.tops = tops, p.chunks = a.chunks, p.floor = w0 > 0 ? a.floor : nullptr;
+      if (a.stored == IN_PLACE) p.listed = a.given, p.n_listed = to.n_given, p.listed_z = a.logp;
       if (r.stored) p.wanted = wanted, p.ld_wanted = r.ld_wanted, p.chunk0 = w0 / 64;
       if (r.few) {
         p.B = (const T*)e.p + w0 * e.ld;
-        DN_TRY((launch_few<T, E_PROBS>(p, st, &a.parts_n, &a.chunk)));
+        if (a.stored == IN_PLACE)
+          DN_TRY((launch_few<T, E_PROBS_LISTED>(p, st, &a.parts_n, &a.chunk)));
+        else
+          DN_TRY((launch_few<T, E_PROBS>(p, st, &a.parts_n, &a.chunk)));
         a.chunks = ceil_div(n, a.chunk);
       } else {
         p.B = (const typename num<T>::op*)e.p + w0 * e.ld;
-        DN_TRY((launch_either<T, true, true, E_PROBS, E_PROBS>(p, nullptr, st, &a.parts_n)));
+        if (a.stored == IN_PLACE)
+          DN_TRY((launch_either<T, true, true, E_PROBS_LISTED, E_PROBS>(p, nullptr, st, &a.parts_n)));
+        else
+          DN_TRY((launch_either<T, true, true, E_PROBS, E_PROBS>(p, nullptr, st, &a.parts_n)));
       }
       a.first = w0 == 0, a.last = w0 + n == words, a.word0 = w0, a.piece = n, a.ldl = padded(n);
       // us of a row in 512 threads and in fewer: 64 rows of 32000 words with 20 alternatives 38 and 54 (two launches), 512 rows 75 and 77

@@ -92,6 +92,20 @@ def test_distillation_at_low_temperatures(rows, words, heat, dt):
     near(loss, exact, 16 * EPS32 * (1 + size), "loss")
 
 
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("heat", [0.05, 1e-6, 1e-36])
+@pytest.mark.parametrize("rows", [1, 12, 40, 200, 700, 1500])
+def test_a_word_that_leads_has_log_p_zero(rows, heat, dt):
+    """Logits of arbitrary numbers: one word a row is ahead by 20, all others together have a probability of 9000 exp(-400) at most."""
+    X, E, first = leading(rows, dt)
+    w = torch.stack([first, torch.zeros_like(first)], 1).contiguous()
+    o = answers(X, E, w, 3, heat)
+    assert torch.equal(o["top_words"][:, 0], first) and torch.isfinite(o["lse"]).all()
+    for name, got in (("logp", o["logp"][:, 0]), ("top_logp", o["top_logp"][:, 0]), ("entropy", o["entropy"])):
+        near(got, torch.zeros(rows, device="cuda").double(), torch.full((rows,), 4 * EPS32, device="cuda").double(), name)
+    assert (o["logp"][:, 1] < -300).all()
+
+
 def leading(rows, dt, n_in=264, words=9000):
     X, E = rand((rows, n_in), dt, 1), rand((words, n_in), "f32", 2, 0.1)
     first = torch.arange(rows, device="cuda") * 5 + 2
