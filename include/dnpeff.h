@@ -656,7 +656,9 @@ int dnpeff_vocab_probs(void* stream, int type, int64_t rows, int64_t n_in, int64
  *   dz_v = (sum_j dlogp_j [v = w_j] - p_v (sum_j dlogp_j + dentropy (log p_v + entropy))) / T,
  * rounded to `type` once for the products as in dnpeff_vocab_loss_backward.  Rows without a gradient (every dlogp of a word and
  * dentropy 0) contribute nothing, whatever their rows of X hold; a given word of n_words and more makes dX's row and dE
- * NaN.  A word may be given twice. */
+ * NaN, and so does an lse that is not finite, of a row with a gradient.  A word may be given twice.  p = exp(z - lse) is off relatively by
+ * what z and lse are as numbers of 32 bits, about 2^-24 |z| / T, and at most 1; below T = 1/16 its sums are formed again with the
+ * products, so that they are 1 at any T. */
 int dnpeff_vocab_probs_backward(void* stream, int type, int64_t rows, int64_t n_in, int64_t n_words, const void* X, int64_t ldx,
                                 const void* E, int64_t lde, float temperature, int n_given, const int32_t* words, const float* logp,
                                 const float* lse, const float* entropy, const float* dlogp, const float* dentropy, void* dX,

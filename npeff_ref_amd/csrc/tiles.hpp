@@ -232,12 +232,14 @@ enum { E_LINEAR = 0, E_STORE = 1, E_LOSS = 2, E_LOSS_GRAD = 3, E_PROBS = 4, E_PR
 constexpr bool is_probs(int e) { return e == E_PROBS || e == E_PROBS_LISTED; }
 constexpr bool is_stats(int e) { return e == E_LOSS || is_probs(e); }
 constexpr bool is_grad(int e) { return e == E_LOSS_GRAD || e == E_PROBS_GRAD; }
-// A row of the logits' gradient but for its listed words: dz = p (a + b log p), and 0 where the row is not alive.
 constexpr float LOG2_E = 1.4426950408889634f;
+// A row of the logits' gradient but for its listed words: dz = p (a + b log p) with log p = (product - top) / T - rest (lse is the rest, of
+// a top of 0, or they are what the row's own sums gave).  Without a gradient, whatever its products are: top is DEAD.
+constexpr int DEAD = 0x7fffffff;  // (a NaN that no sum gives)
 struct slope_row {
-  float lse, a, b;
-  int alive;
+  float top, rest, a, b;
 };
+__device__ __forceinline__ bool is_dead(const slope_row& t) { return __float_as_int(t.top) == DEAD; }
 
 struct args {
   const void *A, *B;        // (of num<T>::op)
@@ -285,7 +287,7 @@ struct args {
   const int32_t* listed;    // [M][n_listed]
   int n_listed;
   float* listed_z;
-  const slope_row* slopes;  // [M]
+  slope_row* slopes;        // [M]
 };
 
 // A kernel's arguments where they lie: read where they are needed, not kept in registers throughout.
@@ -399,17 +401,21 @@ __device__ __forceinline__ void finish_grad(const P& p, int64_t m, int64_t n, fl
   }
   store_op<T, W>((typename num<T>::op*)p.out + m * p.ldc + n, p.M * p.ldc, v);
 }
-// p (a + b log p): the same of probabilities and entropies
-__device__ __forceinline__ float slope_of(float z, const slope_row& t) {
-  const float l = z - t.lse, lp = l < -150.f ? -150.f : l;  // (p is 0 there; NaN stays)
-  return __expf(lp) * fmaf(t.b, lp, t.a);
+// p (a + b log p): the same of probabilities and entropies.  (Past -150 p is 0; above 0 log p is a rounding, which a small T
+// makes large; of rows with NaN a is NaN.)
+__device__ __forceinline__ float slope_of(float log_p, float a, float b) {
+  const float l = __builtin_amdgcn_fmed3f(log_p, -150.f, 0.f);
+  return __expf(l) * fmaf(b, l, a);
+}
+__device__ __forceinline__ float slope_of(float product, const slope_row& t, float inv_heat) {
+  return slope_of(fmaf(product - t.top, inv_heat, -t.rest), t.a, t.b);
 }
 template <class T, int W, class P>
 __device__ __forceinline__ void finish_slope(const P& p, int64_t m, int64_t n, float* v, const slope_row& t, float shrink) {
-  const int there = t.alive == 0 || n >= p.N ? 0 : p.N - n < W ? (int)(p.N - n) : W;
+  const int there = is_dead(t) || n >= p.N ? 0 : p.N - n < W ? (int)(p.N - n) : W;
 #pragma unroll
   for (int e = 0; e < W; e++) {
-    const float g = slope_of(v[e] * p.inv_heat, t) * shrink;
+    const float g = slope_of(v[e], t, p.inv_heat) * shrink;
     v[e] = e < there ? g : 0.f;
   }
   store_op<T, W>((typename num<T>::op*)p.out + m * p.ldc + n, p.M * p.ldc, v);
@@ -1157,13 +1163,13 @@ __global__ __launch_bounds__(512, 2) void k_few(args p, int parts) {
         }
       } else if constexpr (E == E_PROBS_GRAD) {
         if (part == 0) {
-          const slope_row t = m < m_end ? p.slopes[m] : slope_row{0.f, 0.f, 0.f, 0};
+          const slope_row t = m < m_end ? p.slopes[m] : slope_row{__int_as_float(DEAD), 0.f, 0.f, 0.f};
 #pragma unroll
           for (int h = 0; h < COLS; h++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
               const int64_t n = n0 + h * 16 + q * 4 + e;
-              const float g = t.alive ? slope_of(acc[h][e] * p.inv_heat, t) : 0.f;
+              const float g = is_dead(t) ? 0.f : slope_of(acc[h][e], t, p.inv_heat);
               if (n < p.N) ((float*)p.out)[n * 16 + (lane & 15)] = g;
             }
         }

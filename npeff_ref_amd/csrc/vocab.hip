@@ -268,6 +268,11 @@ struct loss_room {  // of the forward pass
     all = packs + parts + round256(rows * 4);
   }
 };
+// Below a temperature of 1/16 given words' products are always the tiles' own: another order of the same sum is off by some 2^-24 |z| / T, which
+// at T = 1e-6 leaves nothing of a log p that should be 0, and of one sum the difference to itself is 0.  (Each tile then looks
+// through the rows' lists.  us from rows of E and here: 2000 rows of 50001 words of 1024 with one given word 202 and 237, with 20 209 and 293, one
+// row of 32000 words of 4096 48 and 46.)
+constexpr float SHARP = 16.f;  // 1 / T
 // The answers' fp32 products of few tiles go through planes.hpp.  (Those of the loss keep the order of their sums.)
 template <class T>
 constexpr bool may_be_planes(int epilogue) {
@@ -361,10 +366,66 @@ int put_spots(const spots& s, int64_t word0, int64_t words, const float* shrink,
   return 0;
 }
 
+// A product of a pass whose logits end in EPILOGUE.
+template <class T, bool A_ROWS, bool B_ROWS, int E, int EPILOGUE>
+int launch_either(const args& p, float* parts, hipStream_t st, int* parts_n = nullptr) {
+  if constexpr (may_be_planes<T>(EPILOGUE)) {
+    if (better_in_planes(p.M, p.N, E == E_STORE)) return launch_planes<A_ROWS, B_ROWS, E>(p, parts, st, parts_n);
+  }
+  return launch_product<T, A_ROWS, B_ROWS, E>(p, parts, st, parts_n);
+}
+
+// Low temperatures (SHARP): lse as the forward pass rounded it, of products summed in another order perhaps, would put p off by the
+// exponential of their difference, 2^-24 |z| / T and more.  There the backward pass sums the exponentials of its own products first
+// (2000 rows of 50001 words of 1024 in bf16, forward and backward: 1104 us instead of 853; 5 rows of 32000 of 2048 147 instead of 121).
+__global__ __launch_bounds__(256) void k_sums_again(int64_t rows, int parts_n, const float2* parts, float inv_heat, int first, int last, slope_row* slopes) {
+  const int lane = threadIdx.x & 63;
+  const float bits = inv_heat * LOG2_E;
+  for (int64_t m = (int64_t)blockIdx.x * 4 + threadIdx.x / 64; m < rows; m += (int64_t)gridDim.x * 4) {
+    slope_row t = slopes[m];
+    if (is_dead(t)) continue;
+    float top = first ? -INFINITY : t.top, sum = 0.f;
+    for (int i = lane; i < parts_n; i += 64) top = fmaxf(top, parts[m * parts_n + i].x);
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
+    const float from = top == -INFINITY ? 0.f : top;
+    auto add = [&](float x, float s) {
+      if (x != -INFINITY || s != 0.f) sum += s * __builtin_amdgcn_exp2f((x - from) * bits);
+    };
+    for (int i = lane; i < parts_n; i += 64) add(parts[m * parts_n + i].x, parts[m * parts_n + i].y);
+    if (!first && lane == 0) add(t.top, t.rest);
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d, 64);
+    if (lane == 0) {
+      t.top = top, t.rest = last ? logf(sum) : sum;
+      if (last && !(fabsf(t.rest) < INFINITY)) t.a = __builtin_nanf("");
+      slopes[m] = t;
+    }
+  }
+}
+// p: of a piece's products; room: of its g (12 bytes a row and 16 or 128 words; g takes more)
+template <class T>
+int sums_again(hipStream_t st, args p, bool few, char* room, bool first, bool last) {
+  p.parts = (float2*)room;
+  p.weighted = (float*)(room + p.M * ceil_div(p.N, few ? 16 : 128) * 8);
+  int parts_n = 0;
+  if (few)
+    DN_TRY((launch_few<T, E_PROBS>(p, st, &parts_n)));
+  else
+    DN_TRY((launch_either<T, true, true, E_PROBS, E_PROBS_GRAD>(p, nullptr, st, &parts_n)));
+  const int64_t blocks = ceil_div(p.M, 4);
+  k_sums_again<<<(unsigned)(blocks < JOIN_MOST ? blocks : JOIN_MOST), 256, 0, st>>>(p.M, parts_n, p.parts, p.inv_heat, first, last, p.slopes);
+  DN_LAUNCH_CHECK();
+  return 0;
+}
+
 // (back_is_few)
 template <class T, int E>
 int few_backward(hipStream_t st, const args& logits, const spots& own, char* g, float* parts, void* dX, int64_t lddx, void* dE, int64_t ldde) {
   args p = logits;
+  if constexpr (E == E_PROBS_GRAD) {
+    if (p.inv_heat > SHARP) DN_TRY(sums_again<T>(st, p, true, g, true, true));
+  }
   p.out = g;
   DN_TRY((launch_few<T, E>(p, st)));
   if constexpr (E == E_PROBS_GRAD) DN_TRY((put_spots<T, true>(own, 0, p.N, nullptr, g, 0, 0, st)));
@@ -386,14 +447,6 @@ int few_backward(hipStream_t st, const args& logits, const spots& own, char* g, 
   k_join<T, E_STORE><<<(unsigned)ceil_div(q.M * ceil_div(q.N, 4), 256), 256, 0, st>>>(q, parts, (int)splits);
   DN_LAUNCH_CHECK();
   return 0;
-}
-// A product of a pass whose logits end in EPILOGUE.
-template <class T, bool A_ROWS, bool B_ROWS, int E, int EPILOGUE>
-int launch_either(const args& p, float* parts, hipStream_t st, int* parts_n = nullptr) {
-  if constexpr (may_be_planes<T>(EPILOGUE)) {
-    if (better_in_planes(p.M, p.N, E == E_STORE)) return launch_planes<A_ROWS, B_ROWS, E>(p, parts, st, parts_n);
-  }
-  return launch_product<T, A_ROWS, B_ROWS, E>(p, parts, st, parts_n);
 }
 // of: what the epilogue of the logits (EPILOGUE) takes of the rows; labels: rows of a negative one have no gradient; dloss: the
 // rows' weights, which k_shrink brings to the range of the type.
@@ -426,15 +479,23 @@ int loss_backward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, con
     DN_LAUNCH_CHECK();
     shrink = both, grow = both + 1;
   }
-  for (int64_t w0 = 0; w0 < words; w0 += r.piece) {
-    const int64_t n = words - w0 < r.piece ? words - w0 : r.piece;
-    const void* Ep = (const typename num<T>::op*)r.m[1].p + w0 * r.m[1].ld;
-    const bool first = w0 == 0, last = w0 + n == words;
+  auto products_of = [&](int64_t w0) {  // of the piece that begins with this word
     args p = of;
-    p.A = r.m[0].p, p.lda = r.m[0].ld, p.B = Ep, p.ldb = r.m[1].ld;
+    p.A = r.m[0].p, p.lda = r.m[0].ld, p.B = (const typename num<T>::op*)r.m[1].p + w0 * r.m[1].ld, p.ldb = r.m[1].ld;
     p.a_plane = r.m[0].plane, p.b_plane = r.m[1].plane;
-    p.M = rows, p.N = n, p.K = n_in;
+    p.M = rows, p.N = words - w0 < r.piece ? words - w0 : r.piece, p.K = n_in;
     p.mode = ONE;
+    return p;
+  };
+  if constexpr (EPILOGUE == E_PROBS_GRAD) {
+    if (of.inv_heat > SHARP && rows > 0)
+      for (int64_t w0 = 0; w0 < words; w0 += r.piece) DN_TRY(sums_again<T>(st, products_of(w0), false, g, w0 == 0, words - w0 <= r.piece));
+  }
+  for (int64_t w0 = 0; w0 < words; w0 += r.piece) {
+    args p = products_of(w0);
+    const int64_t n = p.N;
+    const void* Ep = p.B;
+    const bool first = w0 == 0, last = w0 + n == words;
     p.shrink = shrink, p.word0 = w0, p.words = words;
     p.out = g, p.ldc = padded(n);
     DN_TRY((launch_either<T, true, true, EPILOGUE, EPILOGUE>(p, nullptr, st)));
@@ -492,11 +553,6 @@ constexpr int64_t WHOLE_BYTES = (int64_t)128 << 20; // of all logits that are st
 // Given words' logits: rows of E read again and multiplied in fp32, or, where that would be so many bytes, taken from the tiles (us
 // there and here: 20 words of 2000 rows of 1024, 82 MB, 904 and 924 with the gradients; 100 of 1999 of 1030, 412 MB, 420 and 340).
 constexpr int64_t STORED_FROM = (int64_t)128 << 20;
-// Below a temperature of 1/16 given words' products are always the tiles' own: another order of the same sum is off by some 2^-24 |z| / T, which
-// at T = 1e-6 leaves nothing of a log p that should be 0, and of one sum the difference to itself is 0.  (Each tile then looks
-// through the rows' lists.  us from rows of E and here: 2000 rows of 50001 words of 1024 with one given word 202 and 237, with 20 209 and 293, one
-// row of 32000 words of 4096 48 and 46.)
-constexpr float SHARP = 16.f;  // 1 / T
 // answer_args::stored: given words' products are among the logits of the pieces; are in logp already
 enum { NOT_STORED = 0, IN_LOGITS = 1, IN_PLACE = 2 };
 
@@ -1322,9 +1378,9 @@ __global__ __launch_bounds__(256) void k_slope_rows(slope_args p) {
       // (p |log p + H| is at most 8 with 2^31 words: p (1 - p) log of those, and 1 / e)
       size = (sizes + 8.f * fabsf(dh)) * p.inv_heat;
     }
-    if (bad) a = nan;
+    if (bad || !(fabsf(p.lse[m]) < INFINITY)) a = nan;
     if (lane == 0) {
-      p.slopes[m] = slope_row{p.lse[m], a, b, alive ? 1 : 0};
+      p.slopes[m] = slope_row{alive ? 0.f : __int_as_float(DEAD), p.lse[m], a, b};
       p.alive[m] = alive ? 0 : -1;
       p.size[m] = size;
     }
@@ -1352,10 +1408,8 @@ __global__ __launch_bounds__(256) void k_slope_rows(slope_args p) {
         }
       }
       if (j < p.many) {
-        const float l = p.logp[m * p.many + j];
-        const slope_row t{0.f, a, b, 1};
         p.word[m * p.many + j] = w >= 0 && w < p.words && first && alive ? w : -1;
-        p.g[m * p.many + j] = slope_of(l, t) + sum;
+        p.g[m * p.many + j] = slope_of(p.logp[m * p.many + j], a, b) + sum;
       }
     }
   }

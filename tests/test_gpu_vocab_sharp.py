@@ -136,6 +136,66 @@ def test_large_logits(rows, dt):
     assert (o["logp"] <= 0).all()
 
 
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("heat", TEMPERATURES)
+@pytest.mark.parametrize("rows, words", SHAPES)
+def test_gradients_at_low_temperatures(rows, words, heat, dt):
+    """Weights of the temperature's size, so that the gradients are of the operands' types.  Errors as at other temperatures, but p is off
+    by an exponential and a logarithm alone."""
+    X, E, w = whole((rows, 40), dt, 1), whole((words, 40), dt, 2), words_of(rows, 3, words, 3)
+    x = Sharp(X, E, heat)
+    w[0, 0] = int(x.raw[0].argmax())
+    o = answers(X, E, w, 1, heat)
+    dlogp, dh = rand((rows, 3), "f32", 4) * heat, rand((rows,), "f32", 5, 0.3) * heat
+    dlogp[1::3], dh[::2] = 0, 0
+    dX, dE = torch.zeros_like(X), torch.zeros_like(E)
+    d.op_vocab_probs_backward(X, E, w, o["logp"], o["lse"], o["entropy"], dlogp=dlogp, dentropy=dh, dX=dX, dE=dE, temperature=heat)
+    dl, dh64 = torch.where(w >= 0, dlogp.double(), 0.0), dh.double()[:, None]
+    # (of the largest words log p + H is 0)
+    G = -x.p * dl.sum(1, keepdim=True)
+    G.scatter_add_(1, w.long().clamp(min=0), dl)
+    err = x.p * 32 * EPS32 * (dl.abs().sum(1, keepdim=True) + 2 * dh64.abs() * x.entropy[:, None])
+    err.scatter_add_(1, w.long().clamp(min=0), 16 * EPS32 * dl.abs().sum(1, keepdim=True).expand(rows, 3).contiguous())
+    size = (dl.abs().sum(1) + 8 * dh64[:, 0].abs()) / heat
+    check_grads(x, dt, dX, dE, G / heat, err / heat, size, (size > 0).double())
+
+    logits, loss = whole((rows, 3), "f32", 6), empty(rows)
+    d.op_vocab_distill(X, E, w, logits, loss=loss, logp=o["logp"], lse=o["lse"], temperature=heat)
+    dl = rand((rows,), "f32", 7) * heat
+    d.op_vocab_distill_backward(X, E, w, logits, o["logp"], o["lse"], dl, dX=dX, dE=dE, temperature=heat)
+    there = w >= 0
+    l = torch.where(there, logits.double(), -9.0)
+    q = ((l == l.max(1, keepdim=True).values) & there).double()
+    q /= q.sum(1, keepdim=True).clamp(min=1)
+    weight = torch.where(there.any(1), dl.double(), 0.0)[:, None] / heat
+    G = x.p.clone()
+    G.scatter_add_(1, w.long().clamp(min=0), -q)
+    err = x.p * 32 * EPS32
+    err.scatter_add_(1, w.long().clamp(min=0), 16 * EPS32 * there.double())
+    check_grads(x, dt, dX, dE, G * weight, err * weight.abs(), weight[:, 0].abs(), there.any(1).double())
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("heat", [0.05, 1e-6, 1e-36])
+@pytest.mark.parametrize("rows", [1, 5, 12, 40, 200, 700, 1500])
+def test_gradients_of_a_word_that_leads(rows, heat, dt):
+    """Arbitrary numbers: what one word takes from the leading one is its gradient, and the leading word has none of its own."""
+    X, E, first = leading(rows, dt)
+    w = torch.stack([first, torch.zeros_like(first)], 1).contiguous()
+    o = answers(X, E, w, 1, heat)
+    dlogp = rand((rows, 2), "f32", 4) * heat
+    dX, dE = torch.zeros_like(X), torch.zeros_like(E)
+    d.op_vocab_probs_backward(X, E, w, o["logp"], o["lse"], dlogp=dlogp, dX=dX, dE=dE, temperature=heat)
+    x = Sharp(X, E, heat)
+    G = torch.zeros_like(x.raw)
+    dl = dlogp.double() / torch.tensor(heat, dtype=torch.float32).double().item()
+    G[:, 0] = dl[:, 1]
+    G.scatter_(1, first.long()[:, None], -dl[:, 1:])
+    err = torch.zeros_like(G)
+    err.scatter_add_(1, w.long(), 16 * EPS32 * dl.abs().sum(1, keepdim=True).expand(rows, 2).contiguous())
+    check_grads(x, dt, dX, dE, G, err, dl.abs().sum(1), torch.ones_like(x.lse))
+
+
 def test_temperatures_too_low_for_32_bits_are_refused():
     X, E = rand((3, 64), "bf16", 1), rand((90, 64), "bf16", 2)
     for heat in (1e-39, 3e-39, 4.2e-39):  # (1 / T, or 1 / T in units of log 2, is infinite)
