@@ -1486,6 +1486,15 @@ answer_room answer_room_of(int64_t rows, int64_t n_in, int64_t words, int n_give
   return r;
 }
 
+// Every piece of a call goes the same way, by the size of the largest: planes.hpp and tiles.hpp add an fp32 product's terms in different
+// orders, and of one embedding in two pieces neither copy may lead.  (Tiles of both sizes, and k_few, keep one order.)
+template <class T, int E>
+int launch_answers(const args& p, bool planes, hipStream_t st, int* parts_n) {
+  if constexpr (may_be_planes<T>(E)) {
+    if (planes) return launch_planes<true, true, E>(p, nullptr, st, parts_n);
+  }
+  return launch_product<T, true, true, E>(p, nullptr, st, parts_n);
+}
 // to: what is wanted, of all rows.
 template <class T>
 int answers_forward(hipStream_t st, const char* me, const answer_args& to, char* ws, int64_t ws_bytes) {
@@ -1512,6 +1521,7 @@ int answers_forward(hipStream_t st, const char* me, const answer_args& to, char*
   float* logp_room = (float*)take(r.logp);
   unsigned* wanted = (unsigned*)take(r.wanted);
   a.stored = r.stored ? IN_LOGITS : to.n_given > 0 && to.inv_heat > SHARP ? IN_PLACE : NOT_STORED;
+  const bool planes = may_be_planes<T>(E_PROBS) && better_in_planes(r.each, r.piece > r.first ? r.piece : r.first, false);
   a.parts = parts, a.weighted = weighted, a.tops = tops, a.logits = logits, a.keep = r.keep;
   for (int64_t b = 0; b < r.blocks; b++) {
     const int64_t m0 = b * r.each, rows = to.rows - m0 < r.each ? to.rows - m0 : r.each;
@@ -1558,9 +1568,9 @@ int answers_forward(hipStream_t st, const char* me, const answer_args& to, char*
       } else {
         p.B = (const typename num<T>::op*)e.p + w0 * e.ld;
         if (a.stored == IN_PLACE)
-          DN_TRY((launch_either<T, true, true, E_PROBS_LISTED, E_PROBS>(p, nullptr, st, &a.parts_n)));
+          DN_TRY((launch_answers<T, E_PROBS_LISTED>(p, planes, st, &a.parts_n)));
         else
-          DN_TRY((launch_either<T, true, true, E_PROBS, E_PROBS>(p, nullptr, st, &a.parts_n)));
+          DN_TRY((launch_answers<T, E_PROBS>(p, planes, st, &a.parts_n)));
       }
       a.first = w0 == 0, a.last = w0 + n == words, a.word0 = w0, a.piece = n, a.ldl = padded(n);
       // us of a row in 512 threads and in fewer: 64 rows of 32000 words with 20 alternatives 38 and 54 (two launches), 512 rows 75 and 77
