@@ -202,3 +202,71 @@ def test_temperatures_too_low_for_32_bits_are_refused():
         with pytest.raises(d.DnpeffError, match="temperature"):
             d.op_vocab_probs(X, E, lse=empty(3), temperature=heat)
     d.op_vocab_probs(X * 0, E, lse=empty(3), temperature=4.3e-39)
+
+
+@pytest.mark.parametrize("dt", list(DTYPES))
+@pytest.mark.parametrize("rows, words", [(1, 1), (16, 1), (8, 9), (5, 17), (16, 65), (17, 1), (70, 9), (300, 33)])
+def test_small_vocabularies_and_exact_workspaces(rows, words, dt):
+    """Nothing is written but the results and as much workspace as is asked for: the sums that low temperatures need again lie in it too."""
+    heat, top = 2.0**-30, min(words, 4)
+    X, E, w = whole((rows, 40), dt, 1), whole((words, 40), dt, 2), words_of(rows, 2, words, 3)
+    x = Sharp(X, E, heat)
+    sizes = d.vocab_probs_workspace(rows, 40, words, 2, top, DTYPES[dt], True)
+    buf = torch.full((max(sizes) + 512,), 123, dtype=torch.uint8, device="cuda")
+    o = dict(logp=empty(rows, 2), lse=empty(rows), entropy=empty(rows), top_words=empty(rows, top, dtype=torch.int32), top_logp=empty(rows, top))
+    d.op_vocab_probs(X, E, w, temperature=heat, workspace=buf[256 : 256 + sizes[0]], **o)
+    assert (buf[:256] == 123).all() and (buf[256 + sizes[0] :] == 123).all()
+    want = torch.where(w >= 0, x.log_p.gather(1, w.long().clamp(min=0)), 0.0)
+    near(o["logp"], want, 8 * EPS32 * (1 + want.abs()), "logp")
+    buf.fill_(123)
+    dlogp = rand((rows, 2), "f32", 4) * heat
+    dX, dE = torch.zeros_like(X), torch.zeros_like(E)
+    d.op_vocab_probs_backward(X, E, w, o["logp"], o["lse"], dlogp=dlogp, dX=dX, dE=dE, temperature=heat, workspace=buf[256 : 256 + sizes[1]])
+    assert (buf[:256] == 123).all() and (buf[256 + sizes[1] :] == 123).all()
+    dl = torch.where(w >= 0, dlogp.double(), 0.0) / heat
+    G = -x.p * dl.sum(1, keepdim=True)
+    G.scatter_add_(1, w.long().clamp(min=0), dl)
+    err = x.p * 32 * EPS32 * dl.abs().sum(1, keepdim=True)
+    err.scatter_add_(1, w.long().clamp(min=0), 16 * EPS32 * dl.abs().sum(1, keepdim=True).expand(rows, 2).contiguous())
+    check_grads(x, dt, dX, dE, G, err, dl.abs().sum(1), (dl != 0).any(1).double())
+
+
+@pytest.mark.parametrize("heat", [1e10, 1e38, 3.4e38])
+@pytest.mark.parametrize("rows", [3, 70, 700])
+def test_high_temperatures(rows, heat):
+    """All words are alike then, the order of the alternatives is that of the products still."""
+    X, E, w = whole((rows, 40), "bf16", 1), whole((3000, 40), "bf16", 2), words_of(rows, 3, 3000, 3)
+    o = answers(X, E, w, 9, heat)
+    v, at = (X.double() @ E.double().T).sort(dim=1, descending=True, stable=True)
+    assert torch.equal(o["top_words"], at[:, :9].to(torch.int32))
+    even = torch.full((rows, 1), 3000.0, device="cuda").double().log()
+    # (sums of 3000 terms)
+    near(o["lse"], even[:, 0], 3100 * EPS32 * even[:, 0], "lse")
+    near(o["entropy"], even[:, 0], 3100 * EPS32 * even[:, 0], "entropy")
+    near(o["logp"], torch.where(w >= 0, -even, 0.0), 3100 * EPS32 * even, "logp")
+
+
+@pytest.mark.parametrize("rows, dt", [(5, "bf16"), (300, "f16"), (300, "f32")])
+def test_captured_at_a_low_temperature(rows, dt):
+    X, E, w = whole((rows, 40), dt, 1), whole((9000, 40), dt, 2), words_of(rows, 3, 9000, 3)
+    o = dict(logp=empty(rows, 3), lse=empty(rows), entropy=empty(rows), top_words=empty(rows, 5, dtype=torch.int32), top_logp=empty(rows, 5))
+    dlogp, dX, dE = rand((rows, 3), "f32", 4) * 1e-3, torch.zeros_like(X), torch.zeros_like(E)
+    ws = torch.empty(max(d.vocab_probs_workspace(rows, 40, 9000, 3, 5, DTYPES[dt])), dtype=torch.uint8, device="cuda")
+
+    def step():
+        d.op_vocab_probs(X, E, w, temperature=1e-3, workspace=ws, **o)
+        d.op_vocab_probs_backward(X, E, w, o["logp"], o["lse"], dlogp=dlogp, dX=dX, dE=dE, temperature=1e-3, workspace=ws)
+        return [t.clone() for t in (*o.values(), dX, dE)]
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(4):
+        X.copy_(whole((rows, 40), dt, 10 + i))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
+        torch.cuda.synchronize()
