@@ -643,7 +643,8 @@ int dnpeff_vocab_loss_backward(void* stream, int type, int64_t rows, int64_t n_i
  * log p come from differences of products, not from lse as it is rounded, and are never above 0.  They are off by what those differences
  * are, times 1 / T: alternatives' are of 64 bits; a given word's product is summed in fp32 by itself, below T = 1/16 it is one of the very
  * sums that lse is made of, so that of a word ahead of all others by more than fp32 sums are off log p is 0 at any T.
- * The workspace of alternatives holds logits, up to 2 GB of them at a time.
+ * The workspace of alternatives holds logits, up to 2 GB of them at a time, and so does that of long given or listed words (where the rows of E
+ * of all of them would be 128 MB and more), in distillation too.
  * With n_given = 0 words and logp may be NULL, with n_top = 0 the alternatives; lse and entropy may be NULL.
  * The workspace call serves dnpeff_vocab_distill and its gradients as well (n_given: the listed words, n_top = 0). */
 int dnpeff_vocab_probs_workspace(int type, int64_t rows, int64_t n_in, int64_t n_words, int n_given, int n_top, int aligned,
@@ -674,7 +675,8 @@ int dnpeff_vocab_distill(void* stream, int type, int64_t rows, int64_t n_in, int
                          float* loss, float* logp, float* lse, void* workspace, int64_t workspace_bytes);
 /* Its gradients for dloss [rows], from the logp and lse of the forward call: dz_v = (p_v - sum_j q_j [v = w_j]) dloss / T (the
  * factor T^2 that keeps gradients of different temperatures alike is the caller's, in dloss).  Rows without listed words
- * contribute nothing, whatever their rows of X hold; where the loss is NaN for the lists' sake dX's row and dE are. */
+ * contribute nothing, whatever their rows of X hold; where the loss is NaN for the lists' sake dX's row and dE are.  p, its rounding and
+ * that of dz, and rows whose lse is not finite: as above. */
 int dnpeff_vocab_distill_backward(void* stream, int type, int64_t rows, int64_t n_in, int64_t n_words, const void* X, int64_t ldx,
                                   const void* E, int64_t lde, float temperature, int n_listed, const int32_t* words,
                                   const float* logits, const float* logp, const float* lse, const float* dloss, void* dX,

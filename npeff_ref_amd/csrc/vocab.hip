@@ -542,16 +542,16 @@ int loss_backward(hipStream_t st, int64_t rows, int64_t n_in, int64_t words, con
 // Listed words of the gradients.  The tiles write dz = p (a + b log p) for all words, k_spots what the few listed ones have instead, from
 // their log p of the forward pass: each value is still rounded once.
 //
-// What bounds them: E of few rows (one token of 32000 words of 4096 in bf16: 43 us at 6.2 TB/s, and 20 for the one workgroup that
+// What bounds them: E of few rows (one token of 32000 words of 4096 in bf16: 42 us at 6.3 TB/s, and 21 for the one workgroup that
 // selects and orders, which waits for memory); the matrix cores of many.  8192 tokens of 131072 words of 4096 in bf16 with 64
-// alternatives: products 6.8 ms (1300 TFLOP/s), selection 0.24, 4.8 GB of E's rows read again for their order 0.74 (6.5 TB/s).
+// alternatives: products 6.4 ms (1367 TFLOP/s), selection 0.22, 4.8 GB of E's rows read again for their order 0.74 (6.5 TB/s).
 constexpr int MOST_TOP = 128, SPARE = 8, MOST_KEEP = MOST_TOP + SPARE;
 constexpr int MOST_LISTED = 4096;
 constexpr int64_t BLOCK_ROWS = 65536;                 // rows at a time, for the workspace's sake
-constexpr int64_t LOGIT_BYTES = (int64_t)2 << 30;   // of a piece's logits (512 MB: 9.2 ms where 2 GB take 9.0)
+constexpr int64_t LOGIT_BYTES = (int64_t)2 << 30;   // of a piece's logits (512 MB: 7.89 ms where 2 GB take 7.64)
 constexpr int64_t WHOLE_BYTES = (int64_t)128 << 20; // of all logits that are stored without a small first piece
 // Given words' logits: rows of E read again and multiplied in fp32, or, where that would be so many bytes, taken from the tiles (us
-// there and here: 20 words of 2000 rows of 1024, 82 MB, 904 and 924 with the gradients; 100 of 1999 of 1030, 412 MB, 420 and 340).
+// there and here: 20 words of 2000 rows of 1024, 82 MB, 914 and 922 with the gradients; 100 of 1999 of 1030, 412 MB, 318 and 290).
 constexpr int64_t STORED_FROM = (int64_t)128 << 20;
 // answer_args::stored: given words' products are among the logits of the pieces; are in logp already
 enum { NOT_STORED = 0, IN_LOGITS = 1, IN_PLACE = 2 };
@@ -1465,7 +1465,7 @@ answer_room answer_room_of(int64_t rows, int64_t n_in, int64_t words, int n_give
     int64_t most = LOGIT_BYTES / (4 * r.each) / 256 * 256;
     if (most < 1024) most = 1024;
     // A first piece small enough that storing all of it costs little, and large enough to know a floor for the others from (us with and without: 2000
-    // rows of 50001 words with 20 alternatives 299 and 315, 8192 of 131072 with 64 7620 and 7770, 600 of 128000 with 5 276 and 299).
+    // rows of 50001 words with 20 alternatives 301 and 306, 8192 of 131072 with 64 7640 and 7710, 600 of 128000 of 1024 with 5 276 and 293).
     const int64_t few_words = ceil_div((int64_t)r.keep * 96, 2048) * 2048;
     if (n_top > 0 && !r.few && 4 * r.each * words > WHOLE_BYTES && 6 * few_words <= words) r.first = few_words < most ? few_words : most;
     const int64_t rest = words - r.first;
